@@ -290,6 +290,164 @@ int msplat_hip_copy_intermediate(const char* name, void* dst, size_t* nbytes);
  * counterpart in the reference; it changes no state. */
 int msplat_hip_raster_work(int64_t counts[6]);
 
+/* Operators of a learned head over the features of gaussians or pixels (rows)
+ * that is trained next to a scene: layer norm, a gated feed-forward block and
+ * dropout added to a residual, each with its backward pass.  No counterpart in
+ * the reference.
+ *
+ * dtype names the one type of all of a call's matrices and vectors but mean
+ * and rstd, which are fp32; sums are fp32 in every type, and a gradient has
+ * the type of what it belongs to.  Matrices are row-major with a stride in
+ * elements between rows (>= the row's length; elements of a row are adjacent)
+ * and may start at any element.  rows may be 0 (gradients summed over rows are
+ * then 0), at most 2^31 - 1.
+ *
+ * stream: NULL for the context's stream, or a HIP stream for this call.
+ * Nothing is allocated and no call waits, so all of them may be captured into
+ * a graph.  The workspace is the caller's: 16-byte aligned, of at least the
+ * bytes that the operator's _workspace function gives for the same sizes (it
+ * needs no device, and gives -1 for sizes that the operator refuses); its
+ * contents need not be kept between calls, and calls that may overlap need one
+ * each.  Outputs must not overlap inputs, except that y or dx of layer norm
+ * and of dropout may be exactly an input matrix with the same stride. */
+#define MSPLAT_F32 0
+#define MSPLAT_F16 1
+#define MSPLAT_BF16 2
+
+/* y = (x - mean) rstd weight + bias over the last axis of x [rows, dim], 1 <=
+ * dim <= 8192, with rstd = 1 / sqrt(variance + eps).  weight and bias [dim]:
+ * NULL for ones and zeros.  mean and rstd [rows] are written where not NULL;
+ * the backward pass takes them. */
+typedef struct MsplatLayerNormArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;
+    const void* x;
+    int64_t x_stride;
+    const void* weight;
+    const void* bias;
+    float eps;
+    void* y;
+    int64_t y_stride;
+    float* mean;
+    float* rstd;
+} MsplatLayerNormArgs;
+int msplat_hip_layer_norm(const MsplatLayerNormArgs* args);
+
+/* Gradients of layer norm from dy and the forward pass's x, mean and rstd: dx
+ * [rows, dim], dweight and dbias [dim], each written where not NULL.  The
+ * sums over rows have a fixed order.  The workspace may be NULL where neither
+ * dweight nor dbias is wanted. */
+typedef struct MsplatLayerNormGradArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;
+    int64_t x_stride;
+    const void* weight;
+    const float* mean;
+    const float* rstd;
+    void* dx;
+    int64_t dx_stride;
+    void* dweight;
+    void* dbias;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatLayerNormGradArgs;
+int64_t msplat_hip_layer_norm_backward_workspace(int64_t rows, int32_t dim, int32_t dtype);
+int msplat_hip_layer_norm_backward(const MsplatLayerNormGradArgs* args);
+
+/* y = (a(x w_gate^T) * (x w_up^T)) w_down^T, with x and y [rows, dim], w_gate
+ * and w_up [hidden, dim] and w_down [dim, hidden]; 1 <= dim <= 256, 1 <=
+ * hidden <= 65536.  activation a: MSPLAT_SILU v / (1 + exp(-v)), MSPLAT_GELU
+ * the tanh form of GELU.  The hidden units stay on the chip; in 16-bit types
+ * they are rounded to the type before the last product. */
+#define MSPLAT_SILU 0
+#define MSPLAT_GELU 1
+typedef struct MsplatGatedFfnArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t hidden;
+    int32_t dtype;
+    int32_t activation;
+    const void* x;
+    int64_t x_stride;
+    const void* w_gate;
+    int64_t gate_stride;
+    const void* w_up;
+    int64_t up_stride;
+    const void* w_down;
+    int64_t down_stride;
+    void* y;
+    int64_t y_stride;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatGatedFfnArgs;
+int64_t msplat_hip_gated_ffn_workspace(int64_t rows, int32_t dim, int32_t hidden, int32_t dtype);
+int msplat_hip_gated_ffn(const MsplatGatedFfnArgs* args);
+
+/* Gradients of the gated feed-forward block from dy, x and the weights: dx
+ * [rows, dim] where not NULL, and dw_gate, dw_up [hidden, dim] and dw_down
+ * [dim, hidden], contiguous, all three or (all NULL) none.  The sums over
+ * rows have a fixed order. */
+typedef struct MsplatGatedFfnGradArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t hidden;
+    int32_t dtype;
+    int32_t activation;
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;
+    int64_t x_stride;
+    const void* w_gate;
+    int64_t gate_stride;
+    const void* w_up;
+    int64_t up_stride;
+    const void* w_down;
+    int64_t down_stride;
+    void* dx;
+    int64_t dx_stride;
+    void* dw_gate;
+    void* dw_up;
+    void* dw_down;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatGatedFfnGradArgs;
+int64_t msplat_hip_gated_ffn_backward_workspace(int64_t rows, int32_t dim, int32_t hidden, int32_t dtype);
+int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* args);
+
+/* y = residual + (keep ? x / (1 - p) : 0), x, residual (NULL for none) and y
+ * [rows, dim], 1 <= dim, 0 <= p <= 1; a dropped element counts as 0 whatever it
+ * holds.  The mask is not stored: keep at (row, column) is word >= floor(p
+ * 2^32) for word column % 4 of Philox 4x32 with seven rounds (Salmon, Moraes,
+ * Dror and Shaw, SC 2011), key = (seed's low, high 32 bits), counter = (column
+ * / 4, row, offset's low, high 32 bits).  A training program gives each
+ * layer its seed and each step its offset.  The gradient of x is the same call
+ * on dy without a residual, and the residual's is dy. */
+typedef struct MsplatDropoutArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;
+    double p;
+    uint64_t seed;
+    uint64_t offset;
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+} MsplatDropoutArgs;
+int msplat_hip_dropout_add(const MsplatDropoutArgs* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -170,6 +170,52 @@ class EvalMetrics(ctypes.Structure):
                 ("numGaussians", c_int32)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    """MsplatLayerNormArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("x", c_void_p),
+                ("x_stride", c_int64), ("weight", c_void_p), ("bias", c_void_p), ("eps", c_float), ("y", c_void_p),
+                ("y_stride", c_int64), ("mean", c_void_p), ("rstd", c_void_p)]
+
+
+class LayerNormGradArgs(ctypes.Structure):
+    """MsplatLayerNormGradArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("dy", c_void_p),
+                ("dy_stride", c_int64), ("x", c_void_p), ("x_stride", c_int64), ("weight", c_void_p),
+                ("mean", c_void_p), ("rstd", c_void_p), ("dx", c_void_p), ("dx_stride", c_int64),
+                ("dweight", c_void_p), ("dbias", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+class GatedFfnArgs(ctypes.Structure):
+    """MsplatGatedFfnArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("hidden", c_int32), ("dtype", c_int32),
+                ("activation", c_int32), ("x", c_void_p), ("x_stride", c_int64), ("w_gate", c_void_p),
+                ("gate_stride", c_int64), ("w_up", c_void_p), ("up_stride", c_int64), ("w_down", c_void_p),
+                ("down_stride", c_int64), ("y", c_void_p), ("y_stride", c_int64), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64)]
+
+
+class GatedFfnGradArgs(ctypes.Structure):
+    """MsplatGatedFfnGradArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("hidden", c_int32), ("dtype", c_int32),
+                ("activation", c_int32), ("dy", c_void_p), ("dy_stride", c_int64), ("x", c_void_p),
+                ("x_stride", c_int64), ("w_gate", c_void_p), ("gate_stride", c_int64), ("w_up", c_void_p),
+                ("up_stride", c_int64), ("w_down", c_void_p), ("down_stride", c_int64), ("dx", c_void_p),
+                ("dx_stride", c_int64), ("dw_gate", c_void_p), ("dw_up", c_void_p), ("dw_down", c_void_p),
+                ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
+class DropoutArgs(ctypes.Structure):
+    """MsplatDropoutArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("p", c_double),
+                ("seed", c_uint64), ("offset", c_uint64), ("x", c_void_p), ("x_stride", c_int64),
+                ("residual", c_void_p), ("residual_stride", c_int64), ("y", c_void_p), ("y_stride", c_int64)]
+
+
 # (name, restype, argtypes) for every symbol declared in include/msplat_hip.h,
 # include/msplat_c_api.h and include/msplat_trainer.h
 SIGNATURES = [
@@ -212,6 +258,14 @@ SIGNATURES = [
      [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_float, POINTER(ImageMetrics)]),
     ("msplat_hip_image_metrics_noalloc", c_int,
      [c_void_p, c_void_p, c_int32, c_int32, c_int32, c_float, POINTER(ImageMetrics)]),
+    ("msplat_hip_layer_norm", c_int, [POINTER(LayerNormArgs)]),
+    ("msplat_hip_layer_norm_backward_workspace", c_int64, [c_int64, c_int32, c_int32]),
+    ("msplat_hip_layer_norm_backward", c_int, [POINTER(LayerNormGradArgs)]),
+    ("msplat_hip_gated_ffn_workspace", c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    ("msplat_hip_gated_ffn", c_int, [POINTER(GatedFfnArgs)]),
+    ("msplat_hip_gated_ffn_backward_workspace", c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    ("msplat_hip_gated_ffn_backward", c_int, [POINTER(GatedFfnGradArgs)]),
+    ("msplat_hip_dropout_add", c_int, [POINTER(DropoutArgs)]),
     # include/msplat_c_api.h (the reference's C API)
     ("msplat_dataset_create", c_void_p, [c_char_p, c_float, c_bool, c_int]),
     ("msplat_dataset_destroy", None, [c_void_p]),

@@ -554,6 +554,75 @@ int forward(Ctx* c, const MsplatRenderArgs* a, bool training, float* dst_img = n
     return MSPLAT_OK;
 }
 
+// Checks shared by the learned-head operators.
+int check_rows(int64_t rows, int dim, int max_dim, int dtype) {
+    if (rows < 0 || rows > 0x7FFFFFFF) return fail(MSPLAT_ERR_ARG, "rows %lld outside [0, 2^31)", (long long)rows);
+    if (dim < 1 || dim > max_dim) return fail(MSPLAT_ERR_ARG, "dim %d outside [1, %d]", dim, max_dim);
+    if (dtype != MSPLAT_F32 && dtype != MSPLAT_F16 && dtype != MSPLAT_BF16)
+        return fail(MSPLAT_ERR_ARG, "unknown dtype %d", dtype);
+    return MSPLAT_OK;
+}
+
+// A matrix [rows, dim]; only one without rows may be null.
+int check_matrix(const char* name, const void* p, int64_t rows, int dim, int64_t stride, int dtype) {
+    if (!p && rows > 0) return fail(MSPLAT_ERR_ARG, "%s is null", name);
+    if (stride < dim && rows > 1)
+        return fail(MSPLAT_ERR_ARG, "%s's stride %lld is below its row length %d", name, (long long)stride, dim);
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == MSPLAT_F32 ? 4 : 2) != 0)
+        return fail(MSPLAT_ERR_ARG, "%s is not aligned to its type", name);
+    return MSPLAT_OK;
+}
+
+int check_workspace(const void* ws, int64_t bytes, size_t need) {
+    if (need == 0) return MSPLAT_OK;
+    if (!ws || bytes < 0 || (size_t)bytes < need)
+        return fail(MSPLAT_ERR_ARG, "workspace of %lld bytes, %zu needed", ws ? (long long)bytes : 0LL, need);
+    if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) return fail(MSPLAT_ERR_ARG, "workspace must be 16-byte aligned");
+    return MSPLAT_OK;
+}
+
+#define CHECK(expr)                     \
+    do {                                \
+        int r_ = (expr);                \
+        if (r_ != MSPLAT_OK) return r_; \
+    } while (0)
+
+int check_ffn_sizes(int64_t rows, int dim, int hidden, int dtype) {
+    CHECK(check_rows(rows, dim, FFN_DIM_MAX, dtype));
+    if (hidden < 1 || hidden > FFN_HIDDEN_MAX)
+        return fail(MSPLAT_ERR_ARG, "hidden %d outside [1, %d]", hidden, FFN_HIDDEN_MAX);
+    return MSPLAT_OK;
+}
+
+// What forward and backward of the gated feed-forward block have in common.
+template <class A>
+int check_ffn(const A* a, FfnArgs& f) {
+    CHECK(check_ffn_sizes(a->rows, a->dim, a->hidden, a->dtype));
+    if (a->activation != MSPLAT_SILU && a->activation != MSPLAT_GELU)
+        return fail(MSPLAT_ERR_ARG, "unknown activation %d", a->activation);
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    CHECK(check_matrix("w_gate", a->w_gate, a->hidden, a->dim, a->gate_stride, a->dtype));
+    CHECK(check_matrix("w_up", a->w_up, a->hidden, a->dim, a->up_stride, a->dtype));
+    CHECK(check_matrix("w_down", a->w_down, a->dim, a->hidden, a->down_stride, a->dtype));
+    f = FfnArgs{};
+    f.rows = a->rows;
+    f.dim = a->dim;
+    f.hidden = a->hidden;
+    f.gelu = a->activation == MSPLAT_GELU;
+    f.x = a->x;
+    f.x_stride = a->x_stride;
+    f.w_gate = a->w_gate;
+    f.w_up = a->w_up;
+    f.w_down = a->w_down;
+    f.gate_stride = a->gate_stride;
+    f.up_stride = a->up_stride;
+    f.down_stride = a->down_stride;
+    f.ws = static_cast<char*>(a->workspace);
+    return MSPLAT_OK;
+}
+
+hipStream_t stream_of(void* s) { return s ? reinterpret_cast<hipStream_t>(s) : g_ctx->stream; }
+
 }  // namespace
 
 extern "C" {
@@ -1246,6 +1315,143 @@ int msplat_hip_copy_intermediate(const char* name, void* dst, size_t* nbytes) {
         return MSPLAT_OK;
     }
     return fail(MSPLAT_ERR_ARG, "unknown intermediate '%s'", name);
+}
+
+int msplat_hip_layer_norm(const MsplatLayerNormArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, NORM_DIM_MAX, a->dtype));
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    if (!(a->eps >= 0.f)) return fail(MSPLAT_ERR_ARG, "eps must be at least 0");
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    NormArgs n{};
+    n.rows = a->rows;
+    n.dim = a->dim;
+    n.eps = a->eps;
+    n.x = a->x;
+    n.weight = a->weight;
+    n.bias = a->bias;
+    n.x_stride = a->x_stride;
+    n.out = a->y;
+    n.out_stride = a->y_stride;
+    n.mean = a->mean;
+    n.rstd = a->rstd;
+    launch_norm_fwd(stream_of(a->stream), a->dtype, n);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_layer_norm_backward_workspace(int64_t rows, int32_t dim, int32_t dtype) {
+    if (check_rows(rows, dim, NORM_DIM_MAX, dtype) != MSPLAT_OK) return -1;
+    return (int64_t)norm_groups(rows, dim, dtype) * 2 * dim * 4;
+}
+
+int msplat_hip_layer_norm_backward(const MsplatLayerNormGradArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, NORM_DIM_MAX, a->dtype));
+    CHECK(check_matrix("dy", a->dy, a->rows, a->dim, a->dy_stride, a->dtype));
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->dim, a->dx_stride, a->dtype));
+    if (a->rows > 0 && (!a->mean || !a->rstd)) return fail(MSPLAT_ERR_ARG, "mean or rstd is null");
+    const bool sums = a->dweight || a->dbias;
+    if (sums)
+        CHECK(check_workspace(a->workspace, a->workspace_bytes,
+                              (size_t)norm_groups(a->rows, a->dim, a->dtype) * 2 * a->dim * 4));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    NormArgs n{};
+    n.rows = a->rows;
+    n.dim = a->dim;
+    n.x = a->x;
+    n.dy = a->dy;
+    n.weight = a->weight;
+    n.x_stride = a->x_stride;
+    n.dy_stride = a->dy_stride;
+    n.out = a->dx;
+    n.out_stride = a->dx_stride;
+    n.mean = const_cast<float*>(a->mean);
+    n.rstd = const_cast<float*>(a->rstd);
+    n.part = sums ? static_cast<float*>(a->workspace) : nullptr;
+    if (!sums && (!a->dx || a->rows == 0)) return MSPLAT_OK;
+    launch_norm_bwd(stream_of(a->stream), a->dtype, n, a->dweight, a->dbias);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_gated_ffn_workspace(int64_t rows, int32_t dim, int32_t hidden, int32_t dtype) {
+    if (check_ffn_sizes(rows, dim, hidden, dtype) != MSPLAT_OK) return -1;
+    return (int64_t)ffn_workspace(dtype, rows, dim, hidden, false);
+}
+
+int msplat_hip_gated_ffn(const MsplatGatedFfnArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    FfnArgs f;
+    CHECK(check_ffn(a, f));
+    CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, ffn_workspace(a->dtype, a->rows, a->dim, a->hidden, false)));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    f.out = a->y;
+    f.out_stride = a->y_stride;
+    launch_ffn_fwd(stream_of(a->stream), a->dtype, f);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_gated_ffn_backward_workspace(int64_t rows, int32_t dim, int32_t hidden, int32_t dtype) {
+    if (check_ffn_sizes(rows, dim, hidden, dtype) != MSPLAT_OK) return -1;
+    return (int64_t)ffn_workspace(dtype, rows, dim, hidden, true);
+}
+
+int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    FfnArgs f;
+    CHECK(check_ffn(a, f));
+    CHECK(check_matrix("dy", a->dy, a->rows, a->dim, a->dy_stride, a->dtype));
+    if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->dim, a->dx_stride, a->dtype));
+    const int given = (a->dw_gate != nullptr) + (a->dw_up != nullptr) + (a->dw_down != nullptr);
+    if (given != 0 && given != 3)
+        return fail(MSPLAT_ERR_ARG, "dw_gate, dw_up and dw_down are wanted together or not at all");
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, ffn_workspace(a->dtype, a->rows, a->dim, a->hidden, true)));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (given == 0 && (!a->dx || a->rows == 0)) return MSPLAT_OK;
+    f.dy = a->dy;
+    f.dy_stride = a->dy_stride;
+    f.out = a->dx;
+    f.out_stride = a->dx_stride;
+    f.dw_gate = a->dw_gate;
+    f.dw_up = a->dw_up;
+    f.dw_down = a->dw_down;
+    launch_ffn_bwd(stream_of(a->stream), a->dtype, f);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int msplat_hip_dropout_add(const MsplatDropoutArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, 0x7FFFFF00, a->dtype));
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->dim, a->residual_stride, a->dtype));
+    CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    if (!(a->p >= 0.0 && a->p <= 1.0)) return fail(MSPLAT_ERR_ARG, "p %g outside [0, 1]", a->p);
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    DropArgs d{};
+    d.rows = a->rows;
+    d.dim = a->dim;
+    d.x = a->x;
+    d.x_stride = a->x_stride;
+    d.residual = a->residual;
+    d.residual_stride = a->residual_stride;
+    d.out = a->y;
+    d.out_stride = a->y_stride;
+    d.scale = (float)(1.0 / (1.0 - a->p));
+    d.threshold = (uint64_t)(a->p * 4294967296.0);
+    d.seed = a->seed;
+    d.offset = a->offset;
+    launch_dropout(stream_of(a->stream), a->dtype, d);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
 }
 
 }  // extern "C"

@@ -407,4 +407,54 @@ void launch_resize_area(hipStream_t s, const float* src, int sw, int sh, float* 
 void launch_undistort(hipStream_t s, const float* src, int w, int h, const UndistortParams& u,
                       float* dst);
 
+// Layer norm over the last axis (norm.hip).  Strides in elements; dtype as in
+// msplat_hip.h.  mean / rstd may be null in the forward, weight and bias in
+// both.
+constexpr int NORM_DIM_MAX = 8192;
+struct NormArgs {
+    int64_t rows;
+    int dim;
+    float eps;
+    const void *x, *dy, *weight, *bias;
+    int64_t x_stride, dy_stride, out_stride;
+    void* out;        // y, or dx (may be null in the backward)
+    float *mean, *rstd;
+    float* part;      // backward: [groups][2][dim] sums of dy n and dy
+};
+void launch_norm_fwd(hipStream_t s, int dtype, const NormArgs& a);
+int norm_groups(int64_t rows, int dim, int dtype);
+void launch_norm_bwd(hipStream_t s, int dtype, const NormArgs& a, void* dweight, void* dbias);
+
+// Dropout added to a residual (dropout.hip): out = residual + keep * x * scale,
+// residual null for none.
+struct DropArgs {
+    int64_t rows;
+    int dim;
+    const void *x, *residual;
+    void* out;
+    int64_t x_stride, residual_stride, out_stride;
+    float scale;           // 1 / (1 - p), unused where threshold keeps nothing
+    uint64_t threshold;    // a word below it drops its element
+    uint64_t seed, offset;
+};
+void launch_dropout(hipStream_t s, int dtype, const DropArgs& a);
+
+// Gated feed-forward block (ffn_*.hip): y = (act(x Wg^T) * (x Wu^T)) Wd^T.
+constexpr int FFN_DIM_MAX = 256;
+constexpr int FFN_HIDDEN_MAX = 1 << 16;
+struct FfnArgs {
+    int64_t rows;
+    int dim, hidden;
+    int gelu;
+    const void *x, *dy, *w_gate, *w_up, *w_down;
+    int64_t x_stride, dy_stride, out_stride;
+    int64_t gate_stride, up_stride, down_stride;
+    void* out;                       // y, or dx (may be null in the backward)
+    void *dw_gate, *dw_up, *dw_down; // contiguous; all null: not wanted
+    char* ws;
+};
+size_t ffn_workspace(int dtype, int64_t rows, int dim, int hidden, bool backward);
+void launch_ffn_fwd(hipStream_t s, int dtype, const FfnArgs& a);
+void launch_ffn_bwd(hipStream_t s, int dtype, const FfnArgs& a);
+
 }  // namespace msp
