@@ -25,17 +25,46 @@ struct Piece {
 template <class T>
 using piece_t = typename Piece<T>::type;
 
-// Elements k .. k + E - 1 of a row of n, zero from n on.
+// v's elements moved down by n (0 .. E - 1, the same in every lane), zeros
+// behind them.
+template <class T>
+__device__ __forceinline__ piece_t<T> moved_down(piece_t<T> v, int n) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    u32x4 w;
+    __builtin_memcpy(&w, &v, 16);
+    const int bytes = n * (int)sizeof(T);
+    if (bytes & 8) w = u32x4{w[2], w[3], 0, 0};
+    if (bytes & 4) w = u32x4{w[1], w[2], w[3], 0};
+    if (bytes & 2) w = u32x4{w[0] >> 16 | w[1] << 16, w[1] >> 16 | w[2] << 16, w[2] >> 16 | w[3] << 16, w[3] >> 16};
+    __builtin_memcpy(&v, &w, 16);
+    return v;
+}
+
+// Elements k .. k + E - 1 of a row of n >= E (k a multiple of E), zero from n
+// on, in two steps so that a read may be under way while something else runs.
+// The last piece of a row that E does not divide is read so that it ends with
+// the row, and moved down: one read for every piece.
+template <class T>
+__device__ __forceinline__ piece_t<T> read_piece(const T* row, int k, int n) {
+    piece_t<T> v;
+    __builtin_memcpy(&v, row + min(k, n - E<T>), 16);
+    return v;
+}
+template <class T>
+__device__ __forceinline__ piece_t<T> settle_piece(piece_t<T> v, int k, int n, bool live) {
+    if (n % E<T> != 0 && k > n - E<T>) v = moved_down<T>(v, E<T> - n % E<T>);
+    if (k >= n || !live) v = piece_t<T>{};
+    return v;
+}
+
+// The same in one step, for rows of any length.
 template <class T>
 __device__ __forceinline__ piece_t<T> load_piece(const T* row, int k, int n) {
+    if (n >= E<T>) return settle_piece<T>(read_piece(row, k, n), k, n, true);
     piece_t<T> v = {};
-    if (k + E<T> <= n) {
-        __builtin_memcpy(&v, row + k, 16);
-    } else {
 #pragma unroll
-        for (int j = 0; j < E<T>; ++j)
-            if (k + j < n) v[j] = row[k + j];
-    }
+    for (int j = 0; j < E<T>; ++j)
+        if (k + j < n) v[j] = row[k + j];
     return v;
 }
 

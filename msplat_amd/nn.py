@@ -35,7 +35,8 @@ def _library(t):
 def _stream(t) -> Optional[int]:
     """PyTorch's current stream; None (the library's own stream, which is
     ordered with it) for the default stream."""
-    return torch.cuda.current_stream(t.device).cuda_stream or None
+    # the stream object of torch.cuda.current_stream costs 2 us a call
+    return torch._C._cuda_getCurrentRawStream(t.device.index) or None
 
 
 def _rows(name, t, dim, like):
@@ -80,7 +81,7 @@ def _same_rows(name, t, x2):
 def _workspace(nbytes, like):
     if nbytes < 0:
         raise _abi.MsplatError(f"msplat_hip error: {_abi.load().msplat_hip_last_error().decode()}")
-    return torch.empty(nbytes, dtype=torch.uint8, device=like.device)
+    return like.new_empty(-(-nbytes // like.element_size()))
 
 
 def _ptr(t):
@@ -95,9 +96,9 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5) -> Tuple[to
     rows, dim = x2.shape
     w = None if weight is None else _matrix("weight", weight, (dim,), x)
     b = None if bias is None else _matrix("bias", bias, (dim,), x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
+    y = x.new_empty(x.shape)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = mean.new_empty(mean.shape)
     a = _abi.LayerNormArgs(_stream(x), rows, dim, dtype, x2.data_ptr(), x2.stride(0), _ptr(w), _ptr(b), eps,
                            y.data_ptr(), dim, mean.data_ptr(), rstd.data_ptr())
     _abi.check(lib.msplat_hip_layer_norm(ctypes.byref(a)))
@@ -116,13 +117,13 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
         if t.dtype is not torch.float32 or t.numel() != rows or t.device != x.device:
             raise ValueError(f"{name} must hold one float32 a row on {x.device}")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dweight = torch.empty(dim, dtype=x.dtype, device=x.device)
-    dbias = torch.empty_like(dweight)
+    dx = x.new_empty(x.shape)
+    dweight = x.new_empty(dim)
+    dbias = x.new_empty(dim)
     ws = _workspace(lib.msplat_hip_layer_norm_backward_workspace(rows, dim, dtype), x)
     a = _abi.LayerNormGradArgs(_stream(x), rows, dim, dtype, dy2.data_ptr(), dy2.stride(0), x2.data_ptr(),
                                x2.stride(0), _ptr(w), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dim,
-                               dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.numel())
+                               dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.nbytes)
     _abi.check(lib.msplat_hip_layer_norm_backward(ctypes.byref(a)))
     return dx, dweight, dbias
 
@@ -145,11 +146,11 @@ def gated_ffn_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
     lib, dtype = _library(x), _dtype(x)
     x2, hidden, wg, wu, wd = _ffn_operands(x, w_gate, w_up, w_down, activation)
     rows, dim = x2.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     ws = _workspace(lib.msplat_hip_gated_ffn_workspace(rows, dim, hidden, dtype), x)
     a = _abi.GatedFfnArgs(_stream(x), rows, dim, hidden, dtype, _ACTIVATIONS[activation], x2.data_ptr(),
                           x2.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0), wd.data_ptr(),
-                          wd.stride(0), y.data_ptr(), dim, ws.data_ptr(), ws.numel())
+                          wd.stride(0), y.data_ptr(), dim, ws.data_ptr(), ws.nbytes)
     _abi.check(lib.msplat_hip_gated_ffn(ctypes.byref(a)))
     return y
 
@@ -160,14 +161,14 @@ def gated_ffn_backward(dy, x, w_gate, w_up, w_down, activation: str = "silu"):
     x2, hidden, wg, wu, wd = _ffn_operands(x, w_gate, w_up, w_down, activation)
     rows, dim = x2.shape
     dy2 = _same_rows("dy", dy, x2)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    grads = [torch.empty(s, dtype=x.dtype, device=x.device) for s in ((hidden, dim), (hidden, dim), (dim, hidden))]
+    dx = x.new_empty(x.shape)
+    grads = x.new_empty((hidden, dim)), x.new_empty((hidden, dim)), x.new_empty((dim, hidden))
     ws = _workspace(lib.msplat_hip_gated_ffn_backward_workspace(rows, dim, hidden, dtype), x)
     a = _abi.GatedFfnGradArgs(_stream(x), rows, dim, hidden, dtype, _ACTIVATIONS[activation], dy2.data_ptr(),
                               dy2.stride(0), x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0),
                               wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0), dx.data_ptr(), dim,
                               grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), ws.data_ptr(),
-                              ws.numel())
+                              ws.nbytes)
     _abi.check(lib.msplat_hip_gated_ffn_backward(ctypes.byref(a)))
     return (dx, *grads)
 
@@ -179,7 +180,7 @@ def _dropout(x, residual, p, seed, offset):
     x2 = _feature_rows("x", x)
     rows, dim = x2.shape
     r2 = None if residual is None else _same_rows("residual", residual, x2)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
                          x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
     _abi.check(lib.msplat_hip_dropout_add(ctypes.byref(a)))

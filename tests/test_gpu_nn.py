@@ -137,6 +137,28 @@ def test_gated_ffn(nn, dtype, rows, dim, hidden):
         assert all(torch.equal(p, q) for p, q in zip(got, again))
 
 
+# more rows than workgroups that take all hidden units: weights through LDS,
+# whole (narrow blocks) or block by block
+FFN_MANY = [(16500, 5, 9), (17001, 32, 600), (20011, 45, 100), (16399, 64, 1000), (9007, 96, 64), (8707, 128, 96),
+            (8300, 200, 333), (8201, 256, 40)]
+
+
+@pytest.mark.parametrize("rows,dim,hidden", FFN_MANY)
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_gated_ffn_of_many_rows(nn, dtype, rows, dim, hidden):
+    act = "gelu" if dim % 2 else "silu"
+    ops = _ffn_operands(rows, dim, hidden, dtype)
+    want, bound = orc.gated_ffn_bounds(*ops, act)
+    orc.within(nn.gated_ffn_forward(*ops, act), want, bound, f"y {act}")
+    dy = _normal(30, rows, dim, dtype=dtype)
+    got = nn.gated_ffn_backward(dy, *ops, act)
+    want, bound = orc.gated_ffn_grad_bounds(dy, *ops, act)
+    for g, v, e, what in zip(got, want, bound, ("dx", "dw_gate", "dw_up", "dw_down")):
+        orc.within(g, v, e, f"{what} {act}")
+    again = (nn.gated_ffn_forward(*ops, act), *nn.gated_ffn_backward(dy, *ops, act))
+    assert all(torch.equal(p, q) for p, q in zip(again, (nn.gated_ffn_forward(*ops, act), *got)))
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_gated_ffn_errors_are_those_of_rounding(nn, dtype):
     """Whole outputs: h, dg and du are rounded to the type once and the output
