@@ -69,6 +69,44 @@ __device__ __forceinline__ piece_t<T> join(const f32x4* t) {
     return o;
 }
 
+// A block of KB rows of a matrix [rows, dim] as fragments rows x dim: the piece
+// of row perm(s, r), elements (4 kb + c) E ..., lies at slot(kb, s, c, r).  The
+// order of rows turns with c so that by_dim's reads spread over LDS's banks.
+template <class T>
+__device__ __forceinline__ int slot(int kb, int s, int c, int r) {
+    return (kb * HT<T> + s) * 64 + c * 16 + (r ^ (sizeof(T) == 4 ? c : c * 4));
+}
+// Fragment f = kb HT + s, rows x dim.
+template <class T>
+__device__ __forceinline__ piece_t<T> by_row(const piece_t<T>* block, int f) {
+    const int lane = threadIdx.x & 63;
+    return block[slot<T>(0, 0, lane >> 4, lane & 15) + f * 64];
+}
+// Fragment f = kb HT + s, dim x rows, of a block in LDS: column kb KB + perm(s,
+// r), elements consecutive rows.  16-bit types take the transposing LDS read,
+// in which lane 4 k + c of 16 brings 4 elements of row k and lane i gets
+// element i % 4 of the lanes 4 k + i / 4.
+template <class T>
+__device__ __forceinline__ piece_t<T> by_dim(const piece_t<T>* block, int f) {
+    const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15;
+    piece_t<T> o;
+    if constexpr (sizeof(T) == 2) {
+        typedef short s16x4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const char* base = reinterpret_cast<const char*>(block + slot<T>(0, 0, j & 3, q * 4 + (j >> 2)));
+        s16x4 h[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+            h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + ((f >> 1) * 2 + t) * 1024 + (f & 1) * 8));
+        __builtin_memcpy(&o, h, 16);
+    } else {
+        const float* base = reinterpret_cast<const float*>(block + f * 64);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = base[slot<T>(0, 0, j >> 2, q * 4 + e) * 4 + (j & 3)];
+    }
+    return o;
+}
+
 constexpr float LOG2E = 1.44269504088896341f;
 constexpr float GELU_A = 1.59576912160573071f;             // 2 sqrt(2/pi)
 constexpr float GELU_B = 0.0713548162726009f;              // 0.044715 * GELU_A
@@ -95,9 +133,11 @@ __device__ __forceinline__ void act_grad(float& g, float& u, float& dh) {
 // Fragments of the weights, block of hidden units after block: in a block the
 // matrices in order, DK * HT fragments each.  Rows x contraction index:
 // forward  0 Wg (hidden x dim)  1 Wu  2 Wd (dim x hidden)
-// backward 0 Wg  1 Wu  2 Wd^T (hidden x dim)  3 Wg^T (dim x hidden)  4 Wu^T
+// backward 0 Wg  1 Wu  2 Wd^T (hidden x dim), and for few rows
+//          3 Wg^T (dim x hidden)  4 Wu^T
 template <class T>
-__global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, int dk, int hblocks, int mats, piece_t<T>* out) {
+__global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, bool backward, int dk, int hblocks,
+                                                  int mats, piece_t<T>* out) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int lane = (int)(i & 63), r = lane & 15, q = lane >> 4;
     const int64_t f = i >> 6;
@@ -105,7 +145,7 @@ __global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, int dk, int hblocks
     const int64_t bm = f / (HT<T> * dk);
     const int m = (int)(bm % mats), b = (int)(bm / mats);
     if (b >= hblocks) return;
-    const bool hidden_rows = m < 2 || (mats == 5 && m == 2);
+    const bool hidden_rows = m < 2 || (backward && m == 2);
     const bool down = m == 2;
     const T* w = static_cast<const T*>(down ? a.w_down : (m == 1 || m == 4) ? a.w_up : a.w_gate);
     const int64_t stride = down ? a.down_stride : (m == 1 || m == 4) ? a.up_stride : a.gate_stride;
@@ -116,7 +156,7 @@ __global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, int dk, int hblocks
         const int d = kb * KB<T> + (hidden_rows ? q * E<T> + j : perm<T>(s, r));
         if (h < a.hidden && d < a.dim) v[j] = down ? w[d * stride + h] : w[h * stride + d];
     }
-    out[i] = v;
+    out[f * 64 + slot<T>(0, 0, q, r)] = v;
 }
 
 // Copies n fragments (1 KB each) from memory to LDS without registers in
@@ -131,8 +171,8 @@ __device__ __forceinline__ void fetch(const piece_t<T>* src, piece_t<T>* lds, in
 }
 
 // The pieces of R rows' operand fragments, in two steps (read_piece,
-// settle_piece).  Only a width of one block may be less than a piece.
-template <class T, int DK, int R>
+// settle_piece).  TINY: rows are less than a piece.
+template <class T, int DK, int R, bool TINY>
 __device__ __forceinline__ void read_rows(const void* base, int64_t stride, int64_t row0, int64_t rows, int dim, int q,
                                           piece_t<T> (&f)[R][DK]) {
 #pragma unroll
@@ -140,23 +180,23 @@ __device__ __forceinline__ void read_rows(const void* base, int64_t stride, int6
         const T* row = static_cast<const T*>(base) + min(row0 + 16 * r, rows - 1) * stride;
 #pragma unroll
         for (int kb = 0; kb < DK; ++kb)
-            f[r][kb] = DK == 1 && dim < E<T> ? load_piece(row, q * E<T>, dim) : read_piece(row, kb * KB<T> + q * E<T>, dim);
+            f[r][kb] = TINY ? load_piece(row, q * E<T>, dim) : read_piece(row, kb * KB<T> + q * E<T>, dim);
     }
 }
-template <class T, int DK, int R>
+template <class T, int DK, int R, bool TINY>
 __device__ __forceinline__ void settle_rows(int64_t row0, int64_t rows, int dim, int q, piece_t<T> (&f)[R][DK]) {
-    if (DK == 1 && dim < E<T>) return;
+    if (TINY) return;
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int kb = 0; kb < DK; ++kb)
             f[r][kb] = settle_piece<T>(f[r][kb], kb * KB<T> + q * E<T>, dim, row0 + 16 * r < rows);
 }
-template <class T, int DK, int R>
+template <class T, int DK, int R, bool TINY>
 __device__ __forceinline__ void load_rows(const void* base, int64_t stride, int64_t row0, int64_t rows, int dim, int q,
                                           piece_t<T> (&f)[R][DK]) {
-    read_rows<T, DK, R>(base, stride, row0, rows, dim, q, f);
-    settle_rows<T, DK, R>(row0, rows, dim, q, f);
+    read_rows<T, DK, R, TINY>(base, stride, row0, rows, dim, q, f);
+    settle_rows<T, DK, R, TINY>(row0, rows, dim, q, f);
 }
 
 template <class T, int DK, int R>
@@ -174,6 +214,24 @@ __device__ __forceinline__ void store_rows(void* base, int64_t stride, int64_t r
     }
 }
 
+// Order of issue for a step of `groups` groups of LDS reads and the matrix
+// instructions that take them: reads run `ahead` groups in front, so that
+// their latency passes behind matrix work.  (The compiler by itself reads a
+// group, waits, and multiplies.)
+template <int READS, int MFMAS, int GROUPS, int AHEAD>
+__device__ __forceinline__ void read_ahead() {
+    constexpr int A = AHEAD < GROUPS ? AHEAD : GROUPS;
+    __builtin_amdgcn_sched_group_barrier(0x100, READS * A, 0);
+#pragma unroll
+    for (int g = 0; g < GROUPS - A; ++g) {
+        __builtin_amdgcn_sched_group_barrier(0x8, MFMAS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x8, MFMAS * A, 0);
+}
+template <class T>
+constexpr int MFMAS = sizeof(T) == 4 ? 4 : 1;   // matrix instructions of an mma
+
 // The two steps of a block of hidden units for R tiles of 16 rows: h from x,
 // then its part of y.
 template <class T, int DK, int R, bool GELU>
@@ -183,13 +241,14 @@ __device__ __forceinline__ void fwd_up(const piece_t<T>* up, const piece_t<T> (&
     f32x4 g[R][HT<T>] = {}, u[R][HT<T>] = {};
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-        const piece_t<T> wg = up[f * 64 + lane], wu = up[(F + f) * 64 + lane];
+        const piece_t<T> wg = by_row<T>(up, f), wu = by_row<T>(up, F + f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             g[r][f % HT<T>] = mma(wg, xf[r][f / HT<T>], g[r][f % HT<T>]);
             u[r][f % HT<T>] = mma(wu, xf[r][f / HT<T>], u[r][f % HT<T>]);
         }
     }
+    read_ahead<2, 2 * R * MFMAS<T>, F, 2>();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -202,10 +261,11 @@ __device__ __forceinline__ void fwd_down(const piece_t<T>* down, const piece_t<T
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-        const piece_t<T> wd = down[f * 64 + lane];
+        const piece_t<T> wd = by_row<T>(down, f);
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][f] = mma(wd, h[r], acc[r][f]);
     }
+    read_ahead<1, R * MFMAS<T>, F, 2>();
 }
 
 // dg and du from x and dy, then their part of dx.
@@ -217,7 +277,7 @@ __device__ __forceinline__ void dx_up(const piece_t<T>* up, const piece_t<T> (&x
     f32x4 g[R][HT<T>] = {}, u[R][HT<T>] = {}, dh[R][HT<T>] = {};
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-        const piece_t<T> wg = up[f * 64 + lane], wu = up[(F + f) * 64 + lane], wd = up[(2 * F + f) * 64 + lane];
+        const piece_t<T> wg = by_row<T>(up, f), wu = by_row<T>(up, F + f), wd = by_row<T>(up, 2 * F + f);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             g[r][f % HT<T>] = mma(wg, xf[r][f / HT<T>], g[r][f % HT<T>]);
@@ -225,6 +285,7 @@ __device__ __forceinline__ void dx_up(const piece_t<T>* up, const piece_t<T> (&x
             dh[r][f % HT<T>] = mma(wd, df[r][f / HT<T>], dh[r][f % HT<T>]);
         }
     }
+    read_ahead<3, 3 * R * MFMAS<T>, F, 2>();
 #pragma unroll
     for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -238,62 +299,69 @@ __device__ __forceinline__ void dx_up(const piece_t<T>* up, const piece_t<T> (&x
         du[r] = join<T>(u[r]);
     }
 }
-template <class T, int F, int R>
+// With TURN the fragments dim x hidden are those of Wg and Wu themselves, in
+// LDS; else they were packed too.
+template <class T, int F, int R, bool TURN>
 __device__ __forceinline__ void dx_down(const piece_t<T>* down, const piece_t<T> (&dg)[R], const piece_t<T> (&du)[R],
                                         f32x4 (&acc)[R][F]) {
-    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int f = 0; f < F; ++f) {
-        const piece_t<T> wg = down[f * 64 + lane], wu = down[(F + f) * 64 + lane];
+        const piece_t<T> wg = TURN ? by_dim<T>(down, f) : by_row<T>(down, f);
+        const piece_t<T> wu = TURN ? by_dim<T>(down + F * 64, f) : by_row<T>(down, F + f);
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[r][f] = mma(wu, du[r], mma(wg, dg[r], acc[r][f]));
     }
+    if (TURN) read_ahead<sizeof(T) == 4 ? 8 : 4, 2 * R * MFMAS<T>, F, 2>();
 }
 
 // A wave takes R tiles of 16 rows and walks the hidden units block by block.
 // The workgroup's waves share a block's weights in LDS, in two areas: while
-// one of the two steps of a block computes, the other's weights arrive.
-template <class T, int DK, int R, int WAVES, bool GELU>
-__global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd(FfnArgs a, const piece_t<T>* packed, int hblocks) {
+// one is computed with, the next block's weights arrive in the other.
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
+__global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd(FfnArgs a, const piece_t<T>* packed, int hblocks, int mats) {
     constexpr int F = DK * HT<T>;
-    __shared__ piece_t<T> up[2 * F * 64], down[F * 64];
+    __shared__ piece_t<T> even[3 * F * 64], odd[3 * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    const int64_t row0 = ((int64_t)blockIdx.x * WAVES + wave) * (16 * R) + (lane & 15);
-    fetch<T>(packed, up, 2 * F);
-    piece_t<T> xf[R][DK], h[R];
-    load_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+    const int64_t row0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * (16 * R) + (lane & 15);
+    fetch<T>(packed, even, 3 * F);
+    piece_t<T> xf[R][DK];
+    load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     f32x4 acc[R][F] = {};
-    __syncthreads();
-    for (int b = 0; b < hblocks; ++b) {
-        fetch<T>(packed + ((int64_t)b * 3 * F + 2 * F) * 64, down, F);
-        fwd_up<T, DK, R, GELU>(up, xf, h);
+    auto block = [&](int b, const piece_t<T>* w, piece_t<T>* next) {
         __syncthreads();
-        if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * 3 * F * 64, up, 2 * F);
-        fwd_down<T, F, R>(down, h, acc);
-        __syncthreads();
+        if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * mats * F * 64, next, 3 * F);
+        piece_t<T> h[R];
+        fwd_up<T, DK, R, GELU>(w, xf, h);
+        fwd_down<T, F, R>(w + 2 * F * 64, h, acc);
+    };
+    for (int b = 0; b < hblocks; b += 2) {
+        block(b, even, odd);
+        if (b + 1 < hblocks) block(b + 1, odd, even);
     }
     store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
 }
 
-template <class T, int DK, int R, int WAVES, bool GELU>
-__global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<T>* packed, int hblocks) {
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
+__global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<T>* packed, int hblocks, int mats) {
     constexpr int F = DK * HT<T>;
-    __shared__ piece_t<T> up[3 * F * 64], down[2 * F * 64];
+    __shared__ piece_t<T> even[3 * F * 64], odd[3 * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    const int64_t row0 = ((int64_t)blockIdx.x * WAVES + wave) * (16 * R) + (lane & 15);
-    fetch<T>(packed, up, 3 * F);
-    piece_t<T> xf[R][DK], df[R][DK], dg[R], du[R];
-    load_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
-    load_rows<T, DK, R>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
+    const int64_t row0 = ((int64_t)blockIdx.x * (blockDim.x >> 6) + wave) * (16 * R) + (lane & 15);
+    fetch<T>(packed, even, 3 * F);
+    piece_t<T> xf[R][DK], df[R][DK];
+    load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+    load_rows<T, DK, R, TINY>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
     f32x4 acc[R][F] = {};
-    __syncthreads();
-    for (int b = 0; b < hblocks; ++b) {
-        fetch<T>(packed + ((int64_t)b * 5 * F + 3 * F) * 64, down, 2 * F);
-        dx_up<T, DK, R, GELU>(up, xf, df, dg, du);
+    auto block = [&](int b, const piece_t<T>* w, piece_t<T>* next) {
         __syncthreads();
-        if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * 5 * F * 64, up, 3 * F);
-        dx_down<T, F, R>(down, dg, du, acc);
-        __syncthreads();
+        if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * mats * F * 64, next, 3 * F);
+        piece_t<T> dg[R], du[R];
+        dx_up<T, DK, R, GELU>(w, xf, df, dg, du);
+        dx_down<T, F, R, true>(w, dg, du, acc);
+    };
+    for (int b = 0; b < hblocks; b += 2) {
+        block(b, even, odd);
+        if (b + 1 < hblocks) block(b + 1, odd, even);
     }
     store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
 }
@@ -301,7 +369,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<
 // The same where all packed weights fit in LDS: a workgroup loads them once,
 // then its waves walk row tiles on their own, with no barrier that would hold
 // all of them at the matrix or at the vector instructions at once.
-template <class T, int DK, int R, int WAVES, bool GELU>
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const piece_t<T>* packed, int hblocks) {
     constexpr int F = DK * HT<T>;
     extern __shared__ char smem[];
@@ -309,17 +377,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const pie
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
     fetch<T>(packed, w, hblocks * 3 * F);
     __syncthreads();
-    const int64_t step = (int64_t)gridDim.x * WAVES;
-    int64_t row0 = ((int64_t)blockIdx.x * WAVES + wave) * (16 * R) + (lane & 15);
+    const int64_t waves = blockDim.x >> 6, step = gridDim.x * waves;
+    int64_t row0 = (blockIdx.x * waves + wave) * (16 * R) + (lane & 15);
     piece_t<T> xf[R][DK], xn[R][DK], h[R];
-    read_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xn);
+    read_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xn);
     for (; row0 - (lane & 15) < a.rows; row0 += step * (16 * R)) {
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int kb = 0; kb < DK; ++kb) xf[r][kb] = xn[r][kb];
-        settle_rows<T, DK, R>(row0, a.rows, a.dim, q, xf);
-        read_rows<T, DK, R>(a.x, a.x_stride, row0 + step * (16 * R), a.rows, a.dim, q, xn);
+        settle_rows<T, DK, R, TINY>(row0, a.rows, a.dim, q, xf);
+        read_rows<T, DK, R, TINY>(a.x, a.x_stride, row0 + step * (16 * R), a.rows, a.dim, q, xn);
         f32x4 acc[R][F] = {};
         for (int b = 0; b < hblocks; ++b) {
             fwd_up<T, DK, R, GELU>(w + b * 3 * F * 64, xf, h);
@@ -329,23 +397,24 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const pie
     }
 }
 
-template <class T, int DK, int R, int WAVES, bool GELU>
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_all(FfnArgs a, const piece_t<T>* packed, int hblocks) {
     constexpr int F = DK * HT<T>;
     extern __shared__ char smem[];
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(smem);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    fetch<T>(packed, w, hblocks * 5 * F);
+    fetch<T>(packed, w, hblocks * 3 * F);
     __syncthreads();
-    for (int64_t t = (int64_t)blockIdx.x * WAVES + wave; t * (16 * R) < a.rows; t += (int64_t)gridDim.x * WAVES) {
+    const int64_t waves = blockDim.x >> 6;
+    for (int64_t t = blockIdx.x * waves + wave; t * (16 * R) < a.rows; t += gridDim.x * waves) {
         const int64_t row0 = t * (16 * R) + (lane & 15);
         piece_t<T> xf[R][DK], df[R][DK], dg[R], du[R];
-        load_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
-        load_rows<T, DK, R>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
+        load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+        load_rows<T, DK, R, TINY>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
         f32x4 acc[R][F] = {};
         for (int b = 0; b < hblocks; ++b) {
-            dx_up<T, DK, R, GELU>(w + b * 5 * F * 64, xf, df, dg, du);
-            dx_down<T, F, R>(w + (b * 5 + 3) * F * 64, dg, du, acc);
+            dx_up<T, DK, R, GELU>(w + b * 3 * F * 64, xf, df, dg, du);
+            dx_down<T, F, R, true>(w + b * 3 * F * 64, dg, du, acc);
         }
         store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
     }
@@ -380,14 +449,14 @@ __device__ __forceinline__ void add_waves(f32x4 (&acc)[R][F], f32x4* lds) {
 
 // The forward reads the weights as they are: all three matrices' fragments lie
 // along their rows.
-template <class T, int DK, int R, int WAVES, bool GELU>
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hblocks) {
     constexpr int F = DK * HT<T>;
     __shared__ f32x4 sums[WAVES / 2 * R * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i = lane & 15;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * R) + i;
     piece_t<T> xf[R][DK], h[R];
-    load_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+    load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     f32x4 acc[R][F] = {};
     for (int b = wave; b < hblocks; b += WAVES) {
         piece_t<T> wg[F], wu[F], wd[F];
@@ -432,59 +501,23 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hbloc
     if (wave == 0) store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
 }
 
-template <class T, int DK, int R, int WAVES, bool GELU>
+template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piece_t<T>* packed, int hblocks) {
     constexpr int F = DK * HT<T>;
     __shared__ f32x4 sums[WAVES / 2 * R * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
     const int64_t row0 = (int64_t)blockIdx.x * (16 * R) + (lane & 15);
     piece_t<T> xf[R][DK], df[R][DK], dg[R], du[R];
-    load_rows<T, DK, R>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
-    load_rows<T, DK, R>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
+    load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+    load_rows<T, DK, R, TINY>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
     f32x4 acc[R][F] = {};
     for (int b = wave; b < hblocks; b += WAVES) {
         const piece_t<T>* w = packed + (int64_t)b * 5 * F * 64;
         dx_up<T, DK, R, GELU>(w, xf, df, dg, du);
-        dx_down<T, F, R>(w + 3 * F * 64, dg, du, acc);
+        dx_down<T, F, R, false>(w + 3 * F * 64, dg, du, acc);
     }
     add_waves<T, F, R, WAVES>(acc, sums);
     if (wave == 0) store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
-}
-
-// A block of KB rows of x (or dy) in LDS, as operand fragments rows x dim: the
-// piece of row perm(s, r), elements (4 kb + c) E ..., lies at slot(kb, s, c, r),
-// whose order of rows turns with c so that by_dim's reads spread over the banks.
-template <class T>
-__device__ __forceinline__ int slot(int kb, int s, int c, int r) {
-    return (kb * HT<T> + s) * 64 + c * 16 + (r ^ (sizeof(T) == 4 ? c : (c & 1) * 4));
-}
-template <class T>
-__device__ __forceinline__ piece_t<T> by_row(const piece_t<T>* rows, int f) {
-    const int lane = threadIdx.x & 63;
-    return rows[slot<T>(0, 0, lane >> 4, lane & 15) + f * 64];
-}
-// The fragment dim x rows of 16 columns from 16 dt on, whose elements are
-// consecutive rows: 16-bit types through the transposing LDS read, in which
-// the lanes 4 k + i / 4 of 16 give lane i element i % 4 of their 8 bytes.
-template <class T>
-__device__ __forceinline__ piece_t<T> by_dim(const piece_t<T>* rows, int dt) {
-    const int lane = threadIdx.x & 63, q = lane >> 4, j = lane & 15;
-    piece_t<T> o;
-    if constexpr (sizeof(T) == 2) {
-        typedef short s16x4 __attribute__((ext_vector_type(4)));
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const char* base = reinterpret_cast<const char*>(rows + slot<T>(0, 0, (j & 3) >> 1, q * 4 + (j >> 2))) + (j & 1) * 8;
-        base += (dt >> 1) * (2 * 64 * 16) + (dt & 1) * (2 * 16 * 16);
-        s16x4 h[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(base + s * 64 * 16));
-        __builtin_memcpy(&o, h, 16);
-    } else {
-        const float* base = reinterpret_cast<const float*>(rows + dt * 64);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = base[slot<T>(0, 0, j >> 2, q * 4 + e) * 4 + (j & 3)];
-    }
-    return o;
 }
 
 // Weight gradients: a wave owns NH tiles of 16 hidden units, keeps their
@@ -505,9 +538,9 @@ constexpr int dw_occupancy(int dk, int nh) {
     return dk * nh * (int)sizeof(T) <= 8 ? 2 : 1;
 }
 
-template <class T, int DK, int NH, int WAVES, bool GELU>
+template <class T, int DK, int NH, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES, WAVES / 4 * dw_occupancy<T>(DK, NH)) void k_ffn_dw(
-    FfnArgs a, const piece_t<T>* packed, int hblocks, int slices, int64_t blocks_per_group, f32x4* part) {
+    FfnArgs a, const piece_t<T>* packed, int hblocks, int mats, int slices, int64_t blocks_per_group, f32x4* part) {
     constexpr int F = DK * HT<T>;
     constexpr int ITEMS = (2 * F + WAVES - 1) / WAVES;   // pieces a thread brings
     __shared__ piece_t<T> xy[2][2 * F * 64];             // x, then dy
@@ -522,10 +555,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4 * dw_occupancy<T>(DK, NH)) vo
         for (int kb = 0; kb < DK; ++kb) {
             wg[n][kb] = wu[n][kb] = wd[n][kb] = piece_t<T>{};
             if (b < hblocks) {
-                const piece_t<T>* p = packed + ((int64_t)b * 5 * F + kb * HT<T> + s) * 64 + lane;
-                wg[n][kb] = p[0];
-                wu[n][kb] = p[F * 64];
-                wd[n][kb] = p[2 * F * 64];
+                const piece_t<T>* p = packed + ((int64_t)b * mats * F + kb * HT<T> + s) * 64;
+                wg[n][kb] = by_row<T>(p, 0);
+                wu[n][kb] = by_row<T>(p, F);
+                wd[n][kb] = by_row<T>(p, 2 * F);
             }
         }
     }
@@ -533,33 +566,50 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4 * dw_occupancy<T>(DK, NH)) vo
     const int64_t first = group * blocks_per_group * KB<T>;
     const int64_t last = min(a.rows, first + blocks_per_group * KB<T>);
 
-    // a thread's pieces of a block: read, and on the next turn put into LDS
+    // A thread's pieces of a block: read, and on the next turn put into LDS.
+    // The last block of all is read so that it ends with the rows (the order
+    // of rows in a block does not matter), and rows before it count as zero.
     piece_t<T> in[ITEMS];
+    int64_t off[ITEMS];
+#pragma unroll
+    for (int k = 0; k < ITEMS; ++k) {
+        int i = k * 64 * WAVES + threadIdx.x;
+        const bool y = i >= F * 64;
+        i -= y ? F * 64 : 0;
+        const int64_t row = min((int64_t)(i / (DK * 4)), a.rows - 1);
+        off[k] = row * (y ? a.dy_stride : a.x_stride) + (TINY ? 0 : min(i % (DK * 4) * E<T>, a.dim - E<T>));
+    }
+    const int64_t final_block = a.rows > KB<T> ? a.rows - KB<T> : 0;
     auto load = [&](int64_t row0) {
+        const int64_t from = min(row0, final_block);
+        const T* xb = static_cast<const T*>(a.x) + from * a.x_stride;
+        const T* yb = static_cast<const T*>(a.dy) + from * a.dy_stride;
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
-            int i = k * 64 * WAVES + threadIdx.x;
-            const bool y = i >= F * 64;
-            i -= y ? F * 64 : 0;
-            if (2 * F % WAVES != 0 && i >= F * 64) continue;
-            const int64_t row = min(row0 + i / (DK * 4), a.rows - 1);
-            const T* p = static_cast<const T*>(y ? a.dy : a.x) + row * (y ? a.dy_stride : a.x_stride);
-            const int c = i % (DK * 4) * E<T>;
-            in[k] = DK == 1 && a.dim < E<T> ? load_piece(p, c, a.dim) : read_piece(p, c, a.dim);
+            const int i = k * 64 * WAVES + threadIdx.x;
+            if (2 * F % WAVES != 0 && i >= 2 * F * 64) continue;
+            const T* p = (i >= F * 64 ? yb : xb) + off[k];
+            if (TINY) in[k] = load_piece(p, i % 4 * E<T>, a.dim);
+            else __builtin_memcpy(&in[k], p, 16);
         }
     };
     auto store = [&](piece_t<T>* to, int64_t row0) {
+        const int64_t from = min(row0, final_block);
+        const bool whole = from == row0 && row0 + KB<T> <= last && a.dim == DK * KB<T>;
 #pragma unroll
         for (int k = 0; k < ITEMS; ++k) {
             int i = k * 64 * WAVES + threadIdx.x;
+            if (2 * F % WAVES != 0 && i >= 2 * F * 64) continue;
             const bool y = i >= F * 64;
             i -= y ? F * 64 : 0;
-            if (2 * F % WAVES != 0 && i >= F * 64) continue;
             const int w = i / (DK * 4), ch = i % (DK * 4);   // w = perm(s, r)
             const int s = HT<T> == 2 ? (w >> 2) & 1 : 0, r = w / E<T> * 4 + (w & 3);
             piece_t<T> v = in[k];
-            if (DK == 1 && a.dim < E<T>) v = row0 + w < last ? v : piece_t<T>{};
-            else v = settle_piece<T>(v, ch * E<T>, a.dim, row0 + w < last);
+            if (!whole) {
+                const bool live = from + w >= row0 && from + w < last;
+                if (TINY) v = live ? v : piece_t<T>{};
+                else v = settle_piece<T>(v, ch * E<T>, a.dim, live);
+            }
             to[(y ? F * 64 : 0) + slot<T>(ch >> 2, s, ch & 3, r)] = v;
         }
     };
@@ -583,6 +633,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4 * dw_occupancy<T>(DK, NH)) vo
                 h[n][f % HT<T>] = mma(py, wd[n][f / HT<T>], h[n][f % HT<T>]);
             }
         }
+        read_ahead<2, 3 * NH * MFMAS<T>, F, 2>();
         piece_t<T> pg[NH], pu[NH], ph[NH];
 #pragma unroll
         for (int n = 0; n < NH; ++n) {
@@ -608,6 +659,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4 * dw_occupancy<T>(DK, NH)) vo
                 acc[2][n][f] = mma(ph[n], py, acc[2][n][f]);
             }
         }
+        read_ahead<sizeof(T) == 4 ? 8 : 4, 3 * NH * MFMAS<T>, F, 2>();
         __syncthreads();
     }
 #pragma unroll
@@ -636,7 +688,7 @@ __global__ __launch_bounds__(1024) void k_ffn_fold(FfnArgs a, const f32x4* part,
 #pragma unroll
     for (int k = 1; k < 16; ++k) t += red[k][lane];
     const int f = blockIdx.x % fr, m = blockIdx.x / fr % 3, tile = blockIdx.x / fr / 3;
-    const int d = f * 16 + (lane & 15);
+    const int d = f / HT<T> * KB<T> + perm<T>(f % HT<T>, lane & 15);
     const int h0 = tile / HT<T> * KB<T> + perm<T>(tile % HT<T>, (lane >> 4) * 4);
     if (d >= a.dim) return;
 #pragma unroll
@@ -652,27 +704,34 @@ __global__ __launch_bounds__(1024) void k_ffn_fold(FfnArgs a, const f32x4* part,
 template <class T>
 inline int dim_blocks(int dim) {
     const int n = (dim + KB<T> - 1) / KB<T>;
-    constexpr int made[] = {1, 2, 3, 4, 6, 8, 12, 16};
+    constexpr int made[] = {1, 2, 3, 4, 5, 6, 7, 8, 10, 12, 14, 16};
     for (int m : made)
         if (n <= m) return m;
     return 0;
 }
+// Calls f with the number of blocks and whether rows are less than a piece.
 template <class T, class F>
 inline void with_blocks(int dim, F&& f) {
+    if (dim < E<T>) return f(std::integral_constant<int, 1>{}, std::true_type{});
 #define BLOCKS(n) \
-    case n: f(std::integral_constant<int, n>{}); break
+    case n: return f(std::integral_constant<int, n>{}, std::false_type{})
     switch (dim_blocks<T>(dim)) {
         BLOCKS(1);
         BLOCKS(2);
         BLOCKS(3);
         BLOCKS(4);
+        BLOCKS(5);
         BLOCKS(6);
+        BLOCKS(7);
         BLOCKS(8);
-        default:
-            if constexpr (sizeof(T) == 4) {
-                if (dim_blocks<T>(dim) == 12) f(std::integral_constant<int, 12>{});
-                else f(std::integral_constant<int, 16>{});
-            }
+    }
+    if constexpr (sizeof(T) == 4) {
+        switch (dim_blocks<T>(dim)) {
+            BLOCKS(10);
+            BLOCKS(12);
+            BLOCKS(14);
+            BLOCKS(16);
+        }
     }
 #undef BLOCKS
 }
@@ -714,27 +773,46 @@ size_t workspace(int64_t rows, int dim, int hidden, bool backward) {
 }
 
 template <class T>
-piece_t<T>* pack(hipStream_t s, const FfnArgs& a, int dk, int hblocks, int mats) {
+piece_t<T>* pack(hipStream_t s, const FfnArgs& a, bool backward, int dk, int hblocks, int mats) {
     piece_t<T>* packed = reinterpret_cast<piece_t<T>*>(a.ws);
     const int64_t n = (int64_t)hblocks * mats * dk * HT<T> * 64;
-    k_ffn_pack<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, dk, hblocks, mats, packed);
+    k_ffn_pack<T><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a, backward, dk, hblocks, mats, packed);
     return packed;
 }
 
 constexpr int64_t CUS = 256;
 constexpr size_t LDS_BYTES = 160 * 1024;
-inline unsigned groups_of(int64_t rows, int64_t each) { return (unsigned)((rows + each - 1) / each); }
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows up to which a workgroup takes one or two row tiles for all hidden units
 // (k_ffn_*_few): as long as every one of them finds a CU free, twice that
 // where two fit on one.
 inline int64_t few_rows(int fragments) { return 32 * CUS * (fragments <= 4 ? 2 : 1); }
 
-// Workgroups of k_ffn_*_all: as many as are resident at once (16 waves a CU by
-// registers), or fewer for fewer rows.
-inline unsigned resident_groups(int64_t rows, int64_t each, int waves, size_t lds) {
-    const int64_t fit = std::min<int64_t>((int64_t)(LDS_BYTES / lds), 16 / waves) * CUS;
-    return (unsigned)std::min<int64_t>(fit, (rows + each - 1) / each);
+// Launch shape of the kernels whose waves take `tile` rows each: `most` waves
+// a workgroup, fewer where that would leave CUs without one.
+struct Shape {
+    unsigned groups, threads;
+};
+inline Shape shape_of(int64_t rows, int tile, int most, int64_t max_groups) {
+    const int64_t tiles = ceil_div(rows, tile);
+    const int64_t waves = std::min<int64_t>(most, ceil_div(tiles, CUS));
+    return {(unsigned)std::min(ceil_div(tiles, waves), max_groups), (unsigned)(64 * waves)};
+}
+
+// Rows that the streaming kernels leave to the few-row ones: the start of a
+// last round of workgroups that would hold the GPU as long as a full one.
+inline int64_t tail_rows(int64_t rows, int64_t per_round) {
+    const int64_t rest = rows % per_round;
+    return rows > per_round && rest <= 16 * CUS ? rest : 0;
+}
+inline FfnArgs rows_from(FfnArgs a, int64_t from, size_t size) {
+    auto at = [&](const void* p, int64_t stride) { return p ? static_cast<const char*>(p) + from * stride * size : nullptr; };
+    a.x = at(a.x, a.x_stride);
+    a.dy = at(a.dy, a.dy_stride);
+    a.out = const_cast<char*>(at(a.out, a.out_stride));
+    a.rows -= from;
+    return a;
 }
 
 template <class F>
@@ -743,71 +821,104 @@ inline void with_act(const FfnArgs& a, F&& f) {
     else f(std::false_type{});
 }
 
+// Row tiles of a wave in the streaming kernels, and with eight waves a
+// workgroup the workgroups of a CU, by registers and LDS.
+// (96-384 forward 337 us with two tiles, 300 with one; 256-1024 433 with one,
+// 337 with two; its input gradient 2083 with two, 1490 with one.)
+constexpr int fwd_tiles(int fragments) { return fragments <= 6 ? 1 : 2; }
+constexpr int dx_tiles(int fragments) { return fragments <= 8 ? 2 : 1; }
+constexpr int per_cu(int fragments) { return fragments <= 8 ? 2 : 1; }
+
+template <class T, int DK, bool GELU, bool TINY>
+void few_forward(hipStream_t s, const FfnArgs& a, int hblocks) {
+    if (a.rows <= 16 * CUS) k_ffn_fwd_few<T, DK, 1, 8, GELU, TINY><<<ceil_div(a.rows, 16), 512, 0, s>>>(a, hblocks);
+    else k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<ceil_div(a.rows, 32), 512, 0, s>>>(a, hblocks);
+}
+
 template <class T>
 void forward(hipStream_t s, const FfnArgs& a) {
-    with_blocks<T>(a.dim, [&](auto dk) {
+    with_blocks<T>(a.dim, [&](auto dk, auto tiny) {
         with_act(a, [&](auto gelu) {
-            constexpr int F = dk() * HT<T>;
+            constexpr int F = dk() * HT<T>, R = fwd_tiles(F), W = 8;
             const int hblocks = (a.hidden + KB<T> - 1) / KB<T>;
-            if (a.rows <= 16 * CUS) {
-                k_ffn_fwd_few<T, dk(), 1, 8, gelu()><<<groups_of(a.rows, 16), 512, 0, s>>>(a, hblocks);
-                return;
-            }
-            if (a.rows <= few_rows(F)) {
-                k_ffn_fwd_few<T, dk(), 2, 8, gelu()><<<groups_of(a.rows, 32), 512, 0, s>>>(a, hblocks);
-                return;
-            }
-            const piece_t<T>* packed = pack<T>(s, a, dk(), hblocks, 3);
+            if (a.rows <= few_rows(F)) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks);
+            const piece_t<T>* packed = pack<T>(s, a, false, dk(), hblocks, 3);
             const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
             if constexpr (F <= 4) {
                 if (lds <= LDS_BYTES) {
-                    k_ffn_fwd_all<T, dk(), 2, 16, gelu()><<<resident_groups(a.rows, 32 * 16, 16, lds), 1024, lds, s>>>(
-                        a, packed, hblocks);
+                    const Shape g = shape_of(a.rows, 32, 16, CUS);
+                    k_ffn_fwd_all<T, dk(), 2, 16, gelu(), tiny()><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
                     return;
                 }
             }
-            k_ffn_fwd<T, dk(), 2, 8, gelu()><<<groups_of(a.rows, 32 * 8), 512, 0, s>>>(a, packed, hblocks);
+            FfnArgs main = a;
+            const int64_t tail = tail_rows(a.rows, 16 * R * W * per_cu(F) * CUS);
+            if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks);
+            main.rows -= tail;
+            const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
+            k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
         });
     });
 }
 
-template <class T, int DK, bool GELU>
-void input_gradient(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks) {
-    constexpr int F = DK * HT<T>;
-    if (a.rows <= 16 * CUS) {
-        k_ffn_dx_few<T, DK, 1, 8, GELU><<<groups_of(a.rows, 16), 512, 0, s>>>(a, packed, hblocks);
-        return;
-    }
-    if (a.rows <= few_rows(F)) {
-        k_ffn_dx_few<T, DK, 2, 8, GELU><<<groups_of(a.rows, 32), 512, 0, s>>>(a, packed, hblocks);
-        return;
-    }
-    const size_t lds = packed_bytes<T>(a.dim, a.hidden, 5);
+template <class T, int DK, bool GELU, bool TINY>
+void few_dx(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks) {
+    if (a.rows <= 16 * CUS) k_ffn_dx_few<T, DK, 1, 8, GELU, TINY><<<ceil_div(a.rows, 16), 512, 0, s>>>(a, packed, hblocks);
+    else k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<ceil_div(a.rows, 32), 512, 0, s>>>(a, packed, hblocks);
+}
+
+// How the input's gradient is made: few rows, resident weights, or streamed
+// weights with a tail of few rows; the few-row kernel needs five matrices.
+template <class T>
+struct DxPlan {
+    int64_t tail;
+    int mats;
+    bool all;
+};
+template <class T>
+DxPlan<T> dx_plan(const FfnArgs& a, int fragments) {
+    if (a.rows <= few_rows(fragments)) return {a.rows, 5, false};
+    if (fragments <= 4 && packed_bytes<T>(a.dim, a.hidden, 3) <= LDS_BYTES) return {0, 3, true};
+    const int64_t tail = tail_rows(a.rows, 16 * dx_tiles(fragments) * 8 * per_cu(fragments) * CUS);
+    return {tail, tail ? 5 : 3, false};
+}
+
+template <class T, int DK, bool GELU, bool TINY>
+void input_gradient(hipStream_t s, const FfnArgs& a, const DxPlan<T>& plan, const piece_t<T>* packed, int hblocks) {
+    constexpr int F = DK * HT<T>, R = dx_tiles(F), W = 8;
+    if (plan.tail) few_dx<T, DK, GELU, TINY>(s, rows_from(a, a.rows - plan.tail, sizeof(T)), packed, hblocks);
+    if (plan.tail == a.rows) return;
     if constexpr (F <= 4) {
-        if (lds <= LDS_BYTES) {
-            k_ffn_dx_all<T, DK, 2, 8, GELU><<<resident_groups(a.rows, 32 * 8, 8, lds), 512, lds, s>>>(a, packed, hblocks);
+        if (plan.all) {
+            const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
+            const Shape g = shape_of(a.rows, 32, 8, CUS * (2 * lds <= LDS_BYTES ? 2 : 1));
+            k_ffn_dx_all<T, DK, 2, 8, GELU, TINY><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
             return;
         }
     }
-    constexpr int W = F <= 8 ? 8 : 4;
-    k_ffn_dx<T, DK, 2, W, GELU><<<groups_of(a.rows, 32 * W), 64 * W, 0, s>>>(a, packed, hblocks);
+    FfnArgs main = a;
+    main.rows -= plan.tail;
+    const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
+    k_ffn_dx<T, DK, R, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
 }
 
 template <class T>
 void backward(hipStream_t s, const FfnArgs& a) {
-    with_blocks<T>(a.dim, [&](auto dk) {
+    with_blocks<T>(a.dim, [&](auto dk, auto tiny) {
         constexpr int F = dk() * HT<T>;
         const int hblocks = (a.hidden + KB<T> - 1) / KB<T>;
-        const piece_t<T>* packed = pack<T>(s, a, dk(), hblocks, 5);
+        const DxPlan<T> plan = dx_plan<T>(a, F);
+        const int mats = plan.mats;
+        const piece_t<T>* packed = pack<T>(s, a, true, dk(), hblocks, mats);
         if (a.out && a.rows > 0)
-            with_act(a, [&](auto gelu) { input_gradient<T, dk(), gelu()>(s, a, packed, hblocks); });
+            with_act(a, [&](auto gelu) { input_gradient<T, dk(), gelu(), tiny()>(s, a, plan, packed, hblocks); });
         if (!a.dw_gate) return;
         const Split p = dw_split<T>(a.rows, a.dim, a.hidden);
         f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 5));
         auto dw = [&](auto nh) {
             with_act(a, [&](auto gelu) {
-                k_ffn_dw<T, dk(), nh(), DW_WAVES, gelu()><<<(unsigned)(p.groups * p.slices), 64 * DW_WAVES, 0, s>>>(
-                    a, packed, hblocks, p.slices, p.blocks_per_group, part);
+                k_ffn_dw<T, dk(), nh(), DW_WAVES, gelu(), tiny()><<<(unsigned)(p.groups * p.slices), 64 * DW_WAVES, 0, s>>>(
+                    a, packed, hblocks, mats, p.slices, p.blocks_per_group, part);
             });
         };
         if (p.groups > 0) {

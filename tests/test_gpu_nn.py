@@ -138,9 +138,10 @@ def test_gated_ffn(nn, dtype, rows, dim, hidden):
 
 
 # more rows than workgroups that take all hidden units: weights through LDS,
-# whole (narrow blocks) or block by block
+# whole (narrow blocks) or block by block, the last with a short last round
 FFN_MANY = [(16500, 5, 9), (17001, 32, 600), (20011, 45, 100), (16399, 64, 1000), (9007, 96, 64), (8707, 128, 96),
-            (8300, 200, 333), (8201, 256, 40)]
+            (8300, 200, 333), (8201, 256, 40), (65543, 200, 72),
+            (131079, 112, 33)]
 
 
 @pytest.mark.parametrize("rows,dim,hidden", FFN_MANY)
