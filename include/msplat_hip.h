@@ -302,7 +302,9 @@ int msplat_hip_raster_work(int64_t counts[6]);
  * and may start at any element.  rows may be 0 (gradients summed over rows are
  * then 0), at most 2^31 - 1.
  *
- * stream: NULL for the context's stream, or a HIP stream for this call.
+ * stream: NULL for the context's stream, MSPLAT_DEFAULT_STREAM for the
+ * device's default stream (which is ordered with the context's own), or a HIP
+ * stream for this call.
  * Nothing is allocated and no call waits, so all of them may be captured into
  * a graph.  The workspace is the caller's: 16-byte aligned, of at least the
  * bytes that the operator's _workspace function gives for the same sizes (it
@@ -310,6 +312,7 @@ int msplat_hip_raster_work(int64_t counts[6]);
  * contents need not be kept between calls, and calls that may overlap need one
  * each.  Outputs must not overlap inputs, except that y or dx of layer norm
  * and of dropout may be exactly an input matrix with the same stride. */
+#define MSPLAT_DEFAULT_STREAM ((void*)-1)
 #define MSPLAT_F32 0
 #define MSPLAT_F16 1
 #define MSPLAT_BF16 2

@@ -621,7 +621,10 @@ int check_ffn(const A* a, FfnArgs& f) {
     return MSPLAT_OK;
 }
 
-hipStream_t stream_of(void* s) { return s ? reinterpret_cast<hipStream_t>(s) : g_ctx->stream; }
+hipStream_t stream_of(void* s) {
+    if (s == MSPLAT_DEFAULT_STREAM) return nullptr;
+    return s ? reinterpret_cast<hipStream_t>(s) : g_ctx->stream;
+}
 
 }  // namespace
 

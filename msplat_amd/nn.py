@@ -15,7 +15,7 @@ be captured into a graph.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Tuple
 
 import torch
 
@@ -32,11 +32,14 @@ def _library(t):
     return lib
 
 
-def _stream(t) -> Optional[int]:
-    """PyTorch's current stream; None (the library's own stream, which is
-    ordered with it) for the default stream."""
+_DEFAULT_STREAM = 0xFFFFFFFFFFFFFFFF   # MSPLAT_DEFAULT_STREAM
+
+
+def _stream(t) -> int:
+    """PyTorch's current stream.  The library's own stream would do for the
+    default one, but each change between the two costs the GPU some 10 us."""
     # the stream object of torch.cuda.current_stream costs 2 us a call
-    return torch._C._cuda_getCurrentRawStream(t.device.index) or None
+    return torch._C._cuda_getCurrentRawStream(t.device.index) or _DEFAULT_STREAM
 
 
 def _rows(name, t, dim, like):
