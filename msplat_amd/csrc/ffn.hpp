@@ -447,18 +447,46 @@ __device__ __forceinline__ void add_waves(f32x4 (&acc)[R][F], f32x4* lds) {
     }
 }
 
-// The forward reads the weights as they are: all three matrices' fragments lie
-// along their rows.
+// Where the row tiles are so few that CUs would be left over, `splits`
+// workgroups share a tile's hidden units too and leave their 32-bit parts for
+// k_ffn_join.  The forward reads the weights as they are: all three matrices'
+// fragments lie along their rows.
+template <class T, int F, int R>
+__device__ __forceinline__ void leave_part(const f32x4 (&acc)[R][F], int splits, int split, f32x4* part) {
+    f32x4* at = part + ((int64_t)(blockIdx.x / splits) * splits + split) * R * F * 64 + (threadIdx.x & 63);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < F; ++f) at[(r * F + f) * 64] = acc[r][f];
+}
+
+// Adds a tile's parts in order: a wave per tile of 16 rows and block of
+// columns.
+template <class T>
+__global__ __launch_bounds__(64) void k_ffn_join(FfnArgs a, const f32x4* part, int splits, int tiles_each, int dk) {
+    const int lane = threadIdx.x, kb = blockIdx.x % dk, fr = dk * HT<T>;
+    const int64_t t = blockIdx.x / dk;   // tile of 16 rows
+    const f32x4* at = part + ((t / tiles_each * splits * tiles_each + t % tiles_each) * fr + kb * HT<T>) * 64 + lane;
+    f32x4 sum[HT<T>] = {};
+    for (int s = 0; s < splits; ++s)
+#pragma unroll
+        for (int h = 0; h < HT<T>; ++h) sum[h] += at[((int64_t)s * tiles_each * fr + h) * 64];
+    const int64_t row = t * 16 + (lane & 15);
+    const int k = kb * KB<T> + (lane >> 4) * E<T>;
+    if (row < a.rows && k < a.dim) store_piece(static_cast<T*>(a.out) + row * a.out_stride, k, a.dim, join<T>(sum));
+}
+
 template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
-__global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hblocks) {
+__global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hblocks, int splits, f32x4* part) {
     constexpr int F = DK * HT<T>;
     __shared__ f32x4 sums[WAVES / 2 * R * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, i = lane & 15;
-    const int64_t row0 = (int64_t)blockIdx.x * (16 * R) + i;
+    const int split = blockIdx.x % splits;
+    const int64_t row0 = (int64_t)(blockIdx.x / splits) * (16 * R) + i;
     piece_t<T> xf[R][DK], h[R];
     load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     f32x4 acc[R][F] = {};
-    for (int b = wave; b < hblocks; b += WAVES) {
+    for (int b = split * WAVES + wave; b < hblocks; b += splits * WAVES) {
         piece_t<T> wg[F], wu[F], wd[F];
 #pragma unroll
         for (int s = 0; s < HT<T>; ++s) {
@@ -498,26 +526,32 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hbloc
             for (int r = 0; r < R; ++r) acc[r][f] = mma(wd[f], h[r], acc[r][f]);
     }
     add_waves<T, F, R, WAVES>(acc, sums);
-    if (wave == 0) store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
+    if (wave != 0) return;
+    if (splits > 1) leave_part<T, F, R>(acc, splits, split, part);
+    else store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
 }
 
 template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
-__global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piece_t<T>* packed, int hblocks) {
+__global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piece_t<T>* packed, int hblocks, int splits,
+                                                            f32x4* part) {
     constexpr int F = DK * HT<T>;
     __shared__ f32x4 sums[WAVES / 2 * R * F * 64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
-    const int64_t row0 = (int64_t)blockIdx.x * (16 * R) + (lane & 15);
+    const int split = blockIdx.x % splits;
+    const int64_t row0 = (int64_t)(blockIdx.x / splits) * (16 * R) + (lane & 15);
     piece_t<T> xf[R][DK], df[R][DK], dg[R], du[R];
     load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     load_rows<T, DK, R, TINY>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
     f32x4 acc[R][F] = {};
-    for (int b = wave; b < hblocks; b += WAVES) {
+    for (int b = split * WAVES + wave; b < hblocks; b += splits * WAVES) {
         const piece_t<T>* w = packed + (int64_t)b * 5 * F * 64;
         dx_up<T, DK, R, GELU>(w, xf, df, dg, du);
         dx_down<T, F, R, false>(w + 3 * F * 64, dg, du, acc);
     }
     add_waves<T, F, R, WAVES>(acc, sums);
-    if (wave == 0) store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
+    if (wave != 0) return;
+    if (splits > 1) leave_part<T, F, R>(acc, splits, split, part);
+    else store_rows<T, DK, R>(a.out, a.out_stride, row0, a.rows, a.dim, q, acc);
 }
 
 // Weight gradients: a wave owns NH tiles of 16 hidden units, keeps their
@@ -527,15 +561,17 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piec
 // part[group][tile][matrix][dim tile][lane].
 constexpr int DW_WAVES = 4;
 // Tiles of hidden units a wave of the weight gradient takes, and waves a SIMD,
-// by registers: 12 a tile and 16 columns of sums, as many again for 16-bit
-// weights' halves.
+// by registers: 24 a tile and block of columns for weights and sums.  (Two
+// tiles at three blocks: 96-384 1073 us against 1033; two waves a SIMD at six
+// blocks spill: 192-768 2160 us against 1728.)
 template <class T>
 constexpr int dw_tiles(int dk) {
-    return sizeof(T) == 2 && dk <= 4 ? 2 : 1;
+    return sizeof(T) == 2 && dk <= 2 ? 2 : 1;
 }
 template <class T>
 constexpr int dw_occupancy(int dk, int nh) {
-    return dk * nh * (int)sizeof(T) <= 8 ? 2 : 1;
+    const int n = dk * nh;
+    return n == 1 ? 4 : n == 2 ? 3 : n <= 5 ? 2 : 1;
 }
 
 template <class T, int DK, int NH, int WAVES, bool GELU, bool TINY>
@@ -766,13 +802,6 @@ size_t packed_bytes(int dim, int hidden, int mats) {
 }
 
 template <class T>
-size_t workspace(int64_t rows, int dim, int hidden, bool backward) {
-    if (!backward) return packed_bytes<T>(dim, hidden, 3);
-    const Split p = dw_split<T>(rows, dim, hidden);
-    return packed_bytes<T>(dim, hidden, 5) + (size_t)p.groups * p.tiles * 3 * dim_blocks<T>(dim) * HT<T> * 1024;
-}
-
-template <class T>
 piece_t<T>* pack(hipStream_t s, const FfnArgs& a, bool backward, int dk, int hblocks, int mats) {
     piece_t<T>* packed = reinterpret_cast<piece_t<T>*>(a.ws);
     const int64_t n = (int64_t)hblocks * mats * dk * HT<T> * 64;
@@ -815,6 +844,21 @@ inline FfnArgs rows_from(FfnArgs a, int64_t from, size_t size) {
     return a;
 }
 
+// Bytes of a call's workspace: packed weights, parts that the few-row kernels
+// leave (at most one workgroup a CU shares its tile), the weight gradient's
+// sums.
+template <class T>
+size_t join_bytes(int dim) {
+    return (size_t)CUS * dim_blocks<T>(dim) * HT<T> * 1024;
+}
+template <class T>
+size_t workspace(int64_t rows, int dim, int hidden, bool backward) {
+    if (!backward) return packed_bytes<T>(dim, hidden, 3) + join_bytes<T>(dim);
+    const Split p = dw_split<T>(rows, dim, hidden);
+    return packed_bytes<T>(dim, hidden, 5) + join_bytes<T>(dim) +
+           (size_t)p.groups * p.tiles * 3 * dim_blocks<T>(dim) * HT<T> * 1024;
+}
+
 template <class F>
 inline void with_act(const FfnArgs& a, F&& f) {
     if (a.gelu) f(std::true_type{});
@@ -824,15 +868,41 @@ inline void with_act(const FfnArgs& a, F&& f) {
 // Row tiles of a wave in the streaming kernels, and with eight waves a
 // workgroup the workgroups of a CU, by registers and LDS.
 // (96-384 forward 337 us with two tiles, 300 with one; 256-1024 433 with one,
-// 337 with two; its input gradient 2083 with two, 1490 with one.)
+// 337 with two.  The input gradient holds twice the fragments and has one.)
 constexpr int fwd_tiles(int fragments) { return fragments <= 6 ? 1 : 2; }
-constexpr int dx_tiles(int fragments) { return fragments <= 8 ? 2 : 1; }
 constexpr int per_cu(int fragments) { return fragments <= 8 ? 2 : 1; }
 
+// How the few-row kernels are launched: tiles of a workgroup, workgroups, and
+// the workgroups that share a tile.  A join costs a launch, so it takes three
+// blocks of hidden units a wave to share them out further.
+struct Few {
+    int tiles, splits;
+    unsigned groups;
+    size_t part_bytes;
+};
+template <class T>
+inline Few few_plan(int64_t rows, int dim, int hidden) {
+    Few p;
+    p.tiles = rows <= 16 * CUS ? 1 : 2;
+    const int64_t row_groups = ceil_div(rows, 16 * p.tiles), blocks = ceil_div(hidden, KB<T>);
+    p.splits = blocks > 16 ? (int)std::max<int64_t>(1, std::min(CUS / row_groups, ceil_div(blocks, 8))) : 1;
+    p.groups = (unsigned)(row_groups * p.splits);
+    p.part_bytes = p.splits > 1 ? (size_t)p.groups * p.tiles * dim_blocks<T>(dim) * HT<T> * 1024 : 0;
+    return p;
+}
+template <class T>
+void few_join(hipStream_t s, const FfnArgs& a, const Few& p, const f32x4* part) {
+    if (p.splits == 1) return;
+    const int dk = dim_blocks<T>(a.dim);
+    k_ffn_join<T><<<(unsigned)(ceil_div(a.rows, 16) * dk), 64, 0, s>>>(a, part, p.splits, p.tiles, dk);
+}
+
 template <class T, int DK, bool GELU, bool TINY>
-void few_forward(hipStream_t s, const FfnArgs& a, int hblocks) {
-    if (a.rows <= 16 * CUS) k_ffn_fwd_few<T, DK, 1, 8, GELU, TINY><<<ceil_div(a.rows, 16), 512, 0, s>>>(a, hblocks);
-    else k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<ceil_div(a.rows, 32), 512, 0, s>>>(a, hblocks);
+void few_forward(hipStream_t s, const FfnArgs& a, int hblocks, f32x4* part) {
+    const Few p = few_plan<T>(a.rows, a.dim, a.hidden);
+    if (p.tiles == 1) k_ffn_fwd_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
+    else k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
+    few_join<T>(s, a, p, part);
 }
 
 template <class T>
@@ -841,7 +911,8 @@ void forward(hipStream_t s, const FfnArgs& a) {
         with_act(a, [&](auto gelu) {
             constexpr int F = dk() * HT<T>, R = fwd_tiles(F), W = 8;
             const int hblocks = (a.hidden + KB<T> - 1) / KB<T>;
-            if (a.rows <= few_rows(F)) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks);
+            f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 3));
+            if (a.rows <= few_rows(F)) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks, part);
             const piece_t<T>* packed = pack<T>(s, a, false, dk(), hblocks, 3);
             const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
             if constexpr (F <= 4) {
@@ -853,7 +924,7 @@ void forward(hipStream_t s, const FfnArgs& a) {
             }
             FfnArgs main = a;
             const int64_t tail = tail_rows(a.rows, 16 * R * W * per_cu(F) * CUS);
-            if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks);
+            if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks, part);
             main.rows -= tail;
             const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
             k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
@@ -862,9 +933,11 @@ void forward(hipStream_t s, const FfnArgs& a) {
 }
 
 template <class T, int DK, bool GELU, bool TINY>
-void few_dx(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks) {
-    if (a.rows <= 16 * CUS) k_ffn_dx_few<T, DK, 1, 8, GELU, TINY><<<ceil_div(a.rows, 16), 512, 0, s>>>(a, packed, hblocks);
-    else k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<ceil_div(a.rows, 32), 512, 0, s>>>(a, packed, hblocks);
+void few_dx(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks, f32x4* part) {
+    const Few p = few_plan<T>(a.rows, a.dim, a.hidden);
+    if (p.tiles == 1) k_ffn_dx_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
+    else k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
+    few_join<T>(s, a, p, part);
 }
 
 // How the input's gradient is made: few rows, resident weights, or streamed
@@ -879,27 +952,28 @@ template <class T>
 DxPlan<T> dx_plan(const FfnArgs& a, int fragments) {
     if (a.rows <= few_rows(fragments)) return {a.rows, 5, false};
     if (fragments <= 4 && packed_bytes<T>(a.dim, a.hidden, 3) <= LDS_BYTES) return {0, 3, true};
-    const int64_t tail = tail_rows(a.rows, 16 * dx_tiles(fragments) * 8 * per_cu(fragments) * CUS);
+    const int64_t tail = tail_rows(a.rows, 16 * 8 * per_cu(fragments) * CUS);
     return {tail, tail ? 5 : 3, false};
 }
 
 template <class T, int DK, bool GELU, bool TINY>
-void input_gradient(hipStream_t s, const FfnArgs& a, const DxPlan<T>& plan, const piece_t<T>* packed, int hblocks) {
-    constexpr int F = DK * HT<T>, R = dx_tiles(F), W = 8;
-    if (plan.tail) few_dx<T, DK, GELU, TINY>(s, rows_from(a, a.rows - plan.tail, sizeof(T)), packed, hblocks);
+void input_gradient(hipStream_t s, const FfnArgs& a, const DxPlan<T>& plan, const piece_t<T>* packed, int hblocks,
+                    f32x4* part) {
+    constexpr int F = DK * HT<T>, W = 8;
+    if (plan.tail) few_dx<T, DK, GELU, TINY>(s, rows_from(a, a.rows - plan.tail, sizeof(T)), packed, hblocks, part);
     if (plan.tail == a.rows) return;
     if constexpr (F <= 4) {
         if (plan.all) {
             const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
-            const Shape g = shape_of(a.rows, 32, 8, CUS * (2 * lds <= LDS_BYTES ? 2 : 1));
-            k_ffn_dx_all<T, DK, 2, 8, GELU, TINY><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
+            const Shape g = shape_of(a.rows, 16, 16, CUS);
+            k_ffn_dx_all<T, DK, 1, 16, GELU, TINY><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
             return;
         }
     }
     FfnArgs main = a;
     main.rows -= plan.tail;
-    const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
-    k_ffn_dx<T, DK, R, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
+    const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
+    k_ffn_dx<T, DK, 1, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
 }
 
 template <class T>
@@ -911,10 +985,13 @@ void backward(hipStream_t s, const FfnArgs& a) {
         const int mats = plan.mats;
         const piece_t<T>* packed = pack<T>(s, a, true, dk(), hblocks, mats);
         if (a.out && a.rows > 0)
-            with_act(a, [&](auto gelu) { input_gradient<T, dk(), gelu(), tiny()>(s, a, plan, packed, hblocks); });
+            with_act(a, [&](auto gelu) {
+                f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 5));
+                input_gradient<T, dk(), gelu(), tiny()>(s, a, plan, packed, hblocks, part);
+            });
         if (!a.dw_gate) return;
         const Split p = dw_split<T>(a.rows, a.dim, a.hidden);
-        f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 5));
+        f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 5) + join_bytes<T>(a.dim));
         auto dw = [&](auto nh) {
             with_act(a, [&](auto gelu) {
                 k_ffn_dw<T, dk(), nh(), DW_WAVES, gelu(), tiny()><<<(unsigned)(p.groups * p.slices), 64 * DW_WAVES, 0, s>>>(
