@@ -145,16 +145,26 @@ __global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, bool backward, int 
     const int64_t bm = f / (HT<T> * dk);
     const int m = (int)(bm % mats), b = (int)(bm / mats);
     if (b >= hblocks) return;
-    const bool hidden_rows = m < 2 || (backward && m == 2);
-    const bool down = m == 2;
+    // rows x contraction index of the fragment; the matrix as it lies has
+    // outer x inner
+    const bool hidden_rows = m < 2 || (backward && m == 2), down = m == 2, along = hidden_rows != down;
     const T* w = static_cast<const T*>(down ? a.w_down : (m == 1 || m == 4) ? a.w_up : a.w_gate);
     const int64_t stride = down ? a.down_stride : (m == 1 || m == 4) ? a.up_stride : a.gate_stride;
-    piece_t<T> v = {};
+    const int row = (hidden_rows ? b : kb) * KB<T> + perm<T>(s, r), at = (hidden_rows ? kb : b) * KB<T> + q * E<T>;
+    const int rows = hidden_rows ? a.hidden : a.dim, n = hidden_rows ? a.dim : a.hidden;
+    const int safe = min(row, rows - 1);
+    piece_t<T> v;
+    if (along && n >= E<T>) {
+        v = settle_piece<T>(read_piece(w + safe * stride, at, n), at, n, row < rows);
+    } else {   // all reads go out before the first is looked at
 #pragma unroll
-    for (int j = 0; j < E<T>; ++j) {
-        const int h = b * KB<T> + (hidden_rows ? perm<T>(s, r) : q * E<T> + j);
-        const int d = kb * KB<T> + (hidden_rows ? q * E<T> + j : perm<T>(s, r));
-        if (h < a.hidden && d < a.dim) v[j] = down ? w[d * stride + h] : w[h * stride + d];
+        for (int j = 0; j < E<T>; ++j) {
+            const int k = min(at + j, n - 1);
+            v[j] = along ? w[safe * stride + k] : w[k * stride + safe];
+        }
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j)
+            if (row >= rows || at + j >= n) v[j] = (T)0.f;
     }
     out[f * 64 + slot<T>(0, 0, q, r)] = v;
 }
@@ -378,7 +388,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const pie
     fetch<T>(packed, w, hblocks * 3 * F);
     __syncthreads();
     const int64_t waves = blockDim.x >> 6, step = gridDim.x * waves;
-    int64_t row0 = (blockIdx.x * waves + wave) * (16 * R) + (lane & 15);
+    int64_t row0 = ((int64_t)wave * gridDim.x + blockIdx.x) * (16 * R) + (lane & 15);   // CUs differ by a tile at most
     piece_t<T> xf[R][DK], xn[R][DK], h[R];
     read_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xn);
     for (; row0 - (lane & 15) < a.rows; row0 += step * (16 * R)) {
@@ -406,7 +416,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_all(FfnArgs a, const piec
     fetch<T>(packed, w, hblocks * 3 * F);
     __syncthreads();
     const int64_t waves = blockDim.x >> 6;
-    for (int64_t t = blockIdx.x * waves + wave; t * (16 * R) < a.rows; t += gridDim.x * waves) {
+    for (int64_t t = (int64_t)wave * gridDim.x + blockIdx.x; t * (16 * R) < a.rows; t += gridDim.x * waves) {
         const int64_t row0 = t * (16 * R) + (lane & 15);
         piece_t<T> xf[R][DK], df[R][DK], dg[R], du[R];
         load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
@@ -788,9 +798,9 @@ inline Split dw_split(int64_t rows, int dim, int hidden) {
     p.slices = (tiles + DW_WAVES * p.nh - 1) / (DW_WAVES * p.nh);
     p.tiles = p.slices * DW_WAVES * p.nh;
     const int64_t blocks = (rows + KB<T> - 1) / KB<T>;
-    int64_t groups = 1024 / DW_WAVES * dw_occupancy<T>(dk, p.nh) / p.slices;
-    groups = groups < 1 ? 1 : groups;
-    groups = groups > (blocks + 3) / 4 ? (blocks + 3) / 4 : groups;
+    // four blocks of rows at least, or one where that leaves CUs without work
+    const int64_t most = std::max(1, 1024 / DW_WAVES * dw_occupancy<T>(dk, p.nh) / p.slices);
+    const int64_t groups = std::min(most, std::max((blocks + 3) / 4, std::min<int64_t>(blocks, 256 / p.slices)));
     p.blocks_per_group = groups ? (blocks + groups - 1) / groups : 0;
     p.groups = p.blocks_per_group ? (int)((blocks + p.blocks_per_group - 1) / p.blocks_per_group) : 0;
     return p;
@@ -868,8 +878,16 @@ inline void with_act(const FfnArgs& a, F&& f) {
 // Row tiles of a wave in the streaming kernels, and with eight waves a
 // workgroup the workgroups of a CU, by registers and LDS.
 // (96-384 forward 337 us with two tiles, 300 with one; 256-1024 433 with one,
-// 337 with two.  The input gradient holds twice the fragments and has one.)
-constexpr int fwd_tiles(int fragments) { return fragments <= 6 ? 1 : 2; }
+// 337 with two.  The input gradient holds twice the fragments: 128-512 1510 us
+// with one, 1408 with two; 96-384 1090 and 1112; 256-1024 1490 and 2083.)
+template <class T>
+constexpr int fwd_tiles(int fragments) {
+    return sizeof(T) == 4 || fragments <= 6 ? 1 : 2;
+}
+template <class T>
+constexpr int dx_tiles(int fragments) {
+    return sizeof(T) == 2 && fragments == 8 ? 2 : 1;
+}
 constexpr int per_cu(int fragments) { return fragments <= 8 ? 2 : 1; }
 
 // How the few-row kernels are launched: tiles of a workgroup, workgroups, and
@@ -909,7 +927,7 @@ template <class T>
 void forward(hipStream_t s, const FfnArgs& a) {
     with_blocks<T>(a.dim, [&](auto dk, auto tiny) {
         with_act(a, [&](auto gelu) {
-            constexpr int F = dk() * HT<T>, R = fwd_tiles(F), W = 8;
+            constexpr int F = dk() * HT<T>, R = fwd_tiles<T>(F), W = 8;
             const int hblocks = (a.hidden + KB<T> - 1) / KB<T>;
             f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 3));
             if (a.rows <= few_rows(F)) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks, part);
@@ -917,8 +935,9 @@ void forward(hipStream_t s, const FfnArgs& a) {
             const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
             if constexpr (F <= 4) {
                 if (lds <= LDS_BYTES) {
-                    const Shape g = shape_of(a.rows, 32, 16, CUS);
-                    k_ffn_fwd_all<T, dk(), 2, 16, gelu(), tiny()><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
+                    constexpr int RA = sizeof(T) == 4 ? 1 : 2;
+                    const Shape g = shape_of(a.rows, 16 * RA, 16, CUS);
+                    k_ffn_fwd_all<T, dk(), RA, 16, gelu(), tiny()><<<g.groups, g.threads, lds, s>>>(a, packed, hblocks);
                     return;
                 }
             }
@@ -926,8 +945,14 @@ void forward(hipStream_t s, const FfnArgs& a) {
             const int64_t tail = tail_rows(a.rows, 16 * R * W * per_cu(F) * CUS);
             if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks, part);
             main.rows -= tail;
-            const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
-            k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
+            // two tiles a wave only where that still gives every SIMD a wave
+            if (R == 2 && main.rows >= 32 * 4 * CUS) {
+                const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
+                k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
+            } else {
+                const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
+                k_ffn_fwd<T, dk(), 1, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
+            }
         });
     });
 }
@@ -952,7 +977,7 @@ template <class T>
 DxPlan<T> dx_plan(const FfnArgs& a, int fragments) {
     if (a.rows <= few_rows(fragments)) return {a.rows, 5, false};
     if (fragments <= 4 && packed_bytes<T>(a.dim, a.hidden, 3) <= LDS_BYTES) return {0, 3, true};
-    const int64_t tail = tail_rows(a.rows, 16 * 8 * per_cu(fragments) * CUS);
+    const int64_t tail = tail_rows(a.rows, 16 * dx_tiles<T>(fragments) * 8 * per_cu(fragments) * CUS);
     return {tail, tail ? 5 : 3, false};
 }
 
@@ -972,8 +997,14 @@ void input_gradient(hipStream_t s, const FfnArgs& a, const DxPlan<T>& plan, cons
     }
     FfnArgs main = a;
     main.rows -= plan.tail;
-    const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
-    k_ffn_dx<T, DK, 1, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
+    constexpr int R = dx_tiles<T>(F);
+    if (R == 2 && main.rows >= 32 * 4 * CUS) {
+        const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
+        k_ffn_dx<T, DK, R, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
+    } else {
+        const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
+        k_ffn_dx<T, DK, 1, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
+    }
 }
 
 template <class T>
