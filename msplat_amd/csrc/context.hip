@@ -554,6 +554,12 @@ int forward(Ctx* c, const MsplatRenderArgs* a, bool training, float* dst_img = n
     return MSPLAT_OK;
 }
 
+#define CHECK(expr)                     \
+    do {                                \
+        int r_ = (expr);                \
+        if (r_ != MSPLAT_OK) return r_; \
+    } while (0)
+
 // Checks shared by the learned-head operators.
 int check_rows(int64_t rows, int dim, int max_dim, int dtype) {
     if (rows < 0 || rows > 0x7FFFFFFF) return fail(MSPLAT_ERR_ARG, "rows %lld outside [0, 2^31)", (long long)rows);
@@ -573,6 +579,13 @@ int check_matrix(const char* name, const void* p, int64_t rows, int dim, int64_t
     return MSPLAT_OK;
 }
 
+// A vector [dim] of the call's type, null for none.
+int check_vector(const char* name, const void* p, int dtype) {
+    if (reinterpret_cast<uintptr_t>(p) % (dtype == MSPLAT_F32 ? 4 : 2) != 0)
+        return fail(MSPLAT_ERR_ARG, "%s is not aligned to its type", name);
+    return MSPLAT_OK;
+}
+
 int check_workspace(const void* ws, int64_t bytes, size_t need) {
     if (need == 0) return MSPLAT_OK;
     if (!ws || bytes < 0 || (size_t)bytes < need)
@@ -581,11 +594,6 @@ int check_workspace(const void* ws, int64_t bytes, size_t need) {
     return MSPLAT_OK;
 }
 
-#define CHECK(expr)                     \
-    do {                                \
-        int r_ = (expr);                \
-        if (r_ != MSPLAT_OK) return r_; \
-    } while (0)
 
 int check_ffn_sizes(int64_t rows, int dim, int hidden, int dtype) {
     CHECK(check_rows(rows, dim, FFN_DIM_MAX, dtype));
@@ -1325,6 +1333,10 @@ int msplat_hip_layer_norm(const MsplatLayerNormArgs* a) {
     CHECK(check_rows(a->rows, a->dim, NORM_DIM_MAX, a->dtype));
     CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
     CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    CHECK(check_vector("weight", a->weight, a->dtype));
+    CHECK(check_vector("bias", a->bias, a->dtype));
+    CHECK(check_vector("mean", a->mean, MSPLAT_F32));
+    CHECK(check_vector("rstd", a->rstd, MSPLAT_F32));
     if (!(a->eps >= 0.f)) return fail(MSPLAT_ERR_ARG, "eps must be at least 0");
     if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
     if (a->rows == 0) return MSPLAT_OK;
@@ -1357,6 +1369,11 @@ int msplat_hip_layer_norm_backward(const MsplatLayerNormGradArgs* a) {
     CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
     if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->dim, a->dx_stride, a->dtype));
     if (a->rows > 0 && (!a->mean || !a->rstd)) return fail(MSPLAT_ERR_ARG, "mean or rstd is null");
+    CHECK(check_vector("weight", a->weight, a->dtype));
+    CHECK(check_vector("mean", a->mean, MSPLAT_F32));
+    CHECK(check_vector("rstd", a->rstd, MSPLAT_F32));
+    CHECK(check_vector("dweight", a->dweight, a->dtype));
+    CHECK(check_vector("dbias", a->dbias, a->dtype));
     const bool sums = a->dweight || a->dbias;
     if (sums)
         CHECK(check_workspace(a->workspace, a->workspace_bytes,
@@ -1412,6 +1429,9 @@ int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* a) {
     CHECK(check_ffn(a, f));
     CHECK(check_matrix("dy", a->dy, a->rows, a->dim, a->dy_stride, a->dtype));
     if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->dim, a->dx_stride, a->dtype));
+    CHECK(check_vector("dw_gate", a->dw_gate, a->dtype));
+    CHECK(check_vector("dw_up", a->dw_up, a->dtype));
+    CHECK(check_vector("dw_down", a->dw_down, a->dtype));
     const int given = (a->dw_gate != nullptr) + (a->dw_up != nullptr) + (a->dw_down != nullptr);
     if (given != 0 && given != 3)
         return fail(MSPLAT_ERR_ARG, "dw_gate, dw_up and dw_down are wanted together or not at all");

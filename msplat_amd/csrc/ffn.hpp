@@ -24,10 +24,18 @@
 // registers, and so do dg, du and h to the gradients.
 //
 // Weights are packed into fragments (1 KB each, zero beyond the matrices) by a
-// small kernel first: each is used in up to three orders, and the pack takes
-// up every width and stride.  In 16-bit types h, dg and du are rounded to the
-// type for the next product, as the type's own matrix instructions take them;
-// the error is of the size of the output's own rounding.
+// small kernel first (5 us): each is used in up to three orders, and the pack
+// takes up every width and stride.  In 16-bit types h, dg and du are rounded to
+// the type for the next product, as the type's own matrix instructions take
+// them; the error is of the size of the output's own rounding.
+//
+// What bounds it: on a SIMD vector and matrix instructions hardly overlap (a
+// probe with four waves: 24 matrix instructions 404 cycles, the activations of
+// as many rows 550, both 782), so a block costs about the sum of the two.  At
+// 64 features the activations are the larger half, at 256 an eighth.
+//   64-256-64 bf16 forward over 1.09M rows: 140 us, 765 TFLOP/s
+//   256-1024-256 bf16 forward over 229k rows: 335 us, 1075 TFLOP/s (a library
+//   product of 8192^3 reaches 1111)
 #pragma once
 
 #include "nn.hpp"
@@ -170,14 +178,19 @@ __global__ __launch_bounds__(256) void k_ffn_pack(FfnArgs a, bool backward, int 
 }
 
 // Copies n fragments (1 KB each) from memory to LDS without registers in
-// between; a wave takes every waves-th.  They have arrived after the next
-// __syncthreads.
+// between; a wave takes every waves-th.  They are there after fetched().
 template <class T>
 __device__ __forceinline__ void fetch(const piece_t<T>* src, piece_t<T>* lds, int n) {
     const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     for (int f = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); f < n; f += waves)
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + f * 64 + lane),
                                          (__attribute__((address_space(3))) void*)(lds + f * 64), 16, 0, 0);
+}
+
+// Waits for the wave's own fetches, then for the workgroup.
+__device__ __forceinline__ void fetched() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
 }
 
 // The pieces of R rows' operand fragments, in two steps (read_piece,
@@ -247,7 +260,6 @@ constexpr int MFMAS = sizeof(T) == 4 ? 4 : 1;   // matrix instructions of an mma
 template <class T, int DK, int R, bool GELU>
 __device__ __forceinline__ void fwd_up(const piece_t<T>* up, const piece_t<T> (&xf)[R][DK], piece_t<T> (&h)[R]) {
     constexpr int F = DK * HT<T>;
-    const int lane = threadIdx.x & 63;
     f32x4 g[R][HT<T>] = {}, u[R][HT<T>] = {};
 #pragma unroll
     for (int f = 0; f < F; ++f) {
@@ -268,7 +280,6 @@ __device__ __forceinline__ void fwd_up(const piece_t<T>* up, const piece_t<T> (&
 }
 template <class T, int F, int R>
 __device__ __forceinline__ void fwd_down(const piece_t<T>* down, const piece_t<T> (&h)[R], f32x4 (&acc)[R][F]) {
-    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int f = 0; f < F; ++f) {
         const piece_t<T> wd = by_row<T>(down, f);
@@ -283,7 +294,6 @@ template <class T, int DK, int R, bool GELU>
 __device__ __forceinline__ void dx_up(const piece_t<T>* up, const piece_t<T> (&xf)[R][DK], const piece_t<T> (&df)[R][DK],
                                       piece_t<T> (&dg)[R], piece_t<T> (&du)[R]) {
     constexpr int F = DK * HT<T>;
-    const int lane = threadIdx.x & 63;
     f32x4 g[R][HT<T>] = {}, u[R][HT<T>] = {}, dh[R][HT<T>] = {};
 #pragma unroll
     for (int f = 0; f < F; ++f) {
@@ -338,7 +348,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd(FfnArgs a, const piece_t
     load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     f32x4 acc[R][F] = {};
     auto block = [&](int b, const piece_t<T>* w, piece_t<T>* next) {
-        __syncthreads();
+        fetched();
         if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * mats * F * 64, next, 3 * F);
         piece_t<T> h[R];
         fwd_up<T, DK, R, GELU>(w, xf, h);
@@ -363,7 +373,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<
     load_rows<T, DK, R, TINY>(a.dy, a.dy_stride, row0, a.rows, a.dim, q, df);
     f32x4 acc[R][F] = {};
     auto block = [&](int b, const piece_t<T>* w, piece_t<T>* next) {
-        __syncthreads();
+        fetched();
         if (b + 1 < hblocks) fetch<T>(packed + (int64_t)(b + 1) * mats * F * 64, next, 3 * F);
         piece_t<T> dg[R], du[R];
         dx_up<T, DK, R, GELU>(w, xf, df, dg, du);
@@ -378,7 +388,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<
 
 // The same where all packed weights fit in LDS: a workgroup loads them once,
 // then its waves walk row tiles on their own, with no barrier that would hold
-// all of them at the matrix or at the vector instructions at once.
+// all of them at the matrix or at the vector instructions at once.  (64-256-64
+// bf16 forward over 1.09M rows: streamed 165 us, resident 151.)
 template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const piece_t<T>* packed, int hblocks) {
     constexpr int F = DK * HT<T>;
@@ -386,7 +397,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const pie
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(smem);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
     fetch<T>(packed, w, hblocks * 3 * F);
-    __syncthreads();
+    fetched();
     const int64_t waves = blockDim.x >> 6, step = gridDim.x * waves;
     int64_t row0 = ((int64_t)wave * gridDim.x + blockIdx.x) * (16 * R) + (lane & 15);   // CUs differ by a tile at most
     piece_t<T> xf[R][DK], xn[R][DK], h[R];
@@ -414,7 +425,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_all(FfnArgs a, const piec
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(smem);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4;
     fetch<T>(packed, w, hblocks * 3 * F);
-    __syncthreads();
+    fetched();
     const int64_t waves = blockDim.x >> 6;
     for (int64_t t = (int64_t)wave * gridDim.x + blockIdx.x; t * (16 * R) < a.rows; t += gridDim.x * waves) {
         const int64_t row0 = t * (16 * R) + (lane & 15);
@@ -433,7 +444,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_all(FfnArgs a, const piec
 // Few rows: a workgroup takes R tiles of 16 rows, and its waves share out the
 // hidden units; the waves' parts of y are added in LDS, half of the waves onto
 // the other half until one is left, in the same order every time.  Weights
-// come from the L2 cache into registers, each read once a workgroup.
+// come from the L2 cache into registers, each read once a workgroup.  (128-512
+// bf16 forward, 256 rows: streamed 34 us a call, this way 15; 8192 rows 35 and
+// 20; 16384 rows 35 and 37.)
 template <class T, int F, int R, int WAVES>
 __device__ __forceinline__ void add_waves(f32x4 (&acc)[R][F], f32x4* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -568,7 +581,9 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piec
 // weights and their rows of the three gradients in registers and walks a
 // group's rows. The workgroup's waves share each block of rows in LDS, two
 // blocks in turn: the next is on its way while one is computed.  Sums go to
-// part[group][tile][matrix][dim tile][lane].
+// part[group][tile][matrix][dim tile][lane].  Bound as the forward; wide blocks
+// run one wave a SIMD, whose waits nothing covers.  (64-256 bf16 over 500k rows:
+// 126 us, 256-1024 over 229k rows: 850, 850 TFLOP/s.)
 constexpr int DW_WAVES = 4;
 // Tiles of hidden units a wave of the weight gradient takes, and waves a SIMD,
 // by registers: 24 a tile and block of columns for weights and sums.  (Two
@@ -896,16 +911,14 @@ constexpr int per_cu(int fragments) { return fragments <= 8 ? 2 : 1; }
 struct Few {
     int tiles, splits;
     unsigned groups;
-    size_t part_bytes;
 };
 template <class T>
-inline Few few_plan(int64_t rows, int dim, int hidden) {
+inline Few few_plan(int64_t rows, int hidden) {
     Few p;
     p.tiles = rows <= 16 * CUS ? 1 : 2;
     const int64_t row_groups = ceil_div(rows, 16 * p.tiles), blocks = ceil_div(hidden, KB<T>);
     p.splits = blocks > 16 ? (int)std::max<int64_t>(1, std::min(CUS / row_groups, ceil_div(blocks, 8))) : 1;
     p.groups = (unsigned)(row_groups * p.splits);
-    p.part_bytes = p.splits > 1 ? (size_t)p.groups * p.tiles * dim_blocks<T>(dim) * HT<T> * 1024 : 0;
     return p;
 }
 template <class T>
@@ -917,7 +930,7 @@ void few_join(hipStream_t s, const FfnArgs& a, const Few& p, const f32x4* part) 
 
 template <class T, int DK, bool GELU, bool TINY>
 void few_forward(hipStream_t s, const FfnArgs& a, int hblocks, f32x4* part) {
-    const Few p = few_plan<T>(a.rows, a.dim, a.hidden);
+    const Few p = few_plan<T>(a.rows, a.hidden);
     if (p.tiles == 1) k_ffn_fwd_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
     else k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
     few_join<T>(s, a, p, part);
@@ -959,7 +972,7 @@ void forward(hipStream_t s, const FfnArgs& a) {
 
 template <class T, int DK, bool GELU, bool TINY>
 void few_dx(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks, f32x4* part) {
-    const Few p = few_plan<T>(a.rows, a.dim, a.hidden);
+    const Few p = few_plan<T>(a.rows, a.hidden);
     if (p.tiles == 1) k_ffn_dx_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
     else k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
     few_join<T>(s, a, p, part);

@@ -18,6 +18,7 @@ import ctypes
 from typing import Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _abi, device
 
@@ -42,6 +43,13 @@ def _stream(t) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index) or _DEFAULT_STREAM
 
 
+def _plain(t) -> bool:
+    """Whether a matrix has adjacent columns and rows that do not overlap (an
+    expanded gradient's do)."""
+    rows, cols = t.shape
+    return (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or rows <= 1)
+
+
 def _rows(name, t, dim, like):
     """t as a [rows, dim] matrix with adjacent columns."""
     if t.dtype is not like.dtype or t.device != like.device:
@@ -50,7 +58,7 @@ def _rows(name, t, dim, like):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not [..., {dim}]")
     if t.dim() != 2:
         t = t.reshape(-1, dim)
-    return t if t.stride(1) == 1 or dim == 1 else t.contiguous()
+    return t if _plain(t) else t.contiguous()
 
 
 def _matrix(name, t, shape, like):
@@ -58,7 +66,7 @@ def _matrix(name, t, shape, like):
         raise ValueError(f"{name} is {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
     if tuple(t.shape) != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, not {shape}")
-    return t if t.stride(-1) == 1 or shape[-1] == 1 else t.contiguous()
+    return t if (t.stride(0) == 1 if len(shape) == 1 else _plain(t)) else t.contiguous()
 
 
 def _dtype(t) -> int:
@@ -210,6 +218,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
         dx, dweight, dbias = layer_norm_backward(dy, x, weight, mean, rstd)
@@ -225,6 +234,7 @@ class _GatedFfn(torch.autograd.Function):
         return gated_ffn_forward(x, w_gate, w_up, w_down, activation)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         return (*gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation), None)
 
@@ -236,6 +246,7 @@ class _DropoutAdd(torch.autograd.Function):
         return dropout_add_forward(x, residual, p, seed, offset)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         need = ctx.needs_input_grad
         return (dropout_add_backward(dy, *ctx.args) if need[0] else None, dy if need[1] else None, None, None, None)

@@ -293,6 +293,45 @@ def test_a_block_and_its_gradients(nn):
     assert abs(float((up - down) / (2 * h) - along)) < float(size) * 1e-6
 
 
+def test_expanded_gradients(nn):
+    """The gradients of sums reach the operators as expanded tensors, whose
+    rows or elements are one in memory."""
+    x, wg, wu, wd = (t.requires_grad_() for t in _ffn_operands(50, 40, 60, torch.float32))
+    r = _normal(61, 50, 40).requires_grad_()
+    w = (1 + _normal(62, 40, scale=0.1)).requires_grad_()
+    v = _normal(63, 40)
+    for loss in (lambda y: y.sum(), lambda y: (y.sum(0) * v).sum()):
+        y = nn.dropout_add(nn.gated_ffn(nn.layer_norm(x, w), wg, wu, wd), r, 0.25, 5, 6)
+        leaves = (x, wg, wu, wd, w, r)
+        got = torch.autograd.grad(loss(y), leaves)
+        y = nn.dropout_add(nn.gated_ffn(nn.layer_norm(x, w), wg, wu, wd), r, 0.25, 5, 6)
+        ones = torch.ones_like(y)
+        dy = ones if torch.equal(torch.autograd.grad(loss(r * 1), r)[0], ones) else v.expand(50, 40).contiguous()
+        want = torch.autograd.grad(y, leaves, dy)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_offsets_beyond_32_bits(nn, dtype):
+    """60000 rows 40000 elements apart: the last ones start past 2^31 elements."""
+    rows, dim, stride = 60000, 40, 40000
+    buf = torch.empty((rows - 1) * stride + dim, dtype=dtype, device="cuda")
+
+    def far(t):
+        view = buf.as_strided((rows, dim), (stride, 1))
+        view.copy_(t)
+        return view
+
+    x, wg, wu, wd = _ffn_operands(rows, dim, 48, dtype)
+    w = torch.ones(dim, dtype=dtype, device="cuda")
+    y, mean, rstd = nn.layer_norm_forward(x, w, w)
+    for call in (lambda t: nn.layer_norm_forward(t, w, w), lambda t: nn.layer_norm_backward(x, t, w, mean, rstd),
+                 lambda t: nn.layer_norm_backward(t, x, w, mean, rstd),
+                 lambda t: (nn.gated_ffn_forward(t, wg, wu, wd),), lambda t: nn.gated_ffn_backward(x, t, wg, wu, wd),
+                 lambda t: nn.gated_ffn_backward(t, x, wg, wu, wd), lambda t: (nn.dropout_add_forward(x, t, 0.5, 1, 2),)):
+        assert all(torch.equal(p, q) for p, q in zip(call(far(x)), call(x)))
+
+
 def test_other_streams(nn):
     x, wg, wu, wd = _ffn_operands(3000, 64, 128, torch.bfloat16)
     w = torch.ones(64, dtype=torch.bfloat16, device="cuda")

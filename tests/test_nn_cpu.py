@@ -165,6 +165,17 @@ def test_misaligned_matrix_is_refused(lib, name):
     assert b"aligned" in lib.msplat_hip_last_error()
 
 
+def test_misaligned_vectors_are_refused(lib):
+    for name, fields in (("msplat_hip_layer_norm", ("weight", "bias", "mean", "rstd")),
+                         ("msplat_hip_layer_norm_backward", ("weight", "mean", "rstd", "dweight", "dbias")),
+                         ("msplat_hip_gated_ffn_backward", ("dw_gate", "dw_up", "dw_down"))):
+        for field in fields:
+            h, a = CALLS[name]()
+            setattr(a, field, h.at + 2)
+            assert getattr(lib, name)(ctypes.byref(a)) == -1, (name, field)
+            assert field.encode() in lib.msplat_hip_last_error()
+
+
 def test_misaligned_workspace_is_refused(lib):
     for name in ("msplat_hip_gated_ffn", "msplat_hip_gated_ffn_backward"):
         h, a = CALLS[name]()
