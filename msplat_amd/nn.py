@@ -52,6 +52,9 @@ def _plain(t) -> bool:
 
 def _rows(name, t, dim, like):
     """t as a [rows, dim] matrix with adjacent columns."""
+    if t.dim() == 2 and t.is_contiguous() and t.shape[1] == dim and t.dtype is like.dtype and \
+            t.get_device() == like.get_device():
+        return t
     if t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{name} is {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
     if t.dim() < 1 or t.shape[-1] != dim:
@@ -62,6 +65,8 @@ def _rows(name, t, dim, like):
 
 
 def _matrix(name, t, shape, like):
+    if t.shape == shape and t.is_contiguous() and t.dtype is like.dtype and t.get_device() == like.get_device():
+        return t
     if t.dtype is not like.dtype or t.device != like.device:
         raise ValueError(f"{name} is {t.dtype} on {t.device}, not {like.dtype} on {like.device}")
     if tuple(t.shape) != shape:
@@ -79,7 +84,7 @@ def _dtype(t) -> int:
 def _feature_rows(name, x):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} has shape {tuple(x.shape)}, not [..., dim]")
-    return _rows(name, x, x.shape[-1], x)
+    return x if x.dim() == 2 and x.is_contiguous() else _rows(name, x, x.shape[-1], x)
 
 
 def _same_rows(name, t, x2):
