@@ -507,27 +507,43 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hbloc
     const int split = blockIdx.x % splits;
     const int64_t row0 = (int64_t)(blockIdx.x / splits) * (16 * R) + i;
     piece_t<T> xf[R][DK], h[R];
-    load_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
+    read_rows<T, DK, R, TINY>(a.x, a.x_stride, row0, a.rows, a.dim, q, xf);
     f32x4 acc[R][F] = {};
+    bool first = true;
     for (int b = split * WAVES + wave; b < hblocks; b += splits * WAVES) {
+        // every read of the block goes out before the first piece is looked at
+        // (wide blocks: every read of a step)
         piece_t<T> wg[F], wu[F], wd[F];
 #pragma unroll
-        for (int s = 0; s < HT<T>; ++s) {
-            const int u = b * KB<T> + perm<T>(s, i), at = min(u, a.hidden - 1);
-            const T* pg = static_cast<const T*>(a.w_gate) + at * a.gate_stride;
-            const T* pu = static_cast<const T*>(a.w_up) + at * a.up_stride;
-#pragma unroll
-            for (int kb = 0; kb < DK; ++kb) {
-                wg[kb * HT<T> + s] = load_piece(pg, kb * KB<T> + q * E<T>, a.dim);
-                wu[kb * HT<T> + s] = load_piece(pu, kb * KB<T> + q * E<T>, a.dim);
-                if (u >= a.hidden) wg[kb * HT<T> + s] = wu[kb * HT<T> + s] = piece_t<T>{};
-            }
+        for (int f = 0; f < F; ++f) {
+            const int64_t u = min(b * KB<T> + perm<T>(f % HT<T>, i), a.hidden - 1);
+            const T* pg = static_cast<const T*>(a.w_gate) + u * a.gate_stride;
+            const T* pu = static_cast<const T*>(a.w_up) + u * a.up_stride;
+            const int k = f / HT<T> * KB<T> + q * E<T>;
+            wg[f] = TINY ? load_piece(pg, k, a.dim) : read_piece(pg, k, a.dim);
+            wu[f] = TINY ? load_piece(pu, k, a.dim) : read_piece(pu, k, a.dim);
         }
+        auto read_down = [&]() {
+#pragma unroll
+            for (int f = 0; f < F; ++f) {
+                const int64_t d = min(f / HT<T> * KB<T> + perm<T>(f % HT<T>, i), a.dim - 1);
+                wd[f] = read_piece(static_cast<const T*>(a.w_down) + d * a.down_stride, b * KB<T> + q * E<T>, a.hidden);
+            }
+        };
+        if (F <= 8) read_down();
+        __builtin_amdgcn_sched_barrier(0);
+        if (first) settle_rows<T, DK, R, TINY>(row0, a.rows, a.dim, q, xf);
+        first = false;
 #pragma unroll
         for (int f = 0; f < F; ++f) {
-            const int d = f / HT<T> * KB<T> + perm<T>(f % HT<T>, i);
-            wd[f] = load_piece(static_cast<const T*>(a.w_down) + min(d, a.dim - 1) * a.down_stride, b * KB<T> + q * E<T>, a.hidden);
-            if (d >= a.dim) wd[f] = piece_t<T>{};
+            const bool live = b * KB<T> + perm<T>(f % HT<T>, i) < a.hidden;
+            const int k = f / HT<T> * KB<T> + q * E<T>;
+            if (TINY) {
+                if (!live) wg[f] = wu[f] = piece_t<T>{};
+            } else {
+                wg[f] = settle_piece<T>(wg[f], k, a.dim, live);
+                wu[f] = settle_piece<T>(wu[f], k, a.dim, live);
+            }
         }
         f32x4 g[R][HT<T>] = {}, u[R][HT<T>] = {};
 #pragma unroll
@@ -537,6 +553,10 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hbloc
                 g[r][f % HT<T>] = mma(wg[f], xf[r][f / HT<T>], g[r][f % HT<T>]);
                 u[r][f % HT<T>] = mma(wu[f], xf[r][f / HT<T>], u[r][f % HT<T>]);
             }
+        if (F > 8) {
+            __builtin_amdgcn_sched_barrier(0);
+            read_down();
+        }
 #pragma unroll
         for (int r = 0; r < R; ++r) {
 #pragma unroll
@@ -544,9 +564,12 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_few(FfnArgs a, int hbloc
             h[r] = join<T>(g[r]);
         }
 #pragma unroll
-        for (int f = 0; f < F; ++f)
+        for (int f = 0; f < F; ++f) {
+            const int d = f / HT<T> * KB<T> + perm<T>(f % HT<T>, i);
+            wd[f] = settle_piece<T>(wd[f], b * KB<T> + q * E<T>, a.hidden, d < a.dim);
 #pragma unroll
             for (int r = 0; r < R; ++r) acc[r][f] = mma(wd[f], h[r], acc[r][f]);
+        }
     }
     add_waves<T, F, R, WAVES>(acc, sums);
     if (wave != 0) return;
@@ -840,8 +863,9 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Rows up to which a workgroup takes one or two row tiles for all hidden units
 // (k_ffn_*_few): as long as every one of them finds a CU free, twice that
-// where two fit on one.
-inline int64_t few_rows(int fragments) { return 32 * CUS * (fragments <= 4 ? 2 : 1); }
+// where two fit on one; two tiles of wide blocks do not fit in registers.
+// (256-1024 bf16 forward over 8192 rows: 117 us this way, 58 streamed.)
+inline int64_t few_rows(int fragments) { return fragments <= 4 ? 64 * CUS : fragments <= 8 ? 32 * CUS : 16 * CUS; }
 
 // Launch shape of the kernels whose waves take `tile` rows each: `most` waves
 // a workgroup, fewer where that would leave CUs without one.
@@ -906,8 +930,11 @@ constexpr int dx_tiles(int fragments) {
 constexpr int per_cu(int fragments) { return fragments <= 8 ? 2 : 1; }
 
 // How the few-row kernels are launched: tiles of a workgroup, workgroups, and
-// the workgroups that share a tile.  A join costs a launch, so it takes three
-// blocks of hidden units a wave to share them out further.
+// the workgroups that share a tile, where a wave would have more than three
+// blocks of hidden units: so many that none has a second while CUs are free.
+// (256-1024 bf16 forward over 64 rows: 32 blocks, 33 us on two workgroups a
+// tile, 20 + 4.7 for the join on four.  128-512 over 256 rows, 16 blocks: 15.0
+// on one, 10.0 + 3.9 on two.)
 struct Few {
     int tiles, splits;
     unsigned groups;
@@ -917,7 +944,7 @@ inline Few few_plan(int64_t rows, int hidden) {
     Few p;
     p.tiles = rows <= 16 * CUS ? 1 : 2;
     const int64_t row_groups = ceil_div(rows, 16 * p.tiles), blocks = ceil_div(hidden, KB<T>);
-    p.splits = blocks > 16 ? (int)std::max<int64_t>(1, std::min(CUS / row_groups, ceil_div(blocks, 8))) : 1;
+    p.splits = blocks > 24 ? (int)std::max<int64_t>(1, std::min(CUS / row_groups, ceil_div(blocks, 8))) : 1;
     p.groups = (unsigned)(row_groups * p.splits);
     return p;
 }
@@ -932,7 +959,8 @@ template <class T, int DK, bool GELU, bool TINY>
 void few_forward(hipStream_t s, const FfnArgs& a, int hblocks, f32x4* part) {
     const Few p = few_plan<T>(a.rows, a.hidden);
     if (p.tiles == 1) k_ffn_fwd_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
-    else k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
+    else if constexpr (DK * HT<T> <= 8)
+        k_ffn_fwd_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, hblocks, p.splits, part);
     few_join<T>(s, a, p, part);
 }
 
@@ -943,7 +971,9 @@ void forward(hipStream_t s, const FfnArgs& a) {
             constexpr int F = dk() * HT<T>, R = fwd_tiles<T>(F), W = 8;
             const int hblocks = (a.hidden + KB<T> - 1) / KB<T>;
             f32x4* part = reinterpret_cast<f32x4*>(a.ws + packed_bytes<T>(a.dim, a.hidden, 3));
-            if (a.rows <= few_rows(F)) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks, part);
+            // the few-row kernel reads the weights as they are, in whole pieces
+            const bool pieces = a.hidden >= E<T>;
+            if (a.rows <= few_rows(F) && pieces) return few_forward<T, dk(), gelu(), tiny()>(s, a, hblocks, part);
             const piece_t<T>* packed = pack<T>(s, a, false, dk(), hblocks, 3);
             const size_t lds = packed_bytes<T>(a.dim, a.hidden, 3);
             if constexpr (F <= 4) {
@@ -955,7 +985,7 @@ void forward(hipStream_t s, const FfnArgs& a) {
                 }
             }
             FfnArgs main = a;
-            const int64_t tail = tail_rows(a.rows, 16 * R * W * per_cu(F) * CUS);
+            const int64_t tail = pieces ? tail_rows(a.rows, 16 * R * W * per_cu(F) * CUS) : 0;
             if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks, part);
             main.rows -= tail;
             // two tiles a wave only where that still gives every SIMD a wave
@@ -974,7 +1004,8 @@ template <class T, int DK, bool GELU, bool TINY>
 void few_dx(hipStream_t s, const FfnArgs& a, const piece_t<T>* packed, int hblocks, f32x4* part) {
     const Few p = few_plan<T>(a.rows, a.hidden);
     if (p.tiles == 1) k_ffn_dx_few<T, DK, 1, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
-    else k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
+    else if constexpr (DK * HT<T> <= 8)
+        k_ffn_dx_few<T, DK, 2, 8, GELU, TINY><<<p.groups, 512, 0, s>>>(a, packed, hblocks, p.splits, part);
     few_join<T>(s, a, p, part);
 }
 

@@ -110,7 +110,8 @@ def test_layer_norm_of_a_large_offset(nn):
 
 FFN_SIZES = [(1, 1, 1), (5, 3, 2), (64, 32, 32), (257, 45, 100), (130, 64, 256), (300, 96, 250), (100, 128, 96),
              (77, 130, 40), (90, 200, 333), (65, 256, 64), (33, 250, 1100), (2500, 16, 24), (1300, 48, 192),
-             (1, 64, 5000), (40, 143, 946), (4100, 20, 700)]
+             (1, 64, 5000), (40, 143, 946), (4100, 20, 700),
+             (30, 70, 3), (4200, 250, 70)]
 
 
 def _ffn_operands(rows, dim, hidden, dtype, seed=20):
