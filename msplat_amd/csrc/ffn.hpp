@@ -79,10 +79,13 @@ __device__ __forceinline__ piece_t<T> join(const f32x4* t) {
 
 // A block of KB rows of a matrix [rows, dim] as fragments rows x dim: the piece
 // of row perm(s, r), elements (4 kb + c) E ..., lies at slot(kb, s, c, r).  The
-// order of rows turns with c so that by_dim's reads spread over LDS's banks.
+// order of rows turns with c so that by_dim's reads spread over LDS's banks;
+// in 16-bit types groups of four rows change places so that by_row's 16-byte
+// reads, which the hardware takes as lanes 0-3, 12-15, 20-23, 24-27 and so on,
+// stay free of conflicts too.
 template <class T>
 __device__ __forceinline__ int slot(int kb, int s, int c, int r) {
-    return (kb * HT<T> + s) * 64 + c * 16 + (r ^ (sizeof(T) == 4 ? c : c * 4));
+    return (kb * HT<T> + s) * 64 + c * 16 + (r ^ (sizeof(T) == 4 ? c : (-c & 3) * 4));
 }
 // Fragment f = kb HT + s, rows x dim.
 template <class T>
