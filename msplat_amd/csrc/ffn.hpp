@@ -7,7 +7,8 @@
 // a(v) = v sigmoid(z(v)), with z = v (SiLU) or z = 2 sqrt(2/pi) (v + 0.044715
 // v^3) (GELU in its tanh form).  The rows are many and the width is at most
 // 256, so g, u and h (rows x hidden) never go to memory: 12 bytes a hidden
-// unit and row would cost more than the 6 dim operations that make them again.
+// unit and row would cost more than the 6 dim operations that make them again (at the
+// rates of a large copy and a large library product up to a width of 430).
 //
 // All products run on 16x16 matrix instructions with 32-bit sums.  Indices
 // are taken in blocks of KB = 4 E (one 16-byte piece in each of the four
@@ -33,7 +34,7 @@
 // probe with four waves: 24 matrix instructions 404 cycles, the activations of
 // as many rows 550, both 782), so a block costs about the sum of the two.  At
 // 64 features the activations are the larger half, at 256 an eighth.
-//   64-256-64 bf16 forward over 1.09M rows: 140 us, 765 TFLOP/s
+//   64-256-64 bf16 forward over 1.09M rows: 137 us, 780 TFLOP/s
 //   256-1024-256 bf16 forward over 229k rows: 335 us, 1075 TFLOP/s (a library
 //   product of 8192^3 reaches 1111)
 #pragma once
@@ -392,7 +393,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx(FfnArgs a, const piece_t<
 // The same where all packed weights fit in LDS: a workgroup loads them once,
 // then its waves walk row tiles on their own, with no barrier that would hold
 // all of them at the matrix or at the vector instructions at once.  (64-256-64
-// bf16 forward over 1.09M rows: streamed 165 us, resident 151.)
+// bf16 over 1.09M rows, a call: streamed 165 us, resident 152; backward
+// over 500k rows 246 and 241.)
 template <class T, int DK, int R, int WAVES, bool GELU, bool TINY>
 __global__ __launch_bounds__(64 * WAVES) void k_ffn_fwd_all(FfnArgs a, const piece_t<T>* packed, int hblocks) {
     constexpr int F = DK * HT<T>;
@@ -448,8 +450,8 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_all(FfnArgs a, const piec
 // hidden units; the waves' parts of y are added in LDS, half of the waves onto
 // the other half until one is left, in the same order every time.  Weights
 // come from the L2 cache into registers, each read once a workgroup.  (128-512
-// bf16 forward, 256 rows: streamed 34 us a call, this way 15; 8192 rows 35 and
-// 20; 16384 rows 35 and 37.)
+// bf16 forward, 256 rows: streamed 25 us a call, this way 15; 8192 rows 21.5 and
+// 19; 256-1024 over 64 rows 80 and 23.)
 template <class T, int F, int R, int WAVES>
 __device__ __forceinline__ void add_waves(f32x4 (&acc)[R][F], f32x4* lds) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -609,7 +611,7 @@ __global__ __launch_bounds__(64 * WAVES) void k_ffn_dx_few(FfnArgs a, const piec
 // blocks in turn: the next is on its way while one is computed.  Sums go to
 // part[group][tile][matrix][dim tile][lane].  Bound as the forward; wide blocks
 // run one wave a SIMD, whose waits nothing covers.  (64-256 bf16 over 500k rows:
-// 126 us, 256-1024 over 229k rows: 850, 850 TFLOP/s.)
+// 130 us, 256-1024 over 229k rows: 844, 855 TFLOP/s.)
 constexpr int DW_WAVES = 4;
 // Tiles of hidden units a wave of the weight gradient takes, and waves a SIMD,
 // by registers: 24 a tile and block of columns for weights and sums.  (Two
@@ -867,7 +869,7 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // Rows up to which a workgroup takes one or two row tiles for all hidden units
 // (k_ffn_*_few): as long as every one of them finds a CU free, twice that
 // where two fit on one; two tiles of wide blocks do not fit in registers.
-// (256-1024 bf16 forward over 8192 rows: 117 us this way, 58 streamed.)
+// (256-1024 bf16 forward over 8192 rows: 117 us this way, 60 streamed.)
 inline int64_t few_rows(int fragments) { return fragments <= 4 ? 64 * CUS : fragments <= 8 ? 32 * CUS : 16 * CUS; }
 
 // Launch shape of the kernels whose waves take `tile` rows each: `most` waves
@@ -919,12 +921,14 @@ inline void with_act(const FfnArgs& a, F&& f) {
 
 // Row tiles of a wave in the streaming kernels, and with eight waves a
 // workgroup the workgroups of a CU, by registers and LDS.
-// (96-384 forward 337 us with two tiles, 300 with one; 256-1024 433 with one,
-// 337 with two.  The input gradient holds twice the fragments: 128-512 1510 us
-// with one, 1408 with two; 96-384 1090 and 1112; 256-1024 1490 and 2083.)
+// (bf16 forward, one tile and two: 96-384 over 1.09M rows 288 us and 327,
+// 128-512 over 300k 137 and 137, 192-768 over 100k 117 and 103, 224-896 over 300k
+// 393 and 325, 256-1024 505 and 415.  The backward, whose input gradient holds
+// twice the fragments: 128-512 over 500k rows 795 and 775, 112-300 527 and 539,
+// 96-384 over 1.09M 1039 and 1049, 256-1024 over 229k 1398 and 2047.)
 template <class T>
 constexpr int fwd_tiles(int fragments) {
-    return sizeof(T) == 4 || fragments <= 6 ? 1 : 2;
+    return sizeof(T) == 4 || fragments <= 8 ? 1 : 2;
 }
 template <class T>
 constexpr int dx_tiles(int fragments) {
