@@ -133,9 +133,13 @@ __device__ __forceinline__ float act(float g) {
 // h, dg and du of one hidden unit, in place of g, u and dh.
 template <bool GELU>
 __device__ __forceinline__ void act_grad(float& g, float& u, float& dh) {
+    // a' = s + a (1 - s) z'.  GELU's z' grows as g g, but from |g| of about 20 on
+    // a (1 - s) is 0 and a' is s: z' is kept finite (g g overflows from 2e19 on) and
+    // comes last (a z' overflows from 1e13 on).
     const float s = sigmoid_fast(GELU ? g * fmaf(g * g, GELU_B, GELU_A) : g);
     const float a = g * s;
-    const float da = fmaf(GELU ? a * fmaf(g * g, 3.f * GELU_B, GELU_A) : a, 1.f - s, s);
+    const float da =
+        GELU ? fmaf(a * (1.f - s), fmaf(fminf(g * g, 1e38f), 3.f * GELU_B, GELU_A), s) : fmaf(a, 1.f - s, s);
     const float h = a * u;
     g = dh * u * da;   // dg
     u = dh * a;        // du

@@ -1,0 +1,38 @@
+"""Learned-head operators at the ends of their types' ranges and of their sizes."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+from test_gpu_nn import nn  # noqa: E402, F401
+
+
+@pytest.mark.parametrize("power", [5, 10, 43, 44, 63, 65, 100, 126])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [2, 20000])
+def test_gradients_of_large_gates(nn, rows, dtype, act, power):  # noqa: F811
+    """Gates of +-2^power with u = 1, where a is the gate or 0 and a' 1 or 0 (SiLU
+    at +-32 within 2^-40: below every type's rounding).  All values are powers of
+    two or a sum of two rounded once."""
+    gate = 2.0 ** power
+    x = torch.ones(rows, 1, dtype=dtype, device="cuda")
+    x[1::2] = -1
+
+    def weight(v):
+        return torch.full((1, 1), v, dtype=dtype, device="cuda")
+
+    dy = torch.zeros_like(x)
+    dy[0], dy[rows - 1] = 1, 1           # a row of each sign
+    y = nn.gated_ffn_forward(x, weight(gate), weight(1.0), weight(1.0), act)
+    dx, dg, du, dd = nn.gated_ffn_backward(dy, x, weight(gate), weight(1.0), weight(1.0), act)
+    # x = 1: g = gate, u = 1, y = gate, dg = u, du = a = gate;  x = -1: all 0 (silu(-32) is 4e-13)
+    close = dict(rtol=0, atol=1e-11)
+    assert torch.allclose(y[:2].double().flatten().cpu(), torch.tensor([gate, 0.0], dtype=torch.float64), **close)
+    want = torch.tensor([gate + gate]).to(dtype)
+    assert torch.allclose(dx[0].double().cpu(), want.double(), **close)
+    assert torch.allclose(dx[rows - 1].double().cpu(), torch.zeros(1, dtype=torch.float64), rtol=0, atol=1e-9)
+    for got, value in ((dg, 1.0), (du, gate), (dd, gate)):
+        assert abs(float(got) - value) <= 1e-11 * value, (float(got), value)
