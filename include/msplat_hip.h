@@ -302,9 +302,10 @@ int msplat_hip_raster_work(int64_t counts[6]);
  * and may start at any element.  rows may be 0 (gradients summed over rows are
  * then 0), at most 2^31 - 1.
  *
- * stream: NULL for the context's stream, MSPLAT_DEFAULT_STREAM for the
- * device's default stream (which is ordered with the context's own), or a HIP
- * stream for this call.
+ * Pointers and streams are those of the context's GPU, which need not be the
+ * calling thread's current device.  stream: NULL for the context's stream,
+ * MSPLAT_DEFAULT_STREAM for that GPU's default stream (which is ordered with the
+ * context's own), or a HIP stream for this call.
  * Nothing is allocated and no call waits, so all of them may be captured into
  * a graph.  The workspace is the caller's: 16-byte aligned, of at least the
  * bytes that the operator's _workspace function gives for the same sizes (it

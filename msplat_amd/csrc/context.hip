@@ -634,6 +634,19 @@ hipStream_t stream_of(void* s) {
     return s ? reinterpret_cast<hipStream_t>(s) : g_ctx->stream;
 }
 
+// Makes the context's GPU current while an operator is launched (a null stream
+// is the current GPU's), and the one that was current before current again.
+struct ContextDevice {
+    int before = -1;
+    hipError_t error;
+    ContextDevice() : error(hipGetDevice(&before)) {
+        if (error == hipSuccess && before != g_ctx->device) error = hipSetDevice(g_ctx->device);
+    }
+    ~ContextDevice() {
+        if (before >= 0 && before != g_ctx->device) (void)hipSetDevice(before);
+    }
+};
+
 }  // namespace
 
 extern "C" {
@@ -1352,6 +1365,8 @@ int msplat_hip_layer_norm(const MsplatLayerNormArgs* a) {
     n.out_stride = a->y_stride;
     n.mean = a->mean;
     n.rstd = a->rstd;
+    ContextDevice on;
+    HIP_TRY(on.error);
     launch_norm_fwd(stream_of(a->stream), a->dtype, n);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;
@@ -1393,6 +1408,8 @@ int msplat_hip_layer_norm_backward(const MsplatLayerNormGradArgs* a) {
     n.rstd = const_cast<float*>(a->rstd);
     n.part = sums ? static_cast<float*>(a->workspace) : nullptr;
     if (!sums && (!a->dx || a->rows == 0)) return MSPLAT_OK;
+    ContextDevice on;
+    HIP_TRY(on.error);
     launch_norm_bwd(stream_of(a->stream), a->dtype, n, a->dweight, a->dbias);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;
@@ -1413,6 +1430,8 @@ int msplat_hip_gated_ffn(const MsplatGatedFfnArgs* a) {
     if (a->rows == 0) return MSPLAT_OK;
     f.out = a->y;
     f.out_stride = a->y_stride;
+    ContextDevice on;
+    HIP_TRY(on.error);
     launch_ffn_fwd(stream_of(a->stream), a->dtype, f);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;
@@ -1445,6 +1464,8 @@ int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* a) {
     f.dw_gate = a->dw_gate;
     f.dw_up = a->dw_up;
     f.dw_down = a->dw_down;
+    ContextDevice on;
+    HIP_TRY(on.error);
     launch_ffn_bwd(stream_of(a->stream), a->dtype, f);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;
@@ -1472,6 +1493,8 @@ int msplat_hip_dropout_add(const MsplatDropoutArgs* a) {
     d.threshold = (uint64_t)(a->p * 4294967296.0);
     d.seed = a->seed;
     d.offset = a->offset;
+    ContextDevice on;
+    HIP_TRY(on.error);
     launch_dropout(stream_of(a->stream), a->dtype, d);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;

@@ -15,15 +15,30 @@ import numpy as np
 from . import _abi
 
 _initialised = False
+_lib = None       # of the initialised context
+_device = None    # and its GPU
 
 
 def init(device: int = 0):
-    global _initialised
+    """The library, with its context on GPU `device` if there is none yet."""
+    global _initialised, _lib, _device
     lib = _abi.load()
     if not _initialised:
         _abi.check(lib.msplat_hip_init(device))
-        _initialised = True
+        _initialised, _lib, _device = True, lib, device
     return lib
+
+
+def init_for(index: int):
+    """The library for tensors on GPU `index`, which becomes the context's GPU if
+    there is none yet; the current device stays what it is.  Memory of another
+    GPU than the context's is refused."""
+    if not _initialised:
+        with torch().cuda.device(index):
+            init(index)
+    if index != _device:
+        raise ValueError(f"tensors on cuda:{index}, but the library runs on cuda:{_device}")
+    return _lib
 
 
 def torch():

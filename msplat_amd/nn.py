@@ -2,9 +2,10 @@
 
 Layer norm, a gated feed-forward block and dropout added to a residual, over
 the features of gaussians or pixels: CUDA tensors [..., dim] of float32,
-float16 or bfloat16 (one type a call), with any stride between rows.  Each runs
-hand-written kernels of libmsplat_hip.so on PyTorch's current stream, sums in
-fp32, and has
+float16 or bfloat16 (one type a call), with any stride between rows, on the GPU
+of the library's context (the first call's, if none has made one yet).  Each
+runs hand-written kernels of libmsplat_hip.so on PyTorch's current stream, sums
+in fp32, and has
 
   layer_norm, gated_ffn, dropout_add          differentiable by autograd
   *_forward, *_backward                       the two passes by themselves
@@ -27,10 +28,10 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
 def _library(t):
-    lib = device.init(t.device.index) if t.is_cuda else None
-    if lib is None:
+    index = t.get_device()
+    if index < 0:
         raise ValueError("the operators take CUDA tensors")
-    return lib
+    return device.init_for(index)
 
 
 _DEFAULT_STREAM = 0xFFFFFFFFFFFFFFFF   # MSPLAT_DEFAULT_STREAM

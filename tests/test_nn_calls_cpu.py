@@ -1,0 +1,77 @@
+"""How msplat_amd.nn calls the library, without a GPU: stand-ins for tensors and
+for the library."""
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+import torch
+
+import msplat_amd
+from msplat_amd import device, nn
+
+
+class _On:
+    """A tensor on GPU `index`, as far as the operators look before they call."""
+
+    is_cuda = True
+    dtype = torch.float32
+
+    def __init__(self, index):
+        self.device = torch.device("cuda", index)
+
+    def get_device(self):
+        return self.device.index
+
+
+@pytest.fixture
+def context(monkeypatch):
+    """A context on GPU 0."""
+    library = object()
+    monkeypatch.setattr(device, "_initialised", True)
+    monkeypatch.setattr(device, "_lib", library, raising=False)
+    monkeypatch.setattr(device, "_device", 0, raising=False)
+    monkeypatch.setattr(device._abi, "load", lambda: library)
+    return library
+
+
+def test_another_gpus_tensors_are_refused(context):
+    assert nn._library(_On(0)) is context
+    far = _On(1)
+    for call in (lambda: nn._library(far), lambda: nn.layer_norm_forward(far), lambda: nn.gated_ffn_forward(far, *[far] * 3),
+                 lambda: nn.dropout_add_forward(far, None, 0.5, 1, 2)):
+        with pytest.raises(ValueError, match="cuda:1"):
+            call()
+
+
+def test_the_first_call_leaves_the_current_device(monkeypatch):
+    """The context is made on the tensors' GPU, in a guard of PyTorch's, and again
+    after a cleanup."""
+    seen = []
+
+    @contextlib.contextmanager
+    def guard(index):
+        seen.append(("enter", index))
+        yield
+        seen.append("leave")
+
+    class Library:
+        def msplat_hip_init(self, index):
+            seen.append(("init", index))
+            return 0
+
+        def msplat_hip_shutdown(self):
+            seen.append("cleanup")
+            return 0
+
+    library = Library()
+    monkeypatch.setattr(device, "_initialised", False)
+    monkeypatch.setattr(device, "_lib", None, raising=False)
+    monkeypatch.setattr(device, "_device", None, raising=False)
+    monkeypatch.setattr(device._abi, "load", lambda: library)
+    monkeypatch.setattr(torch.cuda, "device", guard)
+    assert nn._library(_On(3)) is library
+    assert seen == [("enter", 3), ("init", 3), "leave"]
+    msplat_amd.cleanup()
+    assert nn._library(_On(2)) is library
+    assert seen[3:] == ["cleanup", ("enter", 2), ("init", 2), "leave"]
