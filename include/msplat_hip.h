@@ -428,8 +428,8 @@ int64_t msplat_hip_gated_ffn_backward_workspace(int64_t rows, int32_t dim, int32
 int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* args);
 
 /* y = residual + (keep ? x / (1 - p) : 0), x, residual (NULL for none) and y
- * [rows, dim], 1 <= dim, 0 <= p <= 1; a dropped element counts as 0 whatever it
- * holds.  The mask is not stored: keep at (row, column) is word >= floor(p
+ * [rows, dim], 1 <= dim <= 2^31 - 256, 0 <= p <= 1; a dropped element counts as 0
+ * whatever it holds.  The mask is not stored: keep at (row, column) is word >= floor(p
  * 2^32) for word column % 4 of Philox 4x32 with seven rounds (Salmon, Moraes,
  * Dror and Shaw, SC 2011), key = (seed's low, high 32 bits), counter = (column
  * / 4, row, offset's low, high 32 bits).  A training program gives each

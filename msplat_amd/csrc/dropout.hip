@@ -48,7 +48,9 @@ __global__ __launch_bounds__(THREADS) void k_dropout(DropArgs a, int tx) {
     const T* res = static_cast<const T*>(a.residual);
     T* out = static_cast<T*>(a.out);
     for (int64_t row = (int64_t)blockIdx.x * rb + sub; row < a.rows; row += (int64_t)gridDim.x * rb)
-        for (int k = lane * E<T>; k < a.dim; k += tx * E<T>) {
+        // at runs to dim + THREADS * E - 1, which passes 2^31 at the largest widths
+        for (uint32_t at = lane * E<T>; at < (uint32_t)a.dim; at += tx * E<T>) {
+            const int k = (int)at;
             const piece_t<T> v = load_piece(x + row * a.x_stride, k, a.dim);
             piece_t<T> r = {};
             if (RES) r = load_piece(res + row * a.residual_stride, k, a.dim);

@@ -1,11 +1,13 @@
 """Learned-head operators at the ends of their types' ranges and of their sizes."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+import nn_oracle as orc  # noqa: E402
 from test_gpu_nn import nn  # noqa: E402, F401
 
 
@@ -36,3 +38,26 @@ def test_gradients_of_large_gates(nn, rows, dtype, act, power):  # noqa: F811
     assert torch.allclose(dx[rows - 1].double().cpu(), torch.zeros(1, dtype=torch.float64), rtol=0, atol=1e-9)
     for got, value in ((dg, 1.0), (du, gate), (dd, gate)):
         assert abs(float(got) - value) <= 1e-11 * value, (float(got), value)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 2 ** 31 - 256), (torch.float16, 2 ** 31 - 2041),
+                                       (torch.float32, 2 ** 31 - 1021)], ids=["bf16", "f16", "f32"])
+def test_dropout_of_one_row_of_the_largest_width(nn, dtype, dim):  # noqa: F811
+    """The step past the row's end does not fit a signed 32-bit index."""
+    p, seed, offset = 0.25, 0xFEDCBA9876543210, 0x1122334455667788
+    y = nn.dropout_add_forward(torch.ones(dim, dtype=dtype, device="cuda"), None, p, seed, offset)
+    kept = torch.tensor(1.0 / (1.0 - p)).to(dtype).cuda()
+    count = 0
+    for part in y.split(1 << 28):
+        zero = part == 0
+        assert bool((zero | (part == kept)).all())
+        count += part.numel() - int(zero.sum())
+    # five standard deviations of the kept share
+    assert abs(count / dim - (1 - p)) < 5 * (p * (1 - p) / dim) ** 0.5
+    for first in (0, 2 ** 30 - 512, (dim - 1024) // 4 * 4):
+        n = min(1024, dim - first)
+        columns = np.arange(first // 4, (first + n + 3) // 4)
+        words = orc.philox((columns, 0 * columns, 0 * columns + (offset & 0xFFFFFFFF), 0 * columns + (offset >> 32)),
+                           (seed & 0xFFFFFFFF, seed >> 32), 7)
+        keep = np.stack(words, 1).reshape(-1)[:n] >= np.uint64(int(p * 2.0 ** 32))
+        assert torch.equal(y[first:first + n].cpu() != 0, torch.from_numpy(keep)), first

@@ -1,14 +1,16 @@
 """How msplat_amd.nn calls the library, without a GPU: stand-ins for tensors and
-for the library."""
+for the library.  And the widths that the library takes."""
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import os
 
 import pytest
 import torch
 
 import msplat_amd
-from msplat_amd import device, nn
+from msplat_amd import _abi, device, nn
 
 
 class _On:
@@ -75,3 +77,17 @@ def test_the_first_call_leaves_the_current_device(monkeypatch):
     msplat_amd.cleanup()
     assert nn._library(_On(2)) is library
     assert seen[3:] == ["cleanup", ("enter", 2), ("init", 2), "leave"]
+
+
+def test_the_widest_dropout():
+    """Refused from 2^31 - 255 columns on; the widest goes on to the missing context."""
+    if not os.path.exists(_abi.LIB_PATH):
+        pytest.skip("libmsplat_hip.so not built")
+    if device._initialised:
+        pytest.skip("a context already exists in this process")
+    lib = _abi.load()
+    host = (ctypes.c_double * 2)()
+    at = ctypes.addressof(host)
+    for dim, code in ((2 ** 31 - 256, -3), (2 ** 31 - 255, -1)):
+        a = _abi.DropoutArgs(None, 1, dim, 2, 0.5, 1, 2, at, dim, None, 0, at, dim)
+        assert lib.msplat_hip_dropout_add(ctypes.byref(a)) == code
