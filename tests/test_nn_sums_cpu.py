@@ -1,0 +1,69 @@
+"""The mean-square checks of the learned-head operators without a GPU: that they
+fail for a sum that misses rows."""
+from __future__ import annotations
+
+import os
+
+import pytest
+import torch
+
+import nn_dispatch
+import nn_norms as norms
+from msplat_amd import _abi
+from nn_sizes import FFN_MANY
+
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _operands(rows, dim, hidden, dtype):
+    g = torch.Generator().manual_seed(rows + dim)
+    shapes = ((rows, dim, 1.0), (rows, dim, 1.0), (hidden, dim, dim ** -0.5), (hidden, dim, dim ** -0.5),
+              (dim, hidden, hidden ** -0.5))
+    return [(s * torch.randn(a, b, generator=g)).to(dtype) for a, b, s in shapes]
+
+
+# ranges of the operator's sizes in which its launch rules change
+ROWS = (1, 40, 300, 4096, 4100, 8200, 9000, 16384, 16400, 17000, 32768, 33000, 65543, 70000, 131079, 140000, 262149)
+HIDDEN = (1, 3, 7, 8, 24, 64, 200, 256, 400, 800, 1100, 1800, 5000)
+
+
+def test_launch_rules_are_the_librarys():
+    """Through the workspaces' sizes, which follow from them."""
+    if not os.path.exists(_abi.LIB_PATH):
+        pytest.skip("libmsplat_hip.so not built")
+    lib = _abi.load()
+    for dtype, number in DTYPES.items():
+        size = torch.empty(0, dtype=dtype).element_size()
+        for dim in (1, 3, 5, 8, 17, 33, 45, 64, 65, 100, 128, 150, 180, 192, 200, 256):
+            for hidden in HIDDEN:
+                for rows in (0,) + ROWS:
+                    plan = nn_dispatch.Plan(size, rows, dim, hidden)
+                    assert lib.msplat_hip_gated_ffn_workspace(rows, dim, hidden, number) == plan.forward_workspace()
+                    assert lib.msplat_hip_gated_ffn_backward_workspace(rows, dim, hidden, number) == \
+                        plan.backward_workspace(), (dtype, rows, dim, hidden)
+
+
+@pytest.mark.parametrize("rows,dim,hidden", [s for s in FFN_MANY if s[0] * s[2] < 8_000_000])
+def test_a_lost_block_of_rows_fails(rows, dim, hidden):
+    """In bf16, whose limits are the widest, for one block of 32 rows (the last,
+    short one where it has 16 rows or more, else the one before), and for one
+    of the rows at edges."""
+    dtype = torch.bfloat16
+    ops = _operands(rows, dim, hidden, dtype)
+    plan = nn_dispatch.Plan(2, rows, dim, hidden)
+    whole = norms.gated_ffn(*ops, "silu")
+    last = rows // 32 * 32 if rows % 32 >= 16 else (rows // 32 - 1) * 32
+    block = slice(last, min(last + 32, rows))
+    part = norms.gated_ffn(ops[0][block], ops[1][block], *ops[2:], "silu")
+    for (v, q2, n), (lost, _, _), what in list(zip(whole, part, norms.NAMES))[2:]:
+        norms.near(v.to(dtype), v, q2, n, dim, what)
+        with pytest.raises(AssertionError, match="error"):
+            norms.near((v - lost).to(dtype), v, q2, n, dim, what)
+    edges = plan.edge_rows()
+    assert edges[0] == 0 and edges[-1] == rows - 1
+    dy, x = ops[0][edges], ops[1][edges]
+    whole = norms.gated_ffn(dy, x, *ops[2:], "silu")
+    part = norms.gated_ffn(dy[-1:], x[-1:], *ops[2:], "silu")
+    for (v, q2, n), (lost, _, _), what in list(zip(whole, part, norms.NAMES))[2:]:
+        with pytest.raises(AssertionError, match="error"):
+            norms.near((v - lost).to(dtype), v, q2, n, dim, what)
