@@ -1,4 +1,5 @@
-"""Sums over many rows in the learned-head operators: errors in the mean square, which a lost block of rows shows in (nn_norms), and
+"""Sums over many rows, and every kernel form of the learned-head operators:
+errors in the mean square, which a lost block of rows shows in (nn_norms), and
 gradients that come from chosen rows alone."""
 from __future__ import annotations
 

@@ -1,5 +1,5 @@
-"""The mean-square checks of the learned-head operators without a GPU: that they
-fail for a sum that misses rows."""
+"""The mean-square checks of the learned-head operators without a GPU: that their
+sizes reach every kernel, and that they fail for a sum that misses rows."""
 from __future__ import annotations
 
 import os
@@ -10,7 +10,7 @@ import torch
 import nn_dispatch
 import nn_norms as norms
 from msplat_amd import _abi
-from nn_sizes import FFN_MANY
+from nn_sizes import FFN_ALL, FFN_MANY
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -25,6 +25,21 @@ def _operands(rows, dim, hidden, dtype):
 # ranges of the operator's sizes in which its launch rules change
 ROWS = (1, 40, 300, 4096, 4100, 8200, 9000, 16384, 16400, 17000, 32768, 33000, 65543, 70000, 131079, 140000, 262149)
 HIDDEN = (1, 3, 7, 8, 24, 64, 200, 256, 400, 800, 1100, 1800, 5000)
+
+
+@pytest.mark.parametrize("size", [4, 2])
+def test_sizes_reach_every_kernel(size):
+    reach = set()
+    for dim in list(range(1, 40)) + list(range(40, 257, 3)) + [128, 192, 256]:
+        for hidden in HIDDEN:
+            for rows in ROWS:
+                plan = nn_dispatch.Plan(size, rows, dim, hidden)
+                reach.update(plan.forward() + plan.backward())
+    tested = set()
+    for sizes in FFN_ALL:
+        plan = nn_dispatch.Plan(size, *sizes)
+        tested.update(plan.forward() + plan.backward())
+    assert not reach - tested, sorted(reach - tested, key=str)
 
 
 def test_launch_rules_are_the_librarys():
