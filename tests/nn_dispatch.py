@@ -110,3 +110,19 @@ class Plan:
         edges |= {self.rows // self.kb * self.kb, (self.rows // self.kb - 1) * self.kb, self.rows - self.kb, self.kb}
         rows = {r for e in edges for r in (e - 1, e)}
         return sorted(r for r in rows if 0 <= r < self.rows)
+
+
+class NormPlan:
+    """Layer norm's launch: lanes and pieces of a row, rows of a workgroup at
+    once, workgroups of the forward and of the backward."""
+
+    def __init__(self, size, rows, dim):
+        pieces = ceil_div(dim, 16 // size)
+        shapes = [(1 << i, 1) for i in range(7)] + [(64, 2), (64, 4), (256, 2), (256, 4), (256, 8)]
+        self.lanes, self.pieces = next(s for s in shapes if pieces <= s[0] * s[1])
+        self.at_once = 256 // self.lanes
+        self.forward_groups = min(ceil_div(rows, self.at_once), 4096)
+        self.backward_groups = min(ceil_div(rows, self.at_once), 1024)
+
+    def backward_workspace(self, dim):
+        return self.backward_groups * 2 * dim * 4

@@ -58,3 +58,14 @@ def rows_near(got, value, q2, additions, dim, what):
     most = 4 * limit(got.dtype, additions, dim)
     over = (got.double() - value).norm(dim=1) - most * (q2 + value.square()).sum(1).sqrt()
     assert float(over.max()) <= 0, f"{what}: {int((over > 0).sum())} rows off, the first {int((over > 0).nonzero()[0])}"
+
+
+def columns_near(got, terms, what):
+    """got = terms.sum(0) of a sum over rows whose terms are exact up to 32-bit
+    rounding: only the result is rounded to its type."""
+    value, rows = terms.sum(0), terms.shape[0]
+    size = float(value.norm())
+    walk = orc.U * (rows ** 0.5 + 12) * float((terms.square().sum(0) + value.square()).sum().sqrt())
+    most = orc.UT[got.dtype][0] * (1 if value.numel() >= 1000 else 2) * size + walk
+    error = float((got.double() - value).norm())
+    assert error <= most, f"{what}: error {error:.3g}, at most {most:.3g}, size {size:.3g}"

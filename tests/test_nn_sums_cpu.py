@@ -10,7 +10,7 @@ import torch
 import nn_dispatch
 import nn_norms as norms
 from msplat_amd import _abi
-from nn_sizes import FFN_ALL, FFN_MANY
+from nn_sizes import FFN_ALL, FFN_MANY, NORM_MANY
 
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
@@ -40,6 +40,8 @@ def test_sizes_reach_every_kernel(size):
         plan = nn_dispatch.Plan(size, *sizes)
         tested.update(plan.forward() + plan.backward())
     assert not reach - tested, sorted(reach - tested, key=str)
+    shapes = {(p.lanes, p.pieces) for p in (nn_dispatch.NormPlan(size, 1, d) for d in range(1, 8193))}
+    assert shapes == {(p.lanes, p.pieces) for p in (nn_dispatch.NormPlan(size, *s) for s in NORM_MANY)}
 
 
 def test_launch_rules_are_the_librarys():
@@ -56,6 +58,9 @@ def test_launch_rules_are_the_librarys():
                     assert lib.msplat_hip_gated_ffn_workspace(rows, dim, hidden, number) == plan.forward_workspace()
                     assert lib.msplat_hip_gated_ffn_backward_workspace(rows, dim, hidden, number) == \
                         plan.backward_workspace(), (dtype, rows, dim, hidden)
+        for rows, dim in NORM_MANY + [(1, 1), (1000, 45)]:
+            assert lib.msplat_hip_layer_norm_backward_workspace(rows, dim, number) == \
+                nn_dispatch.NormPlan(size, rows, dim).backward_workspace(dim)
 
 
 @pytest.mark.parametrize("rows,dim,hidden", [s for s in FFN_MANY if s[0] * s[2] < 8_000_000])
@@ -82,3 +87,11 @@ def test_a_lost_block_of_rows_fails(rows, dim, hidden):
     for (v, q2, n), (lost, _, _), what in list(zip(whole, part, norms.NAMES))[2:]:
         with pytest.raises(AssertionError, match="error"):
             norms.near((v - lost).to(dtype), v, q2, n, dim, what)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_a_lost_row_of_five_fails(dtype):
+    terms = torch.randn(5, 1000, generator=torch.Generator().manual_seed(1), dtype=torch.float64)
+    norms.columns_near(terms.sum(0).to(dtype), terms, "whole")
+    with pytest.raises(AssertionError, match="error"):
+        norms.columns_near(terms[:4].sum(0).to(dtype), terms, "four of five")
