@@ -902,6 +902,18 @@ inline FfnArgs rows_from(FfnArgs a, int64_t from, size_t size) {
     return a;
 }
 
+// Calls f with a's rows in parts that a launch of the streaming kernels can take:
+// it has fewer than 2^32 threads, and those are up to four a row.
+template <class F>
+inline void in_parts(const FfnArgs& a, size_t size, F&& f) {
+    constexpr int64_t most = int64_t(1) << 29;
+    for (int64_t at = 0; at < a.rows; at += most) {
+        FfnArgs part = rows_from(a, at, size);
+        part.rows = std::min(part.rows, most);
+        f(part);
+    }
+}
+
 // Bytes of a call's workspace: packed weights, parts that the few-row kernels
 // leave (at most one workgroup a CU shares its tile), the weight gradient's
 // sums.
@@ -1000,13 +1012,15 @@ void forward(hipStream_t s, const FfnArgs& a) {
             if (tail) few_forward<T, dk(), gelu(), tiny()>(s, rows_from(a, a.rows - tail, sizeof(T)), hblocks, part);
             main.rows -= tail;
             // two tiles a wave only where that still gives every SIMD a wave
-            if (R == 2 && main.rows >= 32 * 4 * CUS) {
-                const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
-                k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
-            } else {
-                const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
-                k_ffn_fwd<T, dk(), 1, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, 3);
-            }
+            in_parts(main, sizeof(T), [&](const FfnArgs& part) {
+                if (R == 2 && part.rows >= 32 * 4 * CUS) {
+                    const Shape g = shape_of(part.rows, 16 * R, W, INT32_MAX);
+                    k_ffn_fwd<T, dk(), R, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(part, packed, hblocks, 3);
+                } else {
+                    const Shape g = shape_of(part.rows, 16, W, INT32_MAX);
+                    k_ffn_fwd<T, dk(), 1, W, gelu(), tiny()><<<g.groups, g.threads, 0, s>>>(part, packed, hblocks, 3);
+                }
+            });
         });
     });
 }
@@ -1053,13 +1067,15 @@ void input_gradient(hipStream_t s, const FfnArgs& a, const DxPlan<T>& plan, cons
     FfnArgs main = a;
     main.rows -= plan.tail;
     constexpr int R = dx_tiles<T>(F);
-    if (R == 2 && main.rows >= 32 * 4 * CUS) {
-        const Shape g = shape_of(main.rows, 16 * R, W, INT32_MAX);
-        k_ffn_dx<T, DK, R, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
-    } else {
-        const Shape g = shape_of(main.rows, 16, W, INT32_MAX);
-        k_ffn_dx<T, DK, 1, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(main, packed, hblocks, plan.mats);
-    }
+    in_parts(main, sizeof(T), [&](const FfnArgs& p) {
+        if (R == 2 && p.rows >= 32 * 4 * CUS) {
+            const Shape g = shape_of(p.rows, 16 * R, W, INT32_MAX);
+            k_ffn_dx<T, DK, R, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(p, packed, hblocks, plan.mats);
+        } else {
+            const Shape g = shape_of(p.rows, 16, W, INT32_MAX);
+            k_ffn_dx<T, DK, 1, W, GELU, TINY><<<g.groups, g.threads, 0, s>>>(p, packed, hblocks, plan.mats);
+        }
+    });
 }
 
 template <class T>

@@ -7,8 +7,9 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+import nn_norms as norms  # noqa: E402
 import nn_oracle as orc  # noqa: E402
-from test_gpu_nn import nn  # noqa: E402, F401
+from test_gpu_nn import _normal, nn  # noqa: E402, F401
 
 
 @pytest.mark.parametrize("power", [5, 10, 43, 44, 63, 65, 100, 126])
@@ -61,3 +62,21 @@ def test_dropout_of_one_row_of_the_largest_width(nn, dtype, dim):  # noqa: F811
                            (seed & 0xFFFFFFFF, seed >> 32), 7)
         keep = np.stack(words, 1).reshape(-1)[:n] >= np.uint64(int(p * 2.0 ** 32))
         assert torch.equal(y[first:first + n].cpu() != 0, torch.from_numpy(keep)), first
+
+
+def test_gated_ffn_of_more_rows_than_a_launch_has_threads_for(nn):  # noqa: F811
+    """2^30 rows through streamed weights: four threads a row are 2^32."""
+    rows, hidden, dtype = 2 ** 30 + 33, 1800, torch.float16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(rows, 1, generator=g, device="cuda", dtype=dtype)
+    ops = [_normal(2 + i, *s, dtype=dtype, scale=f) for i, (s, f) in
+           enumerate((((hidden, 1), 1.0), ((hidden, 1), 1.0), ((1, hidden), hidden ** -0.5)))]
+    at = torch.tensor([0, 1, 2 ** 29 - 1, 2 ** 29, 2 ** 30 - 1, 2 ** 30, rows - 1], device="cuda")
+    dy = torch.zeros_like(x)
+    dy[at] = _normal(5, len(at), 1, dtype=dtype)
+    want = norms.gated_ffn(dy[at], x[at], *ops, "silu")
+    norms.rows_near(nn.gated_ffn_forward(x, *ops)[at], *want[0], 1, "y")
+    dx, *grads = nn.gated_ffn_backward(dy, x, *ops)
+    norms.rows_near(dx[at], *want[1], 1, "dx")
+    for got, (v, q2, n), what in zip(grads, want[2:], norms.NAMES[2:]):
+        norms.near(got, v, q2, n, 1, what)
