@@ -27,7 +27,12 @@ from . import nn
 
 class AppearanceHead:
     """dim features a pixel, `blocks` blocks of `hidden` units.  Parameters and
-    their optimiser are float32; features and products have the type `dtype`."""
+    their optimiser are float32; features and products have the type `dtype`.
+
+    float16 is for correcting views with a head trained in another type
+    (head.dtype = torch.float16): a pixel's share of a view's mean loss is
+    below its smallest numbers, and scaled up for them the sums over a view's
+    pixels pass its largest, so training in it is refused."""
 
     def __init__(self, num_photos: int, dim: int = 32, hidden: int = 128, blocks: int = 2, dropout: float = 0.05,
                  activation: str = "silu", dtype=torch.bfloat16, seed: int = 0, device: str = "cuda"):
@@ -59,6 +64,8 @@ class AppearanceHead:
 
     def __call__(self, rgb, photo: int, training: bool = False):
         """The (H, W, 3) float32 view in the colours of photo number `photo`."""
+        if training and self.dtype is torch.float16:
+            raise ValueError("a head is trained in bfloat16 or float32, not float16")
         if rgb.dim() != 3 or rgb.shape[2] != 3:
             raise ValueError(f"rgb has shape {tuple(rgb.shape)}, not (H, W, 3)")
         h, w = rgb.shape[:2]

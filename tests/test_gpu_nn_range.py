@@ -80,3 +80,28 @@ def test_gated_ffn_of_more_rows_than_a_launch_has_threads_for(nn):  # noqa: F811
     norms.rows_near(dx[at], *want[1], 1, "dx")
     for got, (v, q2, n), what in zip(grads, want[2:], norms.NAMES[2:]):
         norms.near(got, v, q2, n, 1, what)
+
+
+def test_bf16_gradients_of_a_whole_views_head(nn):  # noqa: F811
+    """A view of 1297 x 840: a pixel's share of the mean loss is 3e-7 of O.  Every
+    parameter's gradient in bf16 is near the float32 one: a pixel's gradient
+    passes some 20 roundings of 2^-8, which may add up (0.08) where a parameter's
+    gradient is mostly one sum over pixels."""
+    from msplat_amd.appearance import AppearanceHead
+    g = torch.Generator(device="cuda").manual_seed(1)
+    view = torch.rand(840, 1297, 3, generator=g, device="cuda")
+    head = AppearanceHead(1, dtype=torch.float32)
+    head.out.data.normal_(generator=g, std=3e-3)   # what a step leaves
+    grads = []
+    for dtype in (torch.float32, torch.bfloat16):
+        head.dtype = dtype
+        loss = (head(view, 0, training=True) - view * 0.8).abs().mean()
+        grads.append(torch.autograd.grad(loss, head.parameters()))
+    for want, got in zip(*grads):
+        assert float(want.norm()) > 0 and float((got - want).norm() / want.norm()) < 0.08
+    head.dtype = torch.float16
+    with torch.no_grad():
+        half = head(view, 0)
+        head.dtype = torch.float32
+        # the correction, of the size of O, in some 20 roundings of 2^-11
+        assert float((half - head(view, 0)).norm()) < 0.01 * float((half - view).norm())
