@@ -14,7 +14,12 @@ msplat_amd.nn.  It has no counterpart in the reference.
 
     head = AppearanceHead(len(photos))
     head.fit(renders, photos, steps=500)     # e.g. renders of GaussianTrainer's cameras
-    corrected = head(render, photo=3)
+    with torch.no_grad():
+        corrected = head(render, photo=3)
+
+Views are (H, W, 3) float32, numpy arrays (as GaussianTrainer.render gives them)
+or tensors.  The head is fitted to finished renders: the scene's own training
+does not see it.
 """
 from __future__ import annotations
 
@@ -63,9 +68,12 @@ class AppearanceHead:
                 *(p for b in self.blocks for p in b.values())]
 
     def __call__(self, rgb, photo: int, training: bool = False):
-        """The (H, W, 3) float32 view in the colours of photo number `photo`."""
+        """The (H, W, 3) float32 view in the colours of photo number `photo`, a
+        tensor on the head's GPU; differentiable, so without torch.no_grad() it
+        keeps what its gradient takes of every pixel."""
         if training and self.dtype is torch.float16:
             raise ValueError("a head is trained in bfloat16 or float32, not float16")
+        rgb = self._view(rgb)
         if rgb.dim() != 3 or rgb.shape[2] != 3:
             raise ValueError(f"rgb has shape {tuple(rgb.shape)}, not (H, W, 3)")
         h, w = rgb.shape[:2]
@@ -82,17 +90,23 @@ class AppearanceHead:
         n = nn.layer_norm(x, self.norm_weight.to(self.dtype), self.norm_bias.to(self.dtype))
         return rgb + (n.float() @ self.out.t()).reshape(h, w, 3)
 
-    def fit(self, renders: Sequence[torch.Tensor], photos: Sequence[torch.Tensor], steps: int,
+    def _view(self, view):
+        return torch.as_tensor(view, dtype=torch.float32, device=self.embed.device)
+
+    def fit(self, renders: Sequence, photos: Sequence, steps: int,
             lr: float = 3e-3, optimiser: Optional[torch.optim.Optimizer] = None) -> List[float]:
         """`steps` steps of the L1 loss between corrected renders and photos,
-        cycling through them; the loss of every step."""
+        cycling through them (a later call goes on where this one stops); the
+        loss of every step.  Without `optimiser` a call starts a new Adam: give
+        one over parameters() to keep its moments from call to call."""
         if len(renders) != len(photos) or not renders:
             raise ValueError("as many photos as renders are needed, and at least one")
+        renders, photos = [self._view(t).detach() for t in renders], [self._view(t) for t in photos]
         optimiser = optimiser or torch.optim.Adam(self.parameters(), lr=lr)
         losses = []
         for _ in range(steps):
             i = self.step % len(renders)
-            loss = (self(renders[i].detach(), i, training=True) - photos[i]).abs().mean()
+            loss = (self(renders[i], i, training=True) - photos[i]).abs().mean()
             optimiser.zero_grad(set_to_none=True)
             loss.backward()
             optimiser.step()
