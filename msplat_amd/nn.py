@@ -122,9 +122,10 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5) -> Tuple[to
     return y, mean, rstd
 
 
-def layer_norm_backward(dy, x, weight, mean, rstd):
+def layer_norm_backward(dy, x, weight, mean, rstd, wanted=(True, True, True)):
     """(dx, dweight, dbias) from the gradient of y and the forward's x, mean
-    and rstd; dweight and dbias have x's type, also where weight is None."""
+    and rstd; dweight and dbias have x's type, also where weight is None.
+    Those not wanted are None and not computed."""
     lib, dtype = _library(x), _dtype(x)
     x2 = _feature_rows("x", x)
     rows, dim = x2.shape
@@ -134,13 +135,13 @@ def layer_norm_backward(dy, x, weight, mean, rstd):
         if t.dtype is not torch.float32 or t.numel() != rows or t.device != x.device:
             raise ValueError(f"{name} must hold one float32 a row on {x.device}")
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    dx = x.new_empty(x.shape)
-    dweight = x.new_empty(dim)
-    dbias = x.new_empty(dim)
+    dx = x.new_empty(x.shape) if wanted[0] else None
+    dweight = x.new_empty(dim) if wanted[1] else None
+    dbias = x.new_empty(dim) if wanted[2] else None
     ws = _workspace(lib.msplat_hip_layer_norm_backward_workspace(rows, dim, dtype), x)
     a = _abi.LayerNormGradArgs(_stream(x), rows, dim, dtype, dy2.data_ptr(), dy2.stride(0), x2.data_ptr(),
-                               x2.stride(0), _ptr(w), mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), dim,
-                               dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), ws.nbytes)
+                               x2.stride(0), _ptr(w), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), dim,
+                               _ptr(dweight), _ptr(dbias), ws.data_ptr(), ws.nbytes)
     _abi.check(lib.msplat_hip_layer_norm_backward(ctypes.byref(a)))
     return dx, dweight, dbias
 
@@ -172,20 +173,22 @@ def gated_ffn_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
     return y
 
 
-def gated_ffn_backward(dy, x, w_gate, w_up, w_down, activation: str = "silu"):
-    """(dx, dw_gate, dw_up, dw_down) from the gradient of y, x and the weights."""
+def gated_ffn_backward(dy, x, w_gate, w_up, w_down, activation: str = "silu", wanted=(True, True)):
+    """(dx, dw_gate, dw_up, dw_down) from the gradient of y, x and the weights.
+    wanted: dx, and the three weights' together; those that are not are None and
+    not computed."""
     lib, dtype = _library(x), _dtype(x)
     x2, hidden, wg, wu, wd = _ffn_operands(x, w_gate, w_up, w_down, activation)
     rows, dim = x2.shape
     dy2 = _same_rows("dy", dy, x2)
-    dx = x.new_empty(x.shape)
-    grads = x.new_empty((hidden, dim)), x.new_empty((hidden, dim)), x.new_empty((dim, hidden))
+    dx = x.new_empty(x.shape) if wanted[0] else None
+    shapes = (hidden, dim), (hidden, dim), (dim, hidden)
+    grads = [x.new_empty(s) if wanted[1] else None for s in shapes]
     ws = _workspace(lib.msplat_hip_gated_ffn_backward_workspace(rows, dim, hidden, dtype), x)
     a = _abi.GatedFfnGradArgs(_stream(x), rows, dim, hidden, dtype, _ACTIVATIONS[activation], dy2.data_ptr(),
                               dy2.stride(0), x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0),
-                              wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0), dx.data_ptr(), dim,
-                              grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), ws.data_ptr(),
-                              ws.nbytes)
+                              wu.data_ptr(), wu.stride(0), wd.data_ptr(), wd.stride(0), _ptr(dx), dim,
+                              _ptr(grads[0]), _ptr(grads[1]), _ptr(grads[2]), ws.data_ptr(), ws.nbytes)
     _abi.check(lib.msplat_hip_gated_ffn_backward(ctypes.byref(a)))
     return (dx, *grads)
 
@@ -227,9 +230,7 @@ class _LayerNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        dx, dweight, dbias = layer_norm_backward(dy, x, weight, mean, rstd)
-        need = ctx.needs_input_grad
-        return dx, dweight if need[1] else None, dbias if need[2] else None, None
+        return (*layer_norm_backward(dy, x, weight, mean, rstd, ctx.needs_input_grad[:3]), None)
 
 
 class _GatedFfn(torch.autograd.Function):
@@ -242,7 +243,9 @@ class _GatedFfn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        return (*gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation), None)
+        need = ctx.needs_input_grad
+        dx, *grads = gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation, (need[0], any(need[1:4])))
+        return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None)
 
 
 class _DropoutAdd(torch.autograd.Function):
