@@ -451,6 +451,11 @@ typedef struct MsplatDropoutArgs {
     int64_t y_stride;
 } MsplatDropoutArgs;
 int msplat_hip_dropout_add(const MsplatDropoutArgs* args);
+/* The same with the offset in device memory (8-byte aligned), read when the
+ * kernel runs, in place of args->offset.  A captured call repeats its arguments
+ * in every replay, so a captured training step takes its masks by this one and
+ * advances the offset in the graph or between replays. */
+int msplat_hip_dropout_add_at(const MsplatDropoutArgs* args, const uint64_t* offset);
 
 #ifdef __cplusplus
 }

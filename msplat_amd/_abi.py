@@ -266,6 +266,7 @@ SIGNATURES = [
     ("msplat_hip_gated_ffn_backward_workspace", c_int64, [c_int64, c_int32, c_int32, c_int32]),
     ("msplat_hip_gated_ffn_backward", c_int, [POINTER(GatedFfnGradArgs)]),
     ("msplat_hip_dropout_add", c_int, [POINTER(DropoutArgs)]),
+    ("msplat_hip_dropout_add_at", c_int, [POINTER(DropoutArgs), c_void_p]),
     # include/msplat_c_api.h (the reference's C API)
     ("msplat_dataset_create", c_void_p, [c_char_p, c_float, c_bool, c_int]),
     ("msplat_dataset_destroy", None, [c_void_p]),

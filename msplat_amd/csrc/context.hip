@@ -647,6 +647,36 @@ struct ContextDevice {
     }
 };
 
+int dropout_add(const MsplatDropoutArgs* a, const uint64_t* offset_at) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, 0x7FFFFF00, a->dtype));
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->dim, a->residual_stride, a->dtype));
+    CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    if (!(a->p >= 0.0 && a->p <= 1.0)) return fail(MSPLAT_ERR_ARG, "p %g outside [0, 1]", a->p);
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    DropArgs d{};
+    d.rows = a->rows;
+    d.dim = a->dim;
+    d.x = a->x;
+    d.x_stride = a->x_stride;
+    d.residual = a->residual;
+    d.residual_stride = a->residual_stride;
+    d.out = a->y;
+    d.out_stride = a->y_stride;
+    d.scale = (float)(1.0 / (1.0 - a->p));
+    d.threshold = (uint64_t)(a->p * 4294967296.0);
+    d.seed = a->seed;
+    d.offset = a->offset;
+    d.offset_at = offset_at;
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch_dropout(stream_of(a->stream), a->dtype, d);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1471,33 +1501,12 @@ int msplat_hip_gated_ffn_backward(const MsplatGatedFfnGradArgs* a) {
     return MSPLAT_OK;
 }
 
-int msplat_hip_dropout_add(const MsplatDropoutArgs* a) {
-    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
-    CHECK(check_rows(a->rows, a->dim, 0x7FFFFF00, a->dtype));
-    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
-    if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->dim, a->residual_stride, a->dtype));
-    CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
-    if (!(a->p >= 0.0 && a->p <= 1.0)) return fail(MSPLAT_ERR_ARG, "p %g outside [0, 1]", a->p);
-    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
-    if (a->rows == 0) return MSPLAT_OK;
-    DropArgs d{};
-    d.rows = a->rows;
-    d.dim = a->dim;
-    d.x = a->x;
-    d.x_stride = a->x_stride;
-    d.residual = a->residual;
-    d.residual_stride = a->residual_stride;
-    d.out = a->y;
-    d.out_stride = a->y_stride;
-    d.scale = (float)(1.0 / (1.0 - a->p));
-    d.threshold = (uint64_t)(a->p * 4294967296.0);
-    d.seed = a->seed;
-    d.offset = a->offset;
-    ContextDevice on;
-    HIP_TRY(on.error);
-    launch_dropout(stream_of(a->stream), a->dtype, d);
-    HIP_TRY(hipGetLastError());
-    return MSPLAT_OK;
+int msplat_hip_dropout_add(const MsplatDropoutArgs* a) { return dropout_add(a, nullptr); }
+
+int msplat_hip_dropout_add_at(const MsplatDropoutArgs* a, const uint64_t* offset) {
+    if (!offset) return fail(MSPLAT_ERR_ARG, "offset is null");
+    if (reinterpret_cast<uintptr_t>(offset) % 8 != 0) return fail(MSPLAT_ERR_ARG, "offset is not 8-byte aligned");
+    return dropout_add(a, offset);
 }
 
 }  // extern "C"

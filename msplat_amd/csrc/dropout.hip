@@ -47,6 +47,7 @@ __global__ __launch_bounds__(THREADS) void k_dropout(DropArgs a, int tx) {
     const T* x = static_cast<const T*>(a.x);
     const T* res = static_cast<const T*>(a.residual);
     T* out = static_cast<T*>(a.out);
+    const uint64_t offset = a.offset_at ? *a.offset_at : a.offset;
     for (int64_t row = (int64_t)blockIdx.x * rb + sub; row < a.rows; row += (int64_t)gridDim.x * rb)
         // at runs to dim + THREADS * E - 1, which passes 2^31 at the largest widths
         for (uint32_t at = lane * E<T>; at < (uint32_t)a.dim; at += tx * E<T>) {
@@ -57,8 +58,8 @@ __global__ __launch_bounds__(THREADS) void k_dropout(DropArgs a, int tx) {
             piece_t<T> o;
 #pragma unroll
             for (int q = 0; q < E<T> / 4; ++q) {
-                const Words w = philox((uint32_t)(k / 4 + q), (uint32_t)row, (uint32_t)a.offset,
-                                       (uint32_t)(a.offset >> 32), (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
+                const Words w = philox((uint32_t)(k / 4 + q), (uint32_t)row, (uint32_t)offset, (uint32_t)(offset >> 32),
+                                       (uint32_t)a.seed, (uint32_t)(a.seed >> 32));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float t = w.w[j] >= a.threshold ? (float)v[4 * q + j] * a.scale : 0.f;

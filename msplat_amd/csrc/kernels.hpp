@@ -436,6 +436,7 @@ struct DropArgs {
     float scale;           // 1 / (1 - p), unused where threshold keeps nothing
     uint64_t threshold;    // a word below it drops its element
     uint64_t seed, offset;
+    const uint64_t* offset_at;   // device memory, read in place of offset where not null
 };
 void launch_dropout(hipStream_t s, int dtype, const DropArgs& a);
 

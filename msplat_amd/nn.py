@@ -11,7 +11,8 @@ in fp32, and has
   *_forward, *_backward                       the two passes by themselves
 
 None of them waits for the GPU or keeps anything between calls, so they may
-be captured into a graph.
+be captured into a graph.  A replay repeats a call's arguments: where each is to
+drop other elements, dropout takes its offset as a tensor.
 """
 from __future__ import annotations
 
@@ -201,20 +202,29 @@ def _dropout(x, residual, p, seed, offset):
     rows, dim = x2.shape
     r2 = None if residual is None else _same_rows("residual", residual, x2)
     y = x.new_empty(x.shape)
-    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
-                         x2.data_ptr(), x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
-    _abi.check(lib.msplat_hip_dropout_add(ctypes.byref(a)))
+    at = offset if torch.is_tensor(offset) else None
+    if at is not None and (at.dtype is not torch.int64 or at.numel() != 1 or at.device != x.device):
+        raise ValueError(f"offset must be a number or one int64 on {x.device}")
+    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, seed & 0xFFFFFFFFFFFFFFFF,
+                         0 if at is not None else offset & 0xFFFFFFFFFFFFFFFF, x2.data_ptr(), x2.stride(0), _ptr(r2),
+                         0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
+    if at is None:
+        _abi.check(lib.msplat_hip_dropout_add(ctypes.byref(a)))
+    else:
+        _abi.check(lib.msplat_hip_dropout_add_at(ctypes.byref(a), at.data_ptr()))
     return y
 
 
-def dropout_add_forward(x, residual, p: float, seed: int, offset: int):
+def dropout_add_forward(x, residual, p: float, seed: int, offset):
     """residual + keep * x / (1 - p); residual None for none.  The mask is
     a function of seed, offset, row and column (the first axes count as one)
-    and is never stored; give each layer its seed and each step its offset."""
+    and is never stored; give each layer its seed and each step its offset: a
+    number, or a tensor of one int64 on x's GPU that is read when the kernel
+    runs, so that replays of a captured step may differ in it."""
     return _dropout(x, residual, p, seed, offset)
 
 
-def dropout_add_backward(dy, p: float, seed: int, offset: int):
+def dropout_add_backward(dy, p: float, seed: int, offset):
     """The gradient of dropout_add's x; the residual's is dy itself."""
     return _dropout(dy, None, p, seed, offset)
 
@@ -252,13 +262,17 @@ class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset):
         ctx.args = (p, seed, offset)
+        if torch.is_tensor(offset):   # saved, so that a change before the backward is an error
+            ctx.args = (p, seed)
+            ctx.save_for_backward(offset)
         return dropout_add_forward(x, residual, p, seed, offset)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        return (dropout_add_backward(dy, *ctx.args) if need[0] else None, dy if need[1] else None, None, None, None)
+        dx = dropout_add_backward(dy, *ctx.args, *ctx.saved_tensors) if need[0] else None
+        return dx, dy if need[1] else None, None, None, None
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
@@ -271,6 +285,7 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu"):
     return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)
 
 
-def dropout_add(x, residual, p: float, seed: int, offset: int):
-    """dropout_add_forward, differentiable in x and residual."""
+def dropout_add(x, residual, p: float, seed: int, offset):
+    """dropout_add_forward, differentiable in x and residual.  An offset tensor
+    must keep its value until the backward has run."""
     return _DropoutAdd.apply(x, residual, p, seed, offset)

@@ -91,3 +91,18 @@ def test_the_widest_dropout():
     for dim, code in ((2 ** 31 - 256, -3), (2 ** 31 - 255, -1)):
         a = _abi.DropoutArgs(None, 1, dim, 2, 0.5, 1, 2, at, dim, None, 0, at, dim)
         assert lib.msplat_hip_dropout_add(ctypes.byref(a)) == code
+
+
+def test_offsets_in_memory_are_checked():
+    if not os.path.exists(_abi.LIB_PATH):
+        pytest.skip("libmsplat_hip.so not built")
+    lib = _abi.load()
+    host = (ctypes.c_double * 8)()
+    at = ctypes.addressof(host)
+    a = _abi.DropoutArgs(None, 1, 4, 0, 0.5, 1, 2, at, 4, None, 0, at, 4)
+    for offset, word in ((None, b"offset is null"), (at + 4, b"aligned")):
+        assert lib.msplat_hip_dropout_add_at(ctypes.byref(a), offset) == -1
+        assert word in lib.msplat_hip_last_error()
+    assert lib.msplat_hip_dropout_add_at(None, at) == -1
+    a.dim = 0
+    assert lib.msplat_hip_dropout_add_at(ctypes.byref(a), at) == -1 and b"dim" in lib.msplat_hip_last_error()
