@@ -17,6 +17,7 @@ drop other elements, dropout takes its offset as a tensor.
 from __future__ import annotations
 
 import ctypes
+from operator import index   # numpy's integers overflow in & where Python's do not
 from typing import Tuple
 
 import torch
@@ -29,10 +30,10 @@ _ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
 def _library(t):
-    index = t.get_device()
-    if index < 0:
+    gpu = t.get_device()
+    if gpu < 0:
         raise ValueError("the operators take CUDA tensors")
-    return device.init_for(index)
+    return device.init_for(gpu)
 
 
 _DEFAULT_STREAM = 0xFFFFFFFFFFFFFFFF   # MSPLAT_DEFAULT_STREAM
@@ -205,8 +206,8 @@ def _dropout(x, residual, p, seed, offset):
     at = offset if torch.is_tensor(offset) else None
     if at is not None and (at.dtype is not torch.int64 or at.numel() != 1 or at.device != x.device):
         raise ValueError(f"offset must be a number or one int64 on {x.device}")
-    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, seed & 0xFFFFFFFFFFFFFFFF,
-                         0 if at is not None else offset & 0xFFFFFFFFFFFFFFFF, x2.data_ptr(), x2.stride(0), _ptr(r2),
+    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, index(seed) & 0xFFFFFFFFFFFFFFFF,
+                         0 if at is not None else index(offset) & 0xFFFFFFFFFFFFFFFF, x2.data_ptr(), x2.stride(0), _ptr(r2),
                          0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
     if at is None:
         _abi.check(lib.msplat_hip_dropout_add(ctypes.byref(a)))

@@ -1,6 +1,7 @@
 """Dropout's masks from an offset in device memory, and in replays of a graph."""
 from __future__ import annotations
 
+import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
@@ -67,3 +68,11 @@ def test_refused_offsets(nn):  # noqa: F811
                 torch.zeros(1, dtype=torch.int64)):
         with pytest.raises(ValueError, match="offset"):
             nn.dropout_add_forward(x, None, 0.5, 1, bad)
+
+
+@pytest.mark.parametrize("kind", [np.int32, np.uint32, np.int64, np.uint64])
+def test_numpy_seeds(nn, kind):  # noqa: F811
+    x = _normal(1, 70, 45)
+    assert torch.equal(nn.dropout_add_forward(x, None, 0.3, kind(5), kind(9)), nn.dropout_add_forward(x, None, 0.3, 5, 9))
+    with pytest.raises(TypeError):
+        nn.dropout_add_forward(x, None, 0.3, 5.0, 9)
