@@ -307,7 +307,8 @@ int msplat_hip_raster_work(int64_t counts[6]);
  * MSPLAT_DEFAULT_STREAM for that GPU's default stream (which is ordered with the
  * context's own), or a HIP stream for this call.
  * Nothing is allocated and no call waits, so all of them may be captured into
- * a graph.  The workspace is the caller's: 16-byte aligned, of at least the
+ * a graph, whose replays repeat the call's arguments (msplat_hip_dropout_add_at).
+ * The workspace is the caller's: 16-byte aligned, of at least the
  * bytes that the operator's _workspace function gives for the same sizes (it
  * needs no device, and gives -1 for sizes that the operator refuses); its
  * contents need not be kept between calls, and calls that may overlap need one
@@ -369,7 +370,9 @@ int msplat_hip_layer_norm_backward(const MsplatLayerNormGradArgs* args);
  * and w_up [hidden, dim] and w_down [dim, hidden]; 1 <= dim <= 256, 1 <=
  * hidden <= 65536.  activation a: MSPLAT_SILU v / (1 + exp(-v)), MSPLAT_GELU
  * the tanh form of GELU.  The hidden units stay on the chip; in 16-bit types
- * they are rounded to the type before the last product. */
+ * they are rounded to the type before the last product, so one beyond float16's
+ * 65504 becomes infinite even where y would not be.  A row of x that holds an
+ * infinity or NaN may come out as NaN throughout; other rows are untouched. */
 #define MSPLAT_SILU 0
 #define MSPLAT_GELU 1
 typedef struct MsplatGatedFfnArgs {
@@ -398,7 +401,10 @@ int msplat_hip_gated_ffn(const MsplatGatedFfnArgs* args);
 /* Gradients of the gated feed-forward block from dy, x and the weights: dx
  * [rows, dim] where not NULL, and dw_gate, dw_up [hidden, dim] and dw_down
  * [dim, hidden], contiguous, all three or (all NULL) none.  The sums over
- * rows have a fixed order. */
+ * rows have a fixed order.  In 16-bit types the gradients of the two products
+ * (dg and du of each hidden unit and row) are rounded to the type too, and in
+ * float16 lose bits below 6e-5 and vanish below 3e-8: scale dy so that they do
+ * not, within what the sums over rows allow (65504), or use bfloat16. */
 typedef struct MsplatGatedFfnGradArgs {
     void* stream;
     int64_t rows;

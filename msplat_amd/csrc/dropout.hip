@@ -10,7 +10,7 @@
 // words again.  A dropped element counts as zero whatever it holds.
 //
 // Bound by HBM: 14 32x32-bit products make four words, which fits behind the 24
-// bytes (16-bit types: 1.09M rows of 64 f16 with a residual 75 us, 5.6 TB/s; a
+// bytes (16-bit types: 1.09M rows of 64 f16 with a residual 74 us, 5.6 TB/s; a
 // large copy 5.1); ten rounds cost 2.5% more, 80.1 against 78.1 us a call.  A thread
 // has a 16-byte piece of a row.
 #include "nn.hpp"

@@ -28,13 +28,20 @@
 // small kernel first (5 us): each is used in up to three orders, and the pack
 // takes up every width and stride.  In 16-bit types h, dg and du are rounded to
 // the type for the next product, as the type's own matrix instructions take
-// them; the error is of the size of the output's own rounding.
+// them; the error is of the size of the output's own rounding (1.4 of it in
+// all), within the type's range: in float16 a hidden unit beyond 65504 becomes
+// infinite though the output may not be, and a dg or du below 6e-5 loses bits
+// and below 3e-8 is zero, though a sum of many rows of it may not be.
 //
-// What bounds it: on a SIMD vector and matrix instructions hardly overlap (a
-// probe with four waves: 24 matrix instructions 404 cycles, the activations of
-// as many rows 550, both 782), so a block costs about the sum of the two.  At
-// 64 features the activations are the larger half, at 256 an eighth.
-//   64-256-64 bf16 forward over 1.09M rows: 137 us, 780 TFLOP/s
+// What bounds it: the activations go through the vector unit and the products
+// through the matrix unit, of which a SIMD has one each and a wave uses one at a
+// time.  The two overlap in part (a probe with four waves a SIMD: 24 matrix
+// instructions 404 cycles, the activations of as many rows 550, both 782: 43% of
+// the matrix cycles pass behind vector ones).  At 64 features the activations
+// are the larger half, at 256 an eighth.  64-256-64 below: the matrix unit is
+// busy in 36% of the cycles, the vector unit in 59% (without issuing matrix
+// instructions, 9%); what hides the rest of the one behind the other is open.
+//   64-256-64 bf16 forward over 1.09M rows: 129-139 us, 770-830 TFLOP/s
 //   256-1024-256 bf16 forward over 229k rows: 335 us, 1075 TFLOP/s (a library
 //   product of 8192^3 reaches 1111)
 #pragma once

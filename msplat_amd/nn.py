@@ -162,7 +162,9 @@ def _ffn_operands(x, w_gate, w_up, w_down, activation):
 
 def gated_ffn_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
     """(a(x w_gate^T) * (x w_up^T)) w_down^T with a = SiLU or GELU (tanh form);
-    w_gate and w_up [hidden, dim], w_down [dim, hidden], dim at most 256."""
+    w_gate and w_up [hidden, dim], w_down [dim, hidden], dim at most 256.  In
+    16-bit types the hidden units are rounded to the type (float16: infinite
+    beyond 65504)."""
     lib, dtype = _library(x), _dtype(x)
     x2, hidden, wg, wu, wd = _ffn_operands(x, w_gate, w_up, w_down, activation)
     rows, dim = x2.shape
@@ -178,7 +180,8 @@ def gated_ffn_forward(x, w_gate, w_up, w_down, activation: str = "silu"):
 def gated_ffn_backward(dy, x, w_gate, w_up, w_down, activation: str = "silu", wanted=(True, True)):
     """(dx, dw_gate, dw_up, dw_down) from the gradient of y, x and the weights.
     wanted: dx, and the three weights' together; those that are not are None and
-    not computed."""
+    not computed.  In 16-bit types the hidden units' gradients are rounded to the
+    type (float16: fewer bits below 6e-5, 0 below 3e-8)."""
     lib, dtype = _library(x), _dtype(x)
     x2, hidden, wg, wu, wd = _ffn_operands(x, w_gate, w_up, w_down, activation)
     rows, dim = x2.shape
