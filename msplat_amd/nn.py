@@ -209,9 +209,9 @@ def _dropout(x, residual, p, seed, offset):
     at = offset if torch.is_tensor(offset) else None
     if at is not None and (at.dtype is not torch.int64 or at.numel() != 1 or at.device != x.device):
         raise ValueError(f"offset must be a number or one int64 on {x.device}")
-    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, index(seed) & 0xFFFFFFFFFFFFFFFF,
-                         0 if at is not None else index(offset) & 0xFFFFFFFFFFFFFFFF, x2.data_ptr(), x2.stride(0), _ptr(r2),
-                         0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
+    number = 0 if at is not None else index(offset) & 0xFFFFFFFFFFFFFFFF
+    a = _abi.DropoutArgs(_stream(x), rows, dim, dtype, p, index(seed) & 0xFFFFFFFFFFFFFFFF, number, x2.data_ptr(),
+                         x2.stride(0), _ptr(r2), 0 if r2 is None else r2.stride(0), y.data_ptr(), dim)
     if at is None:
         _abi.check(lib.msplat_hip_dropout_add(ctypes.byref(a)))
     else:

@@ -71,7 +71,8 @@ def test_outputs_over_inputs(nn, dtype, dim):  # noqa: F811
     that a piece does not divide and that several waves share."""
     lib, number = _abi.load(), nn._DTYPES[dtype]
     for rows in (3, 4200):
-        x, dy, w = (_normal(1, rows, dim, dtype=dtype), _normal(2, rows, dim, dtype=dtype), 1 + _normal(3, dim, dtype=dtype))
+        x, dy = _normal(1, rows, dim, dtype=dtype), _normal(2, rows, dim, dtype=dtype)
+        w = 1 + _normal(3, dim, dtype=dtype)
         y, mean, rstd = nn.layer_norm_forward(x, w, w)
         dx = nn.layer_norm_backward(dy, x, w, mean, rstd, (True, False, False))[0]
         dropped = nn.dropout_add_forward(x, dy, 0.3, 5, 6)

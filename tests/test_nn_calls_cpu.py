@@ -40,8 +40,8 @@ def context(monkeypatch):
 def test_another_gpus_tensors_are_refused(context):
     assert nn._library(_On(0)) is context
     far = _On(1)
-    for call in (lambda: nn._library(far), lambda: nn.layer_norm_forward(far), lambda: nn.gated_ffn_forward(far, *[far] * 3),
-                 lambda: nn.dropout_add_forward(far, None, 0.5, 1, 2)):
+    for call in (lambda: nn._library(far), lambda: nn.layer_norm_forward(far),
+                 lambda: nn.gated_ffn_forward(far, *[far] * 3), lambda: nn.dropout_add_forward(far, None, 0.5, 1, 2)):
         with pytest.raises(ValueError, match="cuda:1"):
             call()
 
