@@ -463,6 +463,89 @@ int msplat_hip_dropout_add(const MsplatDropoutArgs* args);
  * advances the offset in the graph or between replays. */
 int msplat_hip_dropout_add_at(const MsplatDropoutArgs* args, const uint64_t* offset);
 
+/* Rows in 8 bits, as activations are kept for a backward pass and as a product
+ * takes them: the OCP microscaling format MXFP8 with e4m3 elements.  Each 32
+ * adjacent columns of a row are a block with one scale, a power of two 2^(code -
+ * 127), code a byte.  A matrix of dim columns has, row after row, 32 ceil(dim /
+ * 32) bytes of data, zeros from dim on, and 4 ceil(dim / 128) bytes of scales,
+ * one a block and then any bytes; both arrays 16-byte aligned, 1 <= dim <= 2^30.
+ *
+ * Packing takes a block's least scale (2^-126 at least) with which its largest
+ * magnitude is at most 448, and rounds to the nearest element, ties to even: to
+ * within 1/16 of a number, or 2^-10 of the scale where that is more.
+ * Infinities and NaN become NaN, and do not count for the scale.  Magnitudes
+ * over 1.875 2^15 (float16) or 1.875 2^127 count as that, since the next
+ * element is beyond the type. */
+typedef struct MsplatMx8Args {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;      /* of the matrix */
+    void* matrix;       /* read by pack, written by unpack */
+    int64_t stride;
+    void* data;
+    void* scales;
+} MsplatMx8Args;
+int msplat_hip_mx8_pack(const MsplatMx8Args* args);
+int msplat_hip_mx8_unpack(const MsplatMx8Args* args);
+
+/* y = t rstd weight over the last axis of t = x + residual [rows, dim], 1 <= dim
+ * <= 8192, rstd = 1 / sqrt(mean(t^2) + eps); t is rounded to the type before its
+ * norm is taken.  residual NULL for none, weight [dim] NULL for ones.  total [rows,
+ * dim] takes t and rstd [rows] its factors, each where not NULL.  y_scales not NULL:
+ * y is written in 8 bits (y the data, y_stride unused), rounded to them once from
+ * fp32.  y and total may each be exactly x or residual with the same stride, but
+ * not both the same one.  A sum of squares beyond fp32 counts as infinite. */
+typedef struct MsplatRmsNormArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;
+    const void* x;
+    int64_t x_stride;
+    const void* residual;
+    int64_t residual_stride;
+    const void* weight;
+    float eps;
+    void* y;
+    int64_t y_stride;
+    void* y_scales;
+    void* total;
+    int64_t total_stride;
+    float* rstd;
+} MsplatRmsNormArgs;
+int msplat_hip_rms_norm(const MsplatRmsNormArgs* args);
+
+/* Gradients of the norm from dy and the forward pass's total and rstd: dx [rows,
+ * dim], the gradient of x and of residual alike, and dweight [dim], each written
+ * where not NULL.  total_scales not NULL: total is in 8 bits (total its data,
+ * total_stride unused).  dtotal: the gradient that reaches total by other ways,
+ * added to dx, NULL for none.  dx may be exactly dy, dtotal or (not in 8 bits)
+ * total with the same stride.  The sums over rows have a fixed order.  The
+ * workspace may be NULL where dweight is. */
+typedef struct MsplatRmsNormGradArgs {
+    void* stream;
+    int64_t rows;
+    int32_t dim;
+    int32_t dtype;
+    const void* dy;
+    int64_t dy_stride;
+    const void* dtotal;
+    int64_t dtotal_stride;
+    const void* total;
+    int64_t total_stride;
+    const void* total_scales;
+    const void* weight;
+    const float* rstd;
+    void* dx;
+    int64_t dx_stride;
+    void* dweight;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatRmsNormGradArgs;
+int64_t msplat_hip_rms_norm_backward_workspace(int64_t rows, int32_t dim, int32_t dtype);
+int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -216,6 +216,32 @@ class DropoutArgs(ctypes.Structure):
                 ("residual", c_void_p), ("residual_stride", c_int64), ("y", c_void_p), ("y_stride", c_int64)]
 
 
+class Mx8Args(ctypes.Structure):
+    """MsplatMx8Args (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("matrix", c_void_p),
+                ("stride", c_int64), ("data", c_void_p), ("scales", c_void_p)]
+
+
+class RmsNormArgs(ctypes.Structure):
+    """MsplatRmsNormArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("x", c_void_p),
+                ("x_stride", c_int64), ("residual", c_void_p), ("residual_stride", c_int64), ("weight", c_void_p),
+                ("eps", c_float), ("y", c_void_p), ("y_stride", c_int64), ("y_scales", c_void_p), ("total", c_void_p),
+                ("total_stride", c_int64), ("rstd", c_void_p)]
+
+
+class RmsNormGradArgs(ctypes.Structure):
+    """MsplatRmsNormGradArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("dim", c_int32), ("dtype", c_int32), ("dy", c_void_p),
+                ("dy_stride", c_int64), ("dtotal", c_void_p), ("dtotal_stride", c_int64), ("total", c_void_p),
+                ("total_stride", c_int64), ("total_scales", c_void_p), ("weight", c_void_p), ("rstd", c_void_p),
+                ("dx", c_void_p), ("dx_stride", c_int64), ("dweight", c_void_p), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64)]
+
+
 # (name, restype, argtypes) for every symbol declared in include/msplat_hip.h,
 # include/msplat_c_api.h and include/msplat_trainer.h
 SIGNATURES = [
@@ -267,6 +293,11 @@ SIGNATURES = [
     ("msplat_hip_gated_ffn_backward", c_int, [POINTER(GatedFfnGradArgs)]),
     ("msplat_hip_dropout_add", c_int, [POINTER(DropoutArgs)]),
     ("msplat_hip_dropout_add_at", c_int, [POINTER(DropoutArgs), c_void_p]),
+    ("msplat_hip_mx8_pack", c_int, [POINTER(Mx8Args)]),
+    ("msplat_hip_mx8_unpack", c_int, [POINTER(Mx8Args)]),
+    ("msplat_hip_rms_norm", c_int, [POINTER(RmsNormArgs)]),
+    ("msplat_hip_rms_norm_backward_workspace", c_int64, [c_int64, c_int32, c_int32]),
+    ("msplat_hip_rms_norm_backward", c_int, [POINTER(RmsNormGradArgs)]),
     # include/msplat_c_api.h (the reference's C API)
     ("msplat_dataset_create", c_void_p, [c_char_p, c_float, c_bool, c_int]),
     ("msplat_dataset_destroy", None, [c_void_p]),

@@ -595,6 +595,14 @@ int check_workspace(const void* ws, int64_t bytes, size_t need) {
 }
 
 
+// A matrix in 8 bits; only one without rows may be null.
+int check_mx8(const char* name, const void* data, const void* scales, int64_t rows) {
+    if (rows > 0 && (!data || !scales)) return fail(MSPLAT_ERR_ARG, "%s is null", name);
+    if (reinterpret_cast<uintptr_t>(data) % 16 != 0 || reinterpret_cast<uintptr_t>(scales) % 16 != 0)
+        return fail(MSPLAT_ERR_ARG, "%s in 8 bits must be 16-byte aligned", name);
+    return MSPLAT_OK;
+}
+
 int check_ffn_sizes(int64_t rows, int dim, int hidden, int dtype) {
     CHECK(check_rows(rows, dim, FFN_DIM_MAX, dtype));
     if (hidden < 1 || hidden > FFN_HIDDEN_MAX)
@@ -646,6 +654,32 @@ struct ContextDevice {
         if (before >= 0 && before != g_ctx->device) (void)hipSetDevice(before);
     }
 };
+
+int mx8_rows(const MsplatMx8Args* a, void (*launch)(hipStream_t, int, const Mx8Args&)) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, MX8_DIM_MAX, a->dtype));
+    CHECK(check_matrix("matrix", a->matrix, a->rows, a->dim, a->stride, a->dtype));
+    CHECK(check_mx8("the matrix", a->data, a->scales, a->rows));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    Mx8Args m{};
+    m.rows = a->rows;
+    m.dim = a->dim;
+    m.x = m.y = a->matrix;
+    m.x_stride = m.y_stride = a->stride;
+    m.data = static_cast<uint8_t*>(a->data);
+    m.scales = static_cast<uint8_t*>(a->scales);
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch(stream_of(a->stream), a->dtype, m);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+// As many workgroups as either kind of total has.
+size_t rms_workspace(int64_t rows, int dim, int dtype) {
+    return (size_t)std::max(rms_groups(rows, dim, dtype, false), rms_groups(rows, dim, dtype, true)) * dim * 4;
+}
 
 int dropout_add(const MsplatDropoutArgs* a, const uint64_t* offset_at) {
     if (!a) return fail(MSPLAT_ERR_ARG, "null args");
@@ -1507,6 +1541,88 @@ int msplat_hip_dropout_add_at(const MsplatDropoutArgs* a, const uint64_t* offset
     if (!offset) return fail(MSPLAT_ERR_ARG, "offset is null");
     if (reinterpret_cast<uintptr_t>(offset) % 8 != 0) return fail(MSPLAT_ERR_ARG, "offset is not 8-byte aligned");
     return dropout_add(a, offset);
+}
+
+int msplat_hip_mx8_pack(const MsplatMx8Args* a) { return mx8_rows(a, launch_mx8_pack); }
+
+int msplat_hip_mx8_unpack(const MsplatMx8Args* a) { return mx8_rows(a, launch_mx8_unpack); }
+
+int msplat_hip_rms_norm(const MsplatRmsNormArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, NORM_DIM_MAX, a->dtype));
+    CHECK(check_matrix("x", a->x, a->rows, a->dim, a->x_stride, a->dtype));
+    if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->dim, a->residual_stride, a->dtype));
+    if (a->total) CHECK(check_matrix("total", a->total, a->rows, a->dim, a->total_stride, a->dtype));
+    if (a->y_scales) CHECK(check_mx8("y", a->y, a->y_scales, a->rows));
+    else CHECK(check_matrix("y", a->y, a->rows, a->dim, a->y_stride, a->dtype));
+    CHECK(check_vector("weight", a->weight, a->dtype));
+    CHECK(check_vector("rstd", a->rstd, MSPLAT_F32));
+    if (!(a->eps >= 0.f)) return fail(MSPLAT_ERR_ARG, "eps must be at least 0");
+    if (a->total && a->total == a->y) return fail(MSPLAT_ERR_ARG, "y and total are the same matrix");
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    RmsArgs n{};
+    n.rows = a->rows;
+    n.dim = a->dim;
+    n.eps = a->eps;
+    n.x = a->x;
+    n.x_stride = a->x_stride;
+    n.residual = a->residual;
+    n.residual_stride = a->residual_stride;
+    n.weight = a->weight;
+    n.y = a->y;
+    n.y_stride = a->y_stride;
+    n.y_scales = static_cast<uint8_t*>(a->y_scales);
+    n.total = a->total;
+    n.total_stride = a->total_stride;
+    n.rstd = a->rstd;
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch_rms_fwd(stream_of(a->stream), a->dtype, n);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_rms_norm_backward_workspace(int64_t rows, int32_t dim, int32_t dtype) {
+    if (check_rows(rows, dim, NORM_DIM_MAX, dtype) != MSPLAT_OK) return -1;
+    return (int64_t)rms_workspace(rows, dim, dtype);
+}
+
+int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_rows(a->rows, a->dim, NORM_DIM_MAX, a->dtype));
+    CHECK(check_matrix("dy", a->dy, a->rows, a->dim, a->dy_stride, a->dtype));
+    if (a->dtotal) CHECK(check_matrix("dtotal", a->dtotal, a->rows, a->dim, a->dtotal_stride, a->dtype));
+    if (a->total_scales) CHECK(check_mx8("total", a->total, a->total_scales, a->rows));
+    else CHECK(check_matrix("total", a->total, a->rows, a->dim, a->total_stride, a->dtype));
+    if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->dim, a->dx_stride, a->dtype));
+    if (a->rows > 0 && !a->rstd) return fail(MSPLAT_ERR_ARG, "rstd is null");
+    CHECK(check_vector("weight", a->weight, a->dtype));
+    CHECK(check_vector("rstd", a->rstd, MSPLAT_F32));
+    CHECK(check_vector("dweight", a->dweight, a->dtype));
+    if (a->dweight) CHECK(check_workspace(a->workspace, a->workspace_bytes, rms_workspace(a->rows, a->dim, a->dtype)));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (!a->dweight && (!a->dx || a->rows == 0)) return MSPLAT_OK;
+    RmsArgs n{};
+    n.rows = a->rows;
+    n.dim = a->dim;
+    n.dy = a->dy;
+    n.dy_stride = a->dy_stride;
+    n.dtotal = a->dtotal;
+    n.dtotal_stride = a->dtotal_stride;
+    n.x = a->total;
+    n.x_stride = a->total_stride;
+    n.x_scales = static_cast<const uint8_t*>(a->total_scales);
+    n.weight = a->weight;
+    n.rstd = const_cast<float*>(a->rstd);
+    n.dx = a->dx;
+    n.dx_stride = a->dx_stride;
+    n.part = a->dweight ? static_cast<float*>(a->workspace) : nullptr;
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch_rms_bwd(stream_of(a->stream), a->dtype, n, a->dweight);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
 }
 
 }  // extern "C"

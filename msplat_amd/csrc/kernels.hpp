@@ -440,6 +440,36 @@ struct DropArgs {
 };
 void launch_dropout(hipStream_t s, int dtype, const DropArgs& a);
 
+// Rows packed into 8 bits and back (mx8.hip).
+constexpr int MX8_DIM_MAX = 1 << 30;
+struct Mx8Args {
+    int64_t rows;
+    int dim;
+    const void* x;
+    void* y;
+    int64_t x_stride, y_stride;
+    uint8_t *data, *scales;
+};
+void launch_mx8_pack(hipStream_t s, int dtype, const Mx8Args& a);
+void launch_mx8_unpack(hipStream_t s, int dtype, const Mx8Args& a);
+
+// Root-mean-square norm (rms.hip): y = t rstd weight, t = x + residual.
+struct RmsArgs {
+    int64_t rows;
+    int dim;
+    float eps;
+    const void *x, *residual, *weight, *dy, *dtotal;   // backward: x is the sum t; dtotal may be null
+    int64_t x_stride, residual_stride, dy_stride, dtotal_stride, y_stride, total_stride, dx_stride;
+    const uint8_t* x_scales;   // backward: not null where t is in mx8
+    void *y, *total, *dx;      // total and dx may be null
+    uint8_t* y_scales;         // not null where y is in mx8
+    float* rstd;
+    float* part;               // backward: [groups][dim] sums of dy n
+};
+void launch_rms_fwd(hipStream_t s, int dtype, const RmsArgs& a);
+int rms_groups(int64_t rows, int dim, int dtype, bool mx);
+void launch_rms_bwd(hipStream_t s, int dtype, const RmsArgs& a, void* dweight);
+
 // Gated feed-forward block (ffn_*.hip): y = (act(x Wg^T) * (x Wu^T)) Wd^T.
 constexpr int FFN_DIM_MAX = 256;
 constexpr int FFN_HIDDEN_MAX = 1 << 16;

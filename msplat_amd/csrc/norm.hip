@@ -5,63 +5,18 @@
 //   dx = r (g - mean(g) - n mean(g n)),  g = dy w
 //   dw = sum over rows of dy n,  db = sum over rows of dy
 //
-// Bound by HBM: a row is read once, kept in registers and written once.  L
-// lanes share a row, NV pieces of 16 bytes each: the fewest lanes that hold
-// the row (so a wave takes 64 / L rows at once), a whole wave from 64 pieces
-// on and a workgroup of 256 beyond 256 pieces.  The variance is the mean of squared
-// differences, a second pass over registers, so that it does not cancel.
+// Bound by HBM: a row is read once, kept in registers (rows.hpp) and written
+// once.  The variance is the mean of squared differences, a second pass over
+// registers, so that it does not cancel.
 //   forward, 1.09M rows of 64 bf16: 50 us, 5.8 TB/s (a large copy 5.1)
 //   backward, 500k rows of 128 bf16: 71 us, 5.4 TB/s, and 5 us for the sums
 //   backward, 120k rows of 45 f32 (180 bytes, off the 16-byte grid): 15 + 4 us
-#include "nn.hpp"
-
-#include <algorithm>
-#include <type_traits>
+#include "rows.hpp"
 
 namespace msp {
 namespace {
 
-constexpr int THREADS = 256;
-
-// Sum over the L threads of a row: lanes of a wave, or the whole workgroup
-// (L == THREADS; then every thread of the workgroup must call it).
-template <int L>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-    if (L <= 64) return group_sum<L <= 64 ? L : 64>(v);
-    v = group_sum<64>(v);
-    __syncthreads();   // the previous sum has been read
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
-}
-
-// A row's pieces, read ahead while the row before is computed, then settled
-// (read_piece, settle_piece).  Only a row that one lane holds may be less than
-// a piece.
-template <class T, int L, int NV>
-__device__ __forceinline__ void read_row(const void* base, int64_t stride, int64_t row, const NormArgs& a, int lane,
-                                         piece_t<T> (&p)[NV]) {
-    const T* at = static_cast<const T*>(base) + min(row, a.rows - 1) * stride;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int k = (i * L + lane) * E<T>;
-        p[i] = L == 1 && a.dim < E<T> ? load_piece(at, k, a.dim) : read_piece(at, k, a.dim);
-    }
-}
-template <class T, int L, int NV>
-__device__ __forceinline__ void settle_row(int64_t row, const NormArgs& a, int lane, piece_t<T> (&p)[NV]) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int k = (i * L + lane) * E<T>;
-        if (L == 1 && a.dim < E<T>) p[i] = row < a.rows ? p[i] : piece_t<T>{};
-        else p[i] = settle_piece<T>(p[i], k, a.dim, row < a.rows);
-    }
-}
-
-// Rows of at least AHEAD_PIECES are read ahead.  With fewer, a wave has several
-// rows under way at once and the occupancy is worth more: backward over 900k
-// rows of 60 bf16 76 us without, 81 us with; over 40k rows of 1500 215 and 81.
-constexpr int AHEAD_PIECES = 64;
+using namespace rows;
 
 // Workgroups of the backward: each leaves a partial row.  512 left too few
 // reads under way (500k rows of 128 bf16: 105 us, 1024: 71, 2048: 74).
@@ -87,16 +42,16 @@ __global__ __launch_bounds__(THREADS) void k_norm_fwd(NormArgs a) {
     const int64_t step = (int64_t)gridDim.x * RB;
     constexpr bool AHEAD = L * NV >= AHEAD_PIECES;
     piece_t<T> next[NV];
-    if (AHEAD) read_row<T, L, NV>(a.x, a.x_stride, (int64_t)blockIdx.x * RB + sub, a, lane, next);
+    if (AHEAD) read_row<T, L, NV, 1>(a.x, a.x_stride, (int64_t)blockIdx.x * RB + sub, a, lane, next);
     for (int64_t base = (int64_t)blockIdx.x * RB; base < a.rows; base += step) {
         const int64_t row = base + sub;
         const bool live = row < a.rows;
         piece_t<T> p[NV];
-        if (!AHEAD) read_row<T, L, NV>(a.x, a.x_stride, row, a, lane, next);
+        if (!AHEAD) read_row<T, L, NV, 1>(a.x, a.x_stride, row, a, lane, next);
 #pragma unroll
         for (int i = 0; i < NV; ++i) p[i] = next[i];
-        settle_row<T, L, NV>(row, a, lane, p);
-        if (AHEAD) read_row<T, L, NV>(a.x, a.x_stride, row + step, a, lane, next);
+        settle_row<T, L, NV, 1>(row, a, lane, p);
+        if (AHEAD) read_row<T, L, NV, 1>(a.x, a.x_stride, row + step, a, lane, next);
         float v[NV][E<T>];
         float s = 0.f;
 #pragma unroll
@@ -158,27 +113,27 @@ __global__ __launch_bounds__(THREADS) void k_norm_bwd(NormArgs a) {
     constexpr bool AHEAD = L * NV >= AHEAD_PIECES;
     piece_t<T> nx[NV], nd[NV];
     if (AHEAD) {
-        read_row<T, L, NV>(a.x, a.x_stride, (int64_t)blockIdx.x * RB + sub, a, lane, nx);
-        read_row<T, L, NV>(a.dy, a.dy_stride, (int64_t)blockIdx.x * RB + sub, a, lane, nd);
+        read_row<T, L, NV, 1>(a.x, a.x_stride, (int64_t)blockIdx.x * RB + sub, a, lane, nx);
+        read_row<T, L, NV, 1>(a.dy, a.dy_stride, (int64_t)blockIdx.x * RB + sub, a, lane, nd);
     }
     for (int64_t base = (int64_t)blockIdx.x * RB; base < a.rows; base += step) {
         const int64_t row = base + sub;
         const bool live = row < a.rows;
         piece_t<T> px[NV], pd[NV];
         if (!AHEAD) {
-            read_row<T, L, NV>(a.x, a.x_stride, row, a, lane, nx);
-            read_row<T, L, NV>(a.dy, a.dy_stride, row, a, lane, nd);
+            read_row<T, L, NV, 1>(a.x, a.x_stride, row, a, lane, nx);
+            read_row<T, L, NV, 1>(a.dy, a.dy_stride, row, a, lane, nd);
         }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             px[i] = nx[i];
             pd[i] = nd[i];
         }
-        settle_row<T, L, NV>(row, a, lane, px);
-        settle_row<T, L, NV>(row, a, lane, pd);
+        settle_row<T, L, NV, 1>(row, a, lane, px);
+        settle_row<T, L, NV, 1>(row, a, lane, pd);
         if (AHEAD) {
-            read_row<T, L, NV>(a.x, a.x_stride, row + step, a, lane, nx);
-            read_row<T, L, NV>(a.dy, a.dy_stride, row + step, a, lane, nd);
+            read_row<T, L, NV, 1>(a.x, a.x_stride, row + step, a, lane, nx);
+            read_row<T, L, NV, 1>(a.dy, a.dy_stride, row + step, a, lane, nd);
         }
         float n[NV][E<T>], g[NV][E<T>];
         float s1 = 0.f, s2 = 0.f;
@@ -246,37 +201,12 @@ __global__ __launch_bounds__(1024) void k_norm_fold(const float* part, int group
     }
 }
 
-// Calls f with (L, NV) as integral constants for a row of `dim`.
-template <class T, class F>
-void with_shape(int dim, F&& f) {
-    const int c = (dim + E<T> - 1) / E<T>;
-#define SHAPE(l, nv) f(std::integral_constant<int, l>{}, std::integral_constant<int, nv>{})
-    if (c <= 1) SHAPE(1, 1);
-    else if (c <= 2) SHAPE(2, 1);
-    else if (c <= 4) SHAPE(4, 1);
-    else if (c <= 8) SHAPE(8, 1);
-    else if (c <= 16) SHAPE(16, 1);
-    else if (c <= 32) SHAPE(32, 1);
-    else if (c <= 64) SHAPE(64, 1);
-    else if (c <= 128) SHAPE(64, 2);
-    else if (c <= 256) SHAPE(64, 4);
-    else if (c <= 512) SHAPE(256, 2);
-    else if (c <= 1024) SHAPE(256, 4);
-    else if constexpr (sizeof(T) == 4) SHAPE(256, 8);
-#undef SHAPE
-}
-
-int grid_for(int64_t rows, int rows_per_group, int most) {
-    const int64_t g = (rows + rows_per_group - 1) / rows_per_group;
-    return (int)std::min<int64_t>(g, most);
-}
-
 }  // namespace
 
 void launch_norm_fwd(hipStream_t s, int dtype, const NormArgs& a) {
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        with_shape<T>(a.dim, [&](auto l, auto nv) {
+        with_shape<T, 1>(a.dim, [&](auto l, auto nv) {
             k_norm_fwd<T, l(), nv()><<<grid_for(a.rows, THREADS / l(), 4096), THREADS, 0, s>>>(a);
         });
     });
@@ -285,7 +215,7 @@ void launch_norm_fwd(hipStream_t s, int dtype, const NormArgs& a) {
 int norm_groups(int64_t rows, int dim, int dtype) {
     int g = 0;
     with_type(dtype, [&](auto t) {
-        with_shape<decltype(t)>(dim, [&](auto l, auto) { g = grid_for(rows, THREADS / l(), MAX_GROUPS); });
+        with_shape<decltype(t), 1>(dim, [&](auto l, auto) { g = grid_for(rows, THREADS / l(), MAX_GROUPS); });
     });
     return g;
 }
@@ -295,7 +225,7 @@ void launch_norm_bwd(hipStream_t s, int dtype, const NormArgs& a, void* dweight,
     with_type(dtype, [&](auto t) {
         using T = decltype(t);
         if (groups > 0)
-            with_shape<T>(a.dim, [&](auto l, auto nv) { k_norm_bwd<T, l(), nv()><<<groups, THREADS, 0, s>>>(a); });
+            with_shape<T, 1>(a.dim, [&](auto l, auto nv) { k_norm_bwd<T, l(), nv()><<<groups, THREADS, 0, s>>>(a); });
         if (dweight || dbias)
             k_norm_fold<T><<<(2 * a.dim + 31) / 32, 1024, 0, s>>>(a.part, groups, a.dim, static_cast<T*>(dweight),
                                                                   static_cast<T*>(dbias));

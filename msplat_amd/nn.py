@@ -233,6 +233,145 @@ def dropout_add_backward(dy, p: float, seed: int, offset):
     return _dropout(dy, None, p, seed, offset)
 
 
+class Mx8:
+    """Numbers [..., dim] in 8 bits, as mx8_pack and rms_norm_forward write them:
+    the OCP microscaling format MXFP8.  data: e4m3 bytes [..., 32 ceil(dim / 32)],
+    zeros from dim on; scales: a byte for each 32 adjacent columns, 127 + the
+    exponent of a power of two, [..., 4 ceil(dim / 128)]; both contiguous.  dtype:
+    the type that they stand in for."""
+
+    __slots__ = ("data", "scales", "dim", "dtype")
+
+    def __init__(self, data, scales, dim: int, dtype):
+        dim = index(dim)
+        if dtype not in _DTYPES:
+            raise ValueError(f"{dtype} is none of float32, float16, bfloat16")
+        if data.dtype not in (torch.uint8, torch.float8_e4m3fn) or scales.dtype is not torch.uint8:
+            raise ValueError(f"data is {data.dtype} and scales {scales.dtype}, not float8_e4m3fn (or uint8) and uint8")
+        if dim < 1 or data.dim() < 1 or scales.dim() < 1 or scales.shape != (*data.shape[:-1], 4 * -(-dim // 128)) or \
+                data.shape[-1] != 32 * -(-dim // 32):
+            raise ValueError(f"data of shape {tuple(data.shape)} and scales of {tuple(scales.shape)} do not hold "
+                             f"[..., {dim}]")
+        if data.device != scales.device:
+            raise ValueError(f"data is on {data.device}, scales on {scales.device}")
+        self.data, self.scales, self.dim, self.dtype = _aligned(data), _aligned(scales), dim, dtype
+
+    @property
+    def shape(self):
+        return torch.Size((*self.data.shape[:-1], self.dim))
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def get_device(self):
+        return self.data.get_device()
+
+    @property
+    def rows(self) -> int:
+        return self.data.numel() // self.data.shape[-1]
+
+    @staticmethod
+    def _empty(shape, like, dtype):
+        m = object.__new__(Mx8)
+        m.dim, m.dtype = shape[-1], dtype
+        m.data = torch.empty((*shape[:-1], 32 * -(-m.dim // 32)), dtype=torch.float8_e4m3fn, device=like.device)
+        m.scales = torch.empty((*shape[:-1], 4 * -(-m.dim // 128)), dtype=torch.uint8, device=like.device)
+        return m
+
+
+def _aligned(t):
+    """t contiguous from a 16-byte boundary on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _mx8_rows(lib, call, matrix, dim, m, like):
+    a = _abi.Mx8Args(_stream(like), matrix.shape[0], dim, _dtype(matrix), matrix.data_ptr(), matrix.stride(0),
+                     m.data.data_ptr(), m.scales.data_ptr())
+    _abi.check(call(ctypes.byref(a)))
+
+
+def mx8_pack(x) -> Mx8:
+    """x in 8 bits: each 32 adjacent columns share a power of two, and a number is
+    kept to within 1/16 of itself, or 2^-18 of its block's largest where that is
+    more.  Infinities and NaN become NaN; float16 beyond 61440 (the others beyond
+    3.19e38) count as that."""
+    lib, _ = _library(x), _dtype(x)
+    x2 = _feature_rows("x", x)
+    m = Mx8._empty(x.shape, x, x.dtype)
+    _mx8_rows(lib, lib.msplat_hip_mx8_pack, x2, x2.shape[1], m, x)
+    return m
+
+
+def mx8_unpack(m: Mx8, dtype=None):
+    """The numbers that m holds, in its own type or `dtype` (exact but where the
+    type is float16 and they pass its range)."""
+    lib, dtype = _library(m), dtype or m.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"{dtype} is none of float32, float16, bfloat16")
+    y = torch.empty(m.shape, dtype=dtype, device=m.device)
+    _mx8_rows(lib, lib.msplat_hip_mx8_unpack, y.view(-1, m.dim) if y.numel() else y.new_empty(0, m.dim), m.dim, m, y)
+    return y
+
+
+def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5, mx8: bool = False):
+    """(y, total, rstd): total = x + residual of x's type (x itself without a
+    residual), y = total rstd weight over the last axis, rstd = 1 / sqrt(mean(total^2)
+    + eps), one float32 a row.  mx8: y is an Mx8, rounded to 8 bits once."""
+    lib, dtype = _library(x), _dtype(x)
+    x2 = _feature_rows("x", x)
+    rows, dim = x2.shape
+    r2 = None if residual is None else _same_rows("residual", residual, x2)
+    w = None if weight is None else _matrix("weight", weight, (dim,), x)
+    y = Mx8._empty(x.shape, x, x.dtype) if mx8 else x.new_empty(x.shape)
+    total = x if residual is None else x.new_empty(x.shape)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    a = _abi.RmsNormArgs(_stream(x), rows, dim, dtype, x2.data_ptr(), x2.stride(0), _ptr(r2),
+                         0 if r2 is None else r2.stride(0), _ptr(w), eps, (y.data if mx8 else y).data_ptr(), dim,
+                         y.scales.data_ptr() if mx8 else None, None if residual is None else total.data_ptr(), dim,
+                         rstd.data_ptr())
+    _abi.check(lib.msplat_hip_rms_norm(ctypes.byref(a)))
+    return y, total, rstd
+
+
+def rms_norm_backward(dy, total, weight, rstd, dtotal=None, wanted=(True, True)):
+    """(dx, dweight) from the gradients of y and (where not None) of total, and the
+    forward's total, a tensor or an Mx8 of it, and rstd.  dx is the gradient of x
+    and of residual alike; dweight has dy's type, also where weight is None.
+    Those not wanted are None and not computed."""
+    lib, dtype = _library(dy), _dtype(dy)
+    dy2 = _feature_rows("dy", dy)
+    rows, dim = dy2.shape
+    kept = isinstance(total, Mx8)
+    if kept:
+        t2 = _same_mx8("total", total, dy2)
+    else:
+        t2 = _same_rows("total", total, dy2)
+    g2 = None if dtotal is None else _same_rows("dtotal", dtotal, dy2)
+    w = None if weight is None else _matrix("weight", weight, (dim,), dy)
+    if rstd.dtype is not torch.float32 or rstd.numel() != rows or rstd.device != dy.device:
+        raise ValueError(f"rstd must hold one float32 a row on {dy.device}")
+    rstd = rstd.contiguous()
+    dx = dy.new_empty(dy.shape) if wanted[0] else None
+    dweight = dy.new_empty(dim) if wanted[1] else None
+    ws = _workspace(lib.msplat_hip_rms_norm_backward_workspace(rows, dim, dtype), dy) if wanted[1] else None
+    a = _abi.RmsNormGradArgs(_stream(dy), rows, dim, dtype, dy2.data_ptr(), dy2.stride(0), _ptr(g2),
+                             0 if g2 is None else g2.stride(0), (t2.data if kept else t2).data_ptr(),
+                             0 if kept else t2.stride(0), t2.scales.data_ptr() if kept else None, _ptr(w),
+                             rstd.data_ptr(), _ptr(dx), dim, _ptr(dweight), _ptr(ws), 0 if ws is None else ws.nbytes)
+    _abi.check(lib.msplat_hip_rms_norm_backward(ctypes.byref(a)))
+    return dx, dweight
+
+
+def _same_mx8(name, m, x2):
+    if m.dim != x2.shape[1] or m.rows != x2.shape[0]:
+        raise ValueError(f"{name} has shape {tuple(m.shape)}, not {x2.shape[0]} rows of {x2.shape[1]}")
+    if m.device != x2.device or m.dtype is not x2.dtype:
+        raise ValueError(f"{name} stands for {m.dtype} on {m.device}, not {x2.dtype} on {x2.device}")
+    return m
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -277,6 +416,60 @@ class _DropoutAdd(torch.autograd.Function):
         need = ctx.needs_input_grad
         dx = dropout_add_backward(dy, *ctx.args, *ctx.saved_tensors) if need[0] else None
         return dx, dy if need[1] else None, None, None, None
+
+
+_CHECKPOINTS = (None, "mx8")
+
+
+def _check_checkpoint(checkpoint):
+    if checkpoint not in _CHECKPOINTS:
+        raise ValueError(f"checkpoint {checkpoint!r} is none of {_CHECKPOINTS}")
+
+
+def _keep(ctx, checkpoint, kept, *others):
+    """Saves tensors for the backward, those in `kept` (each may be None) as
+    Mx8 where the checkpoint says so."""
+    packed = [None if t is None else mx8_pack(t) for t in kept] if checkpoint else list(kept)
+    ctx.kept = [None if m is None else (m.dim, m.dtype) for m in packed] if checkpoint else None
+    flat = [t for m in packed for t in ((None, None) if m is None else (m.data, m.scales))] if checkpoint else packed
+    ctx.save_for_backward(*flat, *others)
+
+
+def _kept(ctx, n):
+    """What _keep took: the n that it kept, and the others."""
+    saved = ctx.saved_tensors
+    if ctx.kept is None:
+        return list(saved)
+    pairs = [None if k is None else Mx8(saved[2 * i], saved[2 * i + 1], *k) for i, k in enumerate(ctx.kept)]
+    return [*pairs, *saved[2 * n:]]
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, checkpoint):
+        ctx.set_materialize_grads(False)
+        y, total, rstd = rms_norm_forward(x, weight, residual, eps)
+        _keep(ctx, checkpoint, (total,), weight, rstd)
+        return y if residual is None else (y, total)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dtotal=None):
+        total, weight, rstd = _kept(ctx, 1)
+        need = ctx.needs_input_grad
+        along = need[0] or need[2]
+        if dy is None:   # y was not used
+            dweight = None if weight is None or not need[1] else torch.zeros_like(weight)
+            return dtotal if need[0] else None, dweight, dtotal if need[2] else None, None, None
+        dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
+        return dx if need[0] else None, dweight, dx if need[2] else None, None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
+    """rms_norm_forward's y, and with a residual (y, total), differentiable in x,
+    weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits."""
+    _check_checkpoint(checkpoint)
+    return _RmsNorm.apply(x, weight, residual, eps, checkpoint)
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
