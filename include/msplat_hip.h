@@ -546,6 +546,79 @@ typedef struct MsplatRmsNormGradArgs {
 int64_t msplat_hip_rms_norm_backward_workspace(int64_t rows, int32_t dim, int32_t dtype);
 int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* args);
 
+/* y = residual + a(x weight^T + bias), x [rows, inner], weight [outer, inner],
+ * bias [outer] and residual [rows, outer] NULL for none; 1 <= inner, outer <=
+ * 65536.  activation a: MSPLAT_SILU, MSPLAT_GELU (tanh form) or MSPLAT_IDENTITY.
+ * dtype is that of x, weight, bias and z, or MSPLAT_MX8: x and weight in 8 bits
+ * (x and weight their data, x_scales and weight_scales), bias fp32.  y_dtype is
+ * that of y and residual, any of the three.  z takes x weight^T + bias, rounded to
+ * dtype, where not NULL (not with MSPLAT_MX8); the backward pass takes it.  y may be
+ * exactly residual with the same stride. */
+#define MSPLAT_IDENTITY 2
+#define MSPLAT_MX8 3
+typedef struct MsplatLinearArgs {
+    void* stream;
+    int64_t rows;
+    int32_t inner;
+    int32_t outer;
+    int32_t dtype;
+    int32_t y_dtype;
+    int32_t activation;
+    const void* x;
+    int64_t x_stride;
+    const void* x_scales;
+    const void* weight;
+    int64_t weight_stride;
+    const void* weight_scales;
+    const void* bias;
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+    void* z;
+    int64_t z_stride;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatLinearArgs;
+int64_t msplat_hip_linear_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype);
+int msplat_hip_linear(const MsplatLinearArgs* args);
+
+/* Gradients of the linear layer from dy (of y_dtype), x, weight and, unless the
+ * activation is MSPLAT_IDENTITY, z: dx [rows, inner], dweight [outer, inner]
+ * contiguous and dbias [outer], each written where not NULL; residual's gradient is dy.
+ * x_scales, z_scales not NULL: x, z are in 8 bits (x, z their data, the strides
+ * unused).  In 16-bit types dz = dy a'(z) is rounded to the type for the products (in
+ * float16 it loses bits below 6e-5 and vanishes below 3e-8).  The sums over
+ * rows have a fixed order. */
+typedef struct MsplatLinearGradArgs {
+    void* stream;
+    int64_t rows;
+    int32_t inner;
+    int32_t outer;
+    int32_t dtype;
+    int32_t y_dtype;
+    int32_t activation;
+    const void* dy;
+    int64_t dy_stride;
+    const void* x;
+    int64_t x_stride;
+    const void* x_scales;
+    const void* weight;
+    int64_t weight_stride;
+    const void* z;
+    int64_t z_stride;
+    const void* z_scales;
+    void* dx;
+    int64_t dx_stride;
+    void* dweight;
+    void* dbias;
+    void* workspace;
+    int64_t workspace_bytes;
+} MsplatLinearGradArgs;
+int64_t msplat_hip_linear_backward_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype, int32_t y_dtype,
+                                             int32_t activation);
+int msplat_hip_linear_backward(const MsplatLinearGradArgs* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -242,6 +242,27 @@ class RmsNormGradArgs(ctypes.Structure):
                 ("workspace_bytes", c_int64)]
 
 
+class LinearArgs(ctypes.Structure):
+    """MsplatLinearArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("inner", c_int32), ("outer", c_int32), ("dtype", c_int32),
+                ("y_dtype", c_int32), ("activation", c_int32), ("x", c_void_p), ("x_stride", c_int64),
+                ("x_scales", c_void_p), ("weight", c_void_p), ("weight_stride", c_int64), ("weight_scales", c_void_p),
+                ("bias", c_void_p), ("residual", c_void_p), ("residual_stride", c_int64), ("y", c_void_p),
+                ("y_stride", c_int64), ("z", c_void_p), ("z_stride", c_int64), ("workspace", c_void_p),
+                ("workspace_bytes", c_int64)]
+
+
+class LinearGradArgs(ctypes.Structure):
+    """MsplatLinearGradArgs (include/msplat_hip.h)."""
+
+    _fields_ = [("stream", c_void_p), ("rows", c_int64), ("inner", c_int32), ("outer", c_int32), ("dtype", c_int32),
+                ("y_dtype", c_int32), ("activation", c_int32), ("dy", c_void_p), ("dy_stride", c_int64), ("x", c_void_p),
+                ("x_stride", c_int64), ("x_scales", c_void_p), ("weight", c_void_p), ("weight_stride", c_int64),
+                ("z", c_void_p), ("z_stride", c_int64), ("z_scales", c_void_p), ("dx", c_void_p), ("dx_stride", c_int64),
+                ("dweight", c_void_p), ("dbias", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64)]
+
+
 # (name, restype, argtypes) for every symbol declared in include/msplat_hip.h,
 # include/msplat_c_api.h and include/msplat_trainer.h
 SIGNATURES = [
@@ -298,6 +319,10 @@ SIGNATURES = [
     ("msplat_hip_rms_norm", c_int, [POINTER(RmsNormArgs)]),
     ("msplat_hip_rms_norm_backward_workspace", c_int64, [c_int64, c_int32, c_int32]),
     ("msplat_hip_rms_norm_backward", c_int, [POINTER(RmsNormGradArgs)]),
+    ("msplat_hip_linear_workspace", c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    ("msplat_hip_linear", c_int, [POINTER(LinearArgs)]),
+    ("msplat_hip_linear_backward_workspace", c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    ("msplat_hip_linear_backward", c_int, [POINTER(LinearGradArgs)]),
     # include/msplat_c_api.h (the reference's C API)
     ("msplat_dataset_create", c_void_p, [c_char_p, c_float, c_bool, c_int]),
     ("msplat_dataset_destroy", None, [c_void_p]),

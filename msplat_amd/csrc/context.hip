@@ -637,6 +637,16 @@ int check_ffn(const A* a, FfnArgs& f) {
     return MSPLAT_OK;
 }
 
+int check_linear(int64_t rows, int inner, int outer, int dtype, int y_dtype, int act) {
+    CHECK(check_rows(rows, inner, LINEAR_DIM_MAX, dtype));
+    if (outer < 1 || outer > LINEAR_DIM_MAX) return fail(MSPLAT_ERR_ARG, "outer %d outside [1, %d]", outer, LINEAR_DIM_MAX);
+    if (y_dtype != MSPLAT_F32 && y_dtype != MSPLAT_F16 && y_dtype != MSPLAT_BF16)
+        return fail(MSPLAT_ERR_ARG, "unknown y_dtype %d", y_dtype);
+    if (act != MSPLAT_SILU && act != MSPLAT_GELU && act != MSPLAT_IDENTITY)
+        return fail(MSPLAT_ERR_ARG, "unknown activation %d", act);
+    return MSPLAT_OK;
+}
+
 hipStream_t stream_of(void* s) {
     if (s == MSPLAT_DEFAULT_STREAM) return nullptr;
     return s ? reinterpret_cast<hipStream_t>(s) : g_ctx->stream;
@@ -1621,6 +1631,115 @@ int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* a) {
     ContextDevice on;
     HIP_TRY(on.error);
     launch_rms_bwd(stream_of(a->stream), a->dtype, n, a->dweight);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_linear_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype) {
+    if (check_linear(rows, inner, outer, dtype == MSPLAT_MX8 ? MSPLAT_BF16 : dtype, MSPLAT_F32, MSPLAT_IDENTITY) != MSPLAT_OK)
+        return -1;
+    return (int64_t)linear_workspace(dtype == MSPLAT_MX8 ? MSPLAT_BF16 : dtype, dtype == MSPLAT_MX8, rows, inner, outer);
+}
+
+int msplat_hip_linear(const MsplatLinearArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    const bool mx = a->dtype == MSPLAT_MX8;
+    const int dtype = mx ? MSPLAT_BF16 : a->dtype;
+    CHECK(check_linear(a->rows, a->inner, a->outer, dtype, a->y_dtype, a->activation));
+    if (mx) {
+        CHECK(check_mx8("x", a->x, a->x_scales, a->rows));
+        CHECK(check_mx8("weight", a->weight, a->weight_scales, a->outer));
+        CHECK(check_vector("bias", a->bias, MSPLAT_F32));
+        if (a->z) return fail(MSPLAT_ERR_ARG, "z is not kept of a product of 8 bits");
+    } else {
+        CHECK(check_matrix("x", a->x, a->rows, a->inner, a->x_stride, dtype));
+        CHECK(check_matrix("weight", a->weight, a->outer, a->inner, a->weight_stride, dtype));
+        CHECK(check_vector("bias", a->bias, dtype));
+        if (a->x_scales || a->weight_scales) return fail(MSPLAT_ERR_ARG, "scales without MSPLAT_MX8");
+        if (a->z) CHECK(check_matrix("z", a->z, a->rows, a->outer, a->z_stride, dtype));
+    }
+    if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->outer, a->residual_stride, a->y_dtype));
+    CHECK(check_matrix("y", a->y, a->rows, a->outer, a->y_stride, a->y_dtype));
+    if (a->z && a->z == a->y) return fail(MSPLAT_ERR_ARG, "y and z are the same matrix");
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(dtype, mx, a->rows, a->inner, a->outer)));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (a->rows == 0) return MSPLAT_OK;
+    LinearArgs l{};
+    l.rows = a->rows;
+    l.inner = a->inner;
+    l.outer = a->outer;
+    l.act = a->activation;
+    l.y_dtype = a->y_dtype;
+    l.x = a->x;
+    l.x_stride = a->x_stride;
+    l.x_scales = static_cast<const uint8_t*>(a->x_scales);
+    l.w = a->weight;
+    l.w_stride = a->weight_stride;
+    l.w_scales = static_cast<const uint8_t*>(a->weight_scales);
+    l.bias = a->bias;
+    l.residual = a->residual;
+    l.residual_stride = a->residual_stride;
+    l.y = a->y;
+    l.y_stride = a->y_stride;
+    l.z = a->z;
+    l.z_stride = a->z_stride;
+    l.ws = static_cast<char*>(a->workspace);
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch_linear_fwd(stream_of(a->stream), dtype, l);
+    HIP_TRY(hipGetLastError());
+    return MSPLAT_OK;
+}
+
+int64_t msplat_hip_linear_backward_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype, int32_t y_dtype,
+                                             int32_t activation) {
+    if (check_linear(rows, inner, outer, dtype, y_dtype, activation) != MSPLAT_OK) return -1;
+    return (int64_t)linear_grad_workspace(dtype, rows, inner, outer, activation != MSPLAT_IDENTITY || y_dtype != dtype);
+}
+
+int msplat_hip_linear_backward(const MsplatLinearGradArgs* a) {
+    if (!a) return fail(MSPLAT_ERR_ARG, "null args");
+    CHECK(check_linear(a->rows, a->inner, a->outer, a->dtype, a->y_dtype, a->activation));
+    CHECK(check_matrix("dy", a->dy, a->rows, a->outer, a->dy_stride, a->y_dtype));
+    if (a->x_scales) CHECK(check_mx8("x", a->x, a->x_scales, a->rows));
+    else CHECK(check_matrix("x", a->x, a->rows, a->inner, a->x_stride, a->dtype));
+    CHECK(check_matrix("weight", a->weight, a->outer, a->inner, a->weight_stride, a->dtype));
+    if (a->activation != MSPLAT_IDENTITY) {
+        if (a->z_scales) CHECK(check_mx8("z", a->z, a->z_scales, a->rows));
+        else CHECK(check_matrix("z", a->z, a->rows, a->outer, a->z_stride, a->dtype));
+    }
+    if (a->dx) CHECK(check_matrix("dx", a->dx, a->rows, a->inner, a->dx_stride, a->dtype));
+    CHECK(check_vector("dweight", a->dweight, a->dtype));
+    CHECK(check_vector("dbias", a->dbias, a->dtype));
+    LinearGradArgs l{};
+    l.rows = a->rows;
+    l.inner = a->inner;
+    l.outer = a->outer;
+    l.act = a->activation;
+    l.dtype = a->dtype;
+    l.y_dtype = a->y_dtype;
+    CHECK(check_workspace(a->workspace, a->workspace_bytes,
+                          linear_grad_workspace(a->dtype, a->rows, a->inner, a->outer, l.own_dz())));
+    if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
+    if (!a->dweight && !a->dbias && (!a->dx || a->rows == 0)) return MSPLAT_OK;
+    l.dy = a->dy;
+    l.dy_stride = a->dy_stride;
+    l.x = a->x;
+    l.x_stride = a->x_stride;
+    l.x_scales = static_cast<const uint8_t*>(a->x_scales);
+    l.w = a->weight;
+    l.w_stride = a->weight_stride;
+    l.z = a->z;
+    l.z_stride = a->z_stride;
+    l.z_scales = static_cast<const uint8_t*>(a->z_scales);
+    l.dx = a->dx;
+    l.dx_stride = a->dx_stride;
+    l.dweight = a->dweight;
+    l.dbias = a->dbias;
+    l.ws = static_cast<char*>(a->workspace);
+    ContextDevice on;
+    HIP_TRY(on.error);
+    launch_linear_bwd(stream_of(a->stream), l);
     HIP_TRY(hipGetLastError());
     return MSPLAT_OK;
 }

@@ -470,6 +470,36 @@ void launch_rms_fwd(hipStream_t s, int dtype, const RmsArgs& a);
 int rms_groups(int64_t rows, int dim, int dtype, bool mx);
 void launch_rms_bwd(hipStream_t s, int dtype, const RmsArgs& a, void* dweight);
 
+// Linear layer (linear_*.hip): y = residual + act(x W^T + bias).
+constexpr int LINEAR_DIM_MAX = 1 << 16;
+constexpr int LINEAR_SILU = 0, LINEAR_GELU = 1, LINEAR_NONE = 2;
+struct LinearArgs {
+    int64_t rows;
+    int inner, outer;   // columns of x, of y
+    int act, y_dtype;
+    const void *x, *w, *bias, *residual;          // bias and residual may be null
+    const uint8_t *x_scales, *w_scales;           // not null where x and w are in mx8
+    int64_t x_stride, w_stride, residual_stride, y_stride, z_stride;
+    void *y, *z;                                  // z = x W^T + bias, may be null
+    char* ws;
+};
+size_t linear_workspace(int dtype, bool mx, int64_t rows, int inner, int outer);
+void launch_linear_fwd(hipStream_t s, int dtype, const LinearArgs& a);
+struct LinearGradArgs {
+    int64_t rows;
+    int inner, outer;
+    int act, dtype, y_dtype;
+    const void *dy, *x, *w, *z;
+    const uint8_t *x_scales, *z_scales;           // not null where x, z are in mx8
+    int64_t dy_stride, x_stride, w_stride, z_stride, dx_stride;
+    void *dx, *dweight, *dbias;                   // each may be null
+    char* ws;
+    // dy is not the gradient of x W^T + bias as the products take it
+    bool own_dz() const { return act != LINEAR_NONE || y_dtype != dtype; }
+};
+size_t linear_grad_workspace(int dtype, int64_t rows, int inner, int outer, bool own_dz);
+void launch_linear_bwd(hipStream_t s, const LinearGradArgs& a);
+
 // Gated feed-forward block (ffn_*.hip): y = (act(x Wg^T) * (x Wu^T)) Wd^T.
 constexpr int FFN_DIM_MAX = 256;
 constexpr int FFN_HIDDEN_MAX = 1 << 16;

@@ -1,0 +1,38 @@
+// linear.hip — the linear layer's launches by operand type.
+#include "linear.hpp"
+
+namespace msp {
+
+template <>
+void linear_forward<float, false>(hipStream_t, const LinearArgs&);
+template <>
+void linear_forward<_Float16, false>(hipStream_t, const LinearArgs&);
+template <>
+void linear_forward<__bf16, false>(hipStream_t, const LinearArgs&);
+template <>
+void linear_forward<__bf16, true>(hipStream_t, const LinearArgs&);
+template <>
+void linear_backward<float>(hipStream_t, const LinearGradArgs&);
+template <>
+void linear_backward<_Float16>(hipStream_t, const LinearGradArgs&);
+template <>
+void linear_backward<__bf16>(hipStream_t, const LinearGradArgs&);
+
+void launch_linear_fwd(hipStream_t s, int dtype, const LinearArgs& a) {
+    if (a.x_scales) return linear_forward<__bf16, true>(s, a);
+    with_type(dtype, [&](auto t) { linear_forward<decltype(t), false>(s, a); });
+}
+
+size_t linear_workspace(int, bool, int64_t, int, int) { return 0; }
+
+size_t linear_grad_workspace(int dtype, int64_t rows, int inner, int outer, bool own_dz) {
+    size_t n = 0;
+    with_type(dtype, [&](auto t) { n = (size_t)linear::plan<decltype(t)>(rows, inner, outer, own_dz).bytes(); });
+    return n;
+}
+
+void launch_linear_bwd(hipStream_t s, const LinearGradArgs& a) {
+    with_type(a.dtype, [&](auto t) { linear_backward<decltype(t)>(s, a); });
+}
+
+}  // namespace msp

@@ -1,0 +1,482 @@
+// linear.hpp — the linear layer, forward and backward:
+//
+//   z = x W^T + b    y = residual + a(z)    a: identity, SiLU, GELU (tanh form)
+//   dz = dy a'(z)    dx = dz W    dW = dz^T x    db = sum over rows of dz
+//
+// Products run on 16x16 matrix instructions with 32-bit sums, fragments as
+// ffn.hpp lays them out: lane (q, r) has elements q E .. q E + E - 1 of row r in
+// a block of KB indices.  A wave takes 32 columns of the result (outputs) as two
+// tiles, tile s with
+//
+//   column(s, r) = (r / 4) 8 + 4 s + r % 4
+//
+// as its row r, so that the result leaves in each lane eight adjacent columns of
+// one row: a 16-byte piece or two to add bias and residual to and to store.
+//
+// x and W in mx8 become bfloat16 fragments, which hold e4m3 times a power of two
+// exactly (down to 2^-126; smaller counts as 0).  gfx950's scaled instruction,
+// which takes 8 bits as they are, drops bits of small products: a sum of 128 was
+// up to 1.5e-4 of its terms' magnitudes off, where 32-bit sums stay within 6e-8.
+// The layer is bound by memory at the widths it is used at, so that the rate of
+// twice as many operations would not show.
+#pragma once
+
+#include "ffn.hpp"
+#include "mx8.hpp"
+
+namespace msp {
+namespace linear {
+
+using ffn::ceil_div;
+using ffn::KB;
+using ffn::mma;
+
+constexpr int COLS = 32;   // columns of a wave's step
+
+// What is multiplied: the matrices' own type, bfloat16 for mx8.
+template <class T, bool MX>
+struct Operand {
+    typedef T type;
+};
+template <class T>
+struct Operand<T, true> {
+    typedef __bf16 type;
+};
+
+__device__ __forceinline__ int column(int s, int r) { return (r >> 2) * 8 + 4 * s + (r & 3); }
+
+// Eight values of mx8 as bfloat16.
+__device__ __forceinline__ piece_t<__bf16> from_mx8(const uint32_t (&bytes)[2], int code) {
+    float v[8];
+    mx8::values<__bf16>(bytes, code, v);
+    piece_t<__bf16> o;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
+    return o;
+}
+
+// The piece of lane group q in block kb of a row of x.
+template <class T, bool MX>
+__device__ __forceinline__ piece_t<typename Operand<T, MX>::type> x_piece(const LinearArgs& a, int64_t row, int kb, int q) {
+    if constexpr (MX) {
+        uint32_t bytes[2];
+        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.x) + row * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
+        return from_mx8(bytes, a.x_scales[row * mx8::scale_stride(a.inner) + kb]);
+    } else {
+        return load_piece(static_cast<const T*>(a.x) + row * a.x_stride, kb * KB<T> + q * E<T>, a.inner);
+    }
+}
+
+// The same of a row of W, W^T where TRANS, zero from `outer` rows on.
+template <class T, bool MX, bool TRANS>
+__device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const LinearArgs& a, int row, int kb, int q) {
+    using C = typename Operand<T, MX>::type;
+    const int at = min(row, a.outer - 1);
+    piece_t<C> v;
+    if constexpr (MX) {
+        uint32_t bytes[2];
+        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.w) + at * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
+        v = from_mx8(bytes, a.w_scales[at * mx8::scale_stride(a.inner) + kb]);
+    } else if constexpr (TRANS) {
+        const T* w = static_cast<const T*>(a.w) + at;
+        const int k = kb * KB<T> + q * E<T>;
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j) v[j] = w[min(k + j, a.inner - 1) * a.w_stride];
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j)
+            if (k + j >= a.inner) v[j] = (T)0.f;
+    } else {
+        v = load_piece(static_cast<const T*>(a.w) + at * a.w_stride, kb * KB<T> + q * E<T>, a.inner);
+    }
+    return row < a.outer ? v : piece_t<C>{};
+}
+
+__device__ __forceinline__ float activate(float v, int act) {
+    return act == LINEAR_SILU ? ffn::act<false>(v) : act == LINEAR_GELU ? ffn::act<true>(v) : v;
+}
+
+// a'(v); large GELU arguments as in ffn::act_grad.
+__device__ __forceinline__ float slope(float v, int act) {
+    if (act == LINEAR_SILU) {
+        const float s = ffn::sigmoid_fast(v);
+        return fmaf(v * s, 1.f - s, s);
+    }
+    if (act == LINEAR_GELU) {
+        const float s = ffn::sigmoid_fast(v * fmaf(v * v, ffn::GELU_B, ffn::GELU_A));
+        return fmaf(v * s * (1.f - s), fmaf(fminf(v * v, 1e38f), 3.f * ffn::GELU_B, ffn::GELU_A), s);
+    }
+    return 1.f;
+}
+
+// Eight columns from `col` on of a row, zeros from n on, in 32 bits.
+template <class T>
+__device__ __forceinline__ void load8(const T* row, int col, int n, float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 8 / E<T>; ++h) {
+        piece_t<T> p = {};
+        if (col + h * E<T> < n) p = load_piece(row, col + h * E<T>, n);
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j) v[h * E<T> + j] = (float)p[j];
+    }
+}
+template <class T>
+__device__ __forceinline__ void store8(T* row, int col, int n, const float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 8 / E<T>; ++h) {
+        piece_t<T> p;
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j) p[j] = (T)v[h * E<T> + j];
+        if (col + h * E<T> < n) store_piece(row, col + h * E<T>, n, p);
+    }
+}
+// By a type that is an argument.
+__device__ __forceinline__ void load8(const void* base, int dtype, int64_t stride, int64_t row, int col, int n,
+                                      float (&v)[8]) {
+    if (dtype == 0) load8(static_cast<const float*>(base) + row * stride, col, n, v);
+    else if (dtype == 1) load8(static_cast<const _Float16*>(base) + row * stride, col, n, v);
+    else load8(static_cast<const __bf16*>(base) + row * stride, col, n, v);
+}
+__device__ __forceinline__ void store8(void* base, int dtype, int64_t stride, int64_t row, int col, int n,
+                                       const float (&v)[8]) {
+    if (dtype == 0) store8(static_cast<float*>(base) + row * stride, col, n, v);
+    else if (dtype == 1) store8(static_cast<_Float16*>(base) + row * stride, col, n, v);
+    else store8(static_cast<__bf16*>(base) + row * stride, col, n, v);
+}
+
+// What follows the product: v are the eight columns from col on of row.
+template <class T>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col, const float (&bias)[8], float (&v)[8]) {
+    if (col >= a.outer) return;
+    if (a.bias)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += bias[j];
+    if (a.z) store8(static_cast<T*>(a.z) + row * a.z_stride, col, a.outer, v);
+    if (a.act != LINEAR_NONE)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = activate(v[j], a.act);
+    if (a.residual) {
+        float r[8];
+        load8(a.residual, a.y_dtype, a.residual_stride, row, col, a.outer, r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += r[j];
+    }
+    store8(a.y, a.y_dtype, a.y_stride, row, col, a.outer, v);
+}
+
+// The bias is of x's type, 32-bit beside mx8.
+template <class T, bool MX>
+__device__ __forceinline__ void bias8(const LinearArgs& a, int col, float (&v)[8]) {
+    using B = typename std::conditional<MX, float, T>::type;
+    if (a.bias) load8(static_cast<const B*>(a.bias), col, a.outer, v);
+}
+
+// 16 R rows and 32 columns a workgroup, whose waves share the contraction (wave
+// w takes blocks w, w + WAVES, ...) and join their sums in LDS in a fixed order.
+constexpr int FEW_WAVES = 4;
+template <class T, bool MX, bool TRANS, int R>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
+    using C = typename Operand<T, MX>::type;
+    __shared__ f32x4 part[FEW_WAVES][R][2][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
+    const int blocks = (a.outer + COLS - 1) / COLS, kbs = (a.inner + KB<C> - 1) / KB<C>;
+    const int64_t row0 = (int64_t)(blockIdx.x / blocks) * 16 * R;
+    const int col0 = (int)(blockIdx.x % blocks) * COLS;
+    f32x4 acc[R][2] = {};
+    constexpr int U = 4;   // blocks whose reads are under way at once
+    for (int kb0 = wave; kb0 < kbs; kb0 += U * FEW_WAVES) {
+        piece_t<C> x[U][R] = {}, w[U][2] = {};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = kb0 + u * FEW_WAVES;
+            if (kb >= kbs) break;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) w[u][s] = w_piece<T, MX, TRANS>(a, col0 + column(s, r), kb, q);
+#pragma unroll
+            for (int i = 0; i < R; ++i) x[u][i] = x_piece<T, MX>(a, min(row0 + 16 * i + r, a.rows - 1), kb, q);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) acc[i][s] = mma(w[u][s], x[u][i], acc[i][s]);
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) part[wave][i][s][lane] = acc[i][s];
+    __syncthreads();
+    float bias[8];
+    bias8<T, MX>(a, col0 + q * 8, bias);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        if (i % FEW_WAVES != wave) continue;
+        const int64_t row = row0 + 16 * i + r;
+        float v[8];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            f32x4 t = part[0][i][s][lane];
+#pragma unroll
+            for (int p = 1; p < FEW_WAVES; ++p) t += part[p][i][s][lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * s + j] = t[j];
+        }
+        if (row < a.rows) finish<C>(a, row, col0 + q * 8, bias, v);
+    }
+}
+
+template <class T, bool MX, bool TRANS>
+void product(hipStream_t s, const LinearArgs& a) {
+    constexpr int R = 4;
+    constexpr int64_t size = sizeof(T);
+    const int64_t blocks = ceil_div(a.outer, COLS);
+    // a launch has fewer than 2^32 threads
+    const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
+    for (int64_t at = 0; at < a.rows; at += most) {
+        LinearArgs p = a;
+        p.rows = std::min(most, a.rows - at);
+        p.x = static_cast<const char*>(a.x) + at * (MX ? mx8::data_stride(a.inner) : a.x_stride * size);
+        if (MX) p.x_scales = a.x_scales + at * mx8::scale_stride(a.inner);
+        const int64_t ysize = a.y_dtype == 0 ? 4 : 2;
+        if (a.residual) p.residual = static_cast<const char*>(a.residual) + at * a.residual_stride * ysize;
+        p.y = static_cast<char*>(a.y) + at * a.y_stride * ysize;
+        if (a.z) p.z = static_cast<char*>(a.z) + at * a.z_stride * size;
+        const int64_t groups = ceil_div(p.rows, 16 * R) * blocks;
+        k_linear_few<T, MX, TRANS, R><<<(unsigned)groups, 64 * FEW_WAVES, 0, s>>>(p);
+    }
+}
+
+// ---------------------------------------------------------------- backward
+
+// dz = dy a'(z) in T, and the sums of its columns over each workgroup's rows.
+// tx threads along a row, eight columns each; 256 / tx rows at once.
+template <class T, bool MX>
+__global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, float* part, int tx, int64_t rows_per_group) {
+    __shared__ float sums[256][8];
+    const int lane = threadIdx.x & (tx - 1), sub = threadIdx.x / tx, rb = 256 / tx;
+    const int64_t first = (int64_t)blockIdx.x * rows_per_group, last = min(first + rows_per_group, a.rows);
+    for (int base = 0; base < a.outer; base += tx * 8) {
+        const int col = base + lane * 8;
+        float sum[8] = {};
+        if (col < a.outer)
+            for (int64_t row = first + sub; row < last; row += rb) {
+                float v[8];
+                load8(a.dy, a.y_dtype, a.dy_stride, row, col, a.outer, v);
+                if (a.act != LINEAR_NONE) {
+                    float z[8];
+                    if constexpr (MX) {
+                        uint32_t bytes[2];
+                        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.z) + row * mx8::data_stride(a.outer) + col, 8);
+                        mx8::values<__bf16>(bytes, a.z_scales[row * mx8::scale_stride(a.outer) + col / 32], z);
+                    } else {
+                        load8(static_cast<const T*>(a.z) + row * a.z_stride, col, a.outer, z);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] *= slope(z[j], a.act);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum[j] += v[j];
+                if (dz) store8(dz + row * a.outer, col, a.outer, v);
+            }
+        if (!part) continue;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[threadIdx.x][j] = sum[j];
+        __syncthreads();
+        for (int c = threadIdx.x; c < tx * 8; c += 256) {
+            if (base + c >= a.outer) continue;
+            float t = 0.f;
+            for (int p = 0; p < rb; ++p) t += sums[p * tx + c / 8][c % 8];
+            part[(int64_t)blockIdx.x * a.outer + base + c] = t;
+        }
+    }
+}
+
+// Adds `groups` partial rows of n: 32 columns a workgroup at once, 32 threads a
+// column.
+template <class T>
+__global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int groups, int64_t n, T* out) {
+    __shared__ float red[32][33];
+    const int sl = threadIdx.x >> 5;
+    for (int64_t at = (int64_t)blockIdx.x * 32; at < n; at += (int64_t)gridDim.x * 32) {
+        const int64_t col = at + (threadIdx.x & 31);
+        float t = 0.f;
+        if (col < n)
+#pragma unroll 8
+            for (int g = sl; g < groups; g += 32) t += part[g * n + col];
+        red[sl][threadIdx.x & 31] = t;
+        __syncthreads();
+        if (sl == 0 && col < n) {
+            t = 0.f;
+            for (int q = 0; q < 32; ++q) t += red[q][threadIdx.x & 31];
+            out[col] = (T)t;
+        }
+        __syncthreads();
+    }
+}
+template <class T>
+void fold(hipStream_t s, const float* part, int groups, int64_t n, void* out) {
+    k_linear_fold<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 32), 1 << 20), 1024, 0, s>>>(part, groups, n, static_cast<T*>(out));
+}
+
+// dW: a workgroup takes TN rows and TK columns of it (outputs and inputs) over a
+// group of x's rows.  A block of KB rows of dz and x goes through LDS in the order
+// of ffn::slot, whose transposing reads give both operands rows x contraction.
+template <class T>
+struct DwTile {
+    static constexpr int NB = 128 / KB<T>, KBS = 128 / KB<T>;   // blocks of outputs and inputs
+    static constexpr int FN = NB * ffn::HT<T>, FK = KBS * ffn::HT<T>;
+};
+template <class T>
+__device__ __forceinline__ int staged(int rho, int c) {   // piece c of row rho of a block of rows
+    // rho = perm(s, r): s = rho % E / 4, r = rho / E * 4 + rho % 4
+    return ffn::slot<T>(c / 4, rho % E<T> / 4, c % 4, rho / E<T> * 4 + rho % 4);
+}
+template <class T, bool MX>
+__global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void* dz, int64_t dz_stride, int ntiles, int ktiles,
+                                                   int64_t blocks_per_group, float* part) {
+    using D = DwTile<T>;
+    constexpr int NP = D::NB * 4, KP = D::KBS * 4;   // pieces of a row
+    __shared__ piece_t<T> ld[KB<T> * NP], lx[KB<T> * KP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
+    const int kt = (int)(blockIdx.x % ktiles), nt = (int)(blockIdx.x / ktiles % ntiles);
+    const int64_t group = blockIdx.x / ktiles / ntiles;
+    const int n0 = nt * 128, k0 = kt * 128;
+    const int wn = wave >> 1, wk = wave & 1;   // waves two by two, a quarter of the tile each
+    constexpr int HN = D::FN / 2, HK = D::FK / 2;
+    f32x4 acc[HN][HK] = {};
+    const int64_t blocks = (a.rows + KB<T> - 1) / KB<T>;
+    const int64_t end = min((group + 1) * blocks_per_group, blocks);
+    for (int64_t b = group * blocks_per_group; b < end; ++b) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < KB<T> * NP; i += 256) {
+            const int rho = i / NP, c = i % NP;
+            const int64_t row = b * KB<T> + rho;
+            piece_t<T> p = {};
+            if (row < a.rows && n0 + c * E<T> < a.outer)
+                p = load_piece(static_cast<const T*>(dz) + row * dz_stride, n0 + c * E<T>, a.outer);
+            ld[staged<T>(rho, c)] = p;
+        }
+        for (int i = threadIdx.x; i < KB<T> * KP; i += 256) {
+            const int rho = i / KP, c = i % KP, k = k0 + c * E<T>;
+            const int64_t row = b * KB<T> + rho;
+            piece_t<T> p = {};
+            if (row < a.rows && k < a.inner) {
+                if constexpr (MX) {
+                    float v[E<T>];
+                    mx8::load<T>(static_cast<const uint8_t*>(a.x) + row * mx8::data_stride(a.inner),
+                                 a.x_scales + row * mx8::scale_stride(a.inner), k, v);
+#pragma unroll
+                    for (int j = 0; j < E<T>; ++j) p[j] = (T)v[j];
+                } else {
+                    p = load_piece(static_cast<const T*>(a.x) + row * a.x_stride, k, a.inner);
+                }
+            }
+            lx[staged<T>(rho, c)] = p;
+        }
+        __syncthreads();
+        piece_t<T> fx[HK];
+#pragma unroll
+        for (int j = 0; j < HK; ++j) fx[j] = ffn::by_dim<T>(lx, wk * HK + j);
+#pragma unroll
+        for (int i = 0; i < HN; ++i) {
+            const piece_t<T> fd = ffn::by_dim<T>(ld, wn * HN + i);
+#pragma unroll
+            for (int j = 0; j < HK; ++j) acc[i][j] = mma(fd, fx[j], acc[i][j]);
+        }
+    }
+    // lane (q, r): dW rows of the fragment's 4 q .., column r
+    float* out = part + group * a.outer * a.inner;
+#pragma unroll
+    for (int i = 0; i < HN; ++i)
+#pragma unroll
+        for (int j = 0; j < HK; ++j) {
+            const int fi = wn * HN + i, fj = wk * HK + j;
+            const int k = k0 + fj / ffn::HT<T> * KB<T> + ffn::perm<T>(fj % ffn::HT<T>, r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = n0 + fi / ffn::HT<T> * KB<T> + ffn::perm<T>(fi % ffn::HT<T>, 4 * q + e);
+                if (n < a.outer && k < a.inner) out[(int64_t)n * a.inner + k] = acc[i][j][e];
+            }
+        }
+}
+
+// How a backward call is split: dz by itself where an activation or another
+// type stands between it and dy, groups of rows for the sums over rows.
+struct Plan {
+    bool own_dz;
+    int64_t dz_bytes;
+    int dz_tx, dz_groups;
+    int64_t dz_rows;
+    int ntiles, ktiles, dw_groups;
+    int64_t dw_blocks;
+    int64_t bytes() const { return dz_bytes + db_bytes + dw_bytes; }
+    int64_t db_bytes, dw_bytes;
+};
+template <class T>
+Plan plan(int64_t rows, int inner, int outer, bool own_dz) {
+    Plan p;
+    p.own_dz = own_dz;
+    p.dz_bytes = own_dz ? (rows * outer * (int64_t)sizeof(T) + 15) / 16 * 16 : 0;
+    p.dz_tx = 1;
+    while (p.dz_tx < 256 && p.dz_tx * 8 < outer) p.dz_tx *= 2;
+    const int64_t at_once = 256 / p.dz_tx;
+    p.dz_rows = std::max(ceil_div(rows, 1024), 4 * at_once);
+    p.dz_groups = (int)ceil_div(rows, p.dz_rows);
+    p.db_bytes = ((int64_t)p.dz_groups * outer * 4 + 15) / 16 * 16;
+    p.ntiles = (int)ceil_div(outer, 128);
+    p.ktiles = (int)ceil_div(inner, 128);
+    const int64_t blocks = ceil_div(rows, KB<T>), most = std::max<int64_t>(1, 512 / ((int64_t)p.ntiles * p.ktiles));
+    p.dw_blocks = std::max(ceil_div(blocks, most), std::min<int64_t>(blocks, 4));
+    p.dw_groups = p.dw_blocks ? (int)ceil_div(blocks, p.dw_blocks) : 0;
+    p.dw_bytes = (int64_t)p.dw_groups * outer * inner * 4;
+    return p;
+}
+
+template <class T>
+void backward(hipStream_t s, const LinearGradArgs& a) {
+    const Plan p = plan<T>(a.rows, a.inner, a.outer, a.own_dz());
+    T* dz = p.own_dz ? reinterpret_cast<T*>(a.ws) : nullptr;
+    float* db_part = reinterpret_cast<float*>(a.ws + p.dz_bytes);
+    float* dw_part = reinterpret_cast<float*>(a.ws + p.dz_bytes + p.db_bytes);
+    if (p.dz_groups > 0 && (dz || a.dbias)) {
+        if (a.z_scales) k_linear_dz<T, true><<<p.dz_groups, 256, 0, s>>>(a, dz, a.dbias ? db_part : nullptr, p.dz_tx, p.dz_rows);
+        else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, dz, a.dbias ? db_part : nullptr, p.dz_tx, p.dz_rows);
+    }
+    if (a.dbias)
+        fold<T>(s, db_part, p.dz_groups, a.outer, a.dbias);
+    const void* left = dz ? dz : a.dy;
+    const int64_t left_stride = dz ? a.outer : a.dy_stride;
+    if (a.dx && a.rows > 0) {
+        LinearArgs d{};
+        d.rows = a.rows;
+        d.inner = a.outer;
+        d.outer = a.inner;
+        d.x = left;
+        d.x_stride = left_stride;
+        d.w = a.w;
+        d.w_stride = a.w_stride;
+        d.act = LINEAR_NONE;
+        d.y = a.dx;
+        d.y_stride = a.dx_stride;
+        d.y_dtype = a.dtype;
+        product<T, false, true>(s, d);
+    }
+    if (!a.dweight) return;
+    if (p.dw_groups > 0) {
+        const unsigned grid = (unsigned)(p.dw_groups * p.ntiles * p.ktiles);
+        if (a.x_scales) k_linear_dw<T, true><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
+        else k_linear_dw<T, false><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
+    }
+    fold<T>(s, dw_part, p.dw_groups, (int64_t)a.outer * a.inner, a.dweight);
+}
+
+}  // namespace linear
+
+// One translation unit per type and direction.
+template <class T, bool MX>
+void linear_forward(hipStream_t s, const LinearArgs& a);
+template <class T>
+void linear_backward(hipStream_t s, const LinearGradArgs& a);
+
+}  // namespace msp

@@ -343,11 +343,11 @@ def rms_norm_backward(dy, total, weight, rstd, dtotal=None, wanted=(True, True))
     lib, dtype = _library(dy), _dtype(dy)
     dy2 = _feature_rows("dy", dy)
     rows, dim = dy2.shape
-    kept = isinstance(total, Mx8)
-    if kept:
-        t2 = _same_mx8("total", total, dy2)
+    if isinstance(total, Mx8):
+        ts = _mx8_operand("total", total, rows, dim, dy)
     else:
         t2 = _same_rows("total", total, dy2)
+        ts = (t2.data_ptr(), t2.stride(0), None)
     g2 = None if dtotal is None else _same_rows("dtotal", dtotal, dy2)
     w = None if weight is None else _matrix("weight", weight, (dim,), dy)
     if rstd.dtype is not torch.float32 or rstd.numel() != rows or rstd.device != dy.device:
@@ -357,19 +357,123 @@ def rms_norm_backward(dy, total, weight, rstd, dtotal=None, wanted=(True, True))
     dweight = dy.new_empty(dim) if wanted[1] else None
     ws = _workspace(lib.msplat_hip_rms_norm_backward_workspace(rows, dim, dtype), dy) if wanted[1] else None
     a = _abi.RmsNormGradArgs(_stream(dy), rows, dim, dtype, dy2.data_ptr(), dy2.stride(0), _ptr(g2),
-                             0 if g2 is None else g2.stride(0), (t2.data if kept else t2).data_ptr(),
-                             0 if kept else t2.stride(0), t2.scales.data_ptr() if kept else None, _ptr(w),
+                             0 if g2 is None else g2.stride(0), *ts, _ptr(w),
                              rstd.data_ptr(), _ptr(dx), dim, _ptr(dweight), _ptr(ws), 0 if ws is None else ws.nbytes)
     _abi.check(lib.msplat_hip_rms_norm_backward(ctypes.byref(a)))
     return dx, dweight
 
 
-def _same_mx8(name, m, x2):
-    if m.dim != x2.shape[1] or m.rows != x2.shape[0]:
-        raise ValueError(f"{name} has shape {tuple(m.shape)}, not {x2.shape[0]} rows of {x2.shape[1]}")
-    if m.device != x2.device or m.dtype is not x2.dtype:
-        raise ValueError(f"{name} stands for {m.dtype} on {m.device}, not {x2.dtype} on {x2.device}")
-    return m
+_LINEAR_ACTIVATIONS = {"silu": 0, "gelu": 1, None: 2}
+_MX8 = 3   # MSPLAT_MX8
+
+
+def _linear_activation(activation) -> int:
+    if activation not in _LINEAR_ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} is none of None, 'silu', 'gelu'")
+    return _LINEAR_ACTIVATIONS[activation]
+
+
+def linear_forward(x, weight, bias=None, residual=None, activation=None, out_dtype=None, keep: bool = False):
+    """residual + a(x weight^T + bias) with a = None (the identity), "silu" or "gelu"
+    (tanh form); weight [outer, inner], bias [outer].  x and weight are of one type, as
+    is bias, or both Mx8 with a float32 bias.  The result and residual have `out_dtype`,
+    x's own where None.  keep: (result, x weight^T + bias in x's type), the latter
+    for the backward."""
+    act = _linear_activation(activation)
+    kept = isinstance(x, Mx8)
+    if kept is not isinstance(weight, Mx8):
+        raise ValueError("x and weight are both Mx8 or neither is")
+    lib, out_dtype = _library(x), out_dtype or x.dtype
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"{out_dtype} is none of float32, float16, bfloat16")
+    if kept:
+        if keep:
+            raise ValueError("a product of Mx8 has no backward to keep anything for")
+        rows, inner, outer, like = x.rows, x.dim, weight.rows, x.data
+        if weight.data.dim() != 2 or weight.dim != inner or weight.device != x.device:
+            raise ValueError(f"weight has shape {tuple(weight.shape)} on {weight.device}, not [outer, {inner}] on {x.device}")
+        dtype, b = _MX8, None if bias is None else _vector("bias", bias, outer, torch.float32, x.device)
+        ops = (x.data.data_ptr(), 0, x.scales.data_ptr(), weight.data.data_ptr(), 0, weight.scales.data_ptr())
+    else:
+        x2, like, dtype = _feature_rows("x", x), x, _dtype(x)
+        rows, inner = x2.shape
+        if weight.dim() != 2:
+            raise ValueError(f"weight has shape {tuple(weight.shape)}, not (outer, {inner})")
+        outer = weight.shape[0]
+        w = _matrix("weight", weight, (outer, inner), x)
+        b = None if bias is None else _matrix("bias", bias, (outer,), x)
+        ops = (x2.data_ptr(), x2.stride(0), None, w.data_ptr(), w.stride(0), None)
+    shape = (*x.shape[:-1], outer)
+    y = like.new_empty(shape, dtype=out_dtype)
+    r2 = None if residual is None else _rows_of("residual", residual, rows, outer, y)
+    z = like.new_empty(shape) if keep else None
+    nbytes = lib.msplat_hip_linear_workspace(rows, inner, outer, dtype)
+    ws = _workspace(nbytes, y) if nbytes else None
+    a = _abi.LinearArgs(_stream(like), rows, inner, outer, dtype, _DTYPES[out_dtype], act, *ops, _ptr(b), _ptr(r2),
+                        0 if r2 is None else r2.stride(0), y.data_ptr(), outer, _ptr(z), outer, _ptr(ws),
+                        0 if ws is None else ws.nbytes)
+    _abi.check(lib.msplat_hip_linear(ctypes.byref(a)))
+    return (y, z) if keep else y
+
+
+def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, True)):
+    """(dx, dweight, dbias) from the gradient of the result, x, weight and, where there
+    is an activation, what the forward kept; x and z may be Mx8 of them.  The
+    gradients have weight's type.  Those not wanted are None and not computed."""
+    act = _linear_activation(activation)
+    lib, dtype = _library(weight), _dtype(weight)
+    if weight.dim() != 2 or min(weight.shape) < 1:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, not (outer, inner)")
+    outer, inner = weight.shape
+    w = _matrix("weight", weight, (outer, inner), weight)
+    if isinstance(x, Mx8):
+        rows = x.rows
+        xs = _mx8_operand("x", x, rows, inner, weight)
+    else:
+        x2 = _rows("x", x, inner, weight)
+        rows, xs = x2.shape[0], (x2.data_ptr(), x2.stride(0), None)
+    dy2 = _rows_of("dy", dy, rows, outer, dy)
+    if dy.device != weight.device:
+        raise ValueError(f"dy is on {dy.device}, not {weight.device}")
+    if activation is None:
+        zs = (None, 0, None)
+    elif isinstance(z, Mx8):
+        zs = _mx8_operand("z", z, rows, outer, weight)
+    elif z is None:
+        raise ValueError("the backward of an activation takes z")
+    else:
+        z2 = _rows_of("z", z, rows, outer, weight)
+        zs = (z2.data_ptr(), z2.stride(0), None)
+    dx = weight.new_empty(x.shape) if wanted[0] else None
+    dweight = weight.new_empty(outer, inner) if wanted[1] else None
+    dbias = weight.new_empty(outer) if wanted[2] else None
+    ws = _workspace(lib.msplat_hip_linear_backward_workspace(rows, inner, outer, dtype, _dtype(dy), act), weight)
+    a = _abi.LinearGradArgs(_stream(weight), rows, inner, outer, dtype, _dtype(dy), act, dy2.data_ptr(), dy2.stride(0), *xs,
+                            w.data_ptr(), w.stride(0), *zs, _ptr(dx), inner, _ptr(dweight), _ptr(dbias), ws.data_ptr(),
+                            ws.nbytes)
+    _abi.check(lib.msplat_hip_linear_backward(ctypes.byref(a)))
+    return dx, dweight, dbias
+
+
+def _vector(name, t, n, dtype, dev):
+    if t.dtype is not dtype or t.device != dev or tuple(t.shape) != (n,):
+        raise ValueError(f"{name} is {t.dtype} of shape {tuple(t.shape)} on {t.device}, not {dtype} of ({n},) on {dev}")
+    return t.contiguous()
+
+
+def _rows_of(name, t, rows, dim, like):
+    t2 = _rows(name, t, dim, like)
+    if t2.shape[0] != rows:
+        raise ValueError(f"{name} has {t2.shape[0]} rows, not {rows}")
+    return t2
+
+
+def _mx8_operand(name, m, rows, dim, like):
+    if m.dim != dim or m.rows != rows:
+        raise ValueError(f"{name} has shape {tuple(m.shape)}, not {rows} rows of {dim}")
+    if m.device != like.device or m.dtype is not like.dtype:
+        raise ValueError(f"{name} stands for {m.dtype} on {m.device}, not {like.dtype} on {like.device}")
+    return m.data.data_ptr(), 0, m.scales.data_ptr()
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -463,6 +567,34 @@ class _RmsNorm(torch.autograd.Function):
             return dtotal if need[0] else None, dweight, dtotal if need[2] else None, None, None
         dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
         return dx if need[0] else None, dweight, dx if need[2] else None, None, None
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation, out_dtype, checkpoint):
+        keep = activation is not None
+        y = linear_forward(x, weight, bias, residual, activation, out_dtype, keep)
+        y, z = y if keep else (y, None)
+        ctx.activation = activation
+        _keep(ctx, checkpoint, (x, z), weight)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, z, weight = _kept(ctx, 2)
+        need = ctx.needs_input_grad
+        grads = None, None, None
+        if any(need[:3]):
+            grads = linear_backward(dy, x, weight, z, ctx.activation, need[:3])
+        return (*grads, dy if need[3] else None, None, None, None)
+
+
+def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
+    """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
+    "mx8" keeps x and x weight^T + bias for the backward in 8 bits."""
+    _check_checkpoint(checkpoint)
+    return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint)
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
