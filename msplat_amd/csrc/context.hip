@@ -1638,7 +1638,7 @@ int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* a) {
 int64_t msplat_hip_linear_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype) {
     if (check_linear(rows, inner, outer, dtype == MSPLAT_MX8 ? MSPLAT_BF16 : dtype, MSPLAT_F32, MSPLAT_IDENTITY) != MSPLAT_OK)
         return -1;
-    return (int64_t)linear_workspace(dtype == MSPLAT_MX8 ? MSPLAT_BF16 : dtype, dtype == MSPLAT_MX8, rows, inner, outer);
+    return (int64_t)linear_workspace(dtype == MSPLAT_MX8 ? MSPLAT_BF16 : dtype, rows, inner, outer);
 }
 
 int msplat_hip_linear(const MsplatLinearArgs* a) {
@@ -1661,7 +1661,7 @@ int msplat_hip_linear(const MsplatLinearArgs* a) {
     if (a->residual) CHECK(check_matrix("residual", a->residual, a->rows, a->outer, a->residual_stride, a->y_dtype));
     CHECK(check_matrix("y", a->y, a->rows, a->outer, a->y_stride, a->y_dtype));
     if (a->z && a->z == a->y) return fail(MSPLAT_ERR_ARG, "y and z are the same matrix");
-    CHECK(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(dtype, mx, a->rows, a->inner, a->outer)));
+    CHECK(check_workspace(a->workspace, a->workspace_bytes, linear_workspace(dtype, a->rows, a->inner, a->outer)));
     if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
     if (a->rows == 0) return MSPLAT_OK;
     LinearArgs l{};

@@ -483,7 +483,7 @@ struct LinearArgs {
     void *y, *z;                                  // z = x W^T + bias, may be null
     char* ws;
 };
-size_t linear_workspace(int dtype, bool mx, int64_t rows, int inner, int outer);
+size_t linear_workspace(int dtype, int64_t rows, int inner, int outer);
 void launch_linear_fwd(hipStream_t s, int dtype, const LinearArgs& a);
 struct LinearGradArgs {
     int64_t rows;

@@ -23,7 +23,11 @@ void launch_linear_fwd(hipStream_t s, int dtype, const LinearArgs& a) {
     with_type(dtype, [&](auto t) { linear_forward<decltype(t), false>(s, a); });
 }
 
-size_t linear_workspace(int, bool, int64_t, int, int) { return 0; }
+size_t linear_workspace(int dtype, int64_t rows, int inner, int outer) {
+    size_t n = 0;
+    with_type(dtype, [&](auto t) { n = (size_t)linear::product_workspace<decltype(t)>(rows, inner, outer); });
+    return n;
+}
 
 size_t linear_grad_workspace(int dtype, int64_t rows, int inner, int outer, bool own_dz) {
     size_t n = 0;

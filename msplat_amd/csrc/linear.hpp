@@ -225,25 +225,308 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
     }
 }
 
+// A piece of x as it is read, and what the products take of it: two steps, so
+// that reads may be under way while something else runs.
+template <class T, bool MX>
+struct XPiece {
+    piece_t<T> v;
+    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
+        const T* at = static_cast<const T*>(a.x) + row * a.x_stride;
+        v = a.inner < E<T> ? load_piece(at, kb * KB<T> + q * E<T>, a.inner)
+                           : read_piece(at, kb * KB<T> + q * E<T>, a.inner);
+    }
+    __device__ __forceinline__ piece_t<T> settled(const LinearArgs& a, int kb, int q) const {
+        return a.inner < E<T> ? v : settle_piece<T>(v, kb * KB<T> + q * E<T>, a.inner, true);
+    }
+};
+template <class T>
+struct XPiece<T, true> {
+    uint32_t bytes[2];
+    int code;
+    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
+        const int64_t ds = mx8::data_stride(a.inner);
+        // a block behind the last is read from it and multiplied by zeros of W
+        kb = min(kb, (int)(ds / 32) - 1);
+        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.x) + row * ds + kb * 32 + q * 8, 8);
+        code = a.x_scales[row * mx8::scale_stride(a.inner) + kb];
+    }
+    __device__ __forceinline__ piece_t<__bf16> settled(const LinearArgs& a, int kb, int) const {
+        return kb * 32 < a.inner ? from_mx8(bytes, code) : piece_t<__bf16>{};
+    }
+};
+
+// Weights in LDS for all of the contraction (DK blocks) and the columns of a
+// slice; 16 waves a CU go through rows, 16 R at a time, without a barrier, and read
+// the next rows' x ahead.  Workgroups of one XCD share an L2: the slices of the same
+// rows run on one.
+template <class T, bool MX, bool TRANS, int DK, int R>
+__global__ __launch_bounds__(1024) void k_linear_all(LinearArgs a, int slices, int slice_blocks) {
+    using C = typename Operand<T, MX>::type;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    piece_t<C>* w = reinterpret_cast<piece_t<C>*>(lds);
+    float* bias = reinterpret_cast<float*>(lds + slice_blocks * 2 * DK * 1024);
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15, waves = blockDim.x >> 6;
+    const int slice = (int)(blockIdx.x / 8 % slices);
+    const int64_t group = blockIdx.x / 8 / slices * 8 + blockIdx.x % 8;
+    const int64_t groups = gridDim.x / slices;
+    const int first = slice * slice_blocks, blocks = min(slice_blocks, (a.outer + COLS - 1) / COLS - first);
+    for (int i = threadIdx.x; i < blocks * 2 * DK * 64; i += blockDim.x) {
+        const int f = i >> 6, kb = f % DK, s = f / DK % 2, cb = f / DK / 2;
+        w[i] = w_piece<T, MX, TRANS>(a, (first + cb) * COLS + column(s, i & 15), kb, (i >> 4) & 3);
+    }
+    if (a.bias)
+        for (int i = threadIdx.x; i < blocks * COLS; i += blockDim.x) {
+            using B = typename std::conditional<MX, float, T>::type;
+            bias[i] = (float)static_cast<const B*>(a.bias)[min(first * COLS + i, a.outer - 1)];
+        }
+    __syncthreads();
+    const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R), step = groups * waves;
+    int64_t t = group * waves + (threadIdx.x >> 6);
+    XPiece<T, MX> next[R][DK];
+    auto read = [&](int64_t tile) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int kb = 0; kb < DK; ++kb) next[i][kb].read(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
+    };
+    read(t);
+    for (; t < tiles; t += step) {
+        piece_t<C> x[R][DK];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int kb = 0; kb < DK; ++kb) x[i][kb] = next[i][kb].settled(a, kb, q);
+        read(t + step);
+        for (int cb = 0; cb < blocks; ++cb) {
+            f32x4 acc[R][2] = {};
+            const piece_t<C>* wb = w + cb * 2 * DK * 64 + lane;
+#pragma unroll
+            for (int kb = 0; kb < DK; ++kb)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const piece_t<C> wf = wb[(s * DK + kb) * 64];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) acc[i][s] = mma(wf, x[i][kb], acc[i][s]);
+                }
+            float b[8];
+            if (a.bias) __builtin_memcpy(b, bias + cb * COLS + q * 8, 32);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int64_t row = t * 16 * R + 16 * i + r;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = acc[i][j / 4][j % 4];
+                if (row < a.rows) finish<C>(a, row, (first + cb) * COLS + q * 8, b, v);
+            }
+        }
+    }
+}
+
+// Fragments of the weights, zero beyond the matrix: for a slice of NB column blocks
+// after the other, block after block of the contraction (kbs of them), the slice's
+// 2 NB tiles.
+template <class T, bool MX, bool TRANS>
+__global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int kbs, piece_t<typename Operand<T, MX>::type>* out,
+                                                     int64_t pieces) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int lane = (int)(i & 63), live = (a.inner + KB<typename Operand<T, MX>::type> - 1) / KB<typename Operand<T, MX>::type>;
+    const int64_t f = i >> 6;
+    const int t = (int)(f % (2 * nb)), kb = (int)(f / (2 * nb) % kbs), slice = (int)(f / (2 * nb) / kbs);
+    const int row = (slice * nb + t / 2) * COLS + column(t % 2, lane & 15);
+    piece_t<typename Operand<T, MX>::type> v = {};
+    if (kb < live) v = w_piece<T, MX, TRANS>(a, row, kb, lane >> 4);
+    out[i] = v;
+}
+
+// Packed weights streamed through two areas of LDS, KC blocks of the contraction at
+// a time; a wave holds the sums of 16 R rows and a slice of NB column blocks, and
+// reads its rows' x for the next step ahead.
+template <class T, bool MX, int NB, int R, int KC>
+__global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece_t<typename Operand<T, MX>::type>* packed,
+                                                       int slices, int steps) {
+    using C = typename Operand<T, MX>::type;
+    constexpr int F = KC * 2 * NB;   // fragments of a step
+    __shared__ piece_t<C> w[2][F * 64];
+    const int lane = threadIdx.x & 63, q = lane >> 4, r = lane & 15, waves = blockDim.x >> 6;
+    const int slice = (int)(blockIdx.x / 8 % slices);
+    const int64_t group = blockIdx.x / 8 / slices * 8 + blockIdx.x % 8;
+    const int64_t row0 = (group * waves + (threadIdx.x >> 6)) * 16 * R;
+    packed += (int64_t)slice * steps * F * 64;
+    XPiece<T, MX> next[R][KC];
+    auto read = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) next[i][c].read(a, min(row0 + 16 * i + r, a.rows - 1), step * KC + c, q);
+    };
+    f32x4 acc[R][2 * NB] = {};
+    ffn::fetch<C>(packed, w[0], F);
+    read(0);
+    for (int step = 0; step < steps; ++step) {
+        ffn::fetched();
+        piece_t<C> x[R][KC];
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int c = 0; c < KC; ++c) x[i][c] = next[i][c].settled(a, step * KC + c, q);
+        if (step + 1 < steps) {
+            ffn::fetch<C>(packed + (int64_t)(step + 1) * F * 64, w[(step + 1) & 1], F);
+            read(step + 1);
+        }
+        const piece_t<C>* at = w[step & 1] + lane;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int f = 0; f < 2 * NB; ++f) {
+                const piece_t<C> wf = at[(c * 2 * NB + f) * 64];
+#pragma unroll
+                for (int i = 0; i < R; ++i) acc[i][f] = mma(wf, x[i][c], acc[i][f]);
+            }
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int col = (slice * NB + b) * COLS + q * 8;
+        float bias[8];
+        bias8<T, MX>(a, col, bias);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const int64_t row = row0 + 16 * i + r;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * b + j / 4][j % 4];
+            if (row < a.rows) finish<C>(a, row, col, bias, v);
+        }
+    }
+}
+
+constexpr int64_t CUS = 256;
+constexpr int64_t LDS_BYTES = 160 * 1024;
+constexpr int ALL_BLOCKS = 8;   // of the contraction, up to which the weights stay in LDS
+
+// How a product is launched, by its sizes.
+struct Shape {
+    int kbs;            // blocks of the contraction
+    int blocks;         // of columns
+    int slices, nb;     // of columns, and blocks of a slice
+    int steps;          // streamed: of KC blocks of the contraction
+    int64_t packed;     // streamed: bytes of the packed weights
+    bool few, all;
+};
+constexpr int KC = 2;
+template <class C>
+Shape shape(int64_t rows, int inner, int outer) {
+    Shape p{};
+    p.kbs = (int)ceil_div(inner, KB<C>);
+    p.blocks = (int)ceil_div(outer, COLS);
+    p.few = rows <= 1024;
+    p.all = !p.few && p.kbs <= ALL_BLOCKS;
+    if (p.all) {
+        const int most = (int)(LDS_BYTES / (p.kbs * 2048 + COLS * 4));
+        p.slices = (int)ceil_div(p.blocks, most);
+        p.nb = (int)ceil_div(p.blocks, p.slices);
+    } else if (!p.few) {
+        const int64_t most = 8;
+        p.slices = (int)ceil_div(p.blocks, most);
+        p.nb = (int)ceil_div(p.blocks, p.slices);
+        p.steps = (int)ceil_div(p.kbs, KC);
+        p.packed = (int64_t)p.slices * p.steps * KC * 2 * p.nb * 1024;
+    }
+    return p;
+}
+
+// Rows from `at` on.
+template <class T, bool MX>
+LinearArgs rows_from(const LinearArgs& a, int64_t at, int64_t rows) {
+    LinearArgs p = a;
+    const int64_t size = sizeof(T), ysize = a.y_dtype == 0 ? 4 : 2;
+    p.rows = rows;
+    p.x = static_cast<const char*>(a.x) + at * (MX ? mx8::data_stride(a.inner) : a.x_stride * size);
+    if (MX) p.x_scales = a.x_scales + at * mx8::scale_stride(a.inner);
+    if (a.residual) p.residual = static_cast<const char*>(a.residual) + at * a.residual_stride * ysize;
+    p.y = static_cast<char*>(a.y) + at * a.y_stride * ysize;
+    if (a.z) p.z = static_cast<char*>(a.z) + at * a.z_stride * size;
+    return p;
+}
+
+template <class T, bool MX, bool TRANS>
+void few_product(hipStream_t s, const LinearArgs& a) {
+    const int64_t blocks = ceil_div(a.outer, COLS);
+    auto launch = [&](auto r) {
+        constexpr int R = r();
+        // a launch has fewer than 2^32 threads
+        const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
+        for (int64_t at = 0; at < a.rows; at += most) {
+            const LinearArgs p = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
+            k_linear_few<T, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES, 0, s>>>(p);
+        }
+    };
+    if (a.rows <= 16) launch(std::integral_constant<int, 1>{});
+    else launch(std::integral_constant<int, 4>{});
+}
+
+template <class T, bool MX, bool TRANS, int DK>
+void all_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
+    constexpr int R = DK <= 4 ? 2 : 1;
+    const int64_t tiles = ceil_div(a.rows, 16 * R), most = std::max<int64_t>(CUS / p.slices / 8, 1) * 8;
+    const int64_t waves = std::min<int64_t>(16, ceil_div(tiles, most));
+    const int64_t groups = std::min(ceil_div(ceil_div(tiles, waves), 8) * 8, most);   // a multiple of 8, as the kernel numbers them
+    const size_t lds = (size_t)p.nb * (2 * DK * 1024 + COLS * 4);
+    k_linear_all<T, MX, TRANS, DK, R><<<(unsigned)(groups * p.slices), (unsigned)(64 * waves), lds, s>>>(a, p.slices, p.nb);
+}
+
+template <class T, bool MX, int NB>
+void stream_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
+    using C = typename Operand<T, MX>::type;
+    const piece_t<C>* packed = reinterpret_cast<const piece_t<C>*>(a.ws);
+    constexpr int R = 2, WAVES = 8;
+    const int64_t most = (int64_t(1) << 22) / p.slices / 8 * 8 * 16 * R * WAVES;   // fewer than 2^32 threads
+    for (int64_t at = 0; at < a.rows; at += most) {
+        const LinearArgs part = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
+        const int64_t groups = ceil_div(ceil_div(part.rows, 16 * R * WAVES), 8) * 8;
+        k_linear_stream<T, MX, NB, R, KC><<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
+    }
+}
+
 template <class T, bool MX, bool TRANS>
 void product(hipStream_t s, const LinearArgs& a) {
-    constexpr int R = 4;
-    constexpr int64_t size = sizeof(T);
-    const int64_t blocks = ceil_div(a.outer, COLS);
-    // a launch has fewer than 2^32 threads
-    const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
-    for (int64_t at = 0; at < a.rows; at += most) {
-        LinearArgs p = a;
-        p.rows = std::min(most, a.rows - at);
-        p.x = static_cast<const char*>(a.x) + at * (MX ? mx8::data_stride(a.inner) : a.x_stride * size);
-        if (MX) p.x_scales = a.x_scales + at * mx8::scale_stride(a.inner);
-        const int64_t ysize = a.y_dtype == 0 ? 4 : 2;
-        if (a.residual) p.residual = static_cast<const char*>(a.residual) + at * a.residual_stride * ysize;
-        p.y = static_cast<char*>(a.y) + at * a.y_stride * ysize;
-        if (a.z) p.z = static_cast<char*>(a.z) + at * a.z_stride * size;
-        const int64_t groups = ceil_div(p.rows, 16 * R) * blocks;
-        k_linear_few<T, MX, TRANS, R><<<(unsigned)groups, 64 * FEW_WAVES, 0, s>>>(p);
+    using C = typename Operand<T, MX>::type;
+    const Shape p = shape<C>(a.rows, a.inner, a.outer);
+    if (p.few) return few_product<T, MX, TRANS>(s, a);
+    if (p.all) {
+        switch (p.kbs) {
+#define BLOCKS(n) case n: return all_product<T, MX, TRANS, n>(s, a, p)
+            BLOCKS(1);
+            BLOCKS(2);
+            BLOCKS(3);
+            BLOCKS(4);
+            BLOCKS(5);
+            BLOCKS(6);
+            BLOCKS(7);
+            BLOCKS(8);
+#undef BLOCKS
+        }
     }
+    const int64_t pieces = p.packed / 16;
+    k_linear_pack<T, MX, TRANS><<<(unsigned)ceil_div(pieces, 256), 256, 0, s>>>(a, p.nb, p.steps * KC,
+                                                                              reinterpret_cast<piece_t<C>*>(a.ws), pieces);
+    switch (p.nb) {
+#define BLOCKS(n) case n: return stream_product<T, MX, n>(s, a, p)
+        BLOCKS(1);
+        BLOCKS(2);
+        BLOCKS(3);
+        BLOCKS(4);
+        BLOCKS(5);
+        BLOCKS(6);
+        BLOCKS(7);
+        BLOCKS(8);
+#undef BLOCKS
+    }
+}
+
+template <class C>
+int64_t product_workspace(int64_t rows, int inner, int outer) {
+    return shape<C>(rows, inner, outer).packed;
 }
 
 // ---------------------------------------------------------------- backward
@@ -410,8 +693,8 @@ struct Plan {
     int64_t dz_rows;
     int ntiles, ktiles, dw_groups;
     int64_t dw_blocks;
-    int64_t bytes() const { return dz_bytes + db_bytes + dw_bytes; }
-    int64_t db_bytes, dw_bytes;
+    int64_t db_bytes, dw_bytes, dx_bytes;
+    int64_t bytes() const { return dz_bytes + db_bytes + dw_bytes + dx_bytes; }
 };
 template <class T>
 Plan plan(int64_t rows, int inner, int outer, bool own_dz) {
@@ -429,7 +712,8 @@ Plan plan(int64_t rows, int inner, int outer, bool own_dz) {
     const int64_t blocks = ceil_div(rows, KB<T>), most = std::max<int64_t>(1, 512 / ((int64_t)p.ntiles * p.ktiles));
     p.dw_blocks = std::max(ceil_div(blocks, most), std::min<int64_t>(blocks, 4));
     p.dw_groups = p.dw_blocks ? (int)ceil_div(blocks, p.dw_blocks) : 0;
-    p.dw_bytes = (int64_t)p.dw_groups * outer * inner * 4;
+    p.dw_bytes = ((int64_t)p.dw_groups * outer * inner * 4 + 15) / 16 * 16;
+    p.dx_bytes = product_workspace<T>(rows, outer, inner);
     return p;
 }
 
@@ -460,6 +744,7 @@ void backward(hipStream_t s, const LinearGradArgs& a) {
         d.y = a.dx;
         d.y_stride = a.dx_stride;
         d.y_dtype = a.dtype;
+        d.ws = a.ws + p.dz_bytes + p.db_bytes + p.dw_bytes;
         product<T, false, true>(s, d);
     }
     if (!a.dweight) return;

@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 import more_oracle as orc  # noqa: E402
-from linear_sizes import SIZES  # noqa: E402
+from linear_sizes import RESIDENT, SIZES, STREAMED  # noqa: E402
 from nn_oracle import within  # noqa: E402
 from test_gpu_nn import DTYPES, IDS, _normal, _strided, nn  # noqa: E402,F401
 
@@ -28,7 +28,7 @@ def _check_forward(got, x, w, b, r, act, out_dtype, what):
     within(got, y, e_y, what)
 
 
-@pytest.mark.parametrize("rows,inner,outer", SIZES)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_forward(nn, dtype, rows, inner, outer):
     x, w, b = _operands(rows, inner, outer, dtype)
@@ -45,7 +45,7 @@ def test_forward(nn, dtype, rows, inner, outer):
     _check_forward(nn.linear_forward(x, w), x, w, None, None, None, dtype, "product alone")
 
 
-@pytest.mark.parametrize("rows,inner,outer", SIZES)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_forward_of_8_bits(nn, dtype, rows, inner, outer):
     """Values of 8 bits multiply exactly, so the bounds are those of 32-bit sums."""
@@ -79,7 +79,7 @@ def _check_backward(nn, dtype, rows, inner, outer, act, mx, out_dtype):
 
 
 @pytest.mark.parametrize("mx", [False, True], ids=["plain", "mx8"])
-@pytest.mark.parametrize("rows,inner,outer", SIZES)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_backward(nn, dtype, rows, inner, outer, mx):
     for i, act in enumerate(ACTS):
