@@ -45,13 +45,18 @@ struct Operand<T, true> {
 
 __device__ __forceinline__ int column(int s, int r) { return (r >> 2) * 8 + 4 * s + (r & 3); }
 
-// Eight values of mx8 as bfloat16.
+// Eight values of mx8 as bfloat16: the conversion multiplies by the scale (a float)
+// in one instruction a pair.
 __device__ __forceinline__ piece_t<__bf16> from_mx8(const uint32_t (&bytes)[2], int code) {
-    float v[8];
-    mx8::values<__bf16>(bytes, code, v);
+    const float s = mx8::scale_of(code);
     piece_t<__bf16> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = (__bf16)v[j];
+    for (int w = 0; w < 2; ++w) {
+        const auto a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)bytes[w], s, false);
+        const auto b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)bytes[w], s, true);
+        __builtin_memcpy((char*)&o + 8 * w, &a, 4);
+        __builtin_memcpy((char*)&o + 8 * w + 4, &b, 4);
+    }
     return o;
 }
 
@@ -67,13 +72,14 @@ __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> x_piece(const 
     }
 }
 
-// The same of a row of W, W^T where TRANS, zero from `outer` rows on.
+// The same of a row of W, W^T where TRANS, zero beyond the matrix.
 template <class T, bool MX, bool TRANS>
 __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const LinearArgs& a, int row, int kb, int q) {
     using C = typename Operand<T, MX>::type;
     const int at = min(row, a.outer - 1);
     piece_t<C> v;
     if constexpr (MX) {
+        if (kb * 32 >= a.inner) return piece_t<C>{};
         uint32_t bytes[2];
         __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.w) + at * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
         v = from_mx8(bytes, a.w_scales[at * mx8::scale_stride(a.inner) + kb]);
@@ -91,8 +97,26 @@ __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const 
     return row < a.outer ? v : piece_t<C>{};
 }
 
-__device__ __forceinline__ float activate(float v, int act) {
-    return act == LINEAR_SILU ? ffn::act<false>(v) : act == LINEAR_GELU ? ffn::act<true>(v) : v;
+// a(v) = v / (1 + 2^p), p = -log2(e) times the sigmoid's argument (ffn::act with one
+// product less).
+template <int ACT>
+__device__ __forceinline__ float activated(float v) {
+    if (ACT == LINEAR_NONE) return v;
+    const float p = ACT == LINEAR_SILU ? v * -ffn::LOG2E
+                                       : v * fmaf(v * v, -ffn::LOG2E * ffn::GELU_B, -ffn::LOG2E * ffn::GELU_A);
+    return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(p));
+}
+// The same by an argument: branches where ACT is ANY.
+constexpr int ANY = -1;
+template <int ACT, int N>
+__device__ __forceinline__ void activate(int act, float (&v)[N]) {
+    if (ACT == ANY ? act == LINEAR_SILU : ACT == LINEAR_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = activated<LINEAR_SILU>(v[j]);
+    } else if (ACT == ANY ? act == LINEAR_GELU : ACT == LINEAR_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = activated<LINEAR_GELU>(v[j]);
+    }
 }
 
 // a'(v); large GELU arguments as in ffn::act_grad.
@@ -108,13 +132,15 @@ __device__ __forceinline__ float slope(float v, int act) {
     return 1.f;
 }
 
-// Eight columns from `col` on of a row, zeros from n on, in 32 bits.
+// Eight columns from `col` < n on of a row, zeros from n on, in 32 bits.  Where 8
+// divides n all eight are there.
 template <class T>
 __device__ __forceinline__ void load8(const T* row, int col, int n, float (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 8 / E<T>; ++h) {
         piece_t<T> p = {};
-        if (col + h * E<T> < n) p = load_piece(row, col + h * E<T>, n);
+        if (n % 8 == 0) __builtin_memcpy(&p, row + col + h * E<T>, 16);
+        else if (col + h * E<T> < n) p = load_piece(row, col + h * E<T>, n);
 #pragma unroll
         for (int j = 0; j < E<T>; ++j) v[h * E<T> + j] = (float)p[j];
     }
@@ -126,7 +152,8 @@ __device__ __forceinline__ void store8(T* row, int col, int n, const float (&v)[
         piece_t<T> p;
 #pragma unroll
         for (int j = 0; j < E<T>; ++j) p[j] = (T)v[h * E<T> + j];
-        if (col + h * E<T> < n) store_piece(row, col + h * E<T>, n, p);
+        if (n % 8 == 0) __builtin_memcpy(row + col + h * E<T>, &p, 16);
+        else if (col + h * E<T> < n) store_piece(row, col + h * E<T>, n, p);
     }
 }
 // By a type that is an argument.
@@ -143,37 +170,117 @@ __device__ __forceinline__ void store8(void* base, int dtype, int64_t stride, in
     else store8(static_cast<__bf16*>(base) + row * stride, col, n, v);
 }
 
-// What follows the product: v are the eight columns from col on of row.
-template <class T>
-__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col, const float (&bias)[8], float (&v)[8]) {
+// What follows the product: v are the eight columns from col on of row, bias
+// included; C is the products' type, Y the result's.
+template <class C, class Y>
+__device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col, float (&v)[8]) {
     if (col >= a.outer) return;
-    if (a.bias)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += bias[j];
-    if (a.z) store8(static_cast<T*>(a.z) + row * a.z_stride, col, a.outer, v);
-    if (a.act != LINEAR_NONE)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = activate(v[j], a.act);
+    if (a.z) store8(static_cast<C*>(a.z) + row * a.z_stride, col, a.outer, v);
+    activate<ANY>(a.act, v);
     if (a.residual) {
         float r[8];
-        load8(a.residual, a.y_dtype, a.residual_stride, row, col, a.outer, r);
+        load8(static_cast<const Y*>(a.residual) + row * a.residual_stride, col, a.outer, r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += r[j];
     }
-    store8(a.y, a.y_dtype, a.y_stride, row, col, a.outer, v);
+    store8(static_cast<Y*>(a.y) + row * a.y_stride, col, a.outer, v);
 }
 
-// The bias is of x's type, 32-bit beside mx8.
+// Stores of 16 rows in whole 128-byte lines.  Lane (q, r) holds two pieces of row
+// r, at columns ca and cb; lanes r and r ^ 8 change one, so that the first store is
+// all of rows 0 .. 7 and the second all of rows 8 .. 15.  (1.09M x 64 -> 256
+// without an activation: 182 us in the 64-byte parts that a piece a lane makes, 145
+// in lines.)
+template <class T>
+__device__ __forceinline__ void store_lines(void* base, int64_t stride, int64_t row0, int64_t rows, int ca, int cb, int n,
+                                            piece_t<T> pa, piece_t<T> pb) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    i32x4 wa, wb, first, second;
+    __builtin_memcpy(&wa, &pa, 16);
+    __builtin_memcpy(&wb, &pb, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {   // row_ror:8 into lanes 8 .. 15, and into lanes 0 .. 7
+        first[j] = __builtin_amdgcn_update_dpp(wa[j], wb[j], 0x128, 0xF, 0xC, false);
+        second[j] = __builtin_amdgcn_update_dpp(wb[j], wa[j], 0x128, 0xF, 0x3, false);
+    }
+    __builtin_memcpy(&pa, &first, 16);
+    __builtin_memcpy(&pb, &second, 16);
+    const int r = threadIdx.x & 15, col = r < 8 ? ca : cb;
+    const int64_t row = row0 + (r & 7);
+    if (col >= n) return;
+    T* at = static_cast<T*>(base) + row * stride;
+    if (n % 8 == 0) {
+        if (row < rows) __builtin_memcpy(at + col, &pa, 16);
+        if (row + 8 < rows) __builtin_memcpy(at + 8 * stride + col, &pb, 16);
+    } else {
+        if (row < rows) store_piece(at, col, n, pa);
+        if (row + 8 < rows) store_piece(at + 8 * stride, col, n, pb);
+    }
+}
+// Blocks of columns whose results a wave stores at once: as many as make lines.
+template <class Y>
+constexpr int LINE = sizeof(Y) == 4 ? 1 : 2;
+
+// The columns col .. col + 7 of each of N blocks, of which the first `live` are there.
+template <class T, int N>
+__device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0, int64_t rows, int col, int n, int live,
+                                        const float (&v)[N][8]) {
+    piece_t<T> p[N][8 / E<T>];
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[b][j / E<T>][j % E<T>] = (T)v[b][j];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int b = 0; b < N; ++b)
+            if (b < live)
+                store_lines<T>(base, stride, row0, rows, col + b * COLS, col + b * COLS + 4, n, p[b][0], p[b][1]);
+    } else if constexpr (N == 2) {
+        store_lines<T>(base, stride, row0, rows, col, live >= 2 ? col + COLS : n, n, p[0][0], p[1][0]);
+    } else {
+        const int64_t row = row0 + (threadIdx.x & 15);
+        T* at = static_cast<T*>(base) + row * stride;
+        if (row < rows && col < n) {
+            if (n % 8 == 0) __builtin_memcpy(at + col, &p[0][0], 16);
+            else store_piece(at, col, n, p[0][0]);
+        }
+    }
+}
+
+// finish for a wave's 16 rows and N blocks of columns, of which the first `live` are there;
+// col is the lane's in the first.  All lanes must be active.
+template <class C, class Y, int ACT, int N>
+__device__ __forceinline__ void finish16(const LinearArgs& a, int64_t row0, int col, int live, float (&v)[N][8]) {
+    if (a.z) store16<C>(a.z, a.z_stride, row0, a.rows, col, a.outer, live, v);
+#pragma unroll
+    for (int b = 0; b < N; ++b) activate<ACT>(a.act, v[b]);
+    if (a.residual) {
+        const Y* at = static_cast<const Y*>(a.residual) + min(row0 + (threadIdx.x & 15), a.rows - 1) * a.residual_stride;
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+            if (col + b * COLS >= a.outer || b >= live) continue;
+            float r[8];
+            load8(at, col + b * COLS, a.outer, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[b][j] += r[j];
+        }
+    }
+    store16<Y>(a.y, a.y_stride, row0, a.rows, col, a.outer, live, v);
+}
+
+// The bias of eight columns, zeros for none; it is of x's type, 32-bit beside mx8.
 template <class T, bool MX>
 __device__ __forceinline__ void bias8(const LinearArgs& a, int col, float (&v)[8]) {
     using B = typename std::conditional<MX, float, T>::type;
-    if (a.bias) load8(static_cast<const B*>(a.bias), col, a.outer, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    if (a.bias && col < a.outer) load8(static_cast<const B*>(a.bias), col, a.outer, v);
 }
 
 // 16 R rows and 32 columns a workgroup, whose waves share the contraction (wave
 // w takes blocks w, w + WAVES, ...) and join their sums in LDS in a fixed order.
 constexpr int FEW_WAVES = 4;
-template <class T, bool MX, bool TRANS, int R>
+template <class T, class Y, bool MX, bool TRANS, int R>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
     using C = typename Operand<T, MX>::type;
     __shared__ f32x4 part[FEW_WAVES][R][2][64];
@@ -219,9 +326,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
 #pragma unroll
             for (int p = 1; p < FEW_WAVES; ++p) t += part[p][i][s][lane];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * s + j] = t[j];
+            for (int j = 0; j < 4; ++j) v[4 * s + j] = t[j] + bias[4 * s + j];
         }
-        if (row < a.rows) finish<C>(a, row, col0 + q * 8, bias, v);
+        if (row < a.rows) finish<C, Y>(a, row, col0 + q * 8, v);
     }
 }
 
@@ -259,8 +366,8 @@ struct XPiece<T, true> {
 // slice; 16 waves a CU go through rows, 16 R at a time, without a barrier, and read
 // the next rows' x ahead.  Workgroups of one XCD share an L2: the slices of the same
 // rows run on one.
-template <class T, bool MX, bool TRANS, int DK, int R>
-__global__ __launch_bounds__(1024) void k_linear_all(LinearArgs a, int slices, int slice_blocks) {
+template <class T, class Y, bool MX, bool TRANS, int ACT, int DK, int R>
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_all(LinearArgs a, int slices, int slice_blocks) {
     using C = typename Operand<T, MX>::type;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     piece_t<C>* w = reinterpret_cast<piece_t<C>*>(lds);
@@ -274,11 +381,10 @@ __global__ __launch_bounds__(1024) void k_linear_all(LinearArgs a, int slices, i
         const int f = i >> 6, kb = f % DK, s = f / DK % 2, cb = f / DK / 2;
         w[i] = w_piece<T, MX, TRANS>(a, (first + cb) * COLS + column(s, i & 15), kb, (i >> 4) & 3);
     }
-    if (a.bias)
-        for (int i = threadIdx.x; i < blocks * COLS; i += blockDim.x) {
-            using B = typename std::conditional<MX, float, T>::type;
-            bias[i] = (float)static_cast<const B*>(a.bias)[min(first * COLS + i, a.outer - 1)];
-        }
+    for (int i = threadIdx.x; i < blocks * COLS; i += blockDim.x) {
+        using B = typename std::conditional<MX, float, T>::type;
+        bias[i] = a.bias ? (float)static_cast<const B*>(a.bias)[min(first * COLS + i, a.outer - 1)] : 0.f;
+    }
     __syncthreads();
     const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R), step = groups * waves;
     int64_t t = group * waves + (threadIdx.x >> 6);
@@ -297,26 +403,36 @@ __global__ __launch_bounds__(1024) void k_linear_all(LinearArgs a, int slices, i
 #pragma unroll
             for (int kb = 0; kb < DK; ++kb) x[i][kb] = next[i][kb].settled(a, kb, q);
         read(t + step);
-        for (int cb = 0; cb < blocks; ++cb) {
-            f32x4 acc[R][2] = {};
-            const piece_t<C>* wb = w + cb * 2 * DK * 64 + lane;
+        constexpr int N = LINE<Y>;
+        for (int cb = 0; cb < blocks; cb += N) {
+            f32x4 acc[R][N][2];   // starts as the bias
 #pragma unroll
-            for (int kb = 0; kb < DK; ++kb)
+            for (int b = 0; b < N; ++b) {
+                const int at = min(cb + b, blocks - 1);
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    const piece_t<C> wf = wb[(s * DK + kb) * 64];
+                    __builtin_memcpy(&acc[0][b][s], bias + at * COLS + q * 8 + 4 * s, 16);
 #pragma unroll
-                    for (int i = 0; i < R; ++i) acc[i][s] = mma(wf, x[i][kb], acc[i][s]);
+                    for (int i = 1; i < R; ++i) acc[i][b][s] = acc[0][b][s];
                 }
-            float b[8];
-            if (a.bias) __builtin_memcpy(b, bias + cb * COLS + q * 8, 32);
+                const piece_t<C>* wb = w + at * 2 * DK * 64 + lane;
+#pragma unroll
+                for (int kb = 0; kb < DK; ++kb)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const piece_t<C> wf = wb[(s * DK + kb) * 64];
+#pragma unroll
+                        for (int i = 0; i < R; ++i) acc[i][b][s] = mma(wf, x[i][kb], acc[i][b][s]);
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int64_t row = t * 16 * R + 16 * i + r;
-                float v[8];
+                float v[N][8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = acc[i][j / 4][j % 4];
-                if (row < a.rows) finish<C>(a, row, (first + cb) * COLS + q * 8, b, v);
+                for (int b = 0; b < N; ++b)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[b][j] = acc[i][b][j / 4][j % 4];
+                finish16<C, Y, ACT>(a, t * 16 * R + 16 * i, (first + cb) * COLS + q * 8, blocks - cb, v);
             }
         }
     }
@@ -342,7 +458,7 @@ __global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int k
 // Packed weights streamed through two areas of LDS, KC blocks of the contraction at
 // a time; a wave holds the sums of 16 R rows and a slice of NB column blocks, and
 // reads its rows' x for the next step ahead.
-template <class T, bool MX, int NB, int R, int KC>
+template <class T, class Y, bool MX, int NB, int R, int KC>
 __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece_t<typename Operand<T, MX>::type>* packed,
                                                        int slices, int steps) {
     using C = typename Operand<T, MX>::type;
@@ -360,9 +476,18 @@ __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece
 #pragma unroll
             for (int c = 0; c < KC; ++c) next[i][c].read(a, min(row0 + 16 * i + r, a.rows - 1), step * KC + c, q);
     };
-    f32x4 acc[R][2 * NB] = {};
     ffn::fetch<C>(packed, w[0], F);
     read(0);
+    f32x4 acc[R][2 * NB];   // starts as the bias
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        float bias[8];
+        bias8<T, MX>(a, (slice * NB + b) * COLS + q * 8, bias);
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) acc[i][2 * b + j / 4][j % 4] = bias[j];
+    }
     for (int step = 0; step < steps; ++step) {
         ffn::fetched();
         piece_t<C> x[R][KC];
@@ -384,20 +509,19 @@ __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece
                 for (int i = 0; i < R; ++i) acc[i][f] = mma(wf, x[i][c], acc[i][f]);
             }
     }
+    constexpr int N = LINE<Y>;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const int col = (slice * NB + b) * COLS + q * 8;
-        float bias[8];
-        bias8<T, MX>(a, col, bias);
+    for (int b = 0; b < NB; b += N)
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int64_t row = row0 + 16 * i + r;
-            float v[8];
+            float v[N][8] = {};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = acc[i][2 * b + j / 4][j % 4];
-            if (row < a.rows) finish<C>(a, row, col, bias, v);
+            for (int h = 0; h < N; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (b + h < NB) v[h][j] = acc[i][b + h < NB ? 2 * (b + h) + j / 4 : 0][j % 4];
+            finish16<C, Y, ANY>(a, row0 + 16 * i, (slice * NB + b) * COLS + q * 8, NB - b, v);
         }
-    }
 }
 
 constexpr int64_t CUS = 256;
@@ -413,7 +537,7 @@ struct Shape {
     int64_t packed;     // streamed: bytes of the packed weights
     bool few, all;
 };
-constexpr int KC = 2;
+constexpr int KC = 4;
 template <class C>
 Shape shape(int64_t rows, int inner, int outer) {
     Shape p{};
@@ -422,6 +546,7 @@ Shape shape(int64_t rows, int inner, int outer) {
     p.few = rows <= 1024;
     p.all = !p.few && p.kbs <= ALL_BLOCKS;
     if (p.all) {
+        if (p.kbs == 5 || p.kbs == 7) ++p.kbs;   // kernels there are for 1 to 4, 6 and 8
         const int most = (int)(LDS_BYTES / (p.kbs * 2048 + COLS * 4));
         p.slices = (int)ceil_div(p.blocks, most);
         p.nb = (int)ceil_div(p.blocks, p.slices);
@@ -449,7 +574,7 @@ LinearArgs rows_from(const LinearArgs& a, int64_t at, int64_t rows) {
     return p;
 }
 
-template <class T, bool MX, bool TRANS>
+template <class T, class Y, bool MX, bool TRANS>
 void few_product(hipStream_t s, const LinearArgs& a) {
     const int64_t blocks = ceil_div(a.outer, COLS);
     auto launch = [&](auto r) {
@@ -458,24 +583,25 @@ void few_product(hipStream_t s, const LinearArgs& a) {
         const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
         for (int64_t at = 0; at < a.rows; at += most) {
             const LinearArgs p = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
-            k_linear_few<T, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES, 0, s>>>(p);
+            k_linear_few<T, Y, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES, 0, s>>>(p);
         }
     };
     if (a.rows <= 16) launch(std::integral_constant<int, 1>{});
     else launch(std::integral_constant<int, 4>{});
 }
 
-template <class T, bool MX, bool TRANS, int DK>
+template <class T, class Y, bool MX, bool TRANS, int ACT, int DK>
 void all_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     constexpr int R = DK <= 4 ? 2 : 1;
-    const int64_t tiles = ceil_div(a.rows, 16 * R), most = std::max<int64_t>(CUS / p.slices / 8, 1) * 8;
-    const int64_t waves = std::min<int64_t>(16, ceil_div(tiles, most));
+    const size_t bytes = (size_t)p.nb * (2 * DK * 1024 + COLS * 4);
+    const int per_cu = std::min<int>(2, LDS_BYTES / bytes), most_waves = 16 / per_cu;
+    const int64_t tiles = ceil_div(a.rows, 16 * R), most = std::max<int64_t>(per_cu * CUS / p.slices / 8, 1) * 8;
+    const int64_t waves = std::min<int64_t>(most_waves, ceil_div(tiles, most));
     const int64_t groups = std::min(ceil_div(ceil_div(tiles, waves), 8) * 8, most);   // a multiple of 8, as the kernel numbers them
-    const size_t lds = (size_t)p.nb * (2 * DK * 1024 + COLS * 4);
-    k_linear_all<T, MX, TRANS, DK, R><<<(unsigned)(groups * p.slices), (unsigned)(64 * waves), lds, s>>>(a, p.slices, p.nb);
+    k_linear_all<T, Y, MX, TRANS, ACT, DK, R><<<(unsigned)(groups * p.slices), (unsigned)(64 * waves), bytes, s>>>(a, p.slices, p.nb);
 }
 
-template <class T, bool MX, int NB>
+template <class T, class Y, bool MX, int NB>
 void stream_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     using C = typename Operand<T, MX>::type;
     const piece_t<C>* packed = reinterpret_cast<const piece_t<C>*>(a.ws);
@@ -484,25 +610,31 @@ void stream_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     for (int64_t at = 0; at < a.rows; at += most) {
         const LinearArgs part = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
         const int64_t groups = ceil_div(ceil_div(part.rows, 16 * R * WAVES), 8) * 8;
-        k_linear_stream<T, MX, NB, R, KC><<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
+        k_linear_stream<T, Y, MX, NB, R, KC><<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
     }
 }
 
-template <class T, bool MX, bool TRANS>
+// TRANS: W^T in W's place, and no activation.
+template <class T, class Y, bool MX, bool TRANS>
 void product(hipStream_t s, const LinearArgs& a) {
     using C = typename Operand<T, MX>::type;
     const Shape p = shape<C>(a.rows, a.inner, a.outer);
-    if (p.few) return few_product<T, MX, TRANS>(s, a);
+    if (p.few) return few_product<T, Y, MX, TRANS>(s, a);
     if (p.all) {
+        auto all = [&](auto dk) {
+            if constexpr (!TRANS) {
+                if (a.act == LINEAR_SILU) return all_product<T, Y, MX, TRANS, LINEAR_SILU, dk()>(s, a, p);
+                if (a.act == LINEAR_GELU) return all_product<T, Y, MX, TRANS, LINEAR_GELU, dk()>(s, a, p);
+            }
+            all_product<T, Y, MX, TRANS, LINEAR_NONE, dk()>(s, a, p);
+        };
         switch (p.kbs) {
-#define BLOCKS(n) case n: return all_product<T, MX, TRANS, n>(s, a, p)
+#define BLOCKS(n) case n: return all(std::integral_constant<int, n>{})
             BLOCKS(1);
             BLOCKS(2);
             BLOCKS(3);
             BLOCKS(4);
-            BLOCKS(5);
             BLOCKS(6);
-            BLOCKS(7);
             BLOCKS(8);
 #undef BLOCKS
         }
@@ -511,7 +643,7 @@ void product(hipStream_t s, const LinearArgs& a) {
     k_linear_pack<T, MX, TRANS><<<(unsigned)ceil_div(pieces, 256), 256, 0, s>>>(a, p.nb, p.steps * KC,
                                                                               reinterpret_cast<piece_t<C>*>(a.ws), pieces);
     switch (p.nb) {
-#define BLOCKS(n) case n: return stream_product<T, MX, n>(s, a, p)
+#define BLOCKS(n) case n: return stream_product<T, Y, MX, n>(s, a, p)
         BLOCKS(1);
         BLOCKS(2);
         BLOCKS(3);
@@ -745,7 +877,7 @@ void backward(hipStream_t s, const LinearGradArgs& a) {
         d.y_stride = a.dx_stride;
         d.y_dtype = a.dtype;
         d.ws = a.ws + p.dz_bytes + p.db_bytes + p.dw_bytes;
-        product<T, false, true>(s, d);
+        product<T, T, false, true>(s, d);
     }
     if (!a.dweight) return;
     if (p.dw_groups > 0) {
@@ -759,7 +891,7 @@ void backward(hipStream_t s, const LinearGradArgs& a) {
 }  // namespace linear
 
 // One translation unit per type and direction.
-template <class T, bool MX>
+template <class T, class Y, bool MX>
 void linear_forward(hipStream_t s, const LinearArgs& a);
 template <class T>
 void linear_backward(hipStream_t s, const LinearGradArgs& a);

@@ -87,7 +87,9 @@ def rms_norm_grad(dy, total, weight, rstd, dtotal):
 def linear(x, w, bias, residual, act, out_dtype):
     """y, z = x w^T + bias and their bounds, z in x's type and before it was rounded.
     x and w as their values (64 bits or less); a product's sum over dim terms is
-    off by dim U of their magnitudes at most."""
+    off by dim U of their magnitudes at most.  The kernels start the sum from the
+    bias: every partial sum is then at most |b| + sum |x| |w| in magnitude, so that
+    each of the dim additions rounds by U of that at most, dim U (|b| + sum |x| |w|) in all."""
     uT, tiny = UT[out_dtype]
     x, w = x.double().cpu(), w.double().cpu()
     dim = x.shape[1]
@@ -95,7 +97,7 @@ def linear(x, w, bias, residual, act, out_dtype):
     e_z = dim * U * (x.abs() @ w.abs().t())
     if bias is not None:
         z = z + bias.double().cpu()
-        e_z = e_z + U * z.abs()
+        e_z = e_z + dim * U * bias.double().cpu().abs() + U * z.abs()
     if act is None:
         y, e_y = z, e_z
     else:
