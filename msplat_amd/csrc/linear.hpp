@@ -60,19 +60,36 @@ __device__ __forceinline__ piece_t<__bf16> from_mx8(const uint32_t (&bytes)[2], 
     return o;
 }
 
-// The piece of lane group q in block kb of a row of x.
+// The piece of lane group q in block kb of a row of x, as it is read and as the
+// products take it.  The last piece of a row that E does not divide is read so that it
+// ends with the row, and so are pieces behind it: W has zeros in the place of
+// what was there before (w_piece), so that x needs no mask.
 template <class T, bool MX>
-__device__ __forceinline__ piece_t<typename Operand<T, MX>::type> x_piece(const LinearArgs& a, int64_t row, int kb, int q) {
-    if constexpr (MX) {
-        uint32_t bytes[2];
-        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.x) + row * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
-        return from_mx8(bytes, a.x_scales[row * mx8::scale_stride(a.inner) + kb]);
-    } else {
-        return load_piece(static_cast<const T*>(a.x) + row * a.x_stride, kb * KB<T> + q * E<T>, a.inner);
+struct XPiece {
+    piece_t<T> v;
+    template <bool TINY>   // whether a row may be less than a piece
+    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
+        const T* at = static_cast<const T*>(a.x) + row * a.x_stride;
+        v = TINY && a.inner < E<T> ? load_piece(at, kb * KB<T> + q * E<T>, a.inner)
+                                   : read_piece(at, kb * KB<T> + q * E<T>, a.inner);
     }
-}
+    __device__ __forceinline__ piece_t<T> taken() const { return v; }
+};
+template <class T>
+struct XPiece<T, true> {
+    uint32_t bytes[2];
+    int code;
+    template <bool TINY>
+    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
+        const int64_t ds = mx8::data_stride(a.inner);
+        kb = min(kb, (int)(ds / 32) - 1);
+        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.x) + row * ds + kb * 32 + q * 8, 8);
+        code = a.x_scales[row * mx8::scale_stride(a.inner) + kb];
+    }
+    __device__ __forceinline__ piece_t<__bf16> taken() const { return from_mx8(bytes, code); }
+};
 
-// The same of a row of W, W^T where TRANS, zero beyond the matrix.
+// The piece of a row of W that meets it, W^T where TRANS, zero beyond the matrix.
 template <class T, bool MX, bool TRANS>
 __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const LinearArgs& a, int row, int kb, int q) {
     using C = typename Operand<T, MX>::type;
@@ -83,16 +100,18 @@ __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const 
         uint32_t bytes[2];
         __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.w) + at * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
         v = from_mx8(bytes, a.w_scales[at * mx8::scale_stride(a.inner) + kb]);
-    } else if constexpr (TRANS) {
-        const T* w = static_cast<const T*>(a.w) + at;
-        const int k = kb * KB<T> + q * E<T>;
+    } else {
+        const int k = kb * KB<T> + q * E<T>, from = max(min(k, a.inner - E<T>), 0);
+        if constexpr (TRANS) {
+            const T* w = static_cast<const T*>(a.w) + at;
 #pragma unroll
-        for (int j = 0; j < E<T>; ++j) v[j] = w[min(k + j, a.inner - 1) * a.w_stride];
+            for (int j = 0; j < E<T>; ++j) v[j] = w[min(from + j, a.inner - 1) * a.w_stride];
+        } else {
+            v = load_piece(static_cast<const T*>(a.w) + at * a.w_stride, from, a.inner);
+        }
 #pragma unroll
         for (int j = 0; j < E<T>; ++j)
-            if (k + j >= a.inner) v[j] = (T)0.f;
-    } else {
-        v = load_piece(static_cast<const T*>(a.w) + at * a.w_stride, kb * KB<T> + q * E<T>, a.inner);
+            if (from + j < k || from + j >= a.inner) v[j] = (T)0.f;
     }
     return row < a.outer ? v : piece_t<C>{};
 }
@@ -291,7 +310,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
     f32x4 acc[R][2] = {};
     constexpr int U = 4;   // blocks whose reads are under way at once
     for (int kb0 = wave; kb0 < kbs; kb0 += U * FEW_WAVES) {
-        piece_t<C> x[U][R] = {}, w[U][2] = {};
+        XPiece<T, MX> x[U][R] = {};
+        piece_t<C> w[U][2] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int kb = kb0 + u * FEW_WAVES;
@@ -299,14 +319,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) w[u][s] = w_piece<T, MX, TRANS>(a, col0 + column(s, r), kb, q);
 #pragma unroll
-            for (int i = 0; i < R; ++i) x[u][i] = x_piece<T, MX>(a, min(row0 + 16 * i + r, a.rows - 1), kb, q);
+            for (int i = 0; i < R; ++i) x[u][i].template read<true>(a, min(row0 + 16 * i + r, a.rows - 1), kb, q);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < R; ++i)
 #pragma unroll
-                for (int s = 0; s < 2; ++s) acc[i][s] = mma(w[u][s], x[u][i], acc[i][s]);
+                for (int s = 0; s < 2; ++s) acc[i][s] = mma(w[u][s], x[u][i].taken(), acc[i][s]);
     }
 #pragma unroll
     for (int i = 0; i < R; ++i)
@@ -331,36 +351,6 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
         if (row < a.rows) finish<C, Y>(a, row, col0 + q * 8, v);
     }
 }
-
-// A piece of x as it is read, and what the products take of it: two steps, so
-// that reads may be under way while something else runs.
-template <class T, bool MX>
-struct XPiece {
-    piece_t<T> v;
-    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
-        const T* at = static_cast<const T*>(a.x) + row * a.x_stride;
-        v = a.inner < E<T> ? load_piece(at, kb * KB<T> + q * E<T>, a.inner)
-                           : read_piece(at, kb * KB<T> + q * E<T>, a.inner);
-    }
-    __device__ __forceinline__ piece_t<T> settled(const LinearArgs& a, int kb, int q) const {
-        return a.inner < E<T> ? v : settle_piece<T>(v, kb * KB<T> + q * E<T>, a.inner, true);
-    }
-};
-template <class T>
-struct XPiece<T, true> {
-    uint32_t bytes[2];
-    int code;
-    __device__ __forceinline__ void read(const LinearArgs& a, int64_t row, int kb, int q) {
-        const int64_t ds = mx8::data_stride(a.inner);
-        // a block behind the last is read from it and multiplied by zeros of W
-        kb = min(kb, (int)(ds / 32) - 1);
-        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.x) + row * ds + kb * 32 + q * 8, 8);
-        code = a.x_scales[row * mx8::scale_stride(a.inner) + kb];
-    }
-    __device__ __forceinline__ piece_t<__bf16> settled(const LinearArgs& a, int kb, int) const {
-        return kb * 32 < a.inner ? from_mx8(bytes, code) : piece_t<__bf16>{};
-    }
-};
 
 // Weights in LDS for all of the contraction (DK blocks) and the columns of a
 // slice; 16 waves a CU go through rows, 16 R at a time, without a barrier, and read
@@ -393,7 +383,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int kb = 0; kb < DK; ++kb) next[i][kb].read(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
+            for (int kb = 0; kb < DK; ++kb) next[i][kb].template read<DK == 1>(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
     };
     read(t);
     for (; t < tiles; t += step) {
@@ -401,7 +391,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int kb = 0; kb < DK; ++kb) x[i][kb] = next[i][kb].settled(a, kb, q);
+            for (int kb = 0; kb < DK; ++kb) x[i][kb] = next[i][kb].taken();
         read(t + step);
         constexpr int N = LINE<Y>;
         for (int cb = 0; cb < blocks; cb += N) {
@@ -456,8 +446,8 @@ __global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int k
 }
 
 // Packed weights streamed through two areas of LDS, KC blocks of the contraction at
-// a time; a wave holds the sums of 16 R rows and a slice of NB column blocks, and
-// reads its rows' x for the next step ahead.
+// a time; a wave holds the sums of 16 R rows and a slice of NB column blocks.  x is
+// read two steps ahead: a step's products take less than a read from memory does.
 template <class T, class Y, bool MX, int NB, int R, int KC>
 __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece_t<typename Operand<T, MX>::type>* packed,
                                                        int slices, int steps) {
@@ -469,15 +459,15 @@ __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece
     const int64_t group = blockIdx.x / 8 / slices * 8 + blockIdx.x % 8;
     const int64_t row0 = (group * waves + (threadIdx.x >> 6)) * 16 * R;
     packed += (int64_t)slice * steps * F * 64;
-    XPiece<T, MX> next[R][KC];
-    auto read = [&](int step) {
+    XPiece<T, MX> next[2][R][KC];
+    auto read = [&](int step, XPiece<T, MX> (&to)[R][KC]) {
+        step = min(step, steps - 1);
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int c = 0; c < KC; ++c) next[i][c].read(a, min(row0 + 16 * i + r, a.rows - 1), step * KC + c, q);
+            for (int c = 0; c < KC; ++c)
+                to[i][c].template read<false>(a, min(row0 + 16 * i + r, a.rows - 1), step * KC + c, q);
     };
-    ffn::fetch<C>(packed, w[0], F);
-    read(0);
     f32x4 acc[R][2 * NB];   // starts as the bias
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -488,27 +478,37 @@ __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece
 #pragma unroll
             for (int j = 0; j < 8; ++j) acc[i][2 * b + j / 4][j % 4] = bias[j];
     }
-    for (int step = 0; step < steps; ++step) {
-        ffn::fetched();
-        piece_t<C> x[R][KC];
+    read(0, next[0]);
+    ffn::fetch<C>(packed, w[0], F);
+    asm volatile("" ::: "memory");
+    read(1, next[1]);
+    for (int step0 = 0; step0 < steps; step0 += 2)
 #pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int h = 0; h < 2; ++h) {
+            const int step = step0 + h;
+            if (step >= steps) break;
+            // the step's weights are there when at most the reads of x that followed them are
+            // under way: one a piece at least
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(R * KC) : "memory");
+            piece_t<C> x[R][KC];
 #pragma unroll
-            for (int c = 0; c < KC; ++c) x[i][c] = next[i][c].settled(a, step * KC + c, q);
-        if (step + 1 < steps) {
-            ffn::fetch<C>(packed + (int64_t)(step + 1) * F * 64, w[(step + 1) & 1], F);
-            read(step + 1);
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int c = 0; c < KC; ++c) x[i][c] = next[h][i][c].taken();
+            if (step + 1 < steps) ffn::fetch<C>(packed + (int64_t)(step + 1) * F * 64, w[h ^ 1], F);
+            asm volatile("" ::: "memory");
+            read(step + 2, next[h]);
+            const piece_t<C>* at = w[h] + lane;
+#pragma unroll
+            for (int c = 0; c < KC; ++c)
+#pragma unroll
+                for (int f = 0; f < 2 * NB; ++f) {
+                    const piece_t<C> wf = at[(c * 2 * NB + f) * 64];
+#pragma unroll
+                    for (int i = 0; i < R; ++i) acc[i][f] = mma(wf, x[i][c], acc[i][f]);
+                }
+            ffn::read_ahead<1, R * ffn::MFMAS<C>, F, 4>();
         }
-        const piece_t<C>* at = w[step & 1] + lane;
-#pragma unroll
-        for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int f = 0; f < 2 * NB; ++f) {
-                const piece_t<C> wf = at[(c * 2 * NB + f) * 64];
-#pragma unroll
-                for (int i = 0; i < R; ++i) acc[i][f] = mma(wf, x[i][c], acc[i][f]);
-            }
-    }
     constexpr int N = LINE<Y>;
 #pragma unroll
     for (int b = 0; b < NB; b += N)
@@ -537,7 +537,7 @@ struct Shape {
     int64_t packed;     // streamed: bytes of the packed weights
     bool few, all;
 };
-constexpr int KC = 4;
+constexpr int KC = 2;
 template <class C>
 Shape shape(int64_t rows, int inner, int outer) {
     Shape p{};
@@ -601,15 +601,25 @@ void all_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     k_linear_all<T, Y, MX, TRANS, ACT, DK, R><<<(unsigned)(groups * p.slices), (unsigned)(64 * waves), bytes, s>>>(a, p.slices, p.nb);
 }
 
+// Rows that a streamed product leaves to k_linear_few: the start of a last round of
+// workgroups that would take as long as a full one (65543 x 1000 -> 200 f16: 86 us
+// with seven rows in a round of their own).
+constexpr int64_t STREAM_ROWS = 16 * 2 * 8;   // of a workgroup
+inline int64_t tail_rows(int64_t rows, int slices) {
+    const int64_t round = STREAM_ROWS * std::max<int64_t>(CUS / slices, 1), rest = rows % round;
+    return rows > round && rest <= 1024 ? rest : 0;
+}
+
 template <class T, class Y, bool MX, int NB>
 void stream_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     using C = typename Operand<T, MX>::type;
     const piece_t<C>* packed = reinterpret_cast<const piece_t<C>*>(a.ws);
     constexpr int R = 2, WAVES = 8;
-    const int64_t most = (int64_t(1) << 22) / p.slices / 8 * 8 * 16 * R * WAVES;   // fewer than 2^32 threads
+    static_assert(STREAM_ROWS == 16 * R * WAVES, "rows of a workgroup");
+    const int64_t most = (int64_t(1) << 22) / p.slices / 8 * 8 * STREAM_ROWS;   // fewer than 2^32 threads
     for (int64_t at = 0; at < a.rows; at += most) {
         const LinearArgs part = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
-        const int64_t groups = ceil_div(ceil_div(part.rows, 16 * R * WAVES), 8) * 8;
+        const int64_t groups = ceil_div(ceil_div(part.rows, STREAM_ROWS), 8) * 8;
         k_linear_stream<T, Y, MX, NB, R, KC><<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
     }
 }
@@ -642,8 +652,11 @@ void product(hipStream_t s, const LinearArgs& a) {
     const int64_t pieces = p.packed / 16;
     k_linear_pack<T, MX, TRANS><<<(unsigned)ceil_div(pieces, 256), 256, 0, s>>>(a, p.nb, p.steps * KC,
                                                                               reinterpret_cast<piece_t<C>*>(a.ws), pieces);
+    const int64_t tail = tail_rows(a.rows, p.slices);
+    const LinearArgs main = rows_from<T, MX>(a, 0, a.rows - tail);
+    if (tail) few_product<T, Y, MX, TRANS>(s, rows_from<T, MX>(a, a.rows - tail, tail));
     switch (p.nb) {
-#define BLOCKS(n) case n: return stream_product<T, Y, MX, n>(s, a, p)
+#define BLOCKS(n) case n: return stream_product<T, Y, MX, n>(s, main, p)
         BLOCKS(1);
         BLOCKS(2);
         BLOCKS(3);
