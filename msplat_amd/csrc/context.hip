@@ -1694,7 +1694,7 @@ int msplat_hip_linear(const MsplatLinearArgs* a) {
 int64_t msplat_hip_linear_backward_workspace(int64_t rows, int32_t inner, int32_t outer, int32_t dtype, int32_t y_dtype,
                                              int32_t activation) {
     if (check_linear(rows, inner, outer, dtype, y_dtype, activation) != MSPLAT_OK) return -1;
-    return (int64_t)linear_grad_workspace(dtype, rows, inner, outer, activation != MSPLAT_IDENTITY || y_dtype != dtype);
+    return (int64_t)linear_grad_workspace(dtype, y_dtype, rows, inner, outer, activation);
 }
 
 int msplat_hip_linear_backward(const MsplatLinearGradArgs* a) {
@@ -1719,7 +1719,7 @@ int msplat_hip_linear_backward(const MsplatLinearGradArgs* a) {
     l.dtype = a->dtype;
     l.y_dtype = a->y_dtype;
     CHECK(check_workspace(a->workspace, a->workspace_bytes,
-                          linear_grad_workspace(a->dtype, a->rows, a->inner, a->outer, l.own_dz())));
+                          linear_grad_workspace(a->dtype, a->y_dtype, a->rows, a->inner, a->outer, a->activation)));
     if (!g_ctx) return fail(MSPLAT_ERR_NOINIT, "not initialised");
     if (!a->dweight && !a->dbias && (!a->dx || a->rows == 0)) return MSPLAT_OK;
     l.dy = a->dy;

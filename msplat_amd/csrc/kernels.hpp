@@ -497,7 +497,7 @@ struct LinearGradArgs {
     // dy is not the gradient of x W^T + bias as the products take it
     bool own_dz() const { return act != LINEAR_NONE || y_dtype != dtype; }
 };
-size_t linear_grad_workspace(int dtype, int64_t rows, int inner, int outer, bool own_dz);
+size_t linear_grad_workspace(int dtype, int y_dtype, int64_t rows, int inner, int outer, int act);
 void launch_linear_bwd(hipStream_t s, const LinearGradArgs& a);
 
 // Gated feed-forward block (ffn_*.hip): y = (act(x Wg^T) * (x Wu^T)) Wd^T.

@@ -90,7 +90,8 @@ struct XPiece<T, true> {
 };
 
 // The piece of a row of W that meets it, W^T where TRANS, zero beyond the matrix.
-template <class T, bool MX, bool TRANS>
+// ENDS: the last piece ends with the row, as x is read.
+template <class T, bool MX, bool TRANS, bool ENDS = true>
 __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const LinearArgs& a, int row, int kb, int q) {
     using C = typename Operand<T, MX>::type;
     const int at = min(row, a.outer - 1);
@@ -101,7 +102,7 @@ __device__ __forceinline__ piece_t<typename Operand<T, MX>::type> w_piece(const 
         __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.w) + at * mx8::data_stride(a.inner) + kb * 32 + q * 8, 8);
         v = from_mx8(bytes, a.w_scales[at * mx8::scale_stride(a.inner) + kb]);
     } else {
-        const int k = kb * KB<T> + q * E<T>, from = max(min(k, a.inner - E<T>), 0);
+        const int k = kb * KB<T> + q * E<T>, from = ENDS ? max(min(k, a.inner - E<T>), 0) : k;
         if constexpr (TRANS) {
             const T* w = static_cast<const T*>(a.w) + at;
 #pragma unroll
@@ -720,12 +721,13 @@ __global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, floa
     }
 }
 
-// Adds `groups` partial rows of n: 32 columns a workgroup at once, 32 threads a
-// column.
+// Adds `groups` partial rows of n1 + n2 numbers into two results, either of which
+// may be null: 32 columns a workgroup at once, 32 threads a column.
 template <class T>
-__global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int groups, int64_t n, T* out) {
+__global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int groups, int64_t n1, int64_t n2, T* out1, T* out2) {
     __shared__ float red[32][33];
     const int sl = threadIdx.x >> 5;
+    const int64_t n = n1 + n2;
     for (int64_t at = (int64_t)blockIdx.x * 32; at < n; at += (int64_t)gridDim.x * 32) {
         const int64_t col = at + (threadIdx.x & 31);
         float t = 0.f;
@@ -737,14 +739,19 @@ __global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int gro
         if (sl == 0 && col < n) {
             t = 0.f;
             for (int q = 0; q < 32; ++q) t += red[q][threadIdx.x & 31];
-            out[col] = (T)t;
+            if (col < n1) {
+                if (out1) out1[col] = (T)t;
+            } else if (out2) {
+                out2[col - n1] = (T)t;
+            }
         }
         __syncthreads();
     }
 }
 template <class T>
-void fold(hipStream_t s, const float* part, int groups, int64_t n, void* out) {
-    k_linear_fold<T><<<(unsigned)std::min<int64_t>(ceil_div(n, 32), 1 << 20), 1024, 0, s>>>(part, groups, n, static_cast<T*>(out));
+void fold(hipStream_t s, const float* part, int groups, int64_t n1, int64_t n2, void* out1, void* out2) {
+    k_linear_fold<T><<<(unsigned)std::min<int64_t>(ceil_div(n1 + n2, 32), 1 << 20), 1024, 0, s>>>(
+        part, groups, n1, n2, static_cast<T*>(out1), static_cast<T*>(out2));
 }
 
 // dW: a workgroup takes TN rows and TK columns of it (outputs and inputs) over a
@@ -829,9 +836,191 @@ __global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void*
         }
 }
 
+// All gradients in one pass over dy, z and x, where a workgroup's registers hold all
+// of dW: eight waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  A block of KB
+// rows goes through LDS: dz is made of dy and z on the way in, its sums over rows
+// stay in registers, dW takes both blocks through transposing reads, and dx takes
+// dz's rows and W^T, which stays in LDS.  A block's reads are under way while the one
+// before is multiplied.
+template <int N, int K>
+struct BwdShape {
+    static constexpr int n = N, k = K;
+    // waves along outputs and inputs, as square a tile each as there can be
+    static constexpr int WN = N >= 256 ? 8 : N >= 2 * K ? 8 : N * 2 <= K ? 1 : 4, WK = 8 / WN;
+    static constexpr int HN = N / 16 / WN, HK = K / 16 / WK;
+};
+template <class T, bool MX>
+struct Kept {   // a piece of a kept matrix on its way in
+    piece_t<T> v;
+    __device__ __forceinline__ void read(const void* base, int64_t stride, const uint8_t*, int64_t row, int col, int n) {
+        const T* at = static_cast<const T*>(base) + row * stride;
+        v = n < E<T> ? load_piece(at, col, n) : read_piece(at, col, n);
+    }
+    // in 32 bits, zeros from n on
+    __device__ __forceinline__ void values(int col, int n, float (&f)[E<T>]) const {
+        const piece_t<T> p = n < E<T> ? v : settle_piece<T>(v, col, n, true);
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j) f[j] = (float)p[j];
+    }
+};
+template <class T>
+struct Kept<T, true> {
+    uint32_t bytes[E<T> / 4];
+    int code;
+    __device__ __forceinline__ void read(const void* base, int64_t, const uint8_t* scales, int64_t row, int col, int n) {
+        col = min(col, (int)mx8::data_stride(n) - E<T>);
+        __builtin_memcpy(bytes, static_cast<const uint8_t*>(base) + row * mx8::data_stride(n) + col, E<T>);
+        code = scales[row * mx8::scale_stride(n) + col / mx8::BLOCK];
+    }
+    __device__ __forceinline__ void values(int col, int n, float (&f)[E<T>]) const {
+        mx8::values<T>(bytes, code, f);
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j)
+            if (col + j >= n) f[j] = 0.f;
+    }
+};
+
+template <class T, class S, bool HASZ, bool ZMX, bool XMX>
+__global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* part) {
+    constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = KB<T> / 16;
+    constexpr int PD = KB<T> * NP > 512 ? KB<T> * NP / 512 : 1, PX = KB<T> * KP > 512 ? KB<T> * KP / 512 : 1;
+    constexpr int HT = ffn::HT<T>, CB = S::k / COLS;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    piece_t<T>* w = reinterpret_cast<piece_t<T>*>(lds);
+    piece_t<T>* ld = w + CB * 2 * NB * 64;         // two blocks of dz
+    piece_t<T>* lx = ld + 2 * KB<T> * NP;          // and of x
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
+    const int wn = wave / S::WK, wk = wave % S::WK;
+    if (a.dx) {
+        LinearArgs t{};   // W^T [inner, outer]
+        t.w = a.w;
+        t.w_stride = a.w_stride;
+        t.inner = a.outer;
+        t.outer = a.inner;
+        for (int i = tid; i < CB * 2 * NB * 64; i += 512) {
+            const int f = i >> 6, kb = f % NB, s = f / NB % 2, cb = f / NB / 2;
+            w[i] = w_piece<T, false, true, false>(t, cb * COLS + column(s, i & 15), kb, (i >> 4) & 3);
+        }
+    }
+    const int64_t blocks = (a.rows + KB<T> - 1) / KB<T>;
+    const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
+    piece_t<T> dy[PD];
+    Kept<T, ZMX> z[PD];
+    Kept<T, XMX> x[PX];
+    auto read = [&](int64_t b) {
+#pragma unroll
+        for (int p = 0; p < PD; ++p) {
+            const int64_t row = min(b * KB<T> + min(tid / NP + p * (512 / NP), KB<T> - 1), a.rows - 1);
+            const T* at = static_cast<const T*>(a.dy) + row * a.dy_stride;
+            dy[p] = a.outer < E<T> ? load_piece(at, cd, a.outer) : read_piece(at, cd, a.outer);
+            if (HASZ) z[p].read(a.z, a.z_stride, a.z_scales, row, cd, a.outer);
+        }
+#pragma unroll
+        for (int p = 0; p < PX; ++p)
+            x[p].read(a.x, a.x_stride, a.x_scales, min(b * KB<T> + min(tid / KP + p * (512 / KP), KB<T> - 1), a.rows - 1), cx,
+                      a.inner);
+    };
+    f32x4 acc[S::HN][S::HK] = {};
+    float db[E<T>] = {};
+    read(blockIdx.x);
+    int turn = 0;
+    for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x, turn ^= 1) {
+        piece_t<T>* bd = ld + turn * KB<T> * NP;
+        piece_t<T>* bx = lx + turn * KB<T> * KP;
+#pragma unroll
+        for (int p = 0; p < PD; ++p) {
+            const int rho = tid / NP + p * (512 / NP);
+            const bool live = b * KB<T> + rho < a.rows;
+            const piece_t<T> g = a.outer < E<T> ? dy[p] : settle_piece<T>(dy[p], cd, a.outer, true);
+            float f[E<T>];
+            if (HASZ) z[p].values(cd, a.outer, f);
+            piece_t<T> o;
+#pragma unroll
+            for (int j = 0; j < E<T>; ++j) {
+                float v = (float)g[j];
+                if (HASZ) v *= slope(f[j], a.act);
+                v = live ? v : 0.f;
+                if (rho < KB<T>) db[j] += v;
+                o[j] = (T)v;
+            }
+            if (rho < KB<T>) bd[staged<T>(rho, tid % NP)] = o;
+        }
+#pragma unroll
+        for (int p = 0; p < PX; ++p) {
+            const int rho = tid / KP + p * (512 / KP);
+            const bool live = b * KB<T> + rho < a.rows;
+            float f[E<T>];
+            x[p].values(cx, a.inner, f);
+            piece_t<T> o;
+#pragma unroll
+            for (int j = 0; j < E<T>; ++j) o[j] = (T)(live ? f[j] : 0.f);
+            if (rho < KB<T>) bx[staged<T>(rho, tid % KP)] = o;
+        }
+        read(b + gridDim.x);
+        // one barrier a block: who is a block ahead writes the other buffers
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (a.dweight) {
+            piece_t<T> fx[S::HK];
+#pragma unroll
+            for (int j = 0; j < S::HK; ++j) fx[j] = ffn::by_dim<T>(bx, wk * S::HK + j);
+#pragma unroll
+            for (int i = 0; i < S::HN; ++i) {
+                const piece_t<T> fd = ffn::by_dim<T>(bd, wn * S::HN + i);
+#pragma unroll
+                for (int j = 0; j < S::HK; ++j) acc[i][j] = mma(fd, fx[j], acc[i][j]);
+            }
+        }
+        if (a.dx)
+            for (int t = wave; t < CB * RT; t += 8) {
+                const int cb = t / RT, tile = t % RT;
+                if (cb * COLS >= a.inner) break;
+                f32x4 o[2] = {};
+#pragma unroll
+                for (int kb = 0; kb < NB; ++kb) {
+                    const piece_t<T> fd = ffn::by_row<T>(bd, kb * HT + tile);
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) o[s] = mma(w[((cb * 2 + s) * NB + kb) * 64 + lane], fd, o[s]);
+                }
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = o[j / 4][j % 4];
+                const int64_t row = b * KB<T> + ffn::perm<T>(tile, r);
+                const int col = cb * COLS + q * 8;
+                if (row < a.rows && col < a.inner) store8(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
+            }
+    }
+    if (!part) return;
+    const int64_t n = (int64_t)a.outer * a.inner;
+    part += blockIdx.x * (n + a.outer);
+    // lane (q, r): dW rows 4 q .. of the tile, column r
+#pragma unroll
+    for (int i = 0; i < S::HN; ++i)
+#pragma unroll
+        for (int j = 0; j < S::HK; ++j) {
+            const int fi = wn * S::HN + i, fj = wk * S::HK + j;
+            const int kk = fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int nn = fi / HT * KB<T> + ffn::perm<T>(fi % HT, 4 * q + e);
+                if (nn < a.outer && kk < a.inner) part[nn * a.inner + kk] = acc[i][j][e];
+            }
+        }
+    __syncthreads();
+    float* sums = reinterpret_cast<float*>(lds);   // [512 / NP][columns]
+#pragma unroll
+    for (int j = 0; j < E<T>; ++j) sums[tid / NP * (NP * E<T>) + cd + j] = db[j];
+    __syncthreads();
+    for (int c = tid; c < a.outer; c += 512) {
+        float t = 0.f;
+        for (int p = 0; p < 512 / NP; ++p) t += sums[p * NP * E<T> + c];
+        part[n + c] = t;
+    }
+}
+
 // How a backward call is split: dz by itself where an activation or another
 // type stands between it and dy, groups of rows for the sums over rows.
 struct Plan {
+    int fused;   // workgroups of the one pass, 0 for several
     bool own_dz;
     int64_t dz_bytes;
     int dz_tx, dz_groups;
@@ -841,9 +1030,20 @@ struct Plan {
     int64_t db_bytes, dw_bytes, dx_bytes;
     int64_t bytes() const { return dz_bytes + db_bytes + dw_bytes + dx_bytes; }
 };
+// Whether a workgroup of k_linear_bwd holds all of dW, beside W^T in LDS.
 template <class T>
-Plan plan(int64_t rows, int inner, int outer, bool own_dz) {
-    Plan p;
+bool one_pass(int inner, int outer) {
+    return sizeof(T) == 4 ? (outer <= 256 && inner <= 64) || (outer <= 64 && inner <= 256)
+                          : (outer <= 256 && inner <= 128) || (outer <= 128 && inner <= 256);
+}
+template <class T>
+Plan plan(int64_t rows, int inner, int outer, bool own_dz, bool same_type) {
+    Plan p{};
+    if (same_type && one_pass<T>(inner, outer)) {
+        p.fused = (int)std::min<int64_t>(ceil_div(rows, KB<T>), CUS);
+        p.dw_bytes = (int64_t)p.fused * (outer * inner + outer) * 4;
+        return p;
+    }
     p.own_dz = own_dz;
     p.dz_bytes = own_dz ? (rows * outer * (int64_t)sizeof(T) + 15) / 16 * 16 : 0;
     p.dz_tx = 1;
@@ -863,8 +1063,33 @@ Plan plan(int64_t rows, int inner, int outer, bool own_dz) {
 }
 
 template <class T>
+void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
+    float* part = a.dweight || a.dbias ? reinterpret_cast<float*>(a.ws) : nullptr;
+    auto launch = [&](auto shape) {
+        using S = decltype(shape);
+        const size_t lds = (size_t)S::n * S::k * sizeof(T) + 2 * KB<T> * (S::n + S::k) * sizeof(T);
+        auto run = [&](auto hasz, auto zmx, auto xmx) {
+            k_linear_bwd<T, S, hasz(), zmx(), xmx()><<<p.fused, 512, lds, s>>>(a, part);
+        };
+        constexpr std::true_type yes{};
+        constexpr std::false_type no{};
+        if (a.act == LINEAR_NONE) a.x_scales ? run(no, no, yes) : run(no, no, no);
+        else if (a.z_scales) a.x_scales ? run(yes, yes, yes) : run(yes, yes, no);
+        else a.x_scales ? run(yes, no, yes) : run(yes, no, no);
+    };
+    if (a.inner <= 64) launch(BwdShape<256, 64>{});
+    else if (a.outer <= 64) launch(BwdShape<64, 256>{});
+    else if constexpr (sizeof(T) == 2) {
+        if (a.inner <= 128) launch(BwdShape<256, 128>{});
+        else launch(BwdShape<128, 256>{});
+    }
+    if (part) fold<T>(s, part, p.fused, (int64_t)a.outer * a.inner, a.outer, a.dweight, a.dbias);
+}
+
+template <class T>
 void backward(hipStream_t s, const LinearGradArgs& a) {
-    const Plan p = plan<T>(a.rows, a.inner, a.outer, a.own_dz());
+    const Plan p = plan<T>(a.rows, a.inner, a.outer, a.own_dz(), a.y_dtype == a.dtype);
+    if (p.fused) return one_pass_backward<T>(s, a, p);
     T* dz = p.own_dz ? reinterpret_cast<T*>(a.ws) : nullptr;
     float* db_part = reinterpret_cast<float*>(a.ws + p.dz_bytes);
     float* dw_part = reinterpret_cast<float*>(a.ws + p.dz_bytes + p.db_bytes);
@@ -873,7 +1098,7 @@ void backward(hipStream_t s, const LinearGradArgs& a) {
         else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, dz, a.dbias ? db_part : nullptr, p.dz_tx, p.dz_rows);
     }
     if (a.dbias)
-        fold<T>(s, db_part, p.dz_groups, a.outer, a.dbias);
+        fold<T>(s, db_part, p.dz_groups, a.outer, 0, a.dbias, nullptr);
     const void* left = dz ? dz : a.dy;
     const int64_t left_stride = dz ? a.outer : a.dy_stride;
     if (a.dx && a.rows > 0) {
@@ -898,7 +1123,7 @@ void backward(hipStream_t s, const LinearGradArgs& a) {
         if (a.x_scales) k_linear_dw<T, true><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
         else k_linear_dw<T, false><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
     }
-    fold<T>(s, dw_part, p.dw_groups, (int64_t)a.outer * a.inner, a.dweight);
+    fold<T>(s, dw_part, p.dw_groups, (int64_t)a.outer * a.inner, 0, a.dweight, nullptr);
 }
 
 }  // namespace linear

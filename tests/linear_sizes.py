@@ -11,3 +11,8 @@ RESIDENT = [(1025, 20, 5), (1300, 50, 70), (1100, 90, 129), (2050, 120, 64), (15
 # weights streamed: each number of column blocks of a slice
 STREAMED = [(1025, 257, 20), (1100, 300, 50), (1600, 1000, 96), (1040, 333, 120), (1300, 270, 160), (1026, 520, 190),
             (1025, 1000, 200), (1090, 264, 256), (1200, 290, 290), (2200, 600, 3)]
+
+# weight gradients that one workgroup holds (each of its shapes), rows from less than
+# a block to several a workgroup
+ONE_PASS = [(7, 64, 256), (33, 60, 250), (2100, 33, 200), (9000, 64, 96), (500, 128, 256), (4500, 70, 130), (40, 256, 64),
+            (3000, 250, 50), (700, 256, 128), (5000, 129, 65), (20000, 8, 3)]

@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 import more_oracle as orc  # noqa: E402
-from linear_sizes import RESIDENT, SIZES, STREAMED  # noqa: E402
+from linear_sizes import ONE_PASS, RESIDENT, SIZES, STREAMED  # noqa: E402
 from nn_oracle import within  # noqa: E402
 from test_gpu_nn import DTYPES, IDS, _normal, _strided, nn  # noqa: E402,F401
 
@@ -79,17 +79,17 @@ def _check_backward(nn, dtype, rows, inner, outer, act, mx, out_dtype):
 
 
 @pytest.mark.parametrize("mx", [False, True], ids=["plain", "mx8"])
-@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED + ONE_PASS)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_backward(nn, dtype, rows, inner, outer, mx):
     for i, act in enumerate(ACTS):
-        out_dtype = DTYPES[(DTYPES.index(dtype) + i) % 3]
-        call, got = _check_backward(nn, dtype, rows, inner, outer, act, mx, out_dtype)
-        for k in range(3):
-            alone = nn.linear_backward(*call, wanted=tuple(j == k for j in range(3)))
-            assert all(t is None for j, t in enumerate(alone) if j != k)
-            assert torch.equal(alone[k], got[k]), f"gradient {k} by itself"
-        assert all(torch.equal(p, q) for p, q in zip(got, nn.linear_backward(*call)))
+        for out_dtype in {dtype, DTYPES[(DTYPES.index(dtype) + i) % 3]}:
+            call, got = _check_backward(nn, dtype, rows, inner, outer, act, mx, out_dtype)
+            for k in range(3):
+                alone = nn.linear_backward(*call, wanted=tuple(j == k for j in range(3)))
+                assert all(t is None for j, t in enumerate(alone) if j != k)
+                assert torch.equal(alone[k], got[k]), f"gradient {k} by itself"
+            assert all(torch.equal(p, q) for p, q in zip(got, nn.linear_backward(*call)))
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
