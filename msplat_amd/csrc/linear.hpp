@@ -837,11 +837,12 @@ __global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void*
 }
 
 // All gradients in one pass over dy, z and x, where a workgroup's registers hold all
-// of dW: eight waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  A block of KB
-// rows goes through LDS: dz is made of dy and z on the way in, its sums over rows
-// stay in registers, dW takes both blocks through transposing reads, and dx takes
-// dz's rows and W^T, which stays in LDS.  A block's reads are under way while the one
-// before is multiplied.
+// of dW: eight waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
+// KB rows at a time go through LDS: dz is made of dy and z on the way in, its sums
+// over rows stay in registers, dW takes both operands through transposing reads, and
+// dx takes dz's rows and W^T, which stays in LDS.  The next rows' reads are under way
+// while these are multiplied.  A wave's tiles are WN (WK) apart and tiles beyond the
+// matrix are left out, so that the matrix units share what there is.
 template <int N, int K>
 struct BwdShape {
     static constexpr int n = N, k = K;
@@ -880,29 +881,41 @@ struct Kept<T, true> {
     }
 };
 
+template <class T>
+constexpr int STEP = 2 * KB<T>;   // rows at a time
+// Columns of dx that one task makes, and where they are: two tiles of 16-bit results
+// side by side (column), one of 32-bit ones, so that a lane has a piece.
+template <class T>
+constexpr int TASK = 4 * E<T>;
+template <class T>
+__device__ __forceinline__ int dx_column(int tile, int r) {
+    return sizeof(T) == 4 ? tile * 16 + r : tile / 2 * COLS + column(tile % 2, r);
+}
+
 template <class T, class S, bool HASZ, bool ZMX, bool XMX>
 __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* part) {
-    constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = KB<T> / 16;
-    constexpr int PD = KB<T> * NP > 512 ? KB<T> * NP / 512 : 1, PX = KB<T> * KP > 512 ? KB<T> * KP / 512 : 1;
-    constexpr int HT = ffn::HT<T>, CB = S::k / COLS;
+    constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP<T> / 16;
+    constexpr int PD = STEP<T> * NP / 512 > 0 ? STEP<T> * NP / 512 : 1, PX = STEP<T> * KP / 512 > 0 ? STEP<T> * KP / 512 : 1;
+    constexpr int HT = ffn::HT<T>, KT = S::k / 16, TT = TASK<T> / 16;   // tiles of a block, of dx's columns, of a task
     extern __shared__ __attribute__((aligned(16))) char lds[];
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(lds);
-    piece_t<T>* ld = w + CB * 2 * NB * 64;         // two blocks of dz
-    piece_t<T>* lx = ld + 2 * KB<T> * NP;          // and of x
+    piece_t<T>* ld = w + KT * NB * 64;             // two steps of dz
+    piece_t<T>* lx = ld + 2 * STEP<T> * NP;        // and of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
     const int wn = wave / S::WK, wk = wave % S::WK;
+    const int nbs = (a.outer + KB<T> - 1) / KB<T>, ntiles = nbs * HT, ktiles = (a.inner + KB<T> - 1) / KB<T> * HT;
     if (a.dx) {
         LinearArgs t{};   // W^T [inner, outer]
         t.w = a.w;
         t.w_stride = a.w_stride;
         t.inner = a.outer;
         t.outer = a.inner;
-        for (int i = tid; i < CB * 2 * NB * 64; i += 512) {
-            const int f = i >> 6, kb = f % NB, s = f / NB % 2, cb = f / NB / 2;
-            w[i] = w_piece<T, false, true, false>(t, cb * COLS + column(s, i & 15), kb, (i >> 4) & 3);
+        for (int i = tid; i < KT * NB * 64; i += 512) {
+            const int f = i >> 6;
+            w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / NB, i & 15), f % NB, (i >> 4) & 3);
         }
     }
-    const int64_t blocks = (a.rows + KB<T> - 1) / KB<T>;
+    const int64_t steps = (a.rows + STEP<T> - 1) / STEP<T>;
     const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
     piece_t<T> dy[PD];
     Kept<T, ZMX> z[PD];
@@ -910,27 +923,27 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     auto read = [&](int64_t b) {
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
-            const int64_t row = min(b * KB<T> + min(tid / NP + p * (512 / NP), KB<T> - 1), a.rows - 1);
+            const int64_t row = min(b * STEP<T> + min(tid / NP + p * (512 / NP), STEP<T> - 1), a.rows - 1);
             const T* at = static_cast<const T*>(a.dy) + row * a.dy_stride;
             dy[p] = a.outer < E<T> ? load_piece(at, cd, a.outer) : read_piece(at, cd, a.outer);
             if (HASZ) z[p].read(a.z, a.z_stride, a.z_scales, row, cd, a.outer);
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p)
-            x[p].read(a.x, a.x_stride, a.x_scales, min(b * KB<T> + min(tid / KP + p * (512 / KP), KB<T> - 1), a.rows - 1), cx,
-                      a.inner);
+            x[p].read(a.x, a.x_stride, a.x_scales,
+                      min(b * STEP<T> + min(tid / KP + p * (512 / KP), STEP<T> - 1), a.rows - 1), cx, a.inner);
     };
     f32x4 acc[S::HN][S::HK] = {};
     float db[E<T>] = {};
     read(blockIdx.x);
     int turn = 0;
-    for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x, turn ^= 1) {
-        piece_t<T>* bd = ld + turn * KB<T> * NP;
-        piece_t<T>* bx = lx + turn * KB<T> * KP;
+    for (int64_t b = blockIdx.x; b < steps; b += gridDim.x, turn ^= 1) {
+        piece_t<T>* bd = ld + turn * STEP<T> * NP;
+        piece_t<T>* bx = lx + turn * STEP<T> * KP;
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
             const int rho = tid / NP + p * (512 / NP);
-            const bool live = b * KB<T> + rho < a.rows;
+            const bool live = b * STEP<T> + rho < a.rows;
             const piece_t<T> g = a.outer < E<T> ? dy[p] : settle_piece<T>(dy[p], cd, a.outer, true);
             float f[E<T>];
             if (HASZ) z[p].values(cd, a.outer, f);
@@ -940,53 +953,60 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
                 float v = (float)g[j];
                 if (HASZ) v *= slope(f[j], a.act);
                 v = live ? v : 0.f;
-                if (rho < KB<T>) db[j] += v;
+                if (rho < STEP<T>) db[j] += v;
                 o[j] = (T)v;
             }
-            if (rho < KB<T>) bd[staged<T>(rho, tid % NP)] = o;
+            if (rho < STEP<T>) bd[rho / KB<T> * (KB<T> * NP) + staged<T>(rho % KB<T>, tid % NP)] = o;
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
             const int rho = tid / KP + p * (512 / KP);
-            const bool live = b * KB<T> + rho < a.rows;
+            const bool live = b * STEP<T> + rho < a.rows;
             float f[E<T>];
             x[p].values(cx, a.inner, f);
             piece_t<T> o;
 #pragma unroll
             for (int j = 0; j < E<T>; ++j) o[j] = (T)(live ? f[j] : 0.f);
-            if (rho < KB<T>) bx[staged<T>(rho, tid % KP)] = o;
+            if (rho < STEP<T>) bx[rho / KB<T> * (KB<T> * KP) + staged<T>(rho % KB<T>, tid % KP)] = o;
         }
         read(b + gridDim.x);
-        // one barrier a block: who is a block ahead writes the other buffers
+        // one barrier a step: who is a step ahead writes the other buffers
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (a.dweight) {
-            piece_t<T> fx[S::HK];
+        if (a.dweight)
 #pragma unroll
-            for (int j = 0; j < S::HK; ++j) fx[j] = ffn::by_dim<T>(bx, wk * S::HK + j);
+            for (int h = 0; h < 2; ++h) {
+                piece_t<T> fx[S::HK];
 #pragma unroll
-            for (int i = 0; i < S::HN; ++i) {
-                const piece_t<T> fd = ffn::by_dim<T>(bd, wn * S::HN + i);
+                for (int j = 0; j < S::HK; ++j)
+                    if (j * S::WK + wk < ktiles) fx[j] = ffn::by_dim<T>(bx + h * KB<T> * KP, j * S::WK + wk);
 #pragma unroll
-                for (int j = 0; j < S::HK; ++j) acc[i][j] = mma(fd, fx[j], acc[i][j]);
-            }
-        }
-        if (a.dx)
-            for (int t = wave; t < CB * RT; t += 8) {
-                const int cb = t / RT, tile = t % RT;
-                if (cb * COLS >= a.inner) break;
-                f32x4 o[2] = {};
+                for (int i = 0; i < S::HN; ++i) {
+                    if (i * S::WN + wn < ntiles) {
+                        const piece_t<T> fd = ffn::by_dim<T>(bd + h * KB<T> * NP, i * S::WN + wn);
 #pragma unroll
-                for (int kb = 0; kb < NB; ++kb) {
-                    const piece_t<T> fd = ffn::by_row<T>(bd, kb * HT + tile);
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) o[s] = mma(w[((cb * 2 + s) * NB + kb) * 64 + lane], fd, o[s]);
+                        for (int j = 0; j < S::HK; ++j)
+                            if (j * S::WK + wk < ktiles) acc[i][j] = mma(fd, fx[j], acc[i][j]);
+                    }
                 }
-                float v[8];
+            }
+        if (a.dx)
+            for (int t = wave; t < KT / TT * RT; t += 8) {
+                const int task = t / RT, tile = t % RT;   // columns, and 16 rows
+                if (task * TASK<T> >= a.inner) break;
+                const piece_t<T>* rows = bd + tile / HT * (KB<T> * NP);
+                f32x4 o[TT] = {};
+#pragma unroll 4
+                for (int kb = 0; kb < nbs; ++kb) {
+                    const piece_t<T> fd = ffn::by_row<T>(rows, kb * HT + tile % HT);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = o[j / 4][j % 4];
-                const int64_t row = b * KB<T> + ffn::perm<T>(tile, r);
-                const int col = cb * COLS + q * 8;
-                if (row < a.rows && col < a.inner) store8(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
+                    for (int s = 0; s < TT; ++s) o[s] = mma(w[((task * TT + s) * NB + kb) * 64 + lane], fd, o[s]);
+                }
+                piece_t<T> v;
+#pragma unroll
+                for (int j = 0; j < E<T>; ++j) v[j] = (T)o[j / 4][j % 4];
+                const int64_t row = b * STEP<T> + tile / HT * KB<T> + ffn::perm<T>(tile % HT, r);
+                const int col = task * TASK<T> + q * E<T>;
+                if (row < a.rows && col < a.inner) store_piece(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
             }
     }
     if (!part) return;
@@ -997,7 +1017,7 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     for (int i = 0; i < S::HN; ++i)
 #pragma unroll
         for (int j = 0; j < S::HK; ++j) {
-            const int fi = wn * S::HN + i, fj = wk * S::HK + j;
+            const int fi = i * S::WN + wn, fj = j * S::WK + wk;
             const int kk = fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -1040,7 +1060,7 @@ template <class T>
 Plan plan(int64_t rows, int inner, int outer, bool own_dz, bool same_type) {
     Plan p{};
     if (same_type && one_pass<T>(inner, outer)) {
-        p.fused = (int)std::min<int64_t>(ceil_div(rows, KB<T>), CUS);
+        p.fused = (int)std::min<int64_t>(ceil_div(rows, STEP<T>), CUS);
         p.dw_bytes = (int64_t)p.fused * (outer * inner + outer) * 4;
         return p;
     }
@@ -1067,7 +1087,7 @@ void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
     float* part = a.dweight || a.dbias ? reinterpret_cast<float*>(a.ws) : nullptr;
     auto launch = [&](auto shape) {
         using S = decltype(shape);
-        const size_t lds = (size_t)S::n * S::k * sizeof(T) + 2 * KB<T> * (S::n + S::k) * sizeof(T);
+        const size_t lds = (size_t)S::n * S::k * sizeof(T) + 2 * STEP<T> * (S::n + S::k) * sizeof(T);
         auto run = [&](auto hasz, auto zmx, auto xmx) {
             k_linear_bwd<T, S, hasz(), zmx(), xmx()><<<p.fused, 512, lds, s>>>(a, part);
         };
