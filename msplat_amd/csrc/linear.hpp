@@ -140,16 +140,15 @@ __device__ __forceinline__ void activate(int act, float (&v)[N]) {
 }
 
 // a'(v); large GELU arguments as in ffn::act_grad.
-__device__ __forceinline__ float slope(float v, int act) {
-    if (act == LINEAR_SILU) {
+template <int ACT>
+__device__ __forceinline__ float slope(float v) {
+    if (ACT == LINEAR_NONE) return 1.f;
+    if (ACT == LINEAR_SILU) {
         const float s = ffn::sigmoid_fast(v);
         return fmaf(v * s, 1.f - s, s);
     }
-    if (act == LINEAR_GELU) {
-        const float s = ffn::sigmoid_fast(v * fmaf(v * v, ffn::GELU_B, ffn::GELU_A));
-        return fmaf(v * s * (1.f - s), fmaf(fminf(v * v, 1e38f), 3.f * ffn::GELU_B, ffn::GELU_A), s);
-    }
-    return 1.f;
+    const float s = ffn::sigmoid_fast(v * fmaf(v * v, ffn::GELU_B, ffn::GELU_A));
+    return fmaf(v * s * (1.f - s), fmaf(fminf(v * v, 1e38f), 3.f * ffn::GELU_B, ffn::GELU_A), s);
 }
 
 // Eight columns from `col` < n on of a row, zeros from n on, in 32 bits.  Where 8
@@ -701,7 +700,7 @@ __global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, floa
                         load8(static_cast<const T*>(a.z) + row * a.z_stride, col, a.outer, z);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] *= slope(z[j], a.act);
+                    for (int j = 0; j < 8; ++j) v[j] *= a.act == LINEAR_SILU ? slope<LINEAR_SILU>(z[j]) : slope<LINEAR_GELU>(z[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[j] += v[j];
@@ -840,9 +839,11 @@ __global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void*
 // of dW: eight waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
 // KB rows at a time go through LDS: dz is made of dy and z on the way in, its sums
 // over rows stay in registers, dW takes both operands through transposing reads, and
-// dx takes dz's rows and W^T, which stays in LDS.  The next rows' reads are under way
-// while these are multiplied.  A wave's tiles are WN (WK) apart and tiles beyond the
-// matrix are left out, so that the matrix units share what there is.
+// dx takes dz's rows and W^T, which stays in LDS.  A SIMD has two waves: one multiplies
+// a step and then makes dz of the next, the other does it in the other order, so that
+// vector and matrix units work at once.  A wave's tiles are WN (WK) apart and tiles
+// beyond the matrix are left out, so that the matrix units share what there is.
+constexpr int RB = 2;
 template <int N, int K>
 struct BwdShape {
     static constexpr int n = N, k = K;
@@ -881,8 +882,6 @@ struct Kept<T, true> {
     }
 };
 
-template <class T>
-constexpr int STEP = 2 * KB<T>;   // rows at a time
 // Columns of dx that one task makes, and where they are: two tiles of 16-bit results
 // side by side (column), one of 32-bit ones, so that a lane has a piece.
 template <class T>
@@ -892,30 +891,38 @@ __device__ __forceinline__ int dx_column(int tile, int r) {
     return sizeof(T) == 4 ? tile * 16 + r : tile / 2 * COLS + column(tile % 2, r);
 }
 
-template <class T, class S, bool HASZ, bool ZMX, bool XMX>
+template <class T>
+__host__ __device__ inline int dx_tiles(int inner) {
+    return (inner + TASK<T> - 1) / TASK<T> * (TASK<T> / 16);
+}
+
+template <class T, class S, int ACT, bool ZMX, bool XMX>
 __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* part) {
-    constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP<T> / 16;
-    constexpr int PD = STEP<T> * NP / 512 > 0 ? STEP<T> * NP / 512 : 1, PX = STEP<T> * KP / 512 > 0 ? STEP<T> * KP / 512 : 1;
-    constexpr int HT = ffn::HT<T>, KT = S::k / 16, TT = TASK<T> / 16;   // tiles of a block, of dx's columns, of a task
+    constexpr int STEP = RB * KB<T>;
+    constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP / 16;
+    constexpr int PD = STEP * NP / 512 > 0 ? STEP * NP / 512 : 1, PX = STEP * KP / 512 > 0 ? STEP * KP / 512 : 1;
+    constexpr int HT = ffn::HT<T>, TT = TASK<T> / 16;   // tiles of a block, of a task
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    // live blocks of outputs and inputs, tiles of them, pieces of a block of rows
+    const int nbs = (a.outer + KB<T> - 1) / KB<T>, ntiles = nbs * HT, nblock = nbs * KB<T> * 4;
+    const int kbs = (a.inner + KB<T> - 1) / KB<T>, ktiles = kbs * HT, kblock = kbs * KB<T> * 4;
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(lds);
-    piece_t<T>* ld = w + KT * NB * 64;             // two steps of dz
-    piece_t<T>* lx = ld + 2 * STEP<T> * NP;        // and of x
+    piece_t<T>* ld = w + (a.dx ? dx_tiles<T>(a.inner) * nbs * 64 : 0);   // two steps of dz
+    piece_t<T>* lx = ld + 2 * RB * nblock;                              // and of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
     const int wn = wave / S::WK, wk = wave % S::WK;
-    const int nbs = (a.outer + KB<T> - 1) / KB<T>, ntiles = nbs * HT, ktiles = (a.inner + KB<T> - 1) / KB<T> * HT;
     if (a.dx) {
         LinearArgs t{};   // W^T [inner, outer]
         t.w = a.w;
         t.w_stride = a.w_stride;
         t.inner = a.outer;
         t.outer = a.inner;
-        for (int i = tid; i < KT * NB * 64; i += 512) {
+        for (int i = tid; i < dx_tiles<T>(a.inner) * nbs * 64; i += 512) {
             const int f = i >> 6;
-            w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / NB, i & 15), f % NB, (i >> 4) & 3);
+            w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / nbs, i & 15), f % nbs, (i >> 4) & 3);
         }
     }
-    const int64_t steps = (a.rows + STEP<T> - 1) / STEP<T>;
+    const int64_t steps = (a.rows + STEP - 1) / STEP;
     const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
     piece_t<T> dy[PD];
     Kept<T, ZMX> z[PD];
@@ -923,91 +930,114 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     auto read = [&](int64_t b) {
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
-            const int64_t row = min(b * STEP<T> + min(tid / NP + p * (512 / NP), STEP<T> - 1), a.rows - 1);
+            const int64_t row = min(b * STEP + min(tid / NP + p * (512 / NP), STEP - 1), a.rows - 1);
             const T* at = static_cast<const T*>(a.dy) + row * a.dy_stride;
             dy[p] = a.outer < E<T> ? load_piece(at, cd, a.outer) : read_piece(at, cd, a.outer);
-            if (HASZ) z[p].read(a.z, a.z_stride, a.z_scales, row, cd, a.outer);
+            if (ACT != LINEAR_NONE) z[p].read(a.z, a.z_stride, a.z_scales, row, cd, a.outer);
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p)
             x[p].read(a.x, a.x_stride, a.x_scales,
-                      min(b * STEP<T> + min(tid / KP + p * (512 / KP), STEP<T> - 1), a.rows - 1), cx, a.inner);
+                      min(b * STEP + min(tid / KP + p * (512 / KP), STEP - 1), a.rows - 1), cx, a.inner);
     };
     f32x4 acc[S::HN][S::HK] = {};
     float db[E<T>] = {};
-    read(blockIdx.x);
-    int turn = 0;
-    for (int64_t b = blockIdx.x; b < steps; b += gridDim.x, turn ^= 1) {
-        piece_t<T>* bd = ld + turn * STEP<T> * NP;
-        piece_t<T>* bx = lx + turn * STEP<T> * KP;
+    int first = 0;
+    // dz and x of step b into LDS
+    auto form = [&](int64_t b, int turn) {
+        piece_t<T>* bd = ld + turn * RB * nblock;
+        piece_t<T>* bx = lx + turn * RB * kblock;
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
             const int rho = tid / NP + p * (512 / NP);
-            const bool live = b * STEP<T> + rho < a.rows;
+            const bool live = b * STEP + rho < a.rows;
             const piece_t<T> g = a.outer < E<T> ? dy[p] : settle_piece<T>(dy[p], cd, a.outer, true);
             float f[E<T>];
-            if (HASZ) z[p].values(cd, a.outer, f);
+            if (ACT != LINEAR_NONE) z[p].values(cd, a.outer, f);
             piece_t<T> o;
 #pragma unroll
             for (int j = 0; j < E<T>; ++j) {
                 float v = (float)g[j];
-                if (HASZ) v *= slope(f[j], a.act);
+                v *= slope<ACT>(f[j]);
                 v = live ? v : 0.f;
-                if (rho < STEP<T>) db[j] += v;
+                if (rho < STEP) db[j] += v;
                 o[j] = (T)v;
             }
-            if (rho < STEP<T>) bd[rho / KB<T> * (KB<T> * NP) + staged<T>(rho % KB<T>, tid % NP)] = o;
+            if (rho < STEP && tid % NP < nbs * 4) bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
             const int rho = tid / KP + p * (512 / KP);
-            const bool live = b * STEP<T> + rho < a.rows;
+            const bool live = b * STEP + rho < a.rows;
             float f[E<T>];
             x[p].values(cx, a.inner, f);
             piece_t<T> o;
 #pragma unroll
             for (int j = 0; j < E<T>; ++j) o[j] = (T)(live ? f[j] : 0.f);
-            if (rho < STEP<T>) bx[rho / KB<T> * (KB<T> * KP) + staged<T>(rho % KB<T>, tid % KP)] = o;
+            if (rho < STEP && tid % KP < kbs * 4) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
         }
-        read(b + gridDim.x);
-        // one barrier a step: who is a step ahead writes the other buffers
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    // the products of step b
+    auto multiply = [&](int64_t b, int turn) {
+        const piece_t<T>* bd = ld + turn * RB * nblock;
+        const piece_t<T>* bx = lx + turn * RB * kblock;
         if (a.dweight)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < RB; ++h) {
                 piece_t<T> fx[S::HK];
 #pragma unroll
                 for (int j = 0; j < S::HK; ++j)
-                    if (j * S::WK + wk < ktiles) fx[j] = ffn::by_dim<T>(bx + h * KB<T> * KP, j * S::WK + wk);
+                    if (j * S::WK + wk < ktiles) fx[j] = ffn::by_dim<T>(bx + h * kblock, j * S::WK + wk);
 #pragma unroll
                 for (int i = 0; i < S::HN; ++i) {
                     if (i * S::WN + wn < ntiles) {
-                        const piece_t<T> fd = ffn::by_dim<T>(bd + h * KB<T> * NP, i * S::WN + wn);
+                        const piece_t<T> fd = ffn::by_dim<T>(bd + h * nblock, i * S::WN + wn);
 #pragma unroll
                         for (int j = 0; j < S::HK; ++j)
                             if (j * S::WK + wk < ktiles) acc[i][j] = mma(fd, fx[j], acc[i][j]);
                     }
                 }
             }
-        if (a.dx)
-            for (int t = wave; t < KT / TT * RT; t += 8) {
+        if (a.dx) {
+            // tasks go round the waves from step to step
+            const int tasks = dx_tiles<T>(a.inner) / TT * RT;
+            for (int t = (wave + first) & 7; t < tasks; t += 8) {
                 const int task = t / RT, tile = t % RT;   // columns, and 16 rows
-                if (task * TASK<T> >= a.inner) break;
-                const piece_t<T>* rows = bd + tile / HT * (KB<T> * NP);
+                const piece_t<T>* rows = bd + tile / HT * nblock;
                 f32x4 o[TT] = {};
-#pragma unroll 4
+#pragma unroll 2
                 for (int kb = 0; kb < nbs; ++kb) {
                     const piece_t<T> fd = ffn::by_row<T>(rows, kb * HT + tile % HT);
 #pragma unroll
-                    for (int s = 0; s < TT; ++s) o[s] = mma(w[((task * TT + s) * NB + kb) * 64 + lane], fd, o[s]);
+                    for (int s = 0; s < TT; ++s) o[s] = mma(w[((task * TT + s) * nbs + kb) * 64 + lane], fd, o[s]);
                 }
                 piece_t<T> v;
 #pragma unroll
                 for (int j = 0; j < E<T>; ++j) v[j] = (T)o[j / 4][j % 4];
-                const int64_t row = b * STEP<T> + tile / HT * KB<T> + ffn::perm<T>(tile % HT, r);
+                const int64_t row = b * STEP + tile / HT * KB<T> + ffn::perm<T>(tile % HT, r);
                 const int col = task * TASK<T> + q * E<T>;
                 if (row < a.rows && col < a.inner) store_piece(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
             }
+            first += tasks;
+        }
+    };
+    int turn = 0;
+    read(blockIdx.x);
+    form(blockIdx.x, 0);
+    read((int64_t)blockIdx.x + gridDim.x);
+    for (int64_t b = blockIdx.x; b < steps; b += gridDim.x, turn ^= 1) {
+        // one barrier a step: the other buffers' readers have passed it
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int64_t next = b + gridDim.x;
+        if (wave < 4) {
+            multiply(b, turn);
+            if (next < steps) form(next, turn ^ 1);
+            read(next + gridDim.x);
+        } else {
+            if (next < steps) form(next, turn ^ 1);
+            read(next + gridDim.x);
+            multiply(b, turn);
+        }
     }
     if (!part) return;
     const int64_t n = (int64_t)a.outer * a.inner;
@@ -1041,6 +1071,7 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
 // type stands between it and dy, groups of rows for the sums over rows.
 struct Plan {
     int fused;   // workgroups of the one pass, 0 for several
+    size_t lds;
     bool own_dz;
     int64_t dz_bytes;
     int dz_tx, dz_groups;
@@ -1060,7 +1091,10 @@ template <class T>
 Plan plan(int64_t rows, int inner, int outer, bool own_dz, bool same_type) {
     Plan p{};
     if (same_type && one_pass<T>(inner, outer)) {
-        p.fused = (int)std::min<int64_t>(ceil_div(rows, STEP<T>), CUS);
+        const int64_t n = ceil_div(outer, KB<T>) * KB<T>, k = ceil_div(inner, KB<T>) * KB<T>;
+        // W^T, two steps of dz and x; the sums of db at the end
+        p.lds = (size_t)std::max<int64_t>((n * dx_tiles<T>(inner) * 16 + 2 * RB * KB<T> * (n + k)) * sizeof(T), 512 * E<T> * 4);
+        p.fused = (int)std::min<int64_t>(ceil_div(rows, RB * KB<T>), CUS);
         p.dw_bytes = (int64_t)p.fused * (outer * inner + outer) * 4;
         return p;
     }
@@ -1087,15 +1121,17 @@ void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
     float* part = a.dweight || a.dbias ? reinterpret_cast<float*>(a.ws) : nullptr;
     auto launch = [&](auto shape) {
         using S = decltype(shape);
-        const size_t lds = (size_t)S::n * S::k * sizeof(T) + 2 * STEP<T> * (S::n + S::k) * sizeof(T);
-        auto run = [&](auto hasz, auto zmx, auto xmx) {
-            k_linear_bwd<T, S, hasz(), zmx(), xmx()><<<p.fused, 512, lds, s>>>(a, part);
+        auto run = [&](auto act, auto zmx) {
+            if (a.x_scales) k_linear_bwd<T, S, act(), zmx(), true><<<p.fused, 512, p.lds, s>>>(a, part);
+            else k_linear_bwd<T, S, act(), zmx(), false><<<p.fused, 512, p.lds, s>>>(a, part);
         };
-        constexpr std::true_type yes{};
-        constexpr std::false_type no{};
-        if (a.act == LINEAR_NONE) a.x_scales ? run(no, no, yes) : run(no, no, no);
-        else if (a.z_scales) a.x_scales ? run(yes, yes, yes) : run(yes, yes, no);
-        else a.x_scales ? run(yes, no, yes) : run(yes, no, no);
+        auto kept = [&](auto act) {
+            if (a.z_scales) run(act, std::true_type{});
+            else run(act, std::false_type{});
+        };
+        if (a.act == LINEAR_NONE) run(std::integral_constant<int, LINEAR_NONE>{}, std::false_type{});
+        else if (a.act == LINEAR_SILU) kept(std::integral_constant<int, LINEAR_SILU>{});
+        else kept(std::integral_constant<int, LINEAR_GELU>{});
     };
     if (a.inner <= 64) launch(BwdShape<256, 64>{});
     else if (a.outer <= 64) launch(BwdShape<64, 256>{});
