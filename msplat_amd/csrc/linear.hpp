@@ -851,35 +851,65 @@ struct BwdShape {
     static constexpr int WN = N >= 256 ? 8 : N >= 2 * K ? 8 : N * 2 <= K ? 1 : 4, WK = 8 / WN;
     static constexpr int HN = N / 16 / WN, HK = K / 16 / WK;
 };
+// Pieces of a matrix on their way in, the same columns of many rows.
 template <class T, bool MX>
-struct Kept {   // a piece of a kept matrix on its way in
-    piece_t<T> v;
-    __device__ __forceinline__ void read(const void* base, int64_t stride, const uint8_t*, int64_t row, int col, int n) {
-        const T* at = static_cast<const T*>(base) + row * stride;
-        v = n < E<T> ? load_piece(at, col, n) : read_piece(at, col, n);
+struct Kept {
+    const T* at;   // the piece in row 0; the last ends with the row
+    __device__ __forceinline__ Kept(const void* base, const uint8_t*, int col, int n)
+        : at(static_cast<const T*>(base) + max(min(col, n - E<T>), 0)) {}
+    struct Raw {
+        piece_t<T> v;
+    };
+    // offset: the row's, in elements
+    __device__ __forceinline__ void read(Raw& r, int64_t offset, int64_t, int n) const {
+        if (n >= E<T>) __builtin_memcpy(&r.v, at + offset, 16);
+        else r.v = load_piece(at + offset, 0, n);
     }
-    // in 32 bits, zeros from n on
-    __device__ __forceinline__ void values(int col, int n, float (&f)[E<T>]) const {
-        const piece_t<T> p = n < E<T> ? v : settle_piece<T>(v, col, n, true);
+    // the piece itself, zeros from n on where it begins before n
+    static __device__ __forceinline__ piece_t<T> piece(const Raw& r, int col, int n) {
+        return n % E<T> != 0 && n >= E<T> && col > n - E<T> ? moved_down<T>(r.v, E<T> - n % E<T>) : r.v;
+    }
+    static __device__ __forceinline__ void values(const Raw& r, int col, int n, float (&f)[E<T>]) {
+        const piece_t<T> p = piece(r, col, n);
 #pragma unroll
         for (int j = 0; j < E<T>; ++j) f[j] = (float)p[j];
     }
+    static __device__ __forceinline__ int64_t scale_offset(int64_t, int) { return 0; }
+    static __device__ __forceinline__ int64_t stride(int64_t s, int) { return s; }
 };
 template <class T>
 struct Kept<T, true> {
-    uint32_t bytes[E<T> / 4];
-    int code;
-    __device__ __forceinline__ void read(const void* base, int64_t, const uint8_t* scales, int64_t row, int col, int n) {
+    const uint8_t *at, *scale;
+    __device__ __forceinline__ Kept(const void* base, const uint8_t* scales, int col, int n) {
         col = min(col, (int)mx8::data_stride(n) - E<T>);
-        __builtin_memcpy(bytes, static_cast<const uint8_t*>(base) + row * mx8::data_stride(n) + col, E<T>);
-        code = scales[row * mx8::scale_stride(n) + col / mx8::BLOCK];
+        at = static_cast<const uint8_t*>(base) + col;
+        scale = scales + col / mx8::BLOCK;
     }
-    __device__ __forceinline__ void values(int col, int n, float (&f)[E<T>]) const {
-        mx8::values<T>(bytes, code, f);
+    struct Raw {
+        uint32_t bytes[E<T> / 4];
+        int code;
+    };
+    __device__ __forceinline__ void read(Raw& r, int64_t offset, int64_t scale_offset, int) const {
+        __builtin_memcpy(r.bytes, at + offset, E<T>);
+        r.code = scale[scale_offset];
+    }
+    static __device__ __forceinline__ void values(const Raw& r, int col, int n, float (&f)[E<T>]) {
+        mx8::values<T>(r.bytes, r.code, f);
+        if (n % E<T> != 0)   // zeros by the format, NaN where their block's scale is
 #pragma unroll
-        for (int j = 0; j < E<T>; ++j)
-            if (col + j >= n) f[j] = 0.f;
+            for (int j = 0; j < E<T>; ++j)
+                if (col + j >= n) f[j] = 0.f;
     }
+    static __device__ __forceinline__ piece_t<T> piece(const Raw& r, int col, int n) {
+        float f[E<T>];
+        values(r, col, n, f);
+        piece_t<T> o;
+#pragma unroll
+        for (int j = 0; j < E<T>; ++j) o[j] = (T)f[j];
+        return o;
+    }
+    static __device__ __forceinline__ int64_t scale_offset(int64_t row, int n) { return row * mx8::scale_stride(n); }
+    static __device__ __forceinline__ int64_t stride(int64_t, int n) { return mx8::data_stride(n); }
 };
 
 // Columns of dx that one task makes, and where they are: two tiles of 16-bit results
@@ -922,23 +952,47 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
             w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / nbs, i & 15), f % nbs, (i >> 4) & 3);
         }
     }
+    // pieces behind the matrices stay zero
+    for (int i = tid; i < 2 * RB * (nblock + kblock); i += 512) ld[i] = piece_t<T>{};
+    __syncthreads();
     const int64_t steps = (a.rows + STEP - 1) / STEP;
     const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
-    piece_t<T> dy[PD];
-    Kept<T, ZMX> z[PD];
-    Kept<T, XMX> x[PX];
+    const Kept<T, false> fy(a.dy, nullptr, cd, a.outer);
+    const Kept<T, ZMX> fz(a.z, a.z_scales, cd, a.outer);
+    const Kept<T, XMX> fx(a.x, a.x_scales, cx, a.inner);
+    typename Kept<T, false>::Raw dy[PD];
+    typename Kept<T, ZMX>::Raw z[PD];
+    typename Kept<T, XMX>::Raw x[PX];
+    const int64_t zstride = fz.stride(a.z_stride, a.outer), xstride = fx.stride(a.x_stride, a.inner);
+    const int rd = min(tid / NP, STEP - 1), rx = min(tid / KP, STEP - 1);
+    // rows of a whole step are the step's, uniform, and the thread's
     auto read = [&](int64_t b) {
+        const int64_t row0 = b * STEP;
+        const bool whole = row0 + STEP <= a.rows;
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
-            const int64_t row = min(b * STEP + min(tid / NP + p * (512 / NP), STEP - 1), a.rows - 1);
-            const T* at = static_cast<const T*>(a.dy) + row * a.dy_stride;
-            dy[p] = a.outer < E<T> ? load_piece(at, cd, a.outer) : read_piece(at, cd, a.outer);
-            if (ACT != LINEAR_NONE) z[p].read(a.z, a.z_stride, a.z_scales, row, cd, a.outer);
+            if (whole) {
+                const int64_t row = row0 + p * (512 / NP);
+                fy.read(dy[p], row * a.dy_stride + rd * a.dy_stride, 0, a.outer);
+                if (ACT != LINEAR_NONE)
+                    fz.read(z[p], row * zstride + rd * zstride, fz.scale_offset(row, a.outer) + fz.scale_offset(rd, a.outer),
+                            a.outer);
+            } else {
+                const int64_t row = min(row0 + rd + p * (512 / NP), a.rows - 1);
+                fy.read(dy[p], row * a.dy_stride, 0, a.outer);
+                if (ACT != LINEAR_NONE) fz.read(z[p], row * zstride, fz.scale_offset(row, a.outer), a.outer);
+            }
         }
 #pragma unroll
-        for (int p = 0; p < PX; ++p)
-            x[p].read(a.x, a.x_stride, a.x_scales,
-                      min(b * STEP + min(tid / KP + p * (512 / KP), STEP - 1), a.rows - 1), cx, a.inner);
+        for (int p = 0; p < PX; ++p) {
+            if (whole) {
+                const int64_t row = row0 + p * (512 / KP);
+                fx.read(x[p], row * xstride + rx * xstride, fx.scale_offset(row, a.inner) + fx.scale_offset(rx, a.inner), a.inner);
+            } else {
+                const int64_t row = min(row0 + rx + p * (512 / KP), a.rows - 1);
+                fx.read(x[p], row * xstride, fx.scale_offset(row, a.inner), a.inner);
+            }
+        }
     };
     f32x4 acc[S::HN][S::HK] = {};
     float db[E<T>] = {};
@@ -947,34 +1001,35 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     auto form = [&](int64_t b, int turn) {
         piece_t<T>* bd = ld + turn * RB * nblock;
         piece_t<T>* bx = lx + turn * RB * kblock;
+        const int live = (int)min(a.rows - b * STEP, (int64_t)STEP);
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
             const int rho = tid / NP + p * (512 / NP);
-            const bool live = b * STEP + rho < a.rows;
-            const piece_t<T> g = a.outer < E<T> ? dy[p] : settle_piece<T>(dy[p], cd, a.outer, true);
-            float f[E<T>];
-            if (ACT != LINEAR_NONE) z[p].values(cd, a.outer, f);
+            float v[E<T>];
+            fy.values(dy[p], cd, a.outer, v);
+            if (ACT != LINEAR_NONE) {
+                float f[E<T>];
+                fz.values(z[p], cd, a.outer, f);
+#pragma unroll
+                for (int j = 0; j < E<T>; ++j) v[j] *= slope<ACT>(f[j]);
+            }
+            if (live < STEP)
+#pragma unroll
+                for (int j = 0; j < E<T>; ++j) v[j] = rho < live ? v[j] : 0.f;
             piece_t<T> o;
 #pragma unroll
             for (int j = 0; j < E<T>; ++j) {
-                float v = (float)g[j];
-                v *= slope<ACT>(f[j]);
-                v = live ? v : 0.f;
-                if (rho < STEP) db[j] += v;
-                o[j] = (T)v;
+                if (STEP * NP >= 512 || rho < STEP) db[j] += v[j];
+                o[j] = (T)v[j];
             }
-            if (rho < STEP && tid % NP < nbs * 4) bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
+            if (rho < STEP && cd < a.outer) bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
             const int rho = tid / KP + p * (512 / KP);
-            const bool live = b * STEP + rho < a.rows;
-            float f[E<T>];
-            x[p].values(cx, a.inner, f);
-            piece_t<T> o;
-#pragma unroll
-            for (int j = 0; j < E<T>; ++j) o[j] = (T)(live ? f[j] : 0.f);
-            if (rho < STEP && tid % KP < kbs * 4) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
+            piece_t<T> o = fx.piece(x[p], cx, a.inner);
+            if (rho >= live) o = piece_t<T>{};
+            if (rho < STEP && cx < a.inner) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
         }
     };
     // the products of step b
@@ -984,17 +1039,17 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
         if (a.dweight)
 #pragma unroll
             for (int h = 0; h < RB; ++h) {
-                piece_t<T> fx[S::HK];
+                piece_t<T> xs[S::HK];
 #pragma unroll
                 for (int j = 0; j < S::HK; ++j)
-                    if (j * S::WK + wk < ktiles) fx[j] = ffn::by_dim<T>(bx + h * kblock, j * S::WK + wk);
+                    if (j * S::WK + wk < ktiles) xs[j] = ffn::by_dim<T>(bx + h * kblock, j * S::WK + wk);
 #pragma unroll
                 for (int i = 0; i < S::HN; ++i) {
                     if (i * S::WN + wn < ntiles) {
                         const piece_t<T> fd = ffn::by_dim<T>(bd + h * nblock, i * S::WN + wn);
 #pragma unroll
                         for (int j = 0; j < S::HK; ++j)
-                            if (j * S::WK + wk < ktiles) acc[i][j] = mma(fd, fx[j], acc[i][j]);
+                            if (j * S::WK + wk < ktiles) acc[i][j] = mma(fd, xs[j], acc[i][j]);
                     }
                 }
             }
