@@ -836,19 +836,19 @@ __global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void*
 }
 
 // All gradients in one pass over dy, z and x, where a workgroup's registers hold all
-// of dW: eight waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
+// of dW: 16 waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
 // KB rows at a time go through LDS: dz is made of dy and z on the way in, its sums
 // over rows stay in registers, dW takes both operands through transposing reads, and
-// dx takes dz's rows and W^T, which stays in LDS.  A SIMD has two waves: one multiplies
-// a step and then makes dz of the next, the other does it in the other order, so that
+// dx takes dz's rows and W^T, which stays in LDS.  A SIMD has four waves: two multiply
+// a step and then make dz of the next, two do it in the other order, so that
 // vector and matrix units work at once.  A wave's tiles are WN (WK) apart and tiles
 // beyond the matrix are left out, so that the matrix units share what there is.
 constexpr int RB = 2;
+constexpr int BWD_WAVES = 16, BWD_THREADS = 64 * BWD_WAVES;
 template <int N, int K>
 struct BwdShape {
     static constexpr int n = N, k = K;
-    // waves along outputs and inputs, as square a tile each as there can be
-    static constexpr int WN = N >= 256 ? 8 : N >= 2 * K ? 8 : N * 2 <= K ? 1 : 4, WK = 8 / WN;
+    static constexpr int WN = N >= 256 ? 8 : N * 2 <= K ? (N == 64 ? 2 : 4) : 4, WK = BWD_WAVES / WN;
     static constexpr int HN = N / 16 / WN, HK = K / 16 / WK;
 };
 // Pieces of a matrix on their way in, the same columns of many rows.
@@ -867,7 +867,9 @@ struct Kept {
     }
     // the piece itself, zeros from n on where it begins before n
     static __device__ __forceinline__ piece_t<T> piece(const Raw& r, int col, int n) {
-        return n % E<T> != 0 && n >= E<T> && col > n - E<T> ? moved_down<T>(r.v, E<T> - n % E<T>) : r.v;
+        if (n % E<T> == 0 || n < E<T>) return r.v;
+        asm volatile("");   // a branch, so that widths of whole pieces are spared the moves
+        return col > n - E<T> ? moved_down<T>(r.v, E<T> - n % E<T>) : r.v;
     }
     static __device__ __forceinline__ void values(const Raw& r, int col, int n, float (&f)[E<T>]) {
         const piece_t<T> p = piece(r, col, n);
@@ -926,11 +928,24 @@ __host__ __device__ inline int dx_tiles(int inner) {
     return (inner + TASK<T> - 1) / TASK<T> * (TASK<T> / 16);
 }
 
+// Calls f with the least number of tiles that there is code for, MOST at most, that
+// holds n (a multiple of HT where a wave's tiles are neighbours).
+template <int MOST, int HT, class F>
+__device__ __forceinline__ void with_live(int n, F&& f) {
+    if constexpr (MOST >= 8)
+        if (n <= 4) return with_live<4, HT>(n, f);
+    if constexpr (MOST >= 4 && MOST % 2 == 0)
+        if (n <= MOST / 2) return with_live<MOST / 2, HT>(n, f);
+    if constexpr (MOST == 4 && HT == 1)
+        if (n <= 3) return f(std::integral_constant<int, 3>{});
+    f(std::integral_constant<int, MOST>{});
+}
+
 template <class T, class S, int ACT, bool ZMX, bool XMX>
-__global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* part) {
+__global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_bwd(LinearGradArgs a, float* part) {
     constexpr int STEP = RB * KB<T>;
     constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP / 16;
-    constexpr int PD = STEP * NP / 512 > 0 ? STEP * NP / 512 : 1, PX = STEP * KP / 512 > 0 ? STEP * KP / 512 : 1;
+    constexpr int PD = STEP * NP / BWD_THREADS > 0 ? STEP * NP / BWD_THREADS : 1, PX = STEP * KP / BWD_THREADS > 0 ? STEP * KP / BWD_THREADS : 1;
     constexpr int HT = ffn::HT<T>, TT = TASK<T> / 16;   // tiles of a block, of a task
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // live blocks of outputs and inputs, tiles of them, pieces of a block of rows
@@ -940,20 +955,20 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     piece_t<T>* ld = w + (a.dx ? dx_tiles<T>(a.inner) * nbs * 64 : 0);   // two steps of dz
     piece_t<T>* lx = ld + 2 * RB * nblock;                              // and of x
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q = lane >> 4, r = lane & 15;
-    const int wn = wave / S::WK, wk = wave % S::WK;
+    const int wn = wave % S::WN, wk = wave / S::WN;   // so that a SIMD has waves of every wk
     if (a.dx) {
         LinearArgs t{};   // W^T [inner, outer]
         t.w = a.w;
         t.w_stride = a.w_stride;
         t.inner = a.outer;
         t.outer = a.inner;
-        for (int i = tid; i < dx_tiles<T>(a.inner) * nbs * 64; i += 512) {
+        for (int i = tid; i < dx_tiles<T>(a.inner) * nbs * 64; i += BWD_THREADS) {
             const int f = i >> 6;
             w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / nbs, i & 15), f % nbs, (i >> 4) & 3);
         }
     }
     // pieces behind the matrices stay zero
-    for (int i = tid; i < 2 * RB * (nblock + kblock); i += 512) ld[i] = piece_t<T>{};
+    for (int i = tid; i < 2 * RB * (nblock + kblock); i += BWD_THREADS) ld[i] = piece_t<T>{};
     __syncthreads();
     const int64_t steps = (a.rows + STEP - 1) / STEP;
     const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
@@ -966,19 +981,19 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     const int64_t zstride = fz.stride(a.z_stride, a.outer), xstride = fx.stride(a.x_stride, a.inner);
     const int rd = min(tid / NP, STEP - 1), rx = min(tid / KP, STEP - 1);
     // rows of a whole step are the step's, uniform, and the thread's
-    auto read = [&](int64_t b) {
+    auto read = [&](int64_t b) __attribute__((always_inline)) {
         const int64_t row0 = b * STEP;
         const bool whole = row0 + STEP <= a.rows;
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
             if (whole) {
-                const int64_t row = row0 + p * (512 / NP);
+                const int64_t row = row0 + p * (BWD_THREADS / NP);
                 fy.read(dy[p], row * a.dy_stride + rd * a.dy_stride, 0, a.outer);
                 if (ACT != LINEAR_NONE)
                     fz.read(z[p], row * zstride + rd * zstride, fz.scale_offset(row, a.outer) + fz.scale_offset(rd, a.outer),
                             a.outer);
             } else {
-                const int64_t row = min(row0 + rd + p * (512 / NP), a.rows - 1);
+                const int64_t row = min(row0 + rd + p * (BWD_THREADS / NP), a.rows - 1);
                 fy.read(dy[p], row * a.dy_stride, 0, a.outer);
                 if (ACT != LINEAR_NONE) fz.read(z[p], row * zstride, fz.scale_offset(row, a.outer), a.outer);
             }
@@ -986,10 +1001,10 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
             if (whole) {
-                const int64_t row = row0 + p * (512 / KP);
+                const int64_t row = row0 + p * (BWD_THREADS / KP);
                 fx.read(x[p], row * xstride + rx * xstride, fx.scale_offset(row, a.inner) + fx.scale_offset(rx, a.inner), a.inner);
             } else {
-                const int64_t row = min(row0 + rx + p * (512 / KP), a.rows - 1);
+                const int64_t row = min(row0 + rx + p * (BWD_THREADS / KP), a.rows - 1);
                 fx.read(x[p], row * xstride, fx.scale_offset(row, a.inner), a.inner);
             }
         }
@@ -998,13 +1013,13 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
     float db[E<T>] = {};
     int first = 0;
     // dz and x of step b into LDS
-    auto form = [&](int64_t b, int turn) {
+    auto form = [&](int64_t b, int turn) __attribute__((always_inline)) {
         piece_t<T>* bd = ld + turn * RB * nblock;
         piece_t<T>* bx = lx + turn * RB * kblock;
         const int live = (int)min(a.rows - b * STEP, (int64_t)STEP);
 #pragma unroll
         for (int p = 0; p < PD; ++p) {
-            const int rho = tid / NP + p * (512 / NP);
+            const int rho = tid / NP + p * (BWD_THREADS / NP);
             float v[E<T>];
             fy.values(dy[p], cd, a.outer, v);
             if (ACT != LINEAR_NONE) {
@@ -1019,44 +1034,45 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
             piece_t<T> o;
 #pragma unroll
             for (int j = 0; j < E<T>; ++j) {
-                if (STEP * NP >= 512 || rho < STEP) db[j] += v[j];
+                if (STEP * NP >= BWD_THREADS || rho < STEP) db[j] += v[j];
                 o[j] = (T)v[j];
             }
             if (rho < STEP && cd < a.outer) bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
-            const int rho = tid / KP + p * (512 / KP);
+            const int rho = tid / KP + p * (BWD_THREADS / KP);
             piece_t<T> o = fx.piece(x[p], cx, a.inner);
             if (rho >= live) o = piece_t<T>{};
             if (rho < STEP && cx < a.inner) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
         }
     };
     // the products of step b
-    auto multiply = [&](int64_t b, int turn) {
+    auto multiply = [&](int64_t b, int turn) __attribute__((always_inline)) {
         const piece_t<T>* bd = ld + turn * RB * nblock;
         const piece_t<T>* bx = lx + turn * RB * kblock;
         if (a.dweight)
+            // straight code for each number of tiles along the inputs that a wave may have
+            with_live<S::HK, HT>((ktiles - wk + S::WK - 1) / S::WK, [&](auto live) __attribute__((always_inline)) {
+                constexpr int HK = decltype(live)::value;
 #pragma unroll
-            for (int h = 0; h < RB; ++h) {
-                piece_t<T> xs[S::HK];
+                for (int h = 0; h < RB; ++h) {
+                    piece_t<T> ds[S::HN], xs[HK];
 #pragma unroll
-                for (int j = 0; j < S::HK; ++j)
-                    if (j * S::WK + wk < ktiles) xs[j] = ffn::by_dim<T>(bx + h * kblock, j * S::WK + wk);
+                    for (int j = 0; j < HK; ++j) xs[j] = ffn::by_dim<T>(bx + h * kblock, min(j * S::WK + wk, ktiles - 1));
 #pragma unroll
-                for (int i = 0; i < S::HN; ++i) {
-                    if (i * S::WN + wn < ntiles) {
-                        const piece_t<T> fd = ffn::by_dim<T>(bd + h * nblock, i * S::WN + wn);
+                    for (int i = 0; i < S::HN; ++i) ds[i] = ffn::by_dim<T>(bd + h * nblock, min(i * S::WN + wn, ntiles - 1));
 #pragma unroll
-                        for (int j = 0; j < S::HK; ++j)
-                            if (j * S::WK + wk < ktiles) acc[i][j] = mma(fd, xs[j], acc[i][j]);
-                    }
+                    for (int i = 0; i < S::HN; ++i)
+                        if (i * S::WN + wn < ntiles)
+#pragma unroll
+                            for (int j = 0; j < HK; ++j) acc[i][j] = mma(ds[i], xs[j], acc[i][j]);
                 }
-            }
+            });
         if (a.dx) {
             // tasks go round the waves from step to step
             const int tasks = dx_tiles<T>(a.inner) / TT * RT;
-            for (int t = (wave + first) & 7; t < tasks; t += 8) {
+            for (int t = (wave + first) % BWD_WAVES; t < tasks; t += BWD_WAVES) {
                 const int task = t / RT, tile = t % RT;   // columns, and 16 rows
                 const piece_t<T>* rows = bd + tile / HT * nblock;
                 f32x4 o[TT] = {};
@@ -1084,15 +1100,13 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
         // one barrier a step: the other buffers' readers have passed it
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         const int64_t next = b + gridDim.x;
-        if (wave < 4) {
-            multiply(b, turn);
+        auto advance = [&]() __attribute__((always_inline)) {
             if (next < steps) form(next, turn ^ 1);
             read(next + gridDim.x);
-        } else {
-            if (next < steps) form(next, turn ^ 1);
-            read(next + gridDim.x);
-            multiply(b, turn);
-        }
+        };
+        if (wave >= BWD_WAVES / 2) advance();
+        multiply(b, turn);
+        if (wave < BWD_WAVES / 2) advance();
     }
     if (!part) return;
     const int64_t n = (int64_t)a.outer * a.inner;
@@ -1111,13 +1125,13 @@ __global__ __launch_bounds__(512) void k_linear_bwd(LinearGradArgs a, float* par
             }
         }
     __syncthreads();
-    float* sums = reinterpret_cast<float*>(lds);   // [512 / NP][columns]
+    float* sums = reinterpret_cast<float*>(lds);   // [BWD_THREADS / NP][columns]
 #pragma unroll
     for (int j = 0; j < E<T>; ++j) sums[tid / NP * (NP * E<T>) + cd + j] = db[j];
     __syncthreads();
-    for (int c = tid; c < a.outer; c += 512) {
+    for (int c = tid; c < a.outer; c += BWD_THREADS) {
         float t = 0.f;
-        for (int p = 0; p < 512 / NP; ++p) t += sums[p * NP * E<T> + c];
+        for (int p = 0; p < BWD_THREADS / NP; ++p) t += sums[p * NP * E<T> + c];
         part[n + c] = t;
     }
 }
@@ -1148,7 +1162,7 @@ Plan plan(int64_t rows, int inner, int outer, bool own_dz, bool same_type) {
     if (same_type && one_pass<T>(inner, outer)) {
         const int64_t n = ceil_div(outer, KB<T>) * KB<T>, k = ceil_div(inner, KB<T>) * KB<T>;
         // W^T, two steps of dz and x; the sums of db at the end
-        p.lds = (size_t)std::max<int64_t>((n * dx_tiles<T>(inner) * 16 + 2 * RB * KB<T> * (n + k)) * sizeof(T), 512 * E<T> * 4);
+        p.lds = (size_t)std::max<int64_t>((n * dx_tiles<T>(inner) * 16 + 2 * RB * KB<T> * (n + k)) * sizeof(T), BWD_THREADS * E<T> * 4);
         p.fused = (int)std::min<int64_t>(ceil_div(rows, RB * KB<T>), CUS);
         p.dw_bytes = (int64_t)p.fused * (outer * inner + outer) * 4;
         return p;
@@ -1177,8 +1191,8 @@ void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
     auto launch = [&](auto shape) {
         using S = decltype(shape);
         auto run = [&](auto act, auto zmx) {
-            if (a.x_scales) k_linear_bwd<T, S, act(), zmx(), true><<<p.fused, 512, p.lds, s>>>(a, part);
-            else k_linear_bwd<T, S, act(), zmx(), false><<<p.fused, 512, p.lds, s>>>(a, part);
+            if (a.x_scales) k_linear_bwd<T, S, act(), zmx(), true><<<p.fused, BWD_THREADS, p.lds, s>>>(a, part);
+            else k_linear_bwd<T, S, act(), zmx(), false><<<p.fused, BWD_THREADS, p.lds, s>>>(a, part);
         };
         auto kept = [&](auto act) {
             if (a.z_scales) run(act, std::true_type{});
