@@ -494,8 +494,6 @@ struct LinearGradArgs {
     int64_t dy_stride, x_stride, w_stride, z_stride, dx_stride;
     void *dx, *dweight, *dbias;                   // each may be null
     char* ws;
-    // dy is not the gradient of x W^T + bias as the products take it
-    bool own_dz() const { return act != LINEAR_NONE || y_dtype != dtype; }
 };
 size_t linear_grad_workspace(int dtype, int y_dtype, int64_t rows, int inner, int outer, int act);
 void launch_linear_bwd(hipStream_t s, const LinearGradArgs& a);

@@ -753,90 +753,14 @@ void fold(hipStream_t s, const float* part, int groups, int64_t n1, int64_t n2, 
         part, groups, n1, n2, static_cast<T*>(out1), static_cast<T*>(out2));
 }
 
-// dW: a workgroup takes TN rows and TK columns of it (outputs and inputs) over a
-// group of x's rows.  A block of KB rows of dz and x goes through LDS in the order
-// of ffn::slot, whose transposing reads give both operands rows x contraction.
+// Where piece c of row rho of a block of rows lies (ffn::slot): rho = perm(s, r).
 template <class T>
-struct DwTile {
-    static constexpr int NB = 128 / KB<T>, KBS = 128 / KB<T>;   // blocks of outputs and inputs
-    static constexpr int FN = NB * ffn::HT<T>, FK = KBS * ffn::HT<T>;
-};
-template <class T>
-__device__ __forceinline__ int staged(int rho, int c) {   // piece c of row rho of a block of rows
-    // rho = perm(s, r): s = rho % E / 4, r = rho / E * 4 + rho % 4
+__device__ __forceinline__ int staged(int rho, int c) {
     return ffn::slot<T>(c / 4, rho % E<T> / 4, c % 4, rho / E<T> * 4 + rho % 4);
 }
-template <class T, bool MX>
-__global__ __launch_bounds__(256) void k_linear_dw(LinearGradArgs a, const void* dz, int64_t dz_stride, int ntiles, int ktiles,
-                                                   int64_t blocks_per_group, float* part) {
-    using D = DwTile<T>;
-    constexpr int NP = D::NB * 4, KP = D::KBS * 4;   // pieces of a row
-    __shared__ piece_t<T> ld[KB<T> * NP], lx[KB<T> * KP];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
-    const int kt = (int)(blockIdx.x % ktiles), nt = (int)(blockIdx.x / ktiles % ntiles);
-    const int64_t group = blockIdx.x / ktiles / ntiles;
-    const int n0 = nt * 128, k0 = kt * 128;
-    const int wn = wave >> 1, wk = wave & 1;   // waves two by two, a quarter of the tile each
-    constexpr int HN = D::FN / 2, HK = D::FK / 2;
-    f32x4 acc[HN][HK] = {};
-    const int64_t blocks = (a.rows + KB<T> - 1) / KB<T>;
-    const int64_t end = min((group + 1) * blocks_per_group, blocks);
-    for (int64_t b = group * blocks_per_group; b < end; ++b) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < KB<T> * NP; i += 256) {
-            const int rho = i / NP, c = i % NP;
-            const int64_t row = b * KB<T> + rho;
-            piece_t<T> p = {};
-            if (row < a.rows && n0 + c * E<T> < a.outer)
-                p = load_piece(static_cast<const T*>(dz) + row * dz_stride, n0 + c * E<T>, a.outer);
-            ld[staged<T>(rho, c)] = p;
-        }
-        for (int i = threadIdx.x; i < KB<T> * KP; i += 256) {
-            const int rho = i / KP, c = i % KP, k = k0 + c * E<T>;
-            const int64_t row = b * KB<T> + rho;
-            piece_t<T> p = {};
-            if (row < a.rows && k < a.inner) {
-                if constexpr (MX) {
-                    float v[E<T>];
-                    mx8::load<T>(static_cast<const uint8_t*>(a.x) + row * mx8::data_stride(a.inner),
-                                 a.x_scales + row * mx8::scale_stride(a.inner), k, v);
-#pragma unroll
-                    for (int j = 0; j < E<T>; ++j) p[j] = (T)v[j];
-                } else {
-                    p = load_piece(static_cast<const T*>(a.x) + row * a.x_stride, k, a.inner);
-                }
-            }
-            lx[staged<T>(rho, c)] = p;
-        }
-        __syncthreads();
-        piece_t<T> fx[HK];
-#pragma unroll
-        for (int j = 0; j < HK; ++j) fx[j] = ffn::by_dim<T>(lx, wk * HK + j);
-#pragma unroll
-        for (int i = 0; i < HN; ++i) {
-            const piece_t<T> fd = ffn::by_dim<T>(ld, wn * HN + i);
-#pragma unroll
-            for (int j = 0; j < HK; ++j) acc[i][j] = mma(fd, fx[j], acc[i][j]);
-        }
-    }
-    // lane (q, r): dW rows of the fragment's 4 q .., column r
-    float* out = part + group * a.outer * a.inner;
-#pragma unroll
-    for (int i = 0; i < HN; ++i)
-#pragma unroll
-        for (int j = 0; j < HK; ++j) {
-            const int fi = wn * HN + i, fj = wk * HK + j;
-            const int k = k0 + fj / ffn::HT<T> * KB<T> + ffn::perm<T>(fj % ffn::HT<T>, r);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = n0 + fi / ffn::HT<T> * KB<T> + ffn::perm<T>(fi % ffn::HT<T>, 4 * q + e);
-                if (n < a.outer && k < a.inner) out[(int64_t)n * a.inner + k] = acc[i][j][e];
-            }
-        }
-}
 
-// All gradients in one pass over dy, z and x, where a workgroup's registers hold all
-// of dW: 16 waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
+// dW, db and more in one pass over dy, z and x: a workgroup's registers hold dW, or a
+// part of it: 16 waves, WN x WK of them, HN x HK tiles of 16 x 16 each.  Two blocks of
 // KB rows at a time go through LDS: dz is made of dy and z on the way in, its sums
 // over rows stay in registers, dW takes both operands through transposing reads, and
 // dx takes dz's rows and W^T, which stays in LDS.  A SIMD has four waves: two multiply
@@ -942,15 +866,19 @@ __device__ __forceinline__ void with_live(int n, F&& f) {
 }
 
 template <class T, class S, int ACT, bool ZMX, bool XMX>
-__global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_bwd(LinearGradArgs a, float* part) {
+__global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_bwd(LinearGradArgs a, T* dz, float* part, int tiles, int ktiles_all) {
     constexpr int STEP = RB * KB<T>;
     constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP / 16;
     constexpr int PD = STEP * NP / BWD_THREADS > 0 ? STEP * NP / BWD_THREADS : 1, PX = STEP * KP / BWD_THREADS > 0 ? STEP * KP / BWD_THREADS : 1;
     constexpr int HT = ffn::HT<T>, TT = TASK<T> / 16;   // tiles of a block, of a task
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    // the part of dW that is the workgroup's; dx is made where that is all of it
+    const int part_of = (int)(blockIdx.x % tiles), n0 = part_of / ktiles_all * S::n, k0 = part_of % ktiles_all * S::k;
+    const int64_t group = blockIdx.x / tiles, groups = gridDim.x / tiles;
+    const int width = min(a.outer - n0, S::n), depth = min(a.inner - k0, S::k);
     // live blocks of outputs and inputs, tiles of them, pieces of a block of rows
-    const int nbs = (a.outer + KB<T> - 1) / KB<T>, ntiles = nbs * HT, nblock = nbs * KB<T> * 4;
-    const int kbs = (a.inner + KB<T> - 1) / KB<T>, ktiles = kbs * HT, kblock = kbs * KB<T> * 4;
+    const int nbs = (width + KB<T> - 1) / KB<T>, ntiles = nbs * HT, nblock = nbs * KB<T> * 4;
+    const int kbs = (depth + KB<T> - 1) / KB<T>, ktiles = kbs * HT, kblock = kbs * KB<T> * 4;
     piece_t<T>* w = reinterpret_cast<piece_t<T>*>(lds);
     piece_t<T>* ld = w + (a.dx ? dx_tiles<T>(a.inner) * nbs * 64 : 0);   // two steps of dz
     piece_t<T>* lx = ld + 2 * RB * nblock;                              // and of x
@@ -972,9 +900,9 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
     __syncthreads();
     const int64_t steps = (a.rows + STEP - 1) / STEP;
     const int cd = tid % NP * E<T>, cx = tid % KP * E<T>;
-    const Kept<T, false> fy(a.dy, nullptr, cd, a.outer);
-    const Kept<T, ZMX> fz(a.z, a.z_scales, cd, a.outer);
-    const Kept<T, XMX> fx(a.x, a.x_scales, cx, a.inner);
+    const Kept<T, false> fy(a.dy, nullptr, n0 + cd, a.outer);
+    const Kept<T, ZMX> fz(a.z, a.z_scales, n0 + cd, a.outer);
+    const Kept<T, XMX> fx(a.x, a.x_scales, k0 + cx, a.inner);
     typename Kept<T, false>::Raw dy[PD];
     typename Kept<T, ZMX>::Raw z[PD];
     typename Kept<T, XMX>::Raw x[PX];
@@ -1021,10 +949,10 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         for (int p = 0; p < PD; ++p) {
             const int rho = tid / NP + p * (BWD_THREADS / NP);
             float v[E<T>];
-            fy.values(dy[p], cd, a.outer, v);
+            fy.values(dy[p], n0 + cd, a.outer, v);
             if (ACT != LINEAR_NONE) {
                 float f[E<T>];
-                fz.values(z[p], cd, a.outer, f);
+                fz.values(z[p], n0 + cd, a.outer, f);
 #pragma unroll
                 for (int j = 0; j < E<T>; ++j) v[j] *= slope<ACT>(f[j]);
             }
@@ -1037,14 +965,17 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
                 if (STEP * NP >= BWD_THREADS || rho < STEP) db[j] += v[j];
                 o[j] = (T)v[j];
             }
-            if (rho < STEP && cd < a.outer) bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
+            if (rho < STEP && cd < width) {
+                bd[rho / KB<T> * nblock + staged<T>(rho % KB<T>, tid % NP)] = o;
+                if (dz && k0 == 0 && rho < live) store_piece(dz + (b * STEP + rho) * a.outer, n0 + cd, a.outer, o);
+            }
         }
 #pragma unroll
         for (int p = 0; p < PX; ++p) {
             const int rho = tid / KP + p * (BWD_THREADS / KP);
-            piece_t<T> o = fx.piece(x[p], cx, a.inner);
+            piece_t<T> o = fx.piece(x[p], k0 + cx, a.inner);
             if (rho >= live) o = piece_t<T>{};
-            if (rho < STEP && cx < a.inner) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
+            if (rho < STEP && cx < depth) bx[rho / KB<T> * kblock + staged<T>(rho % KB<T>, tid % KP)] = o;
         }
     };
     // the products of step b
@@ -1093,16 +1024,16 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         }
     };
     int turn = 0;
-    read(blockIdx.x);
-    form(blockIdx.x, 0);
-    read((int64_t)blockIdx.x + gridDim.x);
-    for (int64_t b = blockIdx.x; b < steps; b += gridDim.x, turn ^= 1) {
+    read(group);
+    form(group, 0);
+    read(group + groups);
+    for (int64_t b = group; b < steps; b += groups, turn ^= 1) {
         // one barrier a step: the other buffers' readers have passed it
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int64_t next = b + gridDim.x;
+        const int64_t next = b + groups;
         auto advance = [&]() __attribute__((always_inline)) {
             if (next < steps) form(next, turn ^ 1);
-            read(next + gridDim.x);
+            read(next + groups);
         };
         if (wave >= BWD_WAVES / 2) advance();
         multiply(b, turn);
@@ -1110,89 +1041,90 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
     }
     if (!part) return;
     const int64_t n = (int64_t)a.outer * a.inner;
-    part += blockIdx.x * (n + a.outer);
+    part += group * (n + a.outer);
     // lane (q, r): dW rows 4 q .. of the tile, column r
 #pragma unroll
     for (int i = 0; i < S::HN; ++i)
 #pragma unroll
         for (int j = 0; j < S::HK; ++j) {
             const int fi = i * S::WN + wn, fj = j * S::WK + wk;
-            const int kk = fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
+            const int kk = k0 + fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int nn = fi / HT * KB<T> + ffn::perm<T>(fi % HT, 4 * q + e);
-                if (nn < a.outer && kk < a.inner) part[nn * a.inner + kk] = acc[i][j][e];
+                const int nn = n0 + fi / HT * KB<T> + ffn::perm<T>(fi % HT, 4 * q + e);
+                if (nn < a.outer && kk < a.inner) part[(int64_t)nn * a.inner + kk] = acc[i][j][e];
             }
         }
+    if (k0 != 0) return;   // all threads
     __syncthreads();
     float* sums = reinterpret_cast<float*>(lds);   // [BWD_THREADS / NP][columns]
 #pragma unroll
     for (int j = 0; j < E<T>; ++j) sums[tid / NP * (NP * E<T>) + cd + j] = db[j];
     __syncthreads();
-    for (int c = tid; c < a.outer; c += BWD_THREADS) {
+    for (int c = tid; c < width; c += BWD_THREADS) {
         float t = 0.f;
         for (int p = 0; p < BWD_THREADS / NP; ++p) t += sums[p * NP * E<T> + c];
-        part[n + c] = t;
+        part[n + n0 + c] = t;
     }
 }
 
-// How a backward call is split: dz by itself where an activation or another
-// type stands between it and dy, groups of rows for the sums over rows.
+// How a backward call is split.  dy of another type than the products' becomes dz
+// by itself first (own_dz).  Where a workgroup holds all of dW, and W^T beside it in
+// LDS, one pass makes all gradients; else the pass makes dW in parts, dz goes to
+// memory where an activation stands before it, and dx is a product of its own.
 struct Plan {
-    int fused;   // workgroups of the one pass, 0 for several
-    size_t lds;
-    bool own_dz;
-    int64_t dz_bytes;
+    bool own_dz, all;
+    int n, k;                 // of a part of dW
+    int tiles, ktiles, groups;
     int dz_tx, dz_groups;
     int64_t dz_rows;
-    int ntiles, ktiles, dw_groups;
-    int64_t dw_blocks;
-    int64_t db_bytes, dw_bytes, dx_bytes;
+    size_t lds;
+    int64_t dz_bytes, db_bytes, dw_bytes, dx_bytes;
     int64_t bytes() const { return dz_bytes + db_bytes + dw_bytes + dx_bytes; }
 };
-// Whether a workgroup of k_linear_bwd holds all of dW, beside W^T in LDS.
 template <class T>
-bool one_pass(int inner, int outer) {
-    return sizeof(T) == 4 ? (outer <= 256 && inner <= 64) || (outer <= 64 && inner <= 256)
-                          : (outer <= 256 && inner <= 128) || (outer <= 128 && inner <= 256);
-}
-template <class T>
-Plan plan(int64_t rows, int inner, int outer, bool own_dz, bool same_type) {
+Plan plan(int64_t rows, int inner, int outer, int act, bool same_type) {
     Plan p{};
-    if (same_type && one_pass<T>(inner, outer)) {
-        const int64_t n = ceil_div(outer, KB<T>) * KB<T>, k = ceil_div(inner, KB<T>) * KB<T>;
-        // W^T, two steps of dz and x; the sums of db at the end
-        p.lds = (size_t)std::max<int64_t>((n * dx_tiles<T>(inner) * 16 + 2 * RB * KB<T> * (n + k)) * sizeof(T), BWD_THREADS * E<T> * 4);
-        p.fused = (int)std::min<int64_t>(ceil_div(rows, RB * KB<T>), CUS);
-        p.dw_bytes = (int64_t)p.fused * (outer * inner + outer) * 4;
-        return p;
+    auto aligned = [](int64_t n) { return (n + 15) / 16 * 16; };
+    p.own_dz = !same_type;
+    p.all = !p.own_dz && (sizeof(T) == 4 ? (outer <= 256 && inner <= 64) || (outer <= 64 && inner <= 256)
+                                         : (outer <= 256 && inner <= 128) || (outer <= 128 && inner <= 256));
+    // the shapes that there is code for
+    if (inner <= 64) p.n = 256, p.k = 64;
+    else if (outer <= 64) p.n = 64, p.k = 256;
+    else if (sizeof(T) == 4) p.n = 256, p.k = 64;
+    else if (inner <= 128 || outer > 128) p.n = 256, p.k = 128;
+    else p.n = 128, p.k = 256;
+    p.ktiles = (int)ceil_div(inner, p.k);
+    p.tiles = (int)ceil_div(outer, p.n) * p.ktiles;
+    p.groups = (int)std::min<int64_t>(ceil_div(rows, RB * KB<T>), std::max<int64_t>(CUS / p.tiles, 1));
+    const int64_t n = ceil_div(std::min(outer, p.n), KB<T>) * KB<T>, k = ceil_div(std::min(inner, p.k), KB<T>) * KB<T>;
+    // W^T, two steps of dz and x; the sums of db at the end
+    p.lds = (size_t)std::max<int64_t>(((p.all ? n * dx_tiles<T>(inner) * 16 : 0) + 2 * RB * KB<T> * (n + k)) * sizeof(T),
+                                      BWD_THREADS * E<T> * 4);
+    p.dw_bytes = aligned((int64_t)p.groups * ((int64_t)outer * inner + outer) * 4);
+    if (p.own_dz) {
+        p.dz_tx = 1;
+        while (p.dz_tx < 256 && p.dz_tx * 8 < outer) p.dz_tx *= 2;
+        p.dz_rows = std::max<int64_t>(ceil_div(rows, 1024), 4 * 256 / p.dz_tx);
+        p.dz_groups = (int)ceil_div(rows, p.dz_rows);
+        p.db_bytes = aligned((int64_t)p.dz_groups * outer * 4);
     }
-    p.own_dz = own_dz;
-    p.dz_bytes = own_dz ? (rows * outer * (int64_t)sizeof(T) + 15) / 16 * 16 : 0;
-    p.dz_tx = 1;
-    while (p.dz_tx < 256 && p.dz_tx * 8 < outer) p.dz_tx *= 2;
-    const int64_t at_once = 256 / p.dz_tx;
-    p.dz_rows = std::max(ceil_div(rows, 1024), 4 * at_once);
-    p.dz_groups = (int)ceil_div(rows, p.dz_rows);
-    p.db_bytes = ((int64_t)p.dz_groups * outer * 4 + 15) / 16 * 16;
-    p.ntiles = (int)ceil_div(outer, 128);
-    p.ktiles = (int)ceil_div(inner, 128);
-    const int64_t blocks = ceil_div(rows, KB<T>), most = std::max<int64_t>(1, 512 / ((int64_t)p.ntiles * p.ktiles));
-    p.dw_blocks = std::max(ceil_div(blocks, most), std::min<int64_t>(blocks, 4));
-    p.dw_groups = p.dw_blocks ? (int)ceil_div(blocks, p.dw_blocks) : 0;
-    p.dw_bytes = ((int64_t)p.dw_groups * outer * inner * 4 + 15) / 16 * 16;
-    p.dx_bytes = product_workspace<T>(rows, outer, inner);
+    if (p.own_dz || (!p.all && act != LINEAR_NONE)) p.dz_bytes = aligned(rows * outer * (int64_t)sizeof(T));
+    if (!p.all) p.dx_bytes = product_workspace<T>(rows, outer, inner);
     return p;
 }
 
+// dW, db (from dz as it is before it is rounded) and, by the plan, dx or dz.
 template <class T>
-void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
-    float* part = a.dweight || a.dbias ? reinterpret_cast<float*>(a.ws) : nullptr;
+void pass(hipStream_t s, const LinearGradArgs& a, const Plan& p, T* dz, float* part) {
+    const unsigned grid = (unsigned)(p.groups * p.tiles);
     auto launch = [&](auto shape) {
         using S = decltype(shape);
         auto run = [&](auto act, auto zmx) {
-            if (a.x_scales) k_linear_bwd<T, S, act(), zmx(), true><<<p.fused, BWD_THREADS, p.lds, s>>>(a, part);
-            else k_linear_bwd<T, S, act(), zmx(), false><<<p.fused, BWD_THREADS, p.lds, s>>>(a, part);
+            if (a.x_scales)
+                k_linear_bwd<T, S, act(), zmx(), true><<<grid, BWD_THREADS, p.lds, s>>>(a, dz, part, p.tiles, p.ktiles);
+            else k_linear_bwd<T, S, act(), zmx(), false><<<grid, BWD_THREADS, p.lds, s>>>(a, dz, part, p.tiles, p.ktiles);
         };
         auto kept = [&](auto act) {
             if (a.z_scales) run(act, std::true_type{});
@@ -1202,53 +1134,55 @@ void one_pass_backward(hipStream_t s, const LinearGradArgs& a, const Plan& p) {
         else if (a.act == LINEAR_SILU) kept(std::integral_constant<int, LINEAR_SILU>{});
         else kept(std::integral_constant<int, LINEAR_GELU>{});
     };
-    if (a.inner <= 64) launch(BwdShape<256, 64>{});
-    else if (a.outer <= 64) launch(BwdShape<64, 256>{});
+    if (p.k == 64) launch(BwdShape<256, 64>{});
+    else if (p.n == 64) launch(BwdShape<64, 256>{});
     else if constexpr (sizeof(T) == 2) {
-        if (a.inner <= 128) launch(BwdShape<256, 128>{});
+        if (p.k == 128) launch(BwdShape<256, 128>{});
         else launch(BwdShape<128, 256>{});
     }
-    if (part) fold<T>(s, part, p.fused, (int64_t)a.outer * a.inner, a.outer, a.dweight, a.dbias);
 }
 
 template <class T>
-void backward(hipStream_t s, const LinearGradArgs& a) {
-    const Plan p = plan<T>(a.rows, a.inner, a.outer, a.own_dz(), a.y_dtype == a.dtype);
-    if (p.fused) return one_pass_backward<T>(s, a, p);
-    T* dz = p.own_dz ? reinterpret_cast<T*>(a.ws) : nullptr;
+void backward(hipStream_t s, LinearGradArgs a) {
+    const Plan p = plan<T>(a.rows, a.inner, a.outer, a.act, a.y_dtype == a.dtype);
+    T* dz = p.dz_bytes ? reinterpret_cast<T*>(a.ws) : nullptr;
     float* db_part = reinterpret_cast<float*>(a.ws + p.dz_bytes);
-    float* dw_part = reinterpret_cast<float*>(a.ws + p.dz_bytes + p.db_bytes);
-    if (p.dz_groups > 0 && (dz || a.dbias)) {
-        if (a.z_scales) k_linear_dz<T, true><<<p.dz_groups, 256, 0, s>>>(a, dz, a.dbias ? db_part : nullptr, p.dz_tx, p.dz_rows);
-        else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, dz, a.dbias ? db_part : nullptr, p.dz_tx, p.dz_rows);
+    float* part = reinterpret_cast<float*>(a.ws + p.dz_bytes + p.db_bytes);
+    const bool dx = a.dx && a.rows > 0;
+    if (p.own_dz) {
+        float* sums = a.dbias ? db_part : nullptr;
+        if (p.dz_groups > 0) {
+            if (a.z_scales) k_linear_dz<T, true><<<p.dz_groups, 256, 0, s>>>(a, dz, sums, p.dz_tx, p.dz_rows);
+            else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, dz, sums, p.dz_tx, p.dz_rows);
+        }
+        if (sums) fold<T>(s, sums, p.dz_groups, a.outer, 0, a.dbias, nullptr);
+        a.dy = dz;
+        a.dy_stride = a.outer;
+        a.act = LINEAR_NONE;
+        a.z = nullptr;
+        a.z_scales = nullptr;
+        a.dbias = nullptr;
     }
-    if (a.dbias)
-        fold<T>(s, db_part, p.dz_groups, a.outer, 0, a.dbias, nullptr);
-    const void* left = dz ? dz : a.dy;
-    const int64_t left_stride = dz ? a.outer : a.dy_stride;
-    if (a.dx && a.rows > 0) {
-        LinearArgs d{};
-        d.rows = a.rows;
-        d.inner = a.outer;
-        d.outer = a.inner;
-        d.x = left;
-        d.x_stride = left_stride;
-        d.w = a.w;
-        d.w_stride = a.w_stride;
-        d.act = LINEAR_NONE;
-        d.y = a.dx;
-        d.y_stride = a.dx_stride;
-        d.y_dtype = a.dtype;
-        d.ws = a.ws + p.dz_bytes + p.db_bytes + p.dw_bytes;
-        product<T, T, false, true>(s, d);
-    }
-    if (!a.dweight) return;
-    if (p.dw_groups > 0) {
-        const unsigned grid = (unsigned)(p.dw_groups * p.ntiles * p.ktiles);
-        if (a.x_scales) k_linear_dw<T, true><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
-        else k_linear_dw<T, false><<<grid, 256, 0, s>>>(a, left, left_stride, p.ntiles, p.ktiles, p.dw_blocks, dw_part);
-    }
-    fold<T>(s, dw_part, p.dw_groups, (int64_t)a.outer * a.inner, 0, a.dweight, nullptr);
+    LinearGradArgs g = a;
+    if (!p.all) g.dx = nullptr;
+    const bool sums = a.dweight || a.dbias, makes_dz = dz && !p.own_dz && dx;
+    if (p.groups > 0 && (sums || makes_dz || g.dx)) pass<T>(s, g, p, makes_dz ? dz : nullptr, sums ? part : nullptr);
+    if (sums) fold<T>(s, part, p.groups, (int64_t)a.outer * a.inner, a.outer, a.dweight, a.dbias);
+    if (p.all || !dx) return;
+    LinearArgs d{};
+    d.rows = a.rows;
+    d.inner = a.outer;
+    d.outer = a.inner;
+    d.x = dz ? dz : a.dy;
+    d.x_stride = dz ? a.outer : a.dy_stride;
+    d.w = a.w;
+    d.w_stride = a.w_stride;
+    d.act = LINEAR_NONE;
+    d.y = a.dx;
+    d.y_stride = a.dx_stride;
+    d.y_dtype = a.dtype;
+    d.ws = a.ws + p.dz_bytes + p.db_bytes + p.dw_bytes;
+    product<T, T, false, true>(s, d);
 }
 
 }  // namespace linear
