@@ -298,7 +298,7 @@ __device__ __forceinline__ void bias8(const LinearArgs& a, int col, float (&v)[8
 
 // 16 R rows and 32 columns a workgroup, whose waves share the contraction (wave
 // w takes blocks w, w + WAVES, ...) and join their sums in LDS in a fixed order.
-constexpr int FEW_WAVES = 4;
+constexpr int FEW_WAVES = 4, FEW_TILES = 4;
 template <class T, class Y, bool MX, bool TRANS, int R>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
     using C = typename Operand<T, MX>::type;
@@ -367,6 +367,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
     const int64_t group = blockIdx.x / 8 / slices * 8 + blockIdx.x % 8;
     const int64_t groups = gridDim.x / slices;
     const int first = slice * slice_blocks, blocks = min(slice_blocks, (a.outer + COLS - 1) / COLS - first);
+#pragma unroll 4
     for (int i = threadIdx.x; i < blocks * 2 * DK * 64; i += blockDim.x) {
         const int f = i >> 6, kb = f % DK, s = f / DK % 2, cb = f / DK / 2;
         w[i] = w_piece<T, MX, TRANS>(a, (first + cb) * COLS + column(s, i & 15), kb, (i >> 4) & 3);
@@ -377,7 +378,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
     }
     __syncthreads();
     const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R), step = groups * waves;
-    int64_t t = group * waves + (threadIdx.x >> 6);
+    int64_t t = group + (threadIdx.x >> 6) * groups;   // so that few tiles go to as many CUs
     XPiece<T, MX> next[R][DK];
     auto read = [&](int64_t tile) {
 #pragma unroll
@@ -528,7 +529,11 @@ constexpr int64_t CUS = 256;
 constexpr int64_t LDS_BYTES = 160 * 1024;
 constexpr int ALL_BLOCKS = 8;   // of the contraction, up to which the weights stay in LDS
 
-// How a product is launched, by its sizes.
+// How a product is launched, by its sizes: by k_linear_few up to so many of its
+// workgroups that the others' start costs more.  (bf16, us: 256 -> 512 over 8000 rows
+// 21 and 29, 16000 38 and 23; 64 -> 256 over 16000 15 and 21, 32000 26 and 19; 1000 ->
+// 200 over 8000 28 and 38, 16000 48 and 39; 1000 -> 1000 over 2000 22 and 45, 8000 77
+// and 47.)
 struct Shape {
     int kbs;            // blocks of the contraction
     int blocks;         // of columns
@@ -543,7 +548,7 @@ Shape shape(int64_t rows, int inner, int outer) {
     Shape p{};
     p.kbs = (int)ceil_div(inner, KB<C>);
     p.blocks = (int)ceil_div(outer, COLS);
-    p.few = rows <= 1024;
+    p.few = ceil_div(rows, 16 * FEW_TILES) * p.blocks <= (inner > 512 ? 1024 : 2048);
     p.all = !p.few && p.kbs <= ALL_BLOCKS;
     if (p.all) {
         if (p.kbs == 5 || p.kbs == 7) ++p.kbs;   // kernels there are for 1 to 4, 6 and 8
@@ -587,7 +592,7 @@ void few_product(hipStream_t s, const LinearArgs& a) {
         }
     };
     if (a.rows <= 16) launch(std::integral_constant<int, 1>{});
-    else launch(std::integral_constant<int, 4>{});
+    else launch(std::integral_constant<int, FEW_TILES>{});
 }
 
 template <class T, class Y, bool MX, bool TRANS, int ACT, int DK>
@@ -596,9 +601,8 @@ void all_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     const size_t bytes = (size_t)p.nb * (2 * DK * 1024 + COLS * 4);
     const int per_cu = std::min<int>(2, LDS_BYTES / bytes), most_waves = 16 / per_cu;
     const int64_t tiles = ceil_div(a.rows, 16 * R), most = std::max<int64_t>(per_cu * CUS / p.slices / 8, 1) * 8;
-    const int64_t waves = std::min<int64_t>(most_waves, ceil_div(tiles, most));
-    const int64_t groups = std::min(ceil_div(ceil_div(tiles, waves), 8) * 8, most);   // a multiple of 8, as the kernel numbers them
-    k_linear_all<T, Y, MX, TRANS, ACT, DK, R><<<(unsigned)(groups * p.slices), (unsigned)(64 * waves), bytes, s>>>(a, p.slices, p.nb);
+    const int64_t groups = std::min(ceil_div(tiles, 8) * 8, most);   // a multiple of 8, as the kernel numbers them
+    k_linear_all<T, Y, MX, TRANS, ACT, DK, R><<<(unsigned)(groups * p.slices), 64 * most_waves, bytes, s>>>(a, p.slices, p.nb);
 }
 
 // Rows that a streamed product leaves to k_linear_few: the start of a last round of
@@ -890,6 +894,7 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         t.w_stride = a.w_stride;
         t.inner = a.outer;
         t.outer = a.inner;
+#pragma unroll 2
         for (int i = tid; i < dx_tiles<T>(a.inner) * nbs * 64; i += BWD_THREADS) {
             const int f = i >> 6;
             w[i] = w_piece<T, false, true, false>(t, dx_column<T>(f / nbs, i & 15), f % nbs, (i >> 4) & 3);

@@ -91,20 +91,20 @@ def linear(x, w, bias, residual, act, out_dtype):
     bias: every partial sum is then at most |b| + sum |x| |w| in magnitude, so that
     each of the dim additions rounds by U of that at most, dim U (|b| + sum |x| |w|) in all."""
     uT, tiny = UT[out_dtype]
-    x, w = x.double().cpu(), w.double().cpu()
+    x, w = x.double(), w.double()
     dim = x.shape[1]
     z = x @ w.t()
     e_z = dim * U * (x.abs() @ w.abs().t())
     if bias is not None:
-        z = z + bias.double().cpu()
-        e_z = e_z + dim * U * bias.double().cpu().abs() + U * z.abs()
+        z = z + bias.double()
+        e_z = e_z + dim * U * bias.double().abs() + U * z.abs()
     if act is None:
         y, e_y = z, e_z
     else:
         y, _, q = activation(z, act)
         e_y = 1.2 * e_z + y.abs() * (8 + 4 * q) * U
     if residual is not None:
-        y = y + residual.double().cpu()
+        y = y + residual.double()
         e_y = e_y + U * y.abs()
     return y, z, e_y + (uT + U) * y.abs() + tiny, e_z
 
@@ -113,11 +113,11 @@ def linear_grad(dy, x, w, z, act, dtype):
     """(dx, dweight, dbias) and their bounds; x and z as their values.  In 16-bit
     types dz is rounded to the type for the products, not for dbias."""
     uT, tiny = UT[dtype]
-    dy, x, w = (t.double().cpu() for t in (dy, x, w))
+    dy, x, w = (t.double() for t in (dy, x, w))
     rows, outer = dy.shape
     dz, e_dz = dy, torch.zeros_like(dy)
     if act is not None:
-        z = z.double().cpu()
+        z = z.double()
         a, da, q = activation(z, act)
         e_s = (8 + 4 * q) * U
         dz = dy * da
@@ -131,3 +131,13 @@ def linear_grad(dy, x, w, z, act, dtype):
     db = dz.sum(0)
     e_db = e_dz.sum(0) + rows * U * dz.abs().sum(0) + (uT + U) * db.abs() + tiny
     return (dx, dw, db), (e_dx, e_dw, e_db)
+
+
+def near(got, want, bound, what):
+    """nn_oracle.within on the tensors' own device."""
+    got = got.double()
+    assert got.shape == want.shape, f"{what}: {tuple(got.shape)} vs {tuple(want.shape)}"
+    assert torch.isfinite(got).all(), f"{what}: not finite"
+    over = (got - want).abs() - bound
+    assert (over <= 0).all(), (f"{what}: {int((over > 0).sum())} of {got.numel()} beyond the bound, worst by "
+                               f"{float(over.max()):.3g} where that is {float(bound.flatten()[over.argmax()]):.3g}")

@@ -8,8 +8,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 import more_oracle as orc  # noqa: E402
-from linear_sizes import ONE_PASS, RESIDENT, SIZES, STREAMED  # noqa: E402
-from nn_oracle import within  # noqa: E402
+from linear_sizes import FEW, ONE_PASS, RESIDENT, SIZES, STREAMED  # noqa: E402
 from test_gpu_nn import DTYPES, IDS, _normal, _strided, nn  # noqa: E402,F401
 
 ACTS = [None, "silu", "gelu"]
@@ -25,10 +24,10 @@ def _operands(rows, inner, outer, dtype, seed=30):
 def _check_forward(got, x, w, b, r, act, out_dtype, what):
     y, z, e_y, _ = orc.linear(x, w, b, r, act, out_dtype)
     assert got.dtype is out_dtype
-    within(got, y, e_y, what)
+    orc.near(got, y, e_y, what)
 
 
-@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + FEW + RESIDENT + STREAMED)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_forward(nn, dtype, rows, inner, outer):
     x, w, b = _operands(rows, inner, outer, dtype)
@@ -40,12 +39,23 @@ def test_forward(nn, dtype, rows, inner, outer):
         _, want, _, e_z = orc.linear(x, w, b, None, None, dtype)
         uT, tiny = orc.UT[dtype]
         assert z.dtype is dtype
-        within(z, want, e_z + (uT + orc.U) * want.abs() + tiny, "z")
+        orc.near(z, want, e_z + (uT + orc.U) * want.abs() + tiny, "z")
         assert torch.equal(nn.linear_forward(x, w, b, r, act, out_dtype), y)
     _check_forward(nn.linear_forward(x, w), x, w, None, None, None, dtype, "product alone")
 
 
-@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED)
+@pytest.mark.parametrize("rows,inner,outer", FEW + [RESIDENT[1], RESIDENT[7], STREAMED[1], STREAMED[6]])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_forward_of_every_pair_of_types(nn, dtype, rows, inner, outer):
+    x, w, b = _operands(rows, inner, outer, dtype)
+    for out_dtype in DTYPES:
+        for act in ACTS:
+            for bias, r in ((b, None), (None, _normal(44, rows, outer, dtype=out_dtype))):
+                got = nn.linear_forward(x, w, bias, r, act, out_dtype)
+                _check_forward(got, x, w, bias, r, act, out_dtype, f"y {act} in {out_dtype}")
+
+
+@pytest.mark.parametrize("rows,inner,outer", SIZES + FEW + RESIDENT + STREAMED)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_forward_of_8_bits(nn, dtype, rows, inner, outer):
     """Values of 8 bits multiply exactly, so the bounds are those of 32-bit sums."""
@@ -74,12 +84,12 @@ def _check_backward(nn, dtype, rows, inner, outer, act, mx, out_dtype):
     want, bound = orc.linear_grad(dy, xv, w, zv, act, dtype)
     for g, v, e, what in zip(got, want, bound, ("dx", "dweight", "dbias")):
         assert g.dtype is dtype
-        within(g, v, e, f"{what} {act} mx={mx}")
+        orc.near(g, v, e, f"{what} {act} mx={mx}")
     return (dy, xk, w, zk, act), got
 
 
 @pytest.mark.parametrize("mx", [False, True], ids=["plain", "mx8"])
-@pytest.mark.parametrize("rows,inner,outer", SIZES + RESIDENT + STREAMED + ONE_PASS)
+@pytest.mark.parametrize("rows,inner,outer", SIZES + FEW + RESIDENT + STREAMED + ONE_PASS)
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_backward(nn, dtype, rows, inner, outer, mx):
     for i, act in enumerate(ACTS):
@@ -170,9 +180,9 @@ def test_autograd(nn, act, checkpoint):
     z0 = nn.linear_forward(x0, w0, b0)
     xk, zk = (nn.mx8_unpack(nn.mx8_pack(t)) if checkpoint else t for t in (x0, z0))
     (dx, dw, db), bound = orc.linear_grad(g.view(24, 40), xk, w0, zk, act, torch.float32)
-    within(x.grad, dx, bound[0], "x")
-    within(w.grad, dw, bound[1], "weight")
-    within(b.grad, db, bound[2], "bias")
+    orc.near(x.grad, dx, bound[0], "x")
+    orc.near(w.grad, dw, bound[1], "weight")
+    orc.near(b.grad, db, bound[2], "bias")
     assert (r.grad - g.sum((0, 1))).abs().max() < 1e-4
     # half of them, with a result in another type
     y = nn.linear(x0, w, None, None, act, torch.bfloat16, checkpoint)
