@@ -378,7 +378,8 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
     }
     __syncthreads();
     const int64_t tiles = (a.rows + 16 * R - 1) / (16 * R), step = groups * waves;
-    int64_t t = group + (threadIdx.x >> 6) * groups;   // so that few tiles go to as many CUs
+    // neighbours in a workgroup, but few tiles to as many CUs
+    int64_t t = tiles >= step ? group * waves + (threadIdx.x >> 6) : group + (threadIdx.x >> 6) * groups;
     XPiece<T, MX> next[R][DK];
     auto read = [&](int64_t tile) {
 #pragma unroll

@@ -1,14 +1,19 @@
 """Operators of a learned head, trained next to a scene.
 
-Layer norm, a gated feed-forward block and dropout added to a residual, over
-the features of gaussians or pixels: CUDA tensors [..., dim] of float32,
-float16 or bfloat16 (one type a call), with any stride between rows, on the GPU
-of the library's context (the first call's, if none has made one yet).  Each
+Layer norm, root-mean-square norm with the residual's addition, a linear layer
+with bias, activation and residual, a gated feed-forward block and dropout added to
+a residual, over the features of gaussians or pixels: CUDA tensors [..., dim] of
+float32, float16 or bfloat16 (one type a call), with any stride between rows, on the
+GPU of the library's context (the first call's, if none has made one yet).  Each
 runs hand-written kernels of libmsplat_hip.so on PyTorch's current stream, sums
 in fp32, and has
 
-  layer_norm, gated_ffn, dropout_add          differentiable by autograd
-  *_forward, *_backward                       the two passes by themselves
+  layer_norm, rms_norm, linear, gated_ffn, dropout_add   differentiable by autograd
+  *_forward, *_backward                                  the two passes by themselves
+
+Rows in 8 bits (Mx8, mx8_pack, mx8_unpack) are what the backward passes of rms_norm
+and linear take instead of their forward's inputs, rms_norm writes and linear
+multiplies; checkpoint="mx8" keeps a training step's activations so.
 
 None of them waits for the GPU or keeps anything between calls, so they may
 be captured into a graph.  A replay repeats a call's arguments: where each is to
@@ -476,52 +481,6 @@ def _mx8_operand(name, m, rows, dim, like):
     return m.data.data_ptr(), 0, m.scales.data_ptr()
 
 
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        return (*layer_norm_backward(dy, x, weight, mean, rstd, ctx.needs_input_grad[:3]), None)
-
-
-class _GatedFfn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation):
-        ctx.save_for_backward(x, w_gate, w_up, w_down)
-        ctx.activation = activation
-        return gated_ffn_forward(x, w_gate, w_up, w_down, activation)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        need = ctx.needs_input_grad
-        dx, *grads = gated_ffn_backward(dy, *ctx.saved_tensors, ctx.activation, (need[0], any(need[1:4])))
-        return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None)
-
-
-class _DropoutAdd(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        ctx.args = (p, seed, offset)
-        if torch.is_tensor(offset):   # saved, so that a change before the backward is an error
-            ctx.args = (p, seed)
-            ctx.save_for_backward(offset)
-        return dropout_add_forward(x, residual, p, seed, offset)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        need = ctx.needs_input_grad
-        dx = dropout_add_backward(dy, *ctx.args, *ctx.saved_tensors) if need[0] else None
-        return dx, dy if need[1] else None, None, None, None
-
-
 _CHECKPOINTS = (None, "mx8")
 
 
@@ -546,6 +505,54 @@ def _kept(ctx, n):
         return list(saved)
     pairs = [None if k is None else Mx8(saved[2 * i], saved[2 * i + 1], *k) for i, k in enumerate(ctx.kept)]
     return [*pairs, *saved[2 * n:]]
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        return (*layer_norm_backward(dy, x, weight, mean, rstd, ctx.needs_input_grad[:3]), None)
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, activation, checkpoint):
+        _keep(ctx, checkpoint, (x,), w_gate, w_up, w_down)
+        ctx.activation = activation
+        return gated_ffn_forward(x, w_gate, w_up, w_down, activation)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        x, *weights = _kept(ctx, 1)
+        x = mx8_unpack(x) if isinstance(x, Mx8) else x
+        dx, *grads = gated_ffn_backward(dy, x, *weights, ctx.activation, (need[0], any(need[1:4])))
+        return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None, None)
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        ctx.args = (p, seed, offset)
+        if torch.is_tensor(offset):   # saved, so that a change before the backward is an error
+            ctx.args = (p, seed)
+            ctx.save_for_backward(offset)
+        return dropout_add_forward(x, residual, p, seed, offset)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need = ctx.needs_input_grad
+        dx = dropout_add_backward(dy, *ctx.args, *ctx.saved_tensors) if need[0] else None
+        return dx, dy if need[1] else None, None, None, None
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -609,9 +616,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
-def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu"):
-    """gated_ffn_forward, differentiable in x and the three weights."""
-    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation)
+def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", checkpoint=None):
+    """gated_ffn_forward, differentiable in x and the three weights.  checkpoint
+    "mx8" keeps x for the backward in 8 bits."""
+    _check_checkpoint(checkpoint)
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, checkpoint)
 
 
 def dropout_add(x, residual, p: float, seed: int, offset):
