@@ -383,7 +383,8 @@ def linear_forward(x, weight, bias=None, residual=None, activation=None, out_dty
     (tanh form); weight [outer, inner], bias [outer].  x and weight are of one type, as
     is bias, or both Mx8 with a float32 bias.  The result and residual have `out_dtype`,
     x's own where None.  keep: (result, x weight^T + bias in x's type), the latter
-    for the backward."""
+    for the backward.  A row of x that holds an infinity may come out as NaN
+    throughout; other rows are untouched."""
     act = _linear_activation(activation)
     kept = isinstance(x, Mx8)
     if kept is not isinstance(weight, Mx8):
@@ -601,6 +602,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None,
     """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
     "mx8" keeps x and x weight^T + bias for the backward in 8 bits."""
     _check_checkpoint(checkpoint)
+    if not torch.is_grad_enabled():   # nothing to keep
+        return linear_forward(x, weight, bias, residual, activation, out_dtype)
     return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint)
 
 
@@ -608,6 +611,9 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
     """rms_norm_forward's y, and with a residual (y, total), differentiable in x,
     weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits."""
     _check_checkpoint(checkpoint)
+    if not torch.is_grad_enabled():   # nothing to keep
+        y, total, _ = rms_norm_forward(x, weight, residual, eps)
+        return y if residual is None else (y, total)
     return _RmsNorm.apply(x, weight, residual, eps, checkpoint)
 
 
@@ -620,6 +626,8 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", checkpoint=None
     """gated_ffn_forward, differentiable in x and the three weights.  checkpoint
     "mx8" keeps x for the backward in 8 bits."""
     _check_checkpoint(checkpoint)
+    if not torch.is_grad_enabled():
+        checkpoint = None   # nothing to keep
     return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, checkpoint)
 
 

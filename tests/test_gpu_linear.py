@@ -237,3 +237,59 @@ def test_streams_and_replays(nn):
         torch.cuda.synchronize()
         got = [t.clone() for t in held]
         assert all(torch.equal(p, q) for p, q in zip(got, step()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_ends_of_the_activations(nn, dtype):
+    """Far arguments: a(v) is v or 0, a'(v) 1 or 0, whatever the powers between overflow to."""
+    big = 6e4 if dtype is torch.float16 else 1e30
+    v = torch.tensor([big, -big, 100.0, -100.0, 0.0, 30.0, -30.0], dtype=dtype, device="cuda")[:, None]
+    one = torch.ones(1, 1, dtype=dtype, device="cuda")
+    for act in ("silu", "gelu"):
+        y, z = nn.linear_forward(v, one, activation=act, keep=True)
+        assert torch.equal(z, v)
+        want = torch.where(v > 0, v, torch.zeros_like(v))
+        assert float((y - want).abs().max()) < 1e-8
+        dx, _, _ = nn.linear_backward(torch.ones_like(v), v, one, z, act)
+        want = torch.where(v > 0, 1.0, torch.where(v == 0, 0.5, 0.0))
+        assert float((dx.float() - want).abs().max()) < 1e-8
+
+
+def test_rows_with_infinities_and_a_tail(nn):
+    """A width that no piece divides, in every kernel: an infinity stays in its row."""
+    for rows, inner, outer in ((40, 45, 40), (70000, 45, 40), (70000, 300, 40)):
+        x, w, b = _operands(rows, inner, outer, torch.bfloat16)
+        clean = nn.linear_forward(x, w, b)
+        x[7, inner - 1], x[8, 0] = float("inf"), float("nan")
+        y = nn.linear_forward(x, w, b)
+        keep = torch.ones(rows, dtype=torch.bool, device="cuda")
+        keep[7:9] = False
+        assert torch.equal(y[keep], clean[keep]) and not torch.isfinite(y[7]).any() and torch.isnan(y[8]).all()
+        dx, _, _ = nn.linear_backward(y, x, w, wanted=(True, False, False))
+        assert torch.isfinite(dx[keep]).all()
+
+
+def test_without_gradients_nothing_is_kept(nn):
+    x, w, b = _operands(50, 45, 40, torch.bfloat16)
+    w.requires_grad_()
+    with torch.no_grad():
+        y = nn.linear(x, w, b, None, "silu", checkpoint="mx8")
+    assert not y.requires_grad and torch.equal(y, nn.linear(x, w, b, None, "silu"))
+
+
+def test_many_rows(nn):
+    """More rows than one launch of few rows' kernel takes, x beyond 2^32 bytes."""
+    rows = (1 << 27) + 37
+    x = torch.zeros(rows, 17, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = _normal(70, 3, 17, dtype=torch.bfloat16)
+    x[5] = _normal(71, 17, dtype=torch.bfloat16)
+    w, b = _normal(72, 3, 17, dtype=torch.bfloat16), _normal(73, 3, dtype=torch.bfloat16)
+    y = nn.linear_forward(x, w, b)
+    small = nn.linear_forward(x[-3:].contiguous(), w, b)
+    assert float((y[-3:].float() - small.float()).abs().max()) <= 2.0 ** -7 * float(small.abs().max())
+    assert torch.equal(y[6:-3], b.expand(rows - 9, 3))
+    dx, dw, db = nn.linear_backward(y, x, w)
+    want = y[-3:].double().t() @ x[-3:].double() + y[5:6].double().t() @ x[5:6].double()
+    assert float((dw.double() - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
+    assert torch.isfinite(dx).all() and dx.shape == x.shape
+    del y, dx
