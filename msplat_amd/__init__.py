@@ -6,7 +6,7 @@ of include/msplat_hip.h).  Python modules:
   device     device-memory driver (PyTorch tensors as buffers)
   camera     prepareCam (view / projection matrices)
   synthetic  deterministic scenes of the benchmark configurations
-  nn         operators of a learned head: layer norm, gated feed-forward, dropout
+  nn         operators of a learned head: norms, linear layer, gated feed-forward, dropout, rows in 8 bits
   appearance per-photo colour correction of rendered views with them
 """
 __version__ = "0.1.0"
