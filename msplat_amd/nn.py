@@ -299,8 +299,8 @@ def _mx8_rows(lib, call, matrix, dim, m, like):
 
 def mx8_pack(x) -> Mx8:
     """x in 8 bits: each 32 adjacent columns share a power of two, and a number is
-    kept to within 1/16 of itself, or 2^-18 of its block's largest where that is
-    more.  Infinities and NaN become NaN; float16 beyond 61440 (the others beyond
+    kept to within 1/16 of itself, or 2^-17 of its block's largest (and 2^-136) where
+    that is more.  Infinities and NaN become NaN; float16 beyond 61440 (the others beyond
     3.19e38) count as that."""
     lib, _ = _library(x), _dtype(x)
     x2 = _feature_rows("x", x)
@@ -561,6 +561,7 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps, checkpoint):
         ctx.set_materialize_grads(False)
         y, total, rstd = rms_norm_forward(x, weight, residual, eps)
+        ctx.residual_shape = None if residual is None else residual.shape
         _keep(ctx, checkpoint, (total,), weight, rstd)
         return y if residual is None else (y, total)
 
@@ -572,9 +573,10 @@ class _RmsNorm(torch.autograd.Function):
         along = need[0] or need[2]
         if dy is None:   # y was not used
             dweight = None if weight is None or not need[1] else torch.zeros_like(weight)
-            return dtotal if need[0] else None, dweight, dtotal if need[2] else None, None, None
-        dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
-        return dx if need[0] else None, dweight, dx if need[2] else None, None, None
+            dx = dtotal
+        else:
+            dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
+        return dx if need[0] else None, dweight, dx.reshape(ctx.residual_shape) if need[2] else None, None, None
 
 
 class _Linear(torch.autograd.Function):
@@ -584,6 +586,7 @@ class _Linear(torch.autograd.Function):
         y = linear_forward(x, weight, bias, residual, activation, out_dtype, keep)
         y, z = y if keep else (y, None)
         ctx.activation = activation
+        ctx.residual_shape = None if residual is None else residual.shape
         _keep(ctx, checkpoint, (x, z), weight)
         return y
 
@@ -595,13 +598,15 @@ class _Linear(torch.autograd.Function):
         grads = None, None, None
         if any(need[:3]):
             grads = linear_backward(dy, x, weight, z, ctx.activation, need[:3])
-        return (*grads, dy if need[3] else None, None, None, None)
+        return (*grads, dy.reshape(ctx.residual_shape) if need[3] else None, None, None, None)
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
     """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
     "mx8" keeps x and x weight^T + bias for the backward in 8 bits."""
     _check_checkpoint(checkpoint)
+    if isinstance(x, Mx8) or isinstance(weight, Mx8):
+        raise ValueError("a product of Mx8 has no gradients: call linear_forward")
     if not torch.is_grad_enabled():   # nothing to keep
         return linear_forward(x, weight, bias, residual, activation, out_dtype)
     return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint)

@@ -293,3 +293,17 @@ def test_many_rows(nn):
     assert float((dw.double() - want).abs().max()) <= 2.0 ** -7 * float(want.abs().max())
     assert torch.isfinite(dx).all() and dx.shape == x.shape
     del y, dx
+
+
+def test_residuals_of_another_shape(nn):
+    """As many rows in other axes: each gradient has its input's shape."""
+    x, w, b = _operands(24, 45, 40, torch.float32)
+    r = _normal(74, 24, 40).requires_grad_()
+    y = nn.linear(x.view(4, 6, 45), w, b, r, "silu")
+    dr, = torch.autograd.grad(y, r, torch.ones_like(y))
+    assert y.shape == (4, 6, 40) and dr.shape == (24, 40) and (dr == 1).all()
+    n, total = nn.rms_norm(y.detach().requires_grad_(), None, r)
+    dr, = torch.autograd.grad(n.sum() + total.sum(), r)
+    assert dr.shape == (24, 40)
+    dr, = torch.autograd.grad(nn.rms_norm(y.detach(), None, r)[1].sum(), r)
+    assert dr.shape == (24, 40) and (dr == 1).all()

@@ -262,6 +262,7 @@ def test_python_refusals():
     for call, word in ((lambda: nn.linear_forward(x, x, activation="relu"), "activation"),
                        (lambda: nn.linear_forward(m, x), "both Mx8"), (lambda: nn.linear_forward(x, m), "both Mx8"),
                        (lambda: nn.linear(x, x, checkpoint="int4"), "checkpoint"),
+                       (lambda: nn.linear(m, m), "no gradients"), (lambda: nn.linear(x, m), "no gradients"),
                        (lambda: nn.rms_norm(x, checkpoint="fp8"), "checkpoint"),
                        (lambda: nn.gated_ffn(x, x, x, x, checkpoint="fp8"), "checkpoint")):
         with pytest.raises(ValueError, match=word):
