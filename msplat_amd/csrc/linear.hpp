@@ -299,23 +299,28 @@ __device__ __forceinline__ void bias8(const LinearArgs& a, int col, float (&v)[8
 // 16 R rows and 32 columns a workgroup, whose waves share the contraction (wave
 // w takes blocks w, w + WAVES, ...) and join their sums in LDS in a fixed order.
 // Bound by latency: two reads from memory and the join (8 x 256 -> 1000 bf16: 4.0 us).
-constexpr int FEW_WAVES = 4, FEW_TILES = 4;
+constexpr int FEW_TILES = 4;
+// Eight waves for a single row tile: 1000 inputs are then read in one go (4 x 1000 ->
+// 1000 bf16: 5.4 us, 6.7 with four; up to 256 inputs the same).  Four tiles of eight
+// waves would leave room for two workgroups a CU.
+template <int R>
+constexpr int FEW_WAVES = R == 1 ? 8 : 4;
 template <class T, class Y, bool MX, bool TRANS, int R>
-__global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
+__global__ __launch_bounds__(64 * FEW_WAVES<R>) void k_linear_few(LinearArgs a) {
     using C = typename Operand<T, MX>::type;
-    __shared__ f32x4 part[FEW_WAVES][R][2][64];
+    __shared__ f32x4 part[FEW_WAVES<R>][R][2][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, q = lane >> 4, r = lane & 15;
     const int blocks = (a.outer + COLS - 1) / COLS, kbs = (a.inner + KB<C> - 1) / KB<C>;
     const int64_t row0 = (int64_t)(blockIdx.x / blocks) * 16 * R;
     const int col0 = (int)(blockIdx.x % blocks) * COLS;
     f32x4 acc[R][2] = {};
     constexpr int U = 4;   // blocks whose reads are under way at once
-    for (int kb0 = wave; kb0 < kbs; kb0 += U * FEW_WAVES) {
+    for (int kb0 = wave; kb0 < kbs; kb0 += U * FEW_WAVES<R>) {
         XPiece<T, MX> x[U][R] = {};
         piece_t<C> w[U][2] = {};
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = kb0 + u * FEW_WAVES;
+            const int kb = kb0 + u * FEW_WAVES<R>;
             if (kb >= kbs) break;
 #pragma unroll
             for (int s = 0; s < 2; ++s) w[u][s] = w_piece<T, MX, TRANS>(a, col0 + column(s, r), kb, q);
@@ -338,14 +343,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_linear_few(LinearArgs a) {
     bias8<T, MX>(a, col0 + q * 8, bias);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        if (i % FEW_WAVES != wave) continue;
+        if (i % FEW_WAVES<R> != wave) continue;
         const int64_t row = row0 + 16 * i + r;
         float v[8];
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             f32x4 t = part[0][i][s][lane];
 #pragma unroll
-            for (int p = 1; p < FEW_WAVES; ++p) t += part[p][i][s][lane];
+            for (int p = 1; p < FEW_WAVES<R>; ++p) t += part[p][i][s][lane];
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[4 * s + j] = t[j] + bias[4 * s + j];
         }
@@ -594,7 +599,7 @@ void few_product(hipStream_t s, const LinearArgs& a) {
         const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
         for (int64_t at = 0; at < a.rows; at += most) {
             const LinearArgs p = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
-            k_linear_few<T, Y, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES, 0, s>>>(p);
+            k_linear_few<T, Y, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES<R>, 0, s>>>(p);
         }
     };
     if (a.rows <= 16) launch(std::integral_constant<int, 1>{});
