@@ -307,3 +307,40 @@ def test_residuals_of_another_shape(nn):
     assert dr.shape == (24, 40)
     dr, = torch.autograd.grad(nn.rms_norm(y.detach(), None, r)[1].sum(), r)
     assert dr.shape == (24, 40) and (dr == 1).all()
+
+
+def test_two_streams_and_two_graphs_at_once(nn):
+    """Calls that overlap have workspaces of their own: streamed weights, parts of sums."""
+    sizes = [(17000, 264, 256), (9500, 1000, 200)]
+    calls = []
+    for i, (rows, inner, outer) in enumerate(sizes):
+        x, w, b = _operands(rows, inner, outer, torch.bfloat16, seed=80 + 10 * i)
+        dy = _normal(85 + 10 * i, rows, outer, dtype=torch.bfloat16)
+        calls.append(lambda x=x, w=w, b=b, dy=dy: (nn.linear_forward(x, w, b, None, "gelu"), *nn.linear_backward(dy, x, w, dy, "silu")))
+    want = [[t.clone() for t in c()] for c in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = [[], []]
+    for _ in range(4):
+        for i, (s, c) in enumerate(zip(streams, calls)):
+            with torch.cuda.stream(s):
+                got[i].append(c())
+    torch.cuda.synchronize()
+    for g, v in zip(got, want):
+        assert all(torch.equal(p, q) for run in g for p, q in zip(run, v))
+    graphs, held = [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held.append(c())
+        graphs.append(g)
+    for _ in range(3):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for h, v in zip(held, want) for p, q in zip(h, v))
+        for h in held:
+            for t in h:
+                t.zero_()
+        torch.cuda.synchronize()
