@@ -362,7 +362,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES<R>) void k_linear_few(LinearArgs a) 
 // slice; 16 waves a CU go through rows, 16 R at a time, without a barrier, and read
 // the next rows' x ahead.  Workgroups of one XCD share an L2: the slices of the same
 // rows run on one.  Bound by HBM, and by the vector unit where there is an activation
-// (1.09M x 64 -> 256 bf16: 145 us without, 4.8 TB/s, 156 with GELU, vector unit 82%;
+// (1.09M x 64 -> 256 bf16: 145 us without, 4.8 TB/s, 150 to 158 with GELU, vector unit 82%;
 // 500k x 256 -> 256 from 8 bits 110 us, 3.6 TB/s).  With two workgroups of 12 waves or 16
 // the registers of a wave do not suffice (214 us -> 366 and more at an earlier step).
 template <class T, class Y, bool MX, bool TRANS, int ACT, int DK, int R>
@@ -397,12 +397,16 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
             for (int kb = 0; kb < DK; ++kb) next[i][kb].template read<DK == 1>(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
     };
     read(t);
-    for (; t < tiles; t += step) {
-        piece_t<C> x[R][DK];
+    piece_t<C> x[R][DK];
+    auto take = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int kb = 0; kb < DK; ++kb) x[i][kb] = next[i][kb].taken();
+    };
+    if (!MX) take();
+    for (; t < tiles; t += step) {
+        if (MX) take();
         read(t + step);
         constexpr int N = LINE<Y>;
         for (int cb = 0; cb < blocks; cb += N) {
@@ -426,6 +430,9 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
                         for (int i = 0; i < R; ++i) acc[i][b][s] = mma(wf, x[i][kb], acc[i][b][s]);
                     }
             }
+            // the next rows are waited for before the last stores, which the wait would include (1M
+            // x 128 -> 64 bf16 with a residual 151 -> 134 us; 8 bits, which convert here, 117 -> 120)
+            if (!MX && cb + N >= blocks) take();
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 float v[N][8];
