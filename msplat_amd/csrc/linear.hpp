@@ -1055,12 +1055,24 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
                 const int task = t / RT, tile = t % RT;   // columns, and 16 rows
                 const piece_t<T>* rows = bd + tile / HT * nblock;
                 f32x4 o[TT] = {};
-#pragma unroll 2
-                for (int kb = 0; kb < nbs; ++kb) {
-                    const piece_t<T> fd = ffn::by_row<T>(rows, kb * HT + tile % HT);
+                auto some = [&](int kb, auto count) __attribute__((always_inline)) {   // reads go out together
+                    constexpr int U = decltype(count)::value;
+                    piece_t<T> fd[U], fw[U][TT];
 #pragma unroll
-                    for (int s = 0; s < TT; ++s) o[s] = mma(w[((task * TT + s) * nbs + kb) * 64 + lane], fd, o[s]);
-                }
+                    for (int u = 0; u < U; ++u) {
+                        fd[u] = ffn::by_row<T>(rows, (kb + u) * HT + tile % HT);
+#pragma unroll
+                        for (int s = 0; s < TT; ++s) fw[u][s] = w[((task * TT + s) * nbs + kb + u) * 64 + lane];
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+#pragma unroll
+                        for (int s = 0; s < TT; ++s) o[s] = mma(fw[u][s], fd[u], o[s]);
+                };
+                constexpr int U = TT == 1 ? 4 : S::HN * S::HK <= 4 ? 2 : 1;   // by the registers left
+                int kb = 0;
+                for (; kb + U <= nbs; kb += U) some(kb, std::integral_constant<int, U>{});
+                for (; kb < nbs; ++kb) some(kb, std::integral_constant<int, 1>{});
                 piece_t<T> v;
 #pragma unroll
                 for (int j = 0; j < E<T>; ++j) v[j] = (T)o[j / 4][j % 4];
