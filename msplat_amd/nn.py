@@ -558,11 +558,12 @@ class _DropoutAdd(torch.autograd.Function):
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, residual, eps, checkpoint):
+    def forward(ctx, x, weight, residual, eps, checkpoint, grad):
         ctx.set_materialize_grads(False)
         y, total, rstd = rms_norm_forward(x, weight, residual, eps)
-        ctx.residual_shape = None if residual is None else residual.shape
-        _keep(ctx, checkpoint, (total,), weight, rstd)
+        if grad:
+            ctx.residual_shape = None if residual is None else residual.shape
+            _keep(ctx, checkpoint, (total,), weight, rstd)
         return y if residual is None else (y, total)
 
     @staticmethod
@@ -576,18 +577,19 @@ class _RmsNorm(torch.autograd.Function):
             dx = dtotal
         else:
             dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
-        return dx if need[0] else None, dweight, dx.reshape(ctx.residual_shape) if need[2] else None, None, None
+        return dx if need[0] else None, dweight, dx.reshape(ctx.residual_shape) if need[2] else None, None, None, None
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, activation, out_dtype, checkpoint):
-        keep = activation is not None
+    def forward(ctx, x, weight, bias, residual, activation, out_dtype, checkpoint, grad):
+        keep = grad and activation is not None
         y = linear_forward(x, weight, bias, residual, activation, out_dtype, keep)
         y, z = y if keep else (y, None)
-        ctx.activation = activation
-        ctx.residual_shape = None if residual is None else residual.shape
-        _keep(ctx, checkpoint, (x, z), weight)
+        if grad:
+            ctx.activation = activation
+            ctx.residual_shape = None if residual is None else residual.shape
+            _keep(ctx, checkpoint, (x, z), weight)
         return y
 
     @staticmethod
@@ -598,7 +600,7 @@ class _Linear(torch.autograd.Function):
         grads = None, None, None
         if any(need[:3]):
             grads = linear_backward(dy, x, weight, z, ctx.activation, need[:3])
-        return (*grads, dy.reshape(ctx.residual_shape) if need[3] else None, None, None, None)
+        return (*grads, dy.reshape(ctx.residual_shape) if need[3] else None, None, None, None, None)
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
@@ -607,19 +609,15 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None,
     _check_checkpoint(checkpoint)
     if isinstance(x, Mx8) or isinstance(weight, Mx8):
         raise ValueError("a product of Mx8 has no gradients: call linear_forward")
-    if not torch.is_grad_enabled():   # nothing to keep
-        return linear_forward(x, weight, bias, residual, activation, out_dtype)
-    return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint)
+    # without gradients too, for forward mode's tangents to be refused; grad mode is off in there
+    return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint, torch.is_grad_enabled())
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
     """rms_norm_forward's y, and with a residual (y, total), differentiable in x,
     weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits."""
     _check_checkpoint(checkpoint)
-    if not torch.is_grad_enabled():   # nothing to keep
-        y, total, _ = rms_norm_forward(x, weight, residual, eps)
-        return y if residual is None else (y, total)
-    return _RmsNorm.apply(x, weight, residual, eps, checkpoint)
+    return _RmsNorm.apply(x, weight, residual, eps, checkpoint, torch.is_grad_enabled())
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):

@@ -1,0 +1,43 @@
+"""What the differentiable operators of msplat_amd.nn do around their kernels,
+without a GPU: plain operations on the CPU stand in for the passes."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+from msplat_amd import nn
+
+
+def _linear_forward(x, weight, bias=None, residual=None, activation=None, out_dtype=None, keep=False):
+    z = x @ weight.t()
+    z = z if bias is None else z + bias
+    y = z if activation is None else torch.nn.functional.silu(z)
+    y = (y if residual is None else y + residual).to(out_dtype or x.dtype)
+    return (y, z) if keep else y
+
+
+def _rms_norm_forward(x, weight=None, residual=None, eps=1e-5, mx8=False):
+    total = x if residual is None else x + residual
+    rstd = (total.square().mean(-1) + eps).rsqrt()
+    y = total * rstd[..., None]
+    return y if weight is None else y * weight, total, rstd
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    monkeypatch.setattr(nn, "linear_forward", _linear_forward)
+    monkeypatch.setattr(nn, "rms_norm_forward", _rms_norm_forward)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(plain, grad):
+    """No operator has a forward-mode derivative: with a tangent each is an error, with
+    and without gradients, and never a result whose tangent is lost."""
+    w = torch.ones(4, 4)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        x = forward_ad.make_dual(torch.ones(3, 4), torch.ones(3, 4))
+        for call in (lambda: nn.linear(x, w), lambda: nn.linear(w, w, x[0]), lambda: nn.rms_norm(x),
+                     lambda: nn.rms_norm(w[:3], None, x)):
+            with pytest.raises(NotImplementedError):
+                call()
