@@ -569,6 +569,8 @@ class _RmsNorm(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dtotal=None):
+        if dy is None and dtotal is None:   # no gradient reaches either result
+            return (None,) * 6
         total, weight, rstd = _kept(ctx, 1)
         need = ctx.needs_input_grad
         along = need[0] or need[2]

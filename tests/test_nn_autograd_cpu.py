@@ -41,3 +41,23 @@ def test_forward_mode_is_refused(plain, grad):
                      lambda: nn.rms_norm(w[:3], None, x)):
             with pytest.raises(NotImplementedError):
                 call()
+
+
+class _NoGradient(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, t):
+        return t.clone()
+
+    @staticmethod
+    def backward(ctx, dy):
+        return None
+
+
+def test_a_norm_that_no_gradient_reaches(plain):
+    """Whatever follows may have no gradient for either result: then no input has one."""
+    x, r, w = (torch.ones(*s, requires_grad=True) for s in ((3, 4), (3, 4), (4,)))
+    y, total = nn.rms_norm(x, w, r)
+    grads = torch.autograd.grad((_NoGradient.apply(y) + _NoGradient.apply(total)).sum(), (x, w, r), allow_unused=True)
+    assert grads == (None, None, None)
+    y = nn.rms_norm(x, w)
+    assert torch.autograd.grad(_NoGradient.apply(y).sum(), (x, w), allow_unused=True) == (None, None)
