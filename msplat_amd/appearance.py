@@ -37,8 +37,9 @@ class AppearanceHead:
     """dim features a pixel, `blocks` blocks of `hidden` units.  Parameters and
     their optimiser are float32; features and products have the type `dtype`.
     norm: "layer", or "rms" (see above).  checkpoint "mx8" keeps what the backward of
-    feed-forward blocks, rms norms and linear layers takes of every pixel in 8 bits,
-    about half of bfloat16's memory for gradients a few percent off.
+    feed-forward blocks, rms norms and linear layers takes of every pixel in 8 bits (the
+    five numbers of the pixel itself as they are), about half of bfloat16's memory for
+    gradients a few percent off.
 
     float16 is for correcting views with a head trained in another type
     (head.dtype = torch.float16): a pixel's share of a view's mean loss is

@@ -13,7 +13,8 @@ in fp32, and has
 
 Rows in 8 bits (Mx8, mx8_pack, mx8_unpack) are what the backward passes of rms_norm
 and linear take instead of their forward's inputs, rms_norm writes and linear
-multiplies; checkpoint="mx8" keeps a training step's activations so.
+multiplies; checkpoint="mx8" keeps a training step's activations so where they are
+smaller that way (rows of few columns are not).
 
 None of them waits for the GPU or keeps anything between calls, so they may
 be captured into a graph.  A replay repeats a call's arguments: where each is to
@@ -490,21 +491,26 @@ def _check_checkpoint(checkpoint):
         raise ValueError(f"checkpoint {checkpoint!r} is none of {_CHECKPOINTS}")
 
 
+def _smaller_packed(t) -> bool:
+    """Whether a matrix takes less room in 8 bits: a row of those has whole blocks
+    of 32 columns (5 columns of float32: 36 bytes instead of 20)."""
+    dim = t.shape[-1]
+    return 32 * -(-dim // 32) + 4 * -(-dim // 128) < dim * t.element_size()
+
+
 def _keep(ctx, checkpoint, kept, *others):
     """Saves tensors for the backward, those in `kept` (each may be None) as
-    Mx8 where the checkpoint says so."""
-    packed = [None if t is None else mx8_pack(t) for t in kept] if checkpoint else list(kept)
-    ctx.kept = [None if m is None else (m.dim, m.dtype) for m in packed] if checkpoint else None
-    flat = [t for m in packed for t in ((None, None) if m is None else (m.data, m.scales))] if checkpoint else packed
+    Mx8 where the checkpoint says so and that is smaller."""
+    packed = [mx8_pack(t) if checkpoint and t is not None and _smaller_packed(t) else t for t in kept]
+    ctx.kept = [(m.dim, m.dtype) if isinstance(m, Mx8) else None for m in packed]
+    flat = [t for m in packed for t in ((m.data, m.scales) if isinstance(m, Mx8) else (m, None))]
     ctx.save_for_backward(*flat, *others)
 
 
-def _kept(ctx, n):
-    """What _keep took: the n that it kept, and the others."""
-    saved = ctx.saved_tensors
-    if ctx.kept is None:
-        return list(saved)
-    pairs = [None if k is None else Mx8(saved[2 * i], saved[2 * i + 1], *k) for i, k in enumerate(ctx.kept)]
+def _kept(ctx):
+    """What _keep took: those that it kept, and the others."""
+    saved, n = ctx.saved_tensors, len(ctx.kept)
+    pairs = [Mx8(*saved[2 * i:2 * i + 2], *k) if k else saved[2 * i] for i, k in enumerate(ctx.kept)]
     return [*pairs, *saved[2 * n:]]
 
 
@@ -525,15 +531,16 @@ class _LayerNorm(torch.autograd.Function):
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, activation, checkpoint):
+        y = gated_ffn_forward(x, w_gate, w_up, w_down, activation)
         _keep(ctx, checkpoint, (x,), w_gate, w_up, w_down)
         ctx.activation = activation
-        return gated_ffn_forward(x, w_gate, w_up, w_down, activation)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         need = ctx.needs_input_grad
-        x, *weights = _kept(ctx, 1)
+        x, *weights = _kept(ctx)
         x = mx8_unpack(x) if isinstance(x, Mx8) else x
         dx, *grads = gated_ffn_backward(dy, x, *weights, ctx.activation, (need[0], any(need[1:4])))
         return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None, None)
@@ -571,7 +578,7 @@ class _RmsNorm(torch.autograd.Function):
     def backward(ctx, dy, dtotal=None):
         if dy is None and dtotal is None:   # no gradient reaches either result
             return (None,) * 6
-        total, weight, rstd = _kept(ctx, 1)
+        total, weight, rstd = _kept(ctx)
         need = ctx.needs_input_grad
         along = need[0] or need[2]
         if dy is None:   # y was not used
@@ -597,7 +604,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, z, weight = _kept(ctx, 2)
+        x, z, weight = _kept(ctx)
         need = ctx.needs_input_grad
         grads = None, None, None
         if any(need[:3]):
@@ -607,7 +614,7 @@ class _Linear(torch.autograd.Function):
 
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
     """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
-    "mx8" keeps x and x weight^T + bias for the backward in 8 bits."""
+    "mx8" keeps x and x weight^T + bias for the backward in 8 bits, where that is less."""
     _check_checkpoint(checkpoint)
     if isinstance(x, Mx8) or isinstance(weight, Mx8):
         raise ValueError("a product of Mx8 has no gradients: call linear_forward")
@@ -617,7 +624,8 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None,
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
     """rms_norm_forward's y, and with a residual (y, total), differentiable in x,
-    weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits."""
+    weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits, where
+    that is less."""
     _check_checkpoint(checkpoint)
     return _RmsNorm.apply(x, weight, residual, eps, checkpoint, torch.is_grad_enabled())
 
@@ -629,7 +637,7 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 
 def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", checkpoint=None):
     """gated_ffn_forward, differentiable in x and the three weights.  checkpoint
-    "mx8" keeps x for the backward in 8 bits."""
+    "mx8" keeps x for the backward in 8 bits, where that is less."""
     _check_checkpoint(checkpoint)
     if not torch.is_grad_enabled():
         checkpoint = None   # nothing to keep

@@ -24,8 +24,14 @@ def _rms_norm_forward(x, weight=None, residual=None, eps=1e-5, mx8=False):
     return y if weight is None else y * weight, total, rstd
 
 
+def _mx8_pack(x):
+    return nn.Mx8._empty(x.shape, x, x.dtype)
+
+
 @pytest.fixture
 def plain(monkeypatch):
+    monkeypatch.setattr(nn, "mx8_pack", _mx8_pack)
+    monkeypatch.setattr(nn, "gated_ffn_forward", lambda x, *_: x.clone())
     monkeypatch.setattr(nn, "linear_forward", _linear_forward)
     monkeypatch.setattr(nn, "rms_norm_forward", _rms_norm_forward)
 
@@ -61,3 +67,26 @@ def test_a_norm_that_no_gradient_reaches(plain):
     assert grads == (None, None, None)
     y = nn.rms_norm(x, w)
     assert torch.autograd.grad(_NoGradient.apply(y).sum(), (x, w), allow_unused=True) == (None, None)
+
+
+def _kept(call):
+    """The tensors that an operator keeps for its backward, and its result."""
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        y = call()
+    return kept, y
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_checkpoints_are_never_larger_than_what_they_stand_for(plain, dtype):
+    """A row in 8 bits has whole blocks of 32 columns and scales for 128: narrow
+    matrices, and some a little wider than a block, are smaller as they are."""
+    for dim in (1, 3, 5, 8, 9, 16, 17, 18, 19, 32, 33, 34, 35, 64, 129, 132, 200):
+        x = torch.ones(7, dim, dtype=dtype, requires_grad=True)
+        w = torch.ones(dim, dim, dtype=dtype, requires_grad=True)
+        for call in (lambda c: nn.linear(x, w, activation="silu", checkpoint=c), lambda c: nn.rms_norm(x, checkpoint=c),
+                     lambda c: nn.gated_ffn(x, w, w, w, checkpoint=c)):
+            size = [sum(t.nbytes for t in _kept(lambda: call(c))[0]) for c in (None, "mx8")]
+            packed, plain_size = 32 * -(-dim // 32) + 4 * -(-dim // 128), dim * x.element_size()
+            assert size[1] <= size[0]
+            assert (size[1] < size[0]) is (packed < plain_size)
