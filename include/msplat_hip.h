@@ -589,7 +589,7 @@ int msplat_hip_linear(const MsplatLinearArgs* args);
  * activation is MSPLAT_IDENTITY, z: dx [rows, inner], dweight [outer, inner]
  * contiguous and dbias [outer], each written where not NULL; residual's gradient is dy.
  * x_scales, z_scales not NULL: x, z are in 8 bits (x, z their data, the strides
- * unused).  In 16-bit types dz = dy a'(z) is rounded to the type for the products (in
+ * unused).  x is not looked at where dweight is NULL.  In 16-bit types dz = dy a'(z) is rounded to the type for the products (in
  * float16 it loses bits below 6e-5 and vanishes below 3e-8).  The sums over
  * rows have a fixed order. */
 typedef struct MsplatLinearGradArgs {

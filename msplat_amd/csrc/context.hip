@@ -1701,8 +1701,10 @@ int msplat_hip_linear_backward(const MsplatLinearGradArgs* a) {
     if (!a) return fail(MSPLAT_ERR_ARG, "null args");
     CHECK(check_linear(a->rows, a->inner, a->outer, a->dtype, a->y_dtype, a->activation));
     CHECK(check_matrix("dy", a->dy, a->rows, a->outer, a->dy_stride, a->y_dtype));
-    if (a->x_scales) CHECK(check_mx8("x", a->x, a->x_scales, a->rows));
-    else CHECK(check_matrix("x", a->x, a->rows, a->inner, a->x_stride, a->dtype));
+    if (a->dweight) {
+        if (a->x_scales) CHECK(check_mx8("x", a->x, a->x_scales, a->rows));
+        else CHECK(check_matrix("x", a->x, a->rows, a->inner, a->x_stride, a->dtype));
+    }
     CHECK(check_matrix("weight", a->weight, a->outer, a->inner, a->weight_stride, a->dtype));
     if (a->activation != MSPLAT_IDENTITY) {
         if (a->z_scales) CHECK(check_mx8("z", a->z, a->z_scales, a->rows));
@@ -1724,9 +1726,10 @@ int msplat_hip_linear_backward(const MsplatLinearGradArgs* a) {
     if (!a->dweight && !a->dbias && (!a->dx || a->rows == 0)) return MSPLAT_OK;
     l.dy = a->dy;
     l.dy_stride = a->dy_stride;
-    l.x = a->x;
-    l.x_stride = a->x_stride;
-    l.x_scales = static_cast<const uint8_t*>(a->x_scales);
+    // only dweight takes x; without it the kernels read the weights' first row in every row's place
+    l.x = a->dweight ? a->x : a->weight;
+    l.x_stride = a->dweight ? a->x_stride : 0;
+    l.x_scales = a->dweight ? static_cast<const uint8_t*>(a->x_scales) : nullptr;
     l.w = a->weight;
     l.w_stride = a->weight_stride;
     l.z = a->z;

@@ -426,20 +426,25 @@ def linear_forward(x, weight, bias=None, residual=None, activation=None, out_dty
 def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, True)):
     """(dx, dweight, dbias) from the gradient of the result, x, weight and, where there
     is an activation, what the forward kept; x and z may be Mx8 of them.  The
-    gradients have weight's type.  Those not wanted are None and not computed."""
+    gradients have weight's type.  Those not wanted are None and not computed; without
+    dweight x may be None."""
     act = _linear_activation(activation)
+    if x is None and wanted[1]:
+        raise ValueError("the weight's gradient takes x")
     lib, dtype = _library(weight), _dtype(weight)
     if weight.dim() != 2 or min(weight.shape) < 1:
         raise ValueError(f"weight has shape {tuple(weight.shape)}, not (outer, inner)")
     outer, inner = weight.shape
     w = _matrix("weight", weight, (outer, inner), weight)
-    if isinstance(x, Mx8):
-        rows = x.rows
+    dy2 = _rows("dy", dy, outer, dy)
+    rows = dy2.shape[0]
+    if x is None:
+        xs = (None, 0, None)
+    elif isinstance(x, Mx8):
         xs = _mx8_operand("x", x, rows, inner, weight)
     else:
-        x2 = _rows("x", x, inner, weight)
-        rows, xs = x2.shape[0], (x2.data_ptr(), x2.stride(0), None)
-    dy2 = _rows_of("dy", dy, rows, outer, dy)
+        x2 = _rows_of("x", x, rows, inner, weight)
+        xs = (x2.data_ptr(), x2.stride(0), None)
     if dy.device != weight.device:
         raise ValueError(f"dy is on {dy.device}, not {weight.device}")
     if activation is None:
@@ -451,7 +456,7 @@ def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, 
     else:
         z2 = _rows_of("z", z, rows, outer, weight)
         zs = (z2.data_ptr(), z2.stride(0), None)
-    dx = weight.new_empty(x.shape) if wanted[0] else None
+    dx = weight.new_empty((*dy.shape[:-1], inner) if x is None else x.shape) if wanted[0] else None
     dweight = weight.new_empty(outer, inner) if wanted[1] else None
     dbias = weight.new_empty(outer) if wanted[2] else None
     ws = _workspace(lib.msplat_hip_linear_backward_workspace(rows, inner, outer, dtype, _dtype(dy), act), weight)
