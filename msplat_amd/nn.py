@@ -535,10 +535,11 @@ class _LayerNorm(torch.autograd.Function):
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, activation, checkpoint):
+    def forward(ctx, x, w_gate, w_up, w_down, activation, checkpoint, grad):
         y = gated_ffn_forward(x, w_gate, w_up, w_down, activation)
-        _keep(ctx, checkpoint, (x,), w_gate, w_up, w_down)
-        ctx.activation = activation
+        if grad and any(ctx.needs_input_grad[:4]):
+            _keep(ctx, checkpoint, (x,), w_gate, w_up, w_down)
+            ctx.activation = activation
         return y
 
     @staticmethod
@@ -548,7 +549,7 @@ class _GatedFfn(torch.autograd.Function):
         x, *weights = _kept(ctx)
         x = mx8_unpack(x) if isinstance(x, Mx8) else x
         dx, *grads = gated_ffn_backward(dy, x, *weights, ctx.activation, (need[0], any(need[1:4])))
-        return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None, None)
+        return (dx, *(g if n else None for g, n in zip(grads, need[1:4])), None, None, None)
 
 
 class _DropoutAdd(torch.autograd.Function):
@@ -573,7 +574,7 @@ class _RmsNorm(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps, checkpoint, grad):
         ctx.set_materialize_grads(False)
         y, total, rstd = rms_norm_forward(x, weight, residual, eps)
-        if grad:
+        if grad and any(ctx.needs_input_grad[:3]):
             ctx.residual_shape = None if residual is None else residual.shape
             _keep(ctx, checkpoint, (total,), weight, rstd)
         return y if residual is None else (y, total)
@@ -597,22 +598,23 @@ class _RmsNorm(torch.autograd.Function):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, out_dtype, checkpoint, grad):
-        keep = grad and activation is not None
+        need = ctx.needs_input_grad
+        keep = grad and activation is not None and any(need[:3])
         y = linear_forward(x, weight, bias, residual, activation, out_dtype, keep)
         y, z = y if keep else (y, None)
-        if grad:
-            ctx.activation = activation
-            ctx.residual_shape = None if residual is None else residual.shape
-            _keep(ctx, checkpoint, (x, z), weight)
+        ctx.activation = activation
+        ctx.residual_shape = None if residual is None else residual.shape
+        if grad and any(need[:3]):
+            _keep(ctx, checkpoint, (x if need[1] else None, z), weight)   # x is for the weight's gradient alone
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, z, weight = _kept(ctx)
         need = ctx.needs_input_grad
         grads = None, None, None
         if any(need[:3]):
+            x, z, weight = _kept(ctx)
             grads = linear_backward(dy, x, weight, z, ctx.activation, need[:3])
         return (*grads, dy.reshape(ctx.residual_shape) if need[3] else None, None, None, None, None)
 
@@ -644,9 +646,7 @@ def gated_ffn(x, w_gate, w_up, w_down, activation: str = "silu", checkpoint=None
     """gated_ffn_forward, differentiable in x and the three weights.  checkpoint
     "mx8" keeps x for the backward in 8 bits, where that is less."""
     _check_checkpoint(checkpoint)
-    if not torch.is_grad_enabled():
-        checkpoint = None   # nothing to keep
-    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, checkpoint)
+    return _GatedFfn.apply(x, w_gate, w_up, w_down, activation, checkpoint, torch.is_grad_enabled())
 
 
 def dropout_add(x, residual, p: float, seed: int, offset):

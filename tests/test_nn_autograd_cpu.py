@@ -90,3 +90,60 @@ def test_checkpoints_are_never_larger_than_what_they_stand_for(plain, dtype):
             packed, plain_size = 32 * -(-dim // 32) + 4 * -(-dim // 128), dim * x.element_size()
             assert size[1] <= size[0]
             assert (size[1] < size[0]) is (packed < plain_size)
+
+
+def _ids(tensors):
+    return {t.data_ptr() for t in tensors if t is not None}
+
+
+@pytest.mark.parametrize("checkpoint", [None, "mx8"])
+def test_only_what_wanted_gradients_take_is_kept(plain, monkeypatch, checkpoint):
+    """A frozen weight leaves x out, no activation z, and without any operand that
+    requires a gradient nothing is kept, packed or written for one."""
+    packed, kept_z = [], []
+    monkeypatch.setattr(nn, "mx8_pack", lambda t: packed.append(t) or _mx8_pack(t))
+    monkeypatch.setattr(nn, "linear_forward",
+                        lambda *a: kept_z.append(len(a) > 6 and a[6]) or _linear_forward(*a))
+    x, w, b, r = torch.ones(7, 64), torch.ones(64, 64), torch.ones(64), torch.ones(7, 64)
+
+    def leaf(t, needs):
+        return t.clone().requires_grad_(needs)
+
+    for needs in range(16):
+        for act in (None, "silu"):
+            ops = [leaf(t, bool(needs >> i & 1)) for i, t in enumerate((x, w, b, r))]
+            packed.clear(), kept_z.clear()
+            kept, y = _kept(lambda: nn.linear(*ops, act, checkpoint=checkpoint))
+            takes_x, takes_z = bool(needs & 2), act is not None and bool(needs & 7)
+            assert y.requires_grad is bool(needs) and kept_z == [takes_z]
+            assert len(packed) == (takes_x + takes_z if checkpoint else 0)
+            assert (ops[0].data_ptr() in _ids(kept + packed)) is takes_x
+            assert bool(kept) is bool(needs & 7)
+    for needs in range(8):
+        ops = [leaf(t, bool(needs >> i & 1)) for i, t in enumerate((x, b, r))]
+        packed.clear()
+        kept, _ = _kept(lambda: nn.rms_norm(*ops, checkpoint=checkpoint))
+        assert len(packed) == (1 if checkpoint and needs else 0) and bool(kept) is bool(needs)
+        ops = [leaf(t, bool(needs >> i & 1)) for i, t in enumerate((x, w, w))]
+        packed.clear()
+        kept, _ = _kept(lambda: nn.gated_ffn(*ops, w, checkpoint=checkpoint))
+        assert len(packed) == (1 if checkpoint and needs else 0) and bool(kept) is bool(needs)
+    packed.clear()
+    with torch.no_grad():
+        x.requires_grad_(), w.requires_grad_()
+        for call in (lambda: nn.linear(x, w, None, None, "silu", None, checkpoint), lambda: nn.rms_norm(x, checkpoint=checkpoint),
+                     lambda: nn.gated_ffn(x, w, w, w, checkpoint=checkpoint)):
+            assert not _kept(call)[0] and not packed
+
+
+def test_the_backward_is_asked_for_what_is_wanted(plain, monkeypatch):
+    asked = []
+    monkeypatch.setattr(nn, "linear_backward", lambda dy, x, w, z, act, wanted: asked.append((x is None, tuple(wanted))) or
+                        tuple(t if k else None for t, k in zip((dy @ w, torch.zeros_like(w), dy.sum(0)), wanted)))
+    for needs in range(1, 8):
+        ops = [t.clone().requires_grad_(bool(needs >> i & 1))
+               for i, t in enumerate((torch.ones(7, 64), torch.ones(64, 64), torch.ones(64)))]
+        nn.linear(*ops, None, "silu").sum().backward()
+        wanted = tuple(bool(needs >> i & 1) for i in range(3))
+        assert asked.pop() == (not wanted[1], wanted) and not asked
+        assert tuple(t.grad is not None for t in ops) == wanted
