@@ -552,8 +552,9 @@ int msplat_hip_rms_norm_backward(const MsplatRmsNormGradArgs* args);
  * dtype is that of x, weight, bias and z, or MSPLAT_MX8: x and weight in 8 bits
  * (x and weight their data, x_scales and weight_scales), bias fp32.  y_dtype is
  * that of y and residual, any of the three.  z takes x weight^T + bias, rounded to
- * dtype, where not NULL (not with MSPLAT_MX8); the backward pass takes it.  y may be
- * exactly residual with the same stride.  Numbers in 8 bits multiply exactly (those
+ * dtype (in float16 to 65504 at most, whose gradients are those of more), where not
+ * NULL (not with MSPLAT_MX8); the backward pass takes it.  y may be exactly residual
+ * with the same stride.  Numbers in 8 bits multiply exactly (those
  * below 2^-126 count as 0) and every sum is fp32.  A row of x that holds an infinity
  * may come out as NaN throughout; other rows are untouched. */
 #define MSPLAT_IDENTITY 2

@@ -189,12 +189,29 @@ __device__ __forceinline__ void store8(void* base, int dtype, int64_t stride, in
     else store8(static_cast<__bf16*>(base) + row * stride, col, n, v);
 }
 
+// z as it is kept for the backward pass.  Beyond float16's range it is the largest
+// number there, not infinite: a'(z) is 1 or 0 from far smaller arguments on, but of an
+// infinity it would be NaN (infinity times 0), as would z packed into 8 bits.
+template <class C, int N>
+__device__ __forceinline__ void keep_finite(float (&z)[N]) {
+    if constexpr (std::is_same<C, _Float16>::value) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) z[j] = z[j] > 65504.f ? 65504.f : z[j] < -65504.f ? -65504.f : z[j];   // NaN stays
+    }
+}
+
 // What follows the product: v are the eight columns from col on of row, bias
 // included; C is the products' type, Y the result's.
 template <class C, class Y>
 __device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col, float (&v)[8]) {
     if (col >= a.outer) return;
-    if (a.z) store8(static_cast<C*>(a.z) + row * a.z_stride, col, a.outer, v);
+    if (a.z) {
+        float z[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = v[j];
+        keep_finite<C>(z);
+        store8(static_cast<C*>(a.z) + row * a.z_stride, col, a.outer, z);
+    }
     activate<ANY>(a.act, v);
     if (a.residual) {
         float r[8];
@@ -270,7 +287,16 @@ __device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0
 // col is the lane's in the first.  All lanes must be active.
 template <class C, class Y, int ACT, int N>
 __device__ __forceinline__ void finish16(const LinearArgs& a, int64_t row0, int col, int live, float (&v)[N][8]) {
-    if (a.z) store16<C>(a.z, a.z_stride, row0, a.rows, col, a.outer, live, v);
+    if (a.z) {
+        float z[N][8];
+#pragma unroll
+        for (int b = 0; b < N; ++b) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[b][j] = v[b][j];
+            keep_finite<C>(z[b]);
+        }
+        store16<C>(a.z, a.z_stride, row0, a.rows, col, a.outer, live, z);
+    }
 #pragma unroll
     for (int b = 0; b < N; ++b) activate<ACT>(a.act, v[b]);
     if (a.residual) {

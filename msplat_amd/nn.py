@@ -383,8 +383,8 @@ def linear_forward(x, weight, bias=None, residual=None, activation=None, out_dty
     """residual + a(x weight^T + bias) with a = None (the identity), "silu" or "gelu"
     (tanh form); weight [outer, inner], bias [outer].  x and weight are of one type, as
     is bias, or both Mx8 with a float32 bias.  The result and residual have `out_dtype`,
-    x's own where None.  keep: (result, x weight^T + bias in x's type), the latter
-    for the backward.  A row of x that holds an infinity may come out as NaN
+    x's own where None.  keep: (result, x weight^T + bias in x's type, in float16 to
+    65504 at most), the latter for the backward.  A row of x that holds an infinity may come out as NaN
     throughout; other rows are untouched."""
     act = _linear_activation(activation)
     kept = isinstance(x, Mx8)
