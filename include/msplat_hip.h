@@ -590,9 +590,12 @@ int msplat_hip_linear(const MsplatLinearArgs* args);
  * activation is MSPLAT_IDENTITY, z: dx [rows, inner], dweight [outer, inner]
  * contiguous and dbias [outer], each written where not NULL; residual's gradient is dy.
  * x_scales, z_scales not NULL: x, z are in 8 bits (x, z their data, the strides
- * unused).  x is not looked at where dweight is NULL.  In 16-bit types dz = dy a'(z) is rounded to the type for the products (in
- * float16 it loses bits below 6e-5 and vanishes below 3e-8).  The sums over
- * rows have a fixed order. */
+ * unused).  x is not looked at where dweight is NULL.  In 16-bit types dz = dy a'(z),
+ * also of a dy in fp32, is rounded to the type for dx and dweight (not for dbias), and
+ * in float16 loses bits below 6e-5, vanishes below 3e-8 and is infinite beyond 65504:
+ * scale dy so that it does not, or use bfloat16.  A row of dy that holds an infinity
+ * may make its row of dx NaN throughout; other rows are untouched, and so are dweight
+ * and dbias but for that infinity's own output.  The sums over rows have a fixed order. */
 typedef struct MsplatLinearGradArgs {
     void* stream;
     int64_t rows;

@@ -427,7 +427,10 @@ def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, 
     """(dx, dweight, dbias) from the gradient of the result, x, weight and, where there
     is an activation, what the forward kept; x and z may be Mx8 of them.  The
     gradients have weight's type.  Those not wanted are None and not computed; without
-    dweight x may be None."""
+    dweight x may be None.  In 16-bit types dy a'(z), also of a dy in float32, is rounded
+    to the type for dx and dweight (float16: fewer bits below 6e-5, 0 below 3e-8, infinite
+    beyond 65504).  A row of dy that holds an infinity may make its row of dx NaN
+    throughout; other rows are untouched."""
     act = _linear_activation(activation)
     if x is None and wanted[1]:
         raise ValueError("the weight's gradient takes x")
@@ -621,7 +624,9 @@ class _Linear(torch.autograd.Function):
 
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
     """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
-    "mx8" keeps x and x weight^T + bias for the backward in 8 bits, where that is less."""
+    "mx8" keeps x and x weight^T + bias for the backward in 8 bits, where that is less.
+    A float16 weight's backward rounds the result's gradient to float16, whatever
+    out_dtype is: scale the loss so that it stays above 6e-5, or use bfloat16."""
     _check_checkpoint(checkpoint)
     if isinstance(x, Mx8) or isinstance(weight, Mx8):
         raise ValueError("a product of Mx8 has no gradients: call linear_forward")
