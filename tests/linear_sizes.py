@@ -18,3 +18,7 @@ FEW = [(1025, 257, 20), (1100, 300, 50), (1300, 50, 70), (1500, 150, 300)]
 # a block to several a workgroup
 ONE_PASS = [(7, 64, 256), (33, 60, 250), (2100, 33, 200), (9000, 64, 96), (500, 128, 256), (4500, 70, 130), (40, 256, 64),
             (3000, 250, 50), (700, 256, 128), (5000, 129, 65), (20000, 8, 3)]
+# float32 inputs in three blocks of the contraction: resident weights, one slice and several
+THREE_BLOCKS = [(132000, 45, 5), (44000, 33, 70), (33000, 48, 129), (7000, 45, 1100)]
+# gradients whose dx is a product with streamed weights
+STREAMED_DX = [(rows, outer, inner) for rows, inner, outer in STREAMED]
