@@ -175,18 +175,12 @@ __device__ __forceinline__ void store8(T* row, int col, int n, const float (&v)[
         else if (col + h * E<T> < n) store_piece(row, col + h * E<T>, n, p);
     }
 }
-// By a type that is an argument.
+// The same by a type that is an argument.
 __device__ __forceinline__ void load8(const void* base, int dtype, int64_t stride, int64_t row, int col, int n,
                                       float (&v)[8]) {
     if (dtype == 0) load8(static_cast<const float*>(base) + row * stride, col, n, v);
     else if (dtype == 1) load8(static_cast<const _Float16*>(base) + row * stride, col, n, v);
     else load8(static_cast<const __bf16*>(base) + row * stride, col, n, v);
-}
-__device__ __forceinline__ void store8(void* base, int dtype, int64_t stride, int64_t row, int col, int n,
-                                       const float (&v)[8]) {
-    if (dtype == 0) store8(static_cast<float*>(base) + row * stride, col, n, v);
-    else if (dtype == 1) store8(static_cast<_Float16*>(base) + row * stride, col, n, v);
-    else store8(static_cast<__bf16*>(base) + row * stride, col, n, v);
 }
 
 // z as it is kept for the backward pass.  Beyond float16's range it is the largest
@@ -623,17 +617,13 @@ LinearArgs rows_from(const LinearArgs& a, int64_t at, int64_t rows) {
     return p;
 }
 
+// One launch: 2048 workgroups at most, or the tail's 1024 rows.
 template <class T, class Y, bool MX, bool TRANS>
 void few_product(hipStream_t s, const LinearArgs& a) {
-    const int64_t blocks = ceil_div(a.outer, COLS);
     auto launch = [&](auto r) {
         constexpr int R = r();
-        // a launch has fewer than 2^32 threads
-        const int64_t most = (int64_t(1) << 23) / blocks * 16 * R;
-        for (int64_t at = 0; at < a.rows; at += most) {
-            const LinearArgs p = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
-            k_linear_few<T, Y, MX, TRANS, R><<<(unsigned)(ceil_div(p.rows, 16 * R) * blocks), 64 * FEW_WAVES<R>, 0, s>>>(p);
-        }
+        const int64_t groups = ceil_div(a.rows, 16 * R) * ceil_div(a.outer, COLS);
+        k_linear_few<T, Y, MX, TRANS, R><<<(unsigned)groups, 64 * FEW_WAVES<R>, 0, s>>>(a);
     };
     if (a.rows <= 16) launch(std::integral_constant<int, 1>{});
     else launch(std::integral_constant<int, FEW_TILES>{});
@@ -925,16 +915,12 @@ __host__ __device__ inline int dx_tiles(int inner) {
     return (inner + TASK<T> - 1) / TASK<T> * (TASK<T> / 16);
 }
 
-// Calls f with the least number of tiles that there is code for, MOST at most, that
-// holds n (a multiple of HT where a wave's tiles are neighbours).
-template <int MOST, int HT, class F>
+// Calls f with the least number of tiles that there is code for, MOST (2 or 4) or half of
+// four, that holds n.
+template <int MOST, class F>
 __device__ __forceinline__ void with_live(int n, F&& f) {
-    if constexpr (MOST >= 8)
-        if (n <= 4) return with_live<4, HT>(n, f);
-    if constexpr (MOST >= 4 && MOST % 2 == 0)
-        if (n <= MOST / 2) return with_live<MOST / 2, HT>(n, f);
-    if constexpr (MOST == 4 && HT == 1)
-        if (n <= 3) return f(std::integral_constant<int, 3>{});
+    if constexpr (MOST == 4)
+        if (n <= 2) return f(std::integral_constant<int, 2>{});
     f(std::integral_constant<int, MOST>{});
 }
 
@@ -1058,7 +1044,7 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         const piece_t<T>* bx = lx + turn * RB * kblock;
         if (a.dweight)
             // straight code for each number of tiles along the inputs that a wave may have
-            with_live<S::HK, HT>((ktiles - wk + S::WK - 1) / S::WK, [&](auto live) __attribute__((always_inline)) {
+            with_live<S::HK>((ktiles - wk + S::WK - 1) / S::WK, [&](auto live) __attribute__((always_inline)) {
                 constexpr int HK = decltype(live)::value;
 #pragma unroll
                 for (int h = 0; h < RB; ++h) {
