@@ -122,7 +122,8 @@ class AppearanceHead:
             if "w_gate" in q:
                 f = nn.gated_ffn(n, q["w_gate"], q["w_up"], q["w_down"], self.activation, keep)
         h, w = rgb.shape[:2]
-        y = nn.linear(n, self.out.to(self.dtype), residual=rgb.reshape(h * w, 3), out_dtype=torch.float32, checkpoint=keep)
+        y = nn.linear(n, self.out.to(self.dtype), residual=rgb.reshape(h * w, 3), out_dtype=torch.float32,
+                      checkpoint=keep)
         return y.reshape(h, w, 3)
 
     def _view(self, view):

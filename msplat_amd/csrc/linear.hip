@@ -49,7 +49,9 @@ size_t linear_workspace(int dtype, int64_t rows, int inner, int outer) {
 
 size_t linear_grad_workspace(int dtype, int y_dtype, int64_t rows, int inner, int outer, int act) {
     size_t n = 0;
-    with_type(dtype, [&](auto t) { n = (size_t)linear::plan<decltype(t)>(rows, inner, outer, act, y_dtype == dtype).bytes(); });
+    with_type(dtype, [&](auto t) {
+        n = (size_t)linear::plan<decltype(t)>(rows, inner, outer, act, y_dtype == dtype).bytes();
+    });
     return n;
 }
 

@@ -222,8 +222,8 @@ __device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col
 // without an activation: 182 us in the 64-byte parts that a piece a lane makes, 145
 // in lines.)
 template <class T>
-__device__ __forceinline__ void store_lines(void* base, int64_t stride, int64_t row0, int64_t rows, int ca, int cb, int n,
-                                            piece_t<T> pa, piece_t<T> pb) {
+__device__ __forceinline__ void store_lines(void* base, int64_t stride, int64_t row0, int64_t rows, int ca, int cb,
+                                            int n, piece_t<T> pa, piece_t<T> pb) {
     typedef int i32x4 __attribute__((ext_vector_type(4)));
     i32x4 wa, wb, first, second;
     __builtin_memcpy(&wa, &pa, 16);
@@ -253,8 +253,8 @@ constexpr int LINE = sizeof(Y) == 4 ? 1 : 2;
 
 // The columns col .. col + 7 of each of N blocks, of which the first `live` are there.
 template <class T, int N>
-__device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0, int64_t rows, int col, int n, int live,
-                                        const float (&v)[N][8]) {
+__device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0, int64_t rows, int col, int n,
+                                        int live, const float (&v)[N][8]) {
     piece_t<T> p[N][8 / E<T>];
 #pragma unroll
     for (int b = 0; b < N; ++b)
@@ -294,7 +294,8 @@ __device__ __forceinline__ void finish16(const LinearArgs& a, int64_t row0, int 
 #pragma unroll
     for (int b = 0; b < N; ++b) activate<ACT>(a.act, v[b]);
     if (a.residual) {
-        const Y* at = static_cast<const Y*>(a.residual) + min(row0 + (threadIdx.x & 15), a.rows - 1) * a.residual_stride;
+        const int64_t row = min(row0 + (threadIdx.x & 15), a.rows - 1);
+        const Y* at = static_cast<const Y*>(a.residual) + row * a.residual_stride;
 #pragma unroll
         for (int b = 0; b < N; ++b) {
             if (col + b * COLS >= a.outer || b >= live) continue;
@@ -386,7 +387,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES<R>) void k_linear_few(LinearArgs a) 
 // 500k x 256 -> 256 from 8 bits 110 us, 3.6 TB/s).  With two workgroups of 12 waves or 16
 // the registers of a wave do not suffice (214 us -> 366 and more at an earlier step).
 template <class T, class Y, bool MX, bool TRANS, int ACT, int DK, int R>
-__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_all(LinearArgs a, int slices, int slice_blocks) {
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_all(
+    LinearArgs a, int slices, int slice_blocks) {
     using C = typename Operand<T, MX>::type;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     piece_t<C>* w = reinterpret_cast<piece_t<C>*>(lds);
@@ -414,7 +416,8 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
-            for (int kb = 0; kb < DK; ++kb) next[i][kb].template read<DK == 1>(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
+            for (int kb = 0; kb < DK; ++kb)
+                next[i][kb].template read<DK == 1>(a, min(tile * 16 * R + 16 * i + r, a.rows - 1), kb, q);
     };
     read(t);
     piece_t<C> x[R][DK];
@@ -470,15 +473,16 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) vo
 // after the other, block after block of the contraction (kbs of them), the slice's
 // 2 NB tiles.
 template <class T, bool MX, bool TRANS>
-__global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int kbs, piece_t<typename Operand<T, MX>::type>* out,
-                                                     int64_t pieces) {
+__global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int kbs,
+                                                     piece_t<typename Operand<T, MX>::type>* out, int64_t pieces) {
+    using C = typename Operand<T, MX>::type;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
-    const int lane = (int)(i & 63), live = (a.inner + KB<typename Operand<T, MX>::type> - 1) / KB<typename Operand<T, MX>::type>;
+    const int lane = (int)(i & 63), live = (a.inner + KB<C> - 1) / KB<C>;
     const int64_t f = i >> 6;
     const int t = (int)(f % (2 * nb)), kb = (int)(f / (2 * nb) % kbs), slice = (int)(f / (2 * nb) / kbs);
     const int row = (slice * nb + t / 2) * COLS + column(t % 2, lane & 15);
-    piece_t<typename Operand<T, MX>::type> v = {};
+    piece_t<C> v = {};
     if (kb < live) v = w_piece<T, MX, TRANS>(a, row, kb, lane >> 4);
     out[i] = v;
 }
@@ -488,8 +492,9 @@ __global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int k
 // read two steps ahead: a step's products take less than a read from memory does.
 // (65536 x 1000 -> 200 f16: 48 us, 3.8 TB/s, matrix unit 27%; one step ahead 81.)
 template <class T, class Y, bool MX, int NB, int R, int KC>
-__global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a, const piece_t<typename Operand<T, MX>::type>* packed,
-                                                       int slices, int steps) {
+__global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a,
+                                                       const piece_t<typename Operand<T, MX>::type>* packed, int slices,
+                                                       int steps) {
     using C = typename Operand<T, MX>::type;
     constexpr int F = KC * 2 * NB;   // fragments of a step
     __shared__ piece_t<C> w[2][F * 64];
@@ -636,7 +641,8 @@ void all_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     const int per_cu = std::min<int>(2, LDS_BYTES / bytes), most_waves = 16 / per_cu;
     const int64_t tiles = ceil_div(a.rows, 16 * R), most = std::max<int64_t>(per_cu * CUS / p.slices / 8, 1) * 8;
     const int64_t groups = std::min(ceil_div(tiles, 8) * 8, most);   // a multiple of 8, as the kernel numbers them
-    k_linear_all<T, Y, MX, TRANS, ACT, DK, R><<<(unsigned)(groups * p.slices), 64 * most_waves, bytes, s>>>(a, p.slices, p.nb);
+    k_linear_all<T, Y, MX, TRANS, ACT, DK, R>
+        <<<(unsigned)(groups * p.slices), 64 * most_waves, bytes, s>>>(a, p.slices, p.nb);
 }
 
 // Rows that a streamed product leaves to k_linear_few: the start of a last round of
@@ -658,7 +664,8 @@ void stream_product(hipStream_t s, const LinearArgs& a, const Shape& p) {
     for (int64_t at = 0; at < a.rows; at += most) {
         const LinearArgs part = rows_from<T, MX>(a, at, std::min(most, a.rows - at));
         const int64_t groups = ceil_div(ceil_div(part.rows, STREAM_ROWS), 8) * 8;
-        k_linear_stream<T, Y, MX, NB, R, KC><<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
+        k_linear_stream<T, Y, MX, NB, R, KC>
+            <<<(unsigned)(groups * p.slices), 64 * WAVES, 0, s>>>(part, packed, p.slices, p.steps);
     }
 }
 
@@ -688,8 +695,8 @@ void product(hipStream_t s, const LinearArgs& a) {
         }
     }
     const int64_t pieces = p.packed / 16;
-    k_linear_pack<T, MX, TRANS><<<(unsigned)ceil_div(pieces, 256), 256, 0, s>>>(a, p.nb, p.steps * KC,
-                                                                              reinterpret_cast<piece_t<C>*>(a.ws), pieces);
+    piece_t<C>* packed = reinterpret_cast<piece_t<C>*>(a.ws);
+    k_linear_pack<T, MX, TRANS><<<(unsigned)ceil_div(pieces, 256), 256, 0, s>>>(a, p.nb, p.steps * KC, packed, pieces);
     const int64_t tail = tail_rows(a.rows, p.slices);
     const LinearArgs main = rows_from<T, MX>(a, 0, a.rows - tail);
     if (tail) few_product<T, Y, MX, TRANS>(s, rows_from<T, MX>(a, a.rows - tail, tail));
@@ -717,7 +724,8 @@ int64_t product_workspace(int64_t rows, int inner, int outer) {
 // dz = dy a'(z) in T, and the sums of its columns over each workgroup's rows.
 // tx threads along a row, eight columns each; 256 / tx rows at once.
 template <class T, bool MX>
-__global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, float* part, int tx, int64_t rows_per_group) {
+__global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, float* part, int tx,
+                                                   int64_t rows_per_group) {
     __shared__ float sums[256][8];
     const int lane = threadIdx.x & (tx - 1), sub = threadIdx.x / tx, rb = 256 / tx;
     const int64_t first = (int64_t)blockIdx.x * rows_per_group, last = min(first + rows_per_group, a.rows);
@@ -731,14 +739,16 @@ __global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, floa
                 if (a.act != LINEAR_NONE) {
                     float z[8];
                     if constexpr (MX) {
+                        const uint8_t* data = static_cast<const uint8_t*>(a.z) + row * mx8::data_stride(a.outer);
                         uint32_t bytes[2];
-                        __builtin_memcpy(bytes, static_cast<const uint8_t*>(a.z) + row * mx8::data_stride(a.outer) + col, 8);
+                        __builtin_memcpy(bytes, data + col, 8);
                         mx8::values<__bf16>(bytes, a.z_scales[row * mx8::scale_stride(a.outer) + col / 32], z);
                     } else {
                         load8(static_cast<const T*>(a.z) + row * a.z_stride, col, a.outer, z);
                     }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] *= a.act == LINEAR_SILU ? slope<LINEAR_SILU>(z[j]) : slope<LINEAR_GELU>(z[j]);
+                    for (int j = 0; j < 8; ++j)
+                        v[j] *= a.act == LINEAR_SILU ? slope<LINEAR_SILU>(z[j]) : slope<LINEAR_GELU>(z[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum[j] += v[j];
@@ -761,7 +771,8 @@ __global__ __launch_bounds__(256) void k_linear_dz(LinearGradArgs a, T* dz, floa
 // Adds `groups` partial rows of n1 + n2 numbers into two results, either of which
 // may be null: 32 columns a workgroup at once, 32 threads a column.
 template <class T>
-__global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int groups, int64_t n1, int64_t n2, T* out1, T* out2) {
+__global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int groups, int64_t n1, int64_t n2, T* out1,
+                                                      T* out2) {
     __shared__ float red[32][33];
     const int sl = threadIdx.x >> 5;
     const int64_t n = n1 + n2;
@@ -787,7 +798,8 @@ __global__ __launch_bounds__(1024) void k_linear_fold(const float* part, int gro
 }
 // The same for few groups: a thread a column.
 template <class T>
-__global__ __launch_bounds__(256) void k_linear_fold_few(const float* part, int groups, int64_t n1, int64_t n2, T* out1, T* out2) {
+__global__ __launch_bounds__(256) void k_linear_fold_few(const float* part, int groups, int64_t n1, int64_t n2, T* out1,
+                                                         T* out2) {
     const int64_t n = n1 + n2;
     for (int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x; col < n; col += (int64_t)gridDim.x * 256) {
         float t = 0.f;
@@ -925,10 +937,12 @@ __device__ __forceinline__ void with_live(int n, F&& f) {
 }
 
 template <class T, class S, int ACT, bool ZMX, bool XMX>
-__global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_bwd(LinearGradArgs a, T* dz, float* part, int tiles, int ktiles_all) {
+__global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_bwd(
+    LinearGradArgs a, T* dz, float* part, int tiles, int ktiles_all) {
     constexpr int STEP = RB * KB<T>;
     constexpr int NB = S::n / KB<T>, KBS = S::k / KB<T>, NP = NB * 4, KP = KBS * 4, RT = STEP / 16;
-    constexpr int PD = STEP * NP / BWD_THREADS > 0 ? STEP * NP / BWD_THREADS : 1, PX = STEP * KP / BWD_THREADS > 0 ? STEP * KP / BWD_THREADS : 1;
+    constexpr int PD = STEP * NP / BWD_THREADS > 0 ? STEP * NP / BWD_THREADS : 1;
+    constexpr int PX = STEP * KP / BWD_THREADS > 0 ? STEP * KP / BWD_THREADS : 1;
     constexpr int HT = ffn::HT<T>, TT = TASK<T> / 16;   // tiles of a block, of a task
     extern __shared__ __attribute__((aligned(16))) char lds[];
     // the part of dW that is the workgroup's; dx is made where that is all of it
@@ -978,8 +992,8 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
                 const int64_t row = row0 + p * (BWD_THREADS / NP);
                 fy.read(dy[p], row * a.dy_stride + rd * a.dy_stride, 0, a.outer);
                 if (ACT != LINEAR_NONE)
-                    fz.read(z[p], row * zstride + rd * zstride, fz.scale_offset(row, a.outer) + fz.scale_offset(rd, a.outer),
-                            a.outer);
+                    fz.read(z[p], row * zstride + rd * zstride,
+                            fz.scale_offset(row, a.outer) + fz.scale_offset(rd, a.outer), a.outer);
             } else {
                 const int64_t row = min(row0 + rd + p * (BWD_THREADS / NP), a.rows - 1);
                 fy.read(dy[p], row * a.dy_stride, 0, a.outer);
@@ -990,7 +1004,8 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         for (int p = 0; p < PX; ++p) {
             if (whole) {
                 const int64_t row = row0 + p * (BWD_THREADS / KP);
-                fx.read(x[p], row * xstride + rx * xstride, fx.scale_offset(row, a.inner) + fx.scale_offset(rx, a.inner), a.inner);
+                fx.read(x[p], row * xstride + rx * xstride,
+                        fx.scale_offset(row, a.inner) + fx.scale_offset(rx, a.inner), a.inner);
             } else {
                 const int64_t row = min(row0 + rx + p * (BWD_THREADS / KP), a.rows - 1);
                 fx.read(x[p], row * xstride, fx.scale_offset(row, a.inner), a.inner);
@@ -1050,9 +1065,11 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
                 for (int h = 0; h < RB; ++h) {
                     piece_t<T> ds[S::HN], xs[HK];
 #pragma unroll
-                    for (int j = 0; j < HK; ++j) xs[j] = ffn::by_dim<T>(bx + h * kblock, min(j * S::WK + wk, ktiles - 1));
+                    for (int j = 0; j < HK; ++j)
+                        xs[j] = ffn::by_dim<T>(bx + h * kblock, min(j * S::WK + wk, ktiles - 1));
 #pragma unroll
-                    for (int i = 0; i < S::HN; ++i) ds[i] = ffn::by_dim<T>(bd + h * nblock, min(i * S::WN + wn, ntiles - 1));
+                    for (int i = 0; i < S::HN; ++i)
+                        ds[i] = ffn::by_dim<T>(bd + h * nblock, min(i * S::WN + wn, ntiles - 1));
 #pragma unroll
                     for (int i = 0; i < S::HN; ++i)
                         if (i * S::WN + wn < ntiles)
@@ -1090,7 +1107,8 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
                 for (int j = 0; j < E<T>; ++j) v[j] = (T)o[j / 4][j % 4];
                 const int64_t row = b * STEP + tile / HT * KB<T> + ffn::perm<T>(tile % HT, r);
                 const int col = task * TASK<T> + q * E<T>;
-                if (row < a.rows && col < a.inner) store_piece(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
+                if (row < a.rows && col < a.inner)
+                    store_piece(static_cast<T*>(a.dx) + row * a.dx_stride, col, a.inner, v);
             }
             first += tasks;
         }
@@ -1172,8 +1190,8 @@ Plan plan(int64_t rows, int inner, int outer, int act, bool same_type) {
     p.groups = (int)std::min<int64_t>(ceil_div(rows, RB * KB<T>), std::max<int64_t>(CUS / p.tiles, 1));
     const int64_t n = ceil_div(std::min(outer, p.n), KB<T>) * KB<T>, k = ceil_div(std::min(inner, p.k), KB<T>) * KB<T>;
     // W^T, two steps of dz and x; the sums of db at the end
-    p.lds = (size_t)std::max<int64_t>(((p.all ? n * dx_tiles<T>(inner) * 16 : 0) + 2 * RB * KB<T> * (n + k)) * sizeof(T),
-                                      BWD_THREADS * E<T> * 4);
+    const int64_t held = (p.all ? n * dx_tiles<T>(inner) * 16 : 0) + 2 * RB * KB<T> * (n + k);
+    p.lds = (size_t)std::max<int64_t>(held * sizeof(T), BWD_THREADS * E<T> * 4);
     p.dw_bytes = aligned((int64_t)p.groups * ((int64_t)outer * inner + outer) * 4);
     if (p.own_dz) {
         p.dz_tx = 1;
@@ -1194,9 +1212,12 @@ void pass(hipStream_t s, const LinearGradArgs& a, const Plan& p, T* dz, float* p
     auto launch = [&](auto shape) {
         using S = decltype(shape);
         auto run = [&](auto act, auto zmx) {
-            if (a.x_scales)
-                k_linear_bwd<T, S, act(), zmx(), true><<<grid, BWD_THREADS, p.lds, s>>>(a, dz, part, p.tiles, p.ktiles);
-            else k_linear_bwd<T, S, act(), zmx(), false><<<grid, BWD_THREADS, p.lds, s>>>(a, dz, part, p.tiles, p.ktiles);
+            auto with = [&](auto xmx) {
+                k_linear_bwd<T, S, act(), zmx(), xmx()>
+                    <<<grid, BWD_THREADS, p.lds, s>>>(a, dz, part, p.tiles, p.ktiles);
+            };
+            if (a.x_scales) with(std::true_type{});
+            else with(std::false_type{});
         };
         auto kept = [&](auto act) {
             if (a.z_scales) run(act, std::true_type{});

@@ -398,7 +398,8 @@ def linear_forward(x, weight, bias=None, residual=None, activation=None, out_dty
             raise ValueError("a product of Mx8 has no backward to keep anything for")
         rows, inner, outer, like = x.rows, x.dim, weight.rows, x.data
         if weight.data.dim() != 2 or weight.dim != inner or weight.device != x.device:
-            raise ValueError(f"weight has shape {tuple(weight.shape)} on {weight.device}, not [outer, {inner}] on {x.device}")
+            raise ValueError(f"weight has shape {tuple(weight.shape)} on {weight.device}, not [outer, {inner}] on "
+                             f"{x.device}")
         dtype, b = _MX8, None if bias is None else _vector("bias", bias, outer, torch.float32, x.device)
         ops = (x.data.data_ptr(), 0, x.scales.data_ptr(), weight.data.data_ptr(), 0, weight.scales.data_ptr())
     else:
@@ -463,9 +464,9 @@ def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, 
     dweight = weight.new_empty(outer, inner) if wanted[1] else None
     dbias = weight.new_empty(outer) if wanted[2] else None
     ws = _workspace(lib.msplat_hip_linear_backward_workspace(rows, inner, outer, dtype, _dtype(dy), act), weight)
-    a = _abi.LinearGradArgs(_stream(weight), rows, inner, outer, dtype, _dtype(dy), act, dy2.data_ptr(), dy2.stride(0), *xs,
-                            w.data_ptr(), w.stride(0), *zs, _ptr(dx), inner, _ptr(dweight), _ptr(dbias), ws.data_ptr(),
-                            ws.nbytes)
+    a = _abi.LinearGradArgs(_stream(weight), rows, inner, outer, dtype, _dtype(dy), act, dy2.data_ptr(), dy2.stride(0),
+                            *xs, w.data_ptr(), w.stride(0), *zs, _ptr(dx), inner, _ptr(dweight), _ptr(dbias),
+                            ws.data_ptr(), ws.nbytes)
     _abi.check(lib.msplat_hip_linear_backward(ctypes.byref(a)))
     return dx, dweight, dbias
 
