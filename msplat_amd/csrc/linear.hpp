@@ -1130,21 +1130,22 @@ __global__ __launch_bounds__(BWD_THREADS) __attribute__((amdgpu_waves_per_eu(4, 
         if (wave < BWD_WAVES / 2) advance();
     }
     if (!part) return;
-    const int64_t n = (int64_t)a.outer * a.inner;
+    const int64_t n = a.dweight ? (int64_t)a.outer * a.inner : 0;
     part += group * (n + a.outer);
     // lane (q, r): dW rows 4 q .. of the tile, column r
+    if (a.dweight)
 #pragma unroll
-    for (int i = 0; i < S::HN; ++i)
+        for (int i = 0; i < S::HN; ++i)
 #pragma unroll
-        for (int j = 0; j < S::HK; ++j) {
-            const int fi = i * S::WN + wn, fj = j * S::WK + wk;
-            const int kk = k0 + fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
+            for (int j = 0; j < S::HK; ++j) {
+                const int fi = i * S::WN + wn, fj = j * S::WK + wk;
+                const int kk = k0 + fj / HT * KB<T> + ffn::perm<T>(fj % HT, r);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int nn = n0 + fi / HT * KB<T> + ffn::perm<T>(fi % HT, 4 * q + e);
-                if (nn < a.outer && kk < a.inner) part[(int64_t)nn * a.inner + kk] = acc[i][j][e];
+                for (int e = 0; e < 4; ++e) {
+                    const int nn = n0 + fi / HT * KB<T> + ffn::perm<T>(fi % HT, 4 * q + e);
+                    if (nn < a.outer && kk < a.inner) part[(int64_t)nn * a.inner + kk] = acc[i][j][e];
+                }
             }
-        }
     if (k0 != 0) return;   // all threads
     __syncthreads();
     float* sums = reinterpret_cast<float*>(lds);   // [BWD_THREADS / NP][columns]
@@ -1244,9 +1245,10 @@ void backward(hipStream_t s, LinearGradArgs a) {
     const bool dx = a.dx && a.rows > 0;
     if (p.own_dz) {
         float* sums = a.dbias ? db_part : nullptr;
+        T* taken = dx || a.dweight ? dz : nullptr;
         if (p.dz_groups > 0) {
-            if (a.z_scales) k_linear_dz<T, true><<<p.dz_groups, 256, 0, s>>>(a, dz, sums, p.dz_tx, p.dz_rows);
-            else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, dz, sums, p.dz_tx, p.dz_rows);
+            if (a.z_scales) k_linear_dz<T, true><<<p.dz_groups, 256, 0, s>>>(a, taken, sums, p.dz_tx, p.dz_rows);
+            else k_linear_dz<T, false><<<p.dz_groups, 256, 0, s>>>(a, taken, sums, p.dz_tx, p.dz_rows);
         }
         if (sums) fold<T>(s, sums, p.dz_groups, a.outer, 0, a.dbias, nullptr);
         a.dy = dz;
@@ -1260,7 +1262,7 @@ void backward(hipStream_t s, LinearGradArgs a) {
     if (!p.all) g.dx = nullptr;
     const bool sums = a.dweight || a.dbias, makes_dz = dz && !p.own_dz && dx;
     if (p.groups > 0 && (sums || makes_dz || g.dx)) pass<T>(s, g, p, makes_dz ? dz : nullptr, sums ? part : nullptr);
-    if (sums) fold<T>(s, part, p.groups, (int64_t)a.outer * a.inner, a.outer, a.dweight, a.dbias);
+    if (sums) fold<T>(s, part, p.groups, a.dweight ? (int64_t)a.outer * a.inner : 0, a.outer, a.dweight, a.dbias);
     if (p.all || !dx) return;
     LinearArgs d{};
     d.rows = a.rows;
