@@ -164,13 +164,30 @@ __device__ __forceinline__ void load8(const T* row, int col, int n, float (&v)[8
         for (int j = 0; j < E<T>; ++j) v[h * E<T> + j] = (float)p[j];
     }
 }
-template <class T>
+// v's elements with infinities as the type's largest number where FINITE: z as it is kept
+// for the backward pass.  a'(z) is 1 or 0 from far smaller arguments on, but of an
+// infinity it would be NaN (infinity times 0), as would z packed into 8 bits.  Of the types
+// only float16 ends where sums may be; NaN stays.
+template <bool FINITE, class T>
+__device__ __forceinline__ piece_t<T> kept(piece_t<T> v) {
+    if constexpr (FINITE && std::is_same<T, _Float16>::value) {
+        typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+        u16x8 w;
+        __builtin_memcpy(&w, &v, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] -= (w[j] & 0x7FFF) == 0x7C00;   // the number before infinity
+        __builtin_memcpy(&v, &w, 16);
+    }
+    return v;
+}
+template <bool FINITE = false, class T>
 __device__ __forceinline__ void store8(T* row, int col, int n, const float (&v)[8]) {
 #pragma unroll
     for (int h = 0; h < 8 / E<T>; ++h) {
         piece_t<T> p;
 #pragma unroll
         for (int j = 0; j < E<T>; ++j) p[j] = (T)v[h * E<T> + j];
+        p = kept<FINITE, T>(p);
         if (n % 8 == 0) __builtin_memcpy(row + col + h * E<T>, &p, 16);
         else if (col + h * E<T> < n) store_piece(row, col + h * E<T>, n, p);
     }
@@ -183,29 +200,12 @@ __device__ __forceinline__ void load8(const void* base, int dtype, int64_t strid
     else load8(static_cast<const __bf16*>(base) + row * stride, col, n, v);
 }
 
-// z as it is kept for the backward pass.  Beyond float16's range it is the largest
-// number there, not infinite: a'(z) is 1 or 0 from far smaller arguments on, but of an
-// infinity it would be NaN (infinity times 0), as would z packed into 8 bits.
-template <class C, int N>
-__device__ __forceinline__ void keep_finite(float (&z)[N]) {
-    if constexpr (std::is_same<C, _Float16>::value) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) z[j] = z[j] > 65504.f ? 65504.f : z[j] < -65504.f ? -65504.f : z[j];   // NaN stays
-    }
-}
-
 // What follows the product: v are the eight columns from col on of row, bias
 // included; C is the products' type, Y the result's.
 template <class C, class Y>
 __device__ __forceinline__ void finish(const LinearArgs& a, int64_t row, int col, float (&v)[8]) {
     if (col >= a.outer) return;
-    if (a.z) {
-        float z[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = v[j];
-        keep_finite<C>(z);
-        store8(static_cast<C*>(a.z) + row * a.z_stride, col, a.outer, z);
-    }
+    if (a.z) store8<true>(static_cast<C*>(a.z) + row * a.z_stride, col, a.outer, v);
     activate<ANY>(a.act, v);
     if (a.residual) {
         float r[8];
@@ -252,7 +252,7 @@ template <class Y>
 constexpr int LINE = sizeof(Y) == 4 ? 1 : 2;
 
 // The columns col .. col + 7 of each of N blocks, of which the first `live` are there.
-template <class T, int N>
+template <bool FINITE, class T, int N>
 __device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0, int64_t rows, int col, int n,
                                         int live, const float (&v)[N][8]) {
     piece_t<T> p[N][8 / E<T>];
@@ -260,6 +260,10 @@ __device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0
     for (int b = 0; b < N; ++b)
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[b][j / E<T>][j % E<T>] = (T)v[b][j];
+#pragma unroll
+    for (int b = 0; b < N; ++b)
+#pragma unroll
+        for (int h = 0; h < 8 / E<T>; ++h) p[b][h] = kept<FINITE, T>(p[b][h]);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
         for (int b = 0; b < N; ++b)
@@ -281,16 +285,7 @@ __device__ __forceinline__ void store16(void* base, int64_t stride, int64_t row0
 // col is the lane's in the first.  All lanes must be active.
 template <class C, class Y, int ACT, int N>
 __device__ __forceinline__ void finish16(const LinearArgs& a, int64_t row0, int col, int live, float (&v)[N][8]) {
-    if (a.z) {
-        float z[N][8];
-#pragma unroll
-        for (int b = 0; b < N; ++b) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[b][j] = v[b][j];
-            keep_finite<C>(z[b]);
-        }
-        store16<C>(a.z, a.z_stride, row0, a.rows, col, a.outer, live, z);
-    }
+    if (a.z) store16<true, C>(a.z, a.z_stride, row0, a.rows, col, a.outer, live, v);
 #pragma unroll
     for (int b = 0; b < N; ++b) activate<ACT>(a.act, v[b]);
     if (a.residual) {
@@ -305,7 +300,7 @@ __device__ __forceinline__ void finish16(const LinearArgs& a, int64_t row0, int 
             for (int j = 0; j < 8; ++j) v[b][j] += r[j];
         }
     }
-    store16<Y>(a.y, a.y_stride, row0, a.rows, col, a.outer, live, v);
+    store16<false, Y>(a.y, a.y_stride, row0, a.rows, col, a.outer, live, v);
 }
 
 // The bias of eight columns, zeros for none; it is of x's type, 32-bit beside mx8.
