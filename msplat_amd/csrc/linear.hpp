@@ -314,10 +314,10 @@ __device__ __forceinline__ void bias8(const LinearArgs& a, int col, float (&v)[8
 
 // 16 R rows and 32 columns a workgroup, whose waves share the contraction (wave
 // w takes blocks w, w + WAVES, ...) and join their sums in LDS in a fixed order.
-// Bound by latency: two reads from memory and the join (8 x 256 -> 1000 bf16: 4.0 us).
+// Bound by latency: two reads from memory and the join (8 x 256 -> 1000 bf16: 4.1 us).
 constexpr int FEW_TILES = 4;
 // Eight waves for a single row tile: 1000 inputs are then read in one go (4 x 1000 ->
-// 1000 bf16: 5.4 us, 6.7 with four; up to 256 inputs the same).  Four tiles of eight
+// 1000 bf16: 5.6 us, 6.7 with four; up to 256 inputs the same).  Four tiles of eight
 // waves would leave room for two workgroups a CU.
 template <int R>
 constexpr int FEW_WAVES = R == 1 ? 8 : 4;
@@ -378,8 +378,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES<R>) void k_linear_few(LinearArgs a) 
 // slice; 16 waves a CU go through rows, 16 R at a time, without a barrier, and read
 // the next rows' x ahead.  Workgroups of one XCD share an L2: the slices of the same
 // rows run on one.  Bound by HBM, and by the vector unit where there is an activation
-// (1.09M x 64 -> 256 bf16: 145 us without, 4.8 TB/s, 150 to 158 with GELU, vector unit 82%;
-// 500k x 256 -> 256 from 8 bits 110 us, 3.6 TB/s).  With two workgroups of 12 waves or 16
+// (1.09M x 64 -> 256 bf16: 145 us without, 4.8 TB/s, 154 to 160 with GELU, vector unit 83%;
+// 500k x 256 -> 256 from 8 bits 112 us, 3.4 TB/s; 120k x 45 -> 192 f32
+// GELU 39 us).  With two workgroups of 12 waves or 16
 // the registers of a wave do not suffice (214 us -> 366 and more at an earlier step).
 template <class T, class Y, bool MX, bool TRANS, int ACT, int DK, int R>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4, 4))) void k_linear_all(
@@ -485,7 +486,7 @@ __global__ __launch_bounds__(256) void k_linear_pack(LinearArgs a, int nb, int k
 // Packed weights streamed through two areas of LDS, KC blocks of the contraction at
 // a time; a wave holds the sums of 16 R rows and a slice of NB column blocks.  x is
 // read two steps ahead: a step's products take less than a read from memory does.
-// (65536 x 1000 -> 200 f16: 48 us, 3.8 TB/s, matrix unit 27%; one step ahead 81.)
+// (65536 x 1000 -> 200 f16: 49 us, 3.7 TB/s, matrix unit 26%; one step ahead 81.)
 template <class T, class Y, bool MX, int NB, int R, int KC>
 __global__ __launch_bounds__(512) void k_linear_stream(LinearArgs a,
                                                        const piece_t<typename Operand<T, MX>::type>* packed, int slices,
@@ -834,8 +835,8 @@ __device__ __forceinline__ int staged(int rho, int c) {
 // a step and then make dz of the next, two do it in the other order, so that
 // vector and matrix units work at once.  A wave's tiles are WN (WK) apart and tiles
 // beyond the matrix are left out, so that the matrix units share what there is.
-//   500k x 64 -> 256 bf16 SiLU: 135 us, 4.7 TB/s (8 waves a workgroup: 153)
-//   120k x 48 -> 192 f32 GELU from 8 bits: 90 us, 49 TFLOP/s: dz by itself takes 42, dx 24
+//   500k x 64 -> 256 bf16 SiLU: 136 us, 4.7 TB/s (8 waves a workgroup: 153)
+//   120k x 48 -> 192 f32 GELU from 8 bits: 96 us, 46 TFLOP/s: dz by itself takes 42, dx 24
 //   and dW 30, and little of the one passes behind the other
 constexpr int RB = 2;
 constexpr int BWD_WAVES = 16, BWD_THREADS = 64 * BWD_WAVES;

@@ -11,8 +11,8 @@
 //
 // Bound by HBM: a row is read once, kept in registers (rows.hpp) and written
 // once.
-//   forward, 1.09M rows of 64 bf16 with a residual: 107 us, 5.2 TB/s (a large copy 5.2)
-//   the same into 8 bits, 500k rows of 128: 93 us, 4.8 TB/s
+//   forward, 1.09M rows of 64 bf16 with a residual: 106 us, 5.2 TB/s (a large copy 5.2)
+//   the same into 8 bits, 500k rows of 128: 94 us, 4.8 TB/s
 //   backward from 8 bits, 500k rows of 128 bf16: 82 us, 5.5 TB/s, and 5 us for the sums
 #include "mx8.hpp"
 #include "rows.hpp"
