@@ -523,6 +523,14 @@ def _kept(ctx):
     return [*pairs, *saved[2 * n:]]
 
 
+def _shaped(g, shape):
+    """g as the gradient of an input of that shape.  Autograd makes a gradient that
+    nobody else holds a leaf's own, and looks at the tensor, not at its memory: g itself
+    where the shape is its own, and never a view, whose memory is another gradient's or the
+    caller's."""
+    return g if g.shape == shape else g.clone(memory_format=torch.contiguous_format).view(shape)
+
+
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -596,7 +604,7 @@ class _RmsNorm(torch.autograd.Function):
             dx = dtotal
         else:
             dx, dweight = rms_norm_backward(dy, total, weight, rstd, dtotal, (along, need[1]))
-        return dx if need[0] else None, dweight, dx.reshape(ctx.residual_shape) if need[2] else None, None, None, None
+        return dx if need[0] else None, dweight, _shaped(dx, ctx.residual_shape) if need[2] else None, None, None, None
 
 
 class _Linear(torch.autograd.Function):
@@ -620,7 +628,7 @@ class _Linear(torch.autograd.Function):
         if any(need[:3]):
             x, z, weight = _kept(ctx)
             grads = linear_backward(dy, x, weight, z, ctx.activation, need[:3])
-        return (*grads, dy.reshape(ctx.residual_shape) if need[3] else None, None, None, None, None)
+        return (*grads, _shaped(dy, ctx.residual_shape) if need[3] else None, None, None, None, None)
 
 
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):

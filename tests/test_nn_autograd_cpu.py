@@ -13,12 +13,12 @@ def _linear_forward(x, weight, bias=None, residual=None, activation=None, out_dt
     z = x @ weight.t()
     z = z if bias is None else z + bias
     y = z if activation is None else torch.nn.functional.silu(z)
-    y = (y if residual is None else y + residual).to(out_dtype or x.dtype)
+    y = (y if residual is None else y + residual.view(y.shape)).to(out_dtype or x.dtype)
     return (y, z) if keep else y
 
 
 def _rms_norm_forward(x, weight=None, residual=None, eps=1e-5, mx8=False):
-    total = x if residual is None else x + residual
+    total = x if residual is None else x + residual.view(x.shape)
     rstd = (total.square().mean(-1) + eps).rsqrt()
     y = total * rstd[..., None]
     return y if weight is None else y * weight, total, rstd
@@ -147,3 +147,38 @@ def test_the_backward_is_asked_for_what_is_wanted(plain, monkeypatch):
         wanted = tuple(bool(needs >> i & 1) for i in range(3))
         assert asked.pop() == (not wanted[1], wanted) and not asked
         assert tuple(t.grad is not None for t in ops) == wanted
+
+
+def _rms_norm_backward(dy, total, weight, rstd, dtotal=None, wanted=(True, True)):
+    dx = dy * 3.0 if dtotal is None else dy * 3.0 + dtotal
+    return dx if wanted[0] else None, None
+
+
+@pytest.mark.parametrize("shape", [(3, 4), (1, 3, 4)])
+def test_gradients_share_no_memory(plain, monkeypatch, shape):
+    """The gradients of leaves are theirs alone: neither another's nor the one that the
+    caller gave backward, so that a second backward pass adds to each once."""
+    monkeypatch.setattr(nn, "linear_backward", lambda dy, x, w, z, act, wanted: (dy @ w if wanted[0] else None, None, None))
+    monkeypatch.setattr(nn, "rms_norm_backward", _rms_norm_backward)
+
+    def leaves():
+        return torch.ones(3, 4, requires_grad=True), torch.ones(shape, requires_grad=True)
+
+    def check(call, want):
+        x, r = leaves()
+        given = torch.ones(3, 4)
+        for times in (1, 2, 3):
+            call(x, r).backward(given)
+            assert (given == 1).all()
+            for t, g in zip((x, r), want):
+                assert t.grad is None if g is None else (t.grad == times * g).all(), (times, t.grad, g)
+        grads = {t.grad.data_ptr() for t in (x, r, given) if t.grad is not None}
+        assert given.data_ptr() not in grads and len(grads) == sum(g is not None for g in want)
+
+    w = torch.eye(4)
+    check(lambda x, r: nn.linear(x, w, None, r), (1, 1))
+    check(lambda x, r: nn.linear(w[:3], w, None, r), (None, 1))
+    check(lambda x, r: nn.rms_norm(x, None, r)[0], (3, 3))
+    check(lambda x, r: nn.rms_norm(x, None, r)[1], (1, 1))
+    check(lambda x, r: nn.rms_norm(w[:3], None, r)[1], (None, 1))
+    check(lambda x, r: sum(nn.rms_norm(x, None, r)), (4, 4))
