@@ -59,8 +59,14 @@ def _plain(t) -> bool:
     return (t.stride(1) == 1 or cols == 1) and (t.stride(0) >= cols or rows <= 1)
 
 
+def _tensor(name, t):
+    if type(t) is Mx8:
+        raise ValueError(f"{name} is an Mx8 where a tensor is taken")
+
+
 def _rows(name, t, dim, like):
     """t as a [rows, dim] matrix with adjacent columns."""
+    _tensor(name, t)
     if t.dim() == 2 and t.is_contiguous() and t.shape[1] == dim and t.dtype is like.dtype and \
             t.get_device() == like.get_device():
         return t
@@ -74,6 +80,7 @@ def _rows(name, t, dim, like):
 
 
 def _matrix(name, t, shape, like):
+    _tensor(name, t)
     if t.shape == shape and t.is_contiguous() and t.dtype is like.dtype and t.get_device() == like.get_device():
         return t
     if t.dtype is not like.dtype or t.device != like.device:
@@ -91,6 +98,7 @@ def _dtype(t) -> int:
 
 
 def _feature_rows(name, x):
+    _tensor(name, x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name} has shape {tuple(x.shape)}, not [..., dim]")
     return x if x.dim() == 2 and x.is_contiguous() else _rows(name, x, x.shape[-1], x)
@@ -435,6 +443,7 @@ def linear_backward(dy, x, weight, z=None, activation=None, wanted=(True, True, 
     act = _linear_activation(activation)
     if x is None and wanted[1]:
         raise ValueError("the weight's gradient takes x")
+    _tensor("weight", weight)
     lib, dtype = _library(weight), _dtype(weight)
     if weight.dim() != 2 or min(weight.shape) < 1:
         raise ValueError(f"weight has shape {tuple(weight.shape)}, not (outer, inner)")

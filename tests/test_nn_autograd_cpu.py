@@ -182,3 +182,17 @@ def test_gradients_share_no_memory(plain, monkeypatch, shape):
     check(lambda x, r: nn.rms_norm(x, None, r)[1], (1, 1))
     check(lambda x, r: nn.rms_norm(w[:3], None, r)[1], (None, 1))
     check(lambda x, r: sum(nn.rms_norm(x, None, r)), (4, 4))
+
+
+def test_rows_in_8_bits_are_refused_by_name(monkeypatch):
+    """Where a tensor is taken, an Mx8 is a ValueError that says so."""
+    monkeypatch.setattr(nn, "_library", lambda t: None)
+    x = torch.zeros(4, 8)
+    m = nn.Mx8._empty(x.shape, x, x.dtype)
+    for call in (lambda: nn.mx8_pack(m), lambda: nn.rms_norm(m), lambda: nn.rms_norm_backward(m, x, None, x[0]),
+                 lambda: nn.linear_backward(x, x, m), lambda: nn.linear_backward(m, x, x), lambda: nn.layer_norm(m),
+                 lambda: nn.gated_ffn(m, x, x, x), lambda: nn.dropout_add(m, None, 0.5, 1, 2),
+                 lambda: nn.rms_norm(x, None, m), lambda: nn.rms_norm(x, m), lambda: nn.linear(x, x, None, m),
+                 lambda: nn.linear(x, x, m)):
+        with pytest.raises(ValueError, match="Mx8"):
+            call()
