@@ -18,7 +18,9 @@ smaller that way (rows of few columns are not).
 
 None of them waits for the GPU or keeps anything between calls, so they may
 be captured into a graph.  A replay repeats a call's arguments: where each is to
-drop other elements, dropout takes its offset as a tensor.
+drop other elements, dropout takes its offset as a tensor.  As with PyTorch's own
+functions, no graph of autograd's from outside the capture may be alive over the same
+leaves while a backward pass is captured.
 """
 from __future__ import annotations
 
@@ -332,7 +334,8 @@ def mx8_unpack(m: Mx8, dtype=None):
 def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5, mx8: bool = False):
     """(y, total, rstd): total = x + residual of x's type (x itself without a
     residual), y = total rstd weight over the last axis, rstd = 1 / sqrt(mean(total^2)
-    + eps), one float32 a row.  mx8: y is an Mx8, rounded to 8 bits once."""
+    + eps), one float32 a row.  mx8: y is an Mx8, rounded to 8 bits once.  A sum of squares
+    beyond float32 counts as infinite (rstd 0)."""
     lib, dtype = _library(x), _dtype(x)
     x2 = _feature_rows("x", x)
     rows, dim = x2.shape
