@@ -29,6 +29,7 @@ from operator import index   # numpy's integers overflow in & where Python's do 
 from typing import Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _abi, device
@@ -522,7 +523,10 @@ def _smaller_packed(t) -> bool:
 def _keep(ctx, checkpoint, kept, *others):
     """Saves tensors for the backward, those in `kept` (each may be None) as
     Mx8 where the checkpoint says so and that is smaller."""
-    packed = [mx8_pack(t) if checkpoint and t is not None and _smaller_packed(t) else t for t in kept]
+    if checkpoint is None:
+        ctx.kept = None
+        return ctx.save_for_backward(*kept, *others)
+    packed = [mx8_pack(t) if t is not None and _smaller_packed(t) else t for t in kept]
     ctx.kept = [(m.dim, m.dtype) if isinstance(m, Mx8) else None for m in packed]
     flat = [t for m in packed for t in ((m.data, m.scales) if isinstance(m, Mx8) else (m, None))]
     ctx.save_for_backward(*flat, *others)
@@ -530,7 +534,10 @@ def _keep(ctx, checkpoint, kept, *others):
 
 def _kept(ctx):
     """What _keep took: those that it kept, and the others."""
-    saved, n = ctx.saved_tensors, len(ctx.kept)
+    saved = ctx.saved_tensors
+    if ctx.kept is None:
+        return saved
+    n = len(ctx.kept)
     pairs = [Mx8(*saved[2 * i:2 * i + 2], *k) if k else saved[2 * i] for i, k in enumerate(ctx.kept)]
     return [*pairs, *saved[2 * n:]]
 
@@ -643,6 +650,12 @@ class _Linear(torch.autograd.Function):
         return (*grads, _shaped(dy, ctx.residual_shape) if need[3] else None, None, None, None, None)
 
 
+def _no_derivatives(grad) -> bool:
+    """Whether a call may go past autograd, which takes 3 us: without gradients, and outside
+    forward mode, whose tangents autograd refuses whatever the grad mode is."""
+    return not grad and forward_ad._current_level < 0
+
+
 def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None, checkpoint=None):
     """linear_forward, differentiable in x, weight, bias and residual.  checkpoint
     "mx8" keeps x and x weight^T + bias for the backward in 8 bits, where that is less.
@@ -651,8 +664,10 @@ def linear(x, weight, bias=None, residual=None, activation=None, out_dtype=None,
     _check_checkpoint(checkpoint)
     if isinstance(x, Mx8) or isinstance(weight, Mx8):
         raise ValueError("a product of Mx8 has no gradients: call linear_forward")
-    # without gradients too, for forward mode's tangents to be refused; grad mode is off in there
-    return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint, torch.is_grad_enabled())
+    grad = torch.is_grad_enabled()   # off in an autograd function's forward
+    if _no_derivatives(grad):
+        return linear_forward(x, weight, bias, residual, activation, out_dtype)
+    return _Linear.apply(x, weight, bias, residual, activation, out_dtype, checkpoint, grad)
 
 
 def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
@@ -660,7 +675,11 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5, checkpoint=None):
     weight and residual.  checkpoint "mx8" keeps total for the backward in 8 bits, where
     that is less."""
     _check_checkpoint(checkpoint)
-    return _RmsNorm.apply(x, weight, residual, eps, checkpoint, torch.is_grad_enabled())
+    grad = torch.is_grad_enabled()
+    if _no_derivatives(grad):
+        y, total, _ = rms_norm_forward(x, weight, residual, eps)
+        return y if residual is None else (y, total)
+    return _RmsNorm.apply(x, weight, residual, eps, checkpoint, grad)
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
