@@ -587,6 +587,7 @@ class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, p, seed, offset):
         ctx.args = (p, seed, offset)
+        ctx.residual_shape = None if residual is None else residual.shape
         if torch.is_tensor(offset):   # saved, so that a change before the backward is an error
             ctx.args = (p, seed)
             ctx.save_for_backward(offset)
@@ -597,7 +598,7 @@ class _DropoutAdd(torch.autograd.Function):
     def backward(ctx, dy):
         need = ctx.needs_input_grad
         dx = dropout_add_backward(dy, *ctx.args, *ctx.saved_tensors) if need[0] else None
-        return dx, dy if need[1] else None, None, None, None
+        return dx, _shaped(dy, ctx.residual_shape) if need[1] else None, None, None, None
 
 
 class _RmsNorm(torch.autograd.Function):

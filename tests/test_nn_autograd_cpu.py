@@ -196,3 +196,13 @@ def test_rows_in_8_bits_are_refused_by_name(monkeypatch):
                  lambda: nn.linear(x, x, m)):
         with pytest.raises(ValueError, match="Mx8"):
             call()
+
+
+def test_dropouts_residual_of_another_shape(monkeypatch):
+    """As many rows in other axes, which the forward pass takes: its gradient has its shape."""
+    monkeypatch.setattr(nn, "dropout_add_forward", lambda x, r, p, seed, offset: x + r.view(x.shape))
+    x, given = torch.ones(2, 3, 4), torch.ones(2, 3, 4)
+    r = torch.ones(6, 4, requires_grad=True)
+    for times in (1, 2):
+        nn.dropout_add(x, r, 0.5, 1, 2).backward(given)
+        assert r.grad.shape == r.shape and (r.grad == times).all() and (given == 1).all()
